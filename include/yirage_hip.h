@@ -148,6 +148,73 @@ int yr_hip_gqa_prefill(const void* q, const void* k, const void* v, void* out, i
  * argmax_reduce (tasks/ampere/argmax.cuh:71-155). */
 int yr_hip_argmax(const void* x, int64_t* out, int rows, int n, int n_valid, int dtype, void* stream);
 
+/* ------------------------------------------------------- serving step around a paged cache
+ * A ragged batch of new tokens: sequence b owns the rows qo_indptr[b] ..
+ * qo_indptr[b + 1) of q / k / v / out (qo_indptr NULL: one row each, rows ==
+ * batch), the pages kv_indices[kv_indptr[b] .. kv_indptr[b + 1]) of a cache
+ * [num_pages][page_size][hkv][d], and has kv_len[b] tokens, the new ones last: row
+ * i of its n rows has position kv_len[b] - n + i.  d is 64 or 128; dtype f16 or
+ * bf16.  Rows behind the last sequence are left as they were.  The tables are device data
+ * that no call reads on the host: entries are clamped to `rows`, `n_indices`
+ * (length of kv_indices) and `num_pages`, and a token whose page is missing or
+ * outside the cache has no place (it is not written, not chosen, not read). */
+
+/* Writes the new tokens' keys and values into their slots; keys, and q into
+ * q_out[rows][hq][d] (q and q_out may both be NULL), are first multiplied by
+ * rsqrt(mean(x^2) + eps) * norm weight[d] (NULL: not) and rotated (rotate-half,
+ * tables cos / sin [max_pos][d] in fp32 or dtype, NULL: not), all in fp32 with one
+ * rounding.  A key whose position lies outside the tables is not written, its q row
+ * becomes NaN.  page_bounds[num_pages][hkv][2][d] (NULL: none) keeps the
+ * smallest and largest stored key per channel of each page: it starts anew when
+ * slot 0 of the page is written and grows otherwise.  strides7 = {q row, q kv group, q head in the group, k row, k head,
+ * v row, v head} in elements, multiples of 8; the last dim is contiguous.
+ * q_out may be q where the layouts agree.  No two sequences may write one page in one call.
+ * The append, RoPE and qk-norm part of the MPK paged attention task
+ * (tasks/ampere/multitoken_paged_attention_4_16.cuh:348-375, norm.cuh:21-126,
+ * rotary_embedding.cuh:22-81) as a call of its own; page_bounds has no counterpart. */
+int yr_hip_append_kv_paged(const void* q, const void* k, const void* v, void* q_out, void* k_cache, void* v_cache,
+                           void* page_bounds, const void* cos_table, const void* sin_table, int table_dtype,
+                           int max_pos, const void* q_norm, const void* k_norm, float eps, const int32_t* qo_indptr,
+                           const int32_t* kv_indptr, const int32_t* kv_indices, int n_indices, const int32_t* kv_len,
+                           int rows, int batch, int hq, int hkv, int d, int page_size, int num_pages,
+                           const int64_t* strides7, int dtype, void* stream);
+
+/* pages[rows][hkv][top_pages] = for each row and kv head the first first_pages
+ * pages of the sequence, the last last_pages (>= 1) visible ones and those of
+ * the others with the largest Q+ . max + Q- . min (min, max: page_bounds; Q+
+ * and Q-: the positive and negative parts of q summed over the group's heads),
+ * an upper bound of the sum of any token's scores; page numbers within the
+ * sequence, ascending, -1 behind them.  The sum runs in 64 bits; ties take the
+ * lower page, a NaN sum or a missing page ranks last.
+ * max_kv_len bounds kv_len (pages behind it are not seen); at most 16384 pages
+ * of it.  No counterpart in the reference. */
+int yr_hip_select_pages(const void* q, const void* page_bounds, const int32_t* qo_indptr, const int32_t* kv_indptr,
+                        const int32_t* kv_indices, int n_indices, const int32_t* kv_len, int32_t* pages, int rows,
+                        int batch, int hq, int hkv, int d, int page_size, int num_pages, int max_kv_len,
+                        int top_pages, int first_pages, int last_pages, int dtype, void* stream);
+
+/* out[t][h] = softmax(q[t][h] k^T / sqrt(d)) v over the tokens at or before row
+ * t's position in the pages pages[t][h / (hq / hkv)][0 .. top_pages); hq / hkv
+ * <= 16, top_pages <= 1024.  Entries in any order; negative, invisible, missing
+ * and repeated ones count for nothing; a row without a token is 0.  The paged attention
+ * of yr_hip_gqa_decode_paged on a selection; no counterpart in the reference. */
+int yr_hip_gqa_sparse_paged(const void* q, const void* k_cache, const void* v_cache, const int32_t* qo_indptr,
+                            const int32_t* kv_indptr, const int32_t* kv_indices, int n_indices,
+                            const int32_t* kv_len, const int32_t* pages, void* out, int rows, int batch, int hq,
+                            int hkv, int d, int page_size, int num_pages, int top_pages, int dtype, void* stream);
+
+/* Log probabilities of row-wise softmax over the first n_valid of n columns of
+ * x (f16, bf16 or fp32; rows row_stride elements apart): logprob[r] of
+ * tokens[r] (NaN for a token outside [0, n_valid)), entropy[r] in nats, and the
+ * top_n (<= 64) most likely tokens, equal ones by the lowest index, with their
+ * log probabilities.  NaN logits never reach the top (fewer candidates than
+ * top_n: index -1, -inf) and make the row's numbers NaN, as does a row of -inf alone.
+ * Sums in 64 bits over fp32 terms.  Next to yr_hip_argmax; no counterpart in
+ * the reference. */
+int yr_hip_token_logprobs(const void* x, const int64_t* tokens, float* logprob, float* entropy, float* top_logprob,
+                          int64_t* top_ids, int rows, int n, int n_valid, int64_t row_stride, int top_n, int dtype,
+                          void* stream);
+
 /* ------------------------------------------------------- kernel-graph operators */
 /* The operators of the reference's kernel graph (python/yirage/kernel.py:
  * 248-321; shape rules src/kernel/{matmul,element_unary,element_binary,

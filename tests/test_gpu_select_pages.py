@@ -1,0 +1,112 @@
+"""select_pages against 64 bits: the lists are whole numbers and have to be equal,
+ties included."""
+import pytest
+import torch
+
+import yirage_amd.fused as F
+from tests.paged_plain import Batch, score, select
+
+pytestmark = pytest.mark.gpu
+
+
+def _reference(b, q, bounds, hkv, top, first, last, max_pages=1 << 30, ids_of=None):
+    T, hq, d = q.shape
+    G = hq // hkv
+    out = torch.full((T, hkv, top), -1, dtype=torch.int32)
+    for t, p, ids in b.each_row():
+        ids = ids if ids_of is None else ids_of(ids)
+        n = min(p // b.page + 1, len(ids), max_pages) if p >= 0 else 0
+        for h in range(hkv):
+            s = []
+            if n:
+                at = torch.from_numpy(ids[:n]).long()
+                ok = (at >= 0) & (at < b.pool)
+                sc = score(q[t, h * G:(h + 1) * G], bounds[at.clamp(0, b.pool - 1), h, 0], bounds[at.clamp(0, b.pool - 1), h, 1])
+                s = torch.where(ok, sc, float("nan")).tolist()
+            take = select(s, n, top, first, last)
+            out[t, h, : len(take)] = torch.tensor(take, dtype=torch.int32)
+    return out
+
+
+@pytest.mark.parametrize("dt", [torch.float16, torch.bfloat16], ids=["f16", "bf16"])
+@pytest.mark.parametrize("lens,news,hq,hkv,d,page,top,first,last", [
+    ([1], [1], 4, 4, 64, 16, 4, 1, 1), ([64, 65, 1000], [1, 1, 1], 32, 8, 128, 64, 6, 1, 1),
+    ([4097], [1], 8, 1, 128, 16, 32, 1, 2), ([700, 9, 33], [3, 9, 17], 10, 2, 64, 16, 8, 2, 3),
+    ([300], [300], 4, 2, 128, 16, 5, 0, 1), ([2000, 1300], [40, 5], 16, 1, 64, 1, 64, 4, 8),
+    ([900], [20], 14, 2, 128, 128, 20, 1, 1),       # fewer pages than asked for
+    ([5000] * 3, [1] * 3, 2, 2, 64, 48, 3, 1, 2),   # nothing left to choose
+    ([2500], [130], 8, 2, 128, 16, 33, 1, 1),
+    ([20000], [1], 4, 1, 64, 16, 400, 1, 1), ([5000, 4000], [33, 2], 8, 4, 128, 16, 16, 1, 1),
+])
+def test_lists(lens, news, hq, hkv, d, page, top, first, last, dt):
+    print("case", lens, news, hq, hkv, d, page, top, first, last, dt, flush=True)
+    gen = torch.Generator().manual_seed(top + page)
+    b = Batch(lens, news, page, seed=top)
+    q = torch.randn((b.rows, hq, d), generator=gen).to(dt)
+    mid, half = torch.randn((b.pool, hkv, d), generator=gen), torch.rand((b.pool, hkv, d), generator=gen)
+    bounds = torch.stack([mid - half, mid + half], 2).to(dt)
+    got = F.select_pages(q.cuda(), bounds.cuda(), *b.args(), page_size=page, top_pages=top, qo_indptr=b.qo(),
+                         first_pages=first, last_pages=last, max_kv_len=max(lens))
+    ref = _reference(b, q, bounds, hkv, top, first, last)
+    assert torch.equal(got.cpu(), ref)
+    # the bound on the lengths may be larger than they are, or come from them
+    again = F.select_pages(q.cuda(), bounds.cuda(), *b.args(), page_size=page, top_pages=top, qo_indptr=b.qo(),
+                           first_pages=first, last_pages=last, max_kv_len=max(lens) + 5 * page)
+    assert torch.equal(again, got)
+    none = F.select_pages(q.cuda(), bounds.cuda(), *b.args(), page_size=page, top_pages=top, qo_indptr=b.qo(),
+                          first_pages=first, last_pages=last)
+    assert torch.equal(none, got)
+
+
+@pytest.mark.parametrize("rows", [1, 7, 40])
+def test_ties_zeros_and_close_scores(rows):
+    """Equal pages tie to the lower number, -0 equals 0, scores one unit in the last place of 40
+    bits apart are told apart."""
+    dt, d, page, n = torch.float16, 64, 16, 300
+    b = Batch([n * page], [rows], page)
+    gen = torch.Generator().manual_seed(5)
+    q = torch.randn((b.rows, 2, d), generator=gen).to(dt)
+    for kind in range(4):
+        bounds = torch.zeros((b.pool, 1, 2, d))
+        ids = torch.from_numpy(b.indices).long()
+        if kind == 0:    # four kinds of page
+            bounds[ids] = torch.randn((4, 1, 2, d), generator=gen).sort(2).values[torch.arange(n) % 4]
+        elif kind == 1:  # zeros of both signs
+            bounds[ids[::2]] = -0.0
+        elif kind == 2:  # large sums that differ by little
+            bounds[..., 0] = 1000.0
+            bounds[ids, 0, :, 1] = (torch.randperm(n, generator=gen) * 2.0 ** -24)[:, None]
+        else:            # infinities and NaN
+            bounds[ids] = torch.randn((n, 1, 2, d), generator=gen).sort(2).values
+            bounds[ids[10:20], 0, 1, 3] = float("inf")
+            bounds[ids[30:40], 0, 0, 3] = float("-inf")
+            bounds[ids[50:60], 0, 0, 7] = float("nan")
+            bounds[ids[70:80], 0, 0], bounds[ids[70:80], 0, 1] = float("inf"), float("-inf")
+        bounds = bounds.to(dt)
+        got = F.select_pages(q.cuda(), bounds.cuda(), *b.args(), page_size=page, top_pages=37, qo_indptr=b.qo(),
+                             max_kv_len=n * page)
+        assert torch.equal(got.cpu(), _reference(b, q, bounds, 1, 37, 1, 1)), kind
+
+
+@pytest.mark.parametrize("news", [[1, 1, 1], [4, 1, 30]])
+def test_missing_pages_and_short_bounds(news):
+    """Ids outside the pool rank last, a short page table or max_kv_len hides what lies behind,
+    rows behind the last sequence are left alone."""
+    gen = torch.Generator().manual_seed(6)
+    dt, d, page = torch.bfloat16, 64, 16
+    b = Batch([400, 300, 350], news, page)
+    b.indices[3:9] = [-1, b.pool, 1 << 30, -5, b.pool + 1, -(1 << 31)]
+    pad = 0 if max(news) == 1 else 3
+    q = torch.randn((b.rows + pad, 4, d), generator=gen).to(dt)
+    bounds = torch.randn((b.pool, 2, 2, d), generator=gen).sort(2).values.to(dt)
+    out = torch.full((b.rows + pad, 2, 20), 99, dtype=torch.int32, device="cuda")
+    F.select_pages(q.cuda(), bounds.cuda(), *b.args(), page_size=page, top_pages=20, qo_indptr=b.qo(),
+                   max_kv_len=320, out=out)
+    assert torch.equal(out[: b.rows].cpu(), _reference(b, q[: b.rows], bounds, 2, 20, 1, 1, max_pages=20))
+    assert (out[b.rows:] == 99).all()
+    ptr, idx, lens = b.args()
+    got = F.select_pages(q.cuda(), bounds.cuda(), ptr, idx[:30], lens, page_size=page, top_pages=6,
+                         qo_indptr=b.qo(), max_kv_len=400)
+    assert torch.equal(got[: b.news[0]].cpu(), _reference(b, q[: b.rows], bounds, 2, 6, 1, 1)[: b.news[0]])
+    assert int(got[b.news[0]: b.news[0] + b.news[1]].max()) < 30 - int(ptr[1])  # the second sequence lost pages
+    assert (got[b.news[0] + b.news[1]: b.rows] == -1).all()                     # the third all of them

@@ -8,8 +8,10 @@ per-device cache that is zero-filled once at allocation.
 """
 from __future__ import annotations
 
+import contextlib
 import ctypes
 import struct
+from typing import NamedTuple
 
 import torch
 
@@ -174,6 +176,222 @@ def argmax(x, n_valid: int | None = None, out=None):
     check(lib().yr_hip_argmax(_ptr(x), _ptr(out), rows, n, n if n_valid is None else n_valid,
                               dtype_code(x.dtype), _stream(x.device)), "argmax")
     return out
+
+
+# ---------------------------------------------------------------- serving step around a paged cache
+# Operators on a ragged batch: sequence b owns the rows qo_indptr[b] ..
+# qo_indptr[b + 1) of the new tokens (qo_indptr None: one row each), the pages
+# kv_indices[kv_indptr[b] .. kv_indptr[b + 1]) and kv_len[b] tokens, the new ones
+# last.  Their kernels run on the tensors' device and its current stream.
+_DTYPE_ALL = {**_TORCH_DT, torch.float32: _lib.DTYPE_F32}
+
+
+def _fail(msg: str):
+    raise _lib.YirageHipError(f"hip backend: {msg}")
+
+
+def _on(device):
+    """Makes the tensors' device current for a launch."""
+    if torch.cuda.current_device() == device.index:
+        return contextlib.nullcontext()
+    return torch.cuda.device(device)
+
+
+def _one_device(x, *others):
+    dev = x.device
+    if dev.type != "cuda":
+        _fail("tensors must live on the GPU")
+    for t in others:
+        if t is not None and t.device != dev:
+            _fail(f"tensors on different devices ({t.device}, {dev})")
+
+
+def _dense(**ts):
+    for name, t in ts.items():
+        if t is not None and not t.is_contiguous():
+            _fail(f"{name} must be contiguous (row-major)")
+
+
+def _at(t):
+    return None if t is None else t.data_ptr()
+
+
+def _page_table(rows, kv_indptr, kv_indices, kv_len, qo_indptr):
+    """Checks of a ragged batch's tables -> batch size."""
+    for t in (kv_indptr, kv_indices, kv_len, qo_indptr):
+        if t is not None and (t.dtype != torch.int32 or t.dim() != 1):
+            _fail("page table tensors must be 1-D int32")
+    _dense(kv_indptr=kv_indptr, kv_indices=kv_indices, kv_len=kv_len, qo_indptr=qo_indptr)
+    batch = kv_len.numel()
+    if kv_indptr.numel() != batch + 1 or (qo_indptr is not None and qo_indptr.numel() != batch + 1):
+        _fail(f"kv_indptr and qo_indptr must have {batch + 1} entries (kv_len has {batch})")
+    if qo_indptr is None and rows != batch:
+        _fail(f"without qo_indptr every sequence has one row ({rows} rows, {batch} sequences)")
+    return batch
+
+
+def _output(out, shape, dtype, device):
+    if out is None:
+        return torch.empty(shape, dtype=dtype, device=device)
+    if out.shape != torch.Size(shape) or out.dtype != dtype:
+        _fail(f"out must be {tuple(shape)} {dtype}, got {tuple(out.shape)} {out.dtype}")
+    _dense(out=out)
+    return out
+
+
+def append_kv_paged(k, v, k_cache, v_cache, kv_indptr, kv_indices, kv_len, q=None, cos=None, sin=None, q_norm=None,
+                    k_norm=None, eps: float = 1e-6, qo_indptr=None, page_bounds=None, out=None):
+    """Writes new tokens k, v [T, Hkv, D] into the paged caches [P, page, Hkv, D]; returns q as the
+    attention reads it, [T, Hq, D] (None without q).
+
+    kv_len counts the new tokens, so row i of a sequence's n rows has position kv_len - n + i.
+    Keys and q are normalised per head (q_norm / k_norm [D]) and rotated (rotate-half, cos / sin
+    [positions, D], fp32 or k's dtype), in fp32 with one rounding; a q row whose position lies
+    outside the tables is NaN and its key is not written.  page_bounds [P, Hkv, 2, D] keeps each page's smallest and
+    largest key per channel (what select_pages reads).  q is [T, Hq, D] or [T, Hkv, Hq / Hkv, D];
+    q, k and v may be slices of one projection (last dim contiguous, 16-byte aligned)."""
+    _same_dtype(k, v, k_cache, v_cache, q, q_norm, k_norm, page_bounds)
+    dt = dtype_code(k.dtype)
+    if k.dim() != 3 or v.shape != k.shape or k_cache.dim() != 4 or v_cache.shape != k_cache.shape:
+        _fail("k and v must be [T, Hkv, D], the caches [P, page, Hkv, D]")
+    T, hkv, D = k.shape
+    P, page = k_cache.shape[:2]
+    if tuple(k_cache.shape[2:]) != (hkv, D):
+        _fail(f"cache heads {tuple(k_cache.shape[2:])} differ from k's {(hkv, D)}")
+    batch = _page_table(T, kv_indptr, kv_indices, kv_len, qo_indptr)
+    _dense(k_cache=k_cache, v_cache=v_cache, cos=cos, sin=sin, q_norm=q_norm, k_norm=k_norm, page_bounds=page_bounds)
+    if page_bounds is not None and tuple(page_bounds.shape) != (P, hkv, 2, D):
+        _fail(f"page_bounds must be {(P, hkv, 2, D)}")
+    for w in (q_norm, k_norm):
+        if w is not None and tuple(w.shape) != (D,):
+            _fail(f"norm weights must be [{D}]")
+    if (cos is None) != (sin is None):
+        _fail("cos and sin come together")
+    tdt, npos = 0, 0
+    if cos is not None:
+        if cos.dim() != 2 or cos.shape[1] != D or sin.shape != cos.shape or sin.dtype != cos.dtype:
+            _fail(f"cos and sin must be [positions, {D}] of one dtype")
+        if cos.dtype != k.dtype and cos.dtype != torch.float32:
+            _fail(f"tables must be float32 or {k.dtype}, got {cos.dtype}")
+        tdt, npos = _DTYPE_ALL[cos.dtype], cos.shape[0]
+    hq, qs = 0, (0, 0, 0)
+    if q is not None:
+        if q.dim() == 4:
+            if q.shape[0] != T or q.shape[1] != hkv or q.shape[3] != D:
+                _fail(f"q must be [{T}, {hkv}, heads, {D}]")
+            hq, qs = hkv * q.shape[2], q.stride()[:3]
+        else:
+            if q.dim() != 3 or q.shape[0] != T or q.shape[2] != D or q.shape[1] % hkv:
+                _fail(f"q must be [{T}, heads, {D}] with a multiple of {hkv} heads")
+            hq = q.shape[1]
+            qs = (q.stride(0), q.stride(1) * (hq // hkv), q.stride(1))
+        out = _output(out, (T, hq, D), q.dtype, q.device)
+    elif out is not None or q_norm is not None:
+        _fail("out and q_norm need q")
+    for t in (q, k, v):
+        if t is not None and t.numel() and t.stride(-1) != 1:
+            _fail("the last dim of q, k and v must be contiguous")
+    _one_device(k, v, k_cache, v_cache, kv_indptr, kv_indices, kv_len, q, cos, sin, q_norm, k_norm, qo_indptr,
+                page_bounds, out)
+    if T == 0:
+        return out
+    strides = (ctypes.c_int64 * 7)(*qs, k.stride(0), k.stride(1), v.stride(0), v.stride(1))
+    with _on(k.device):
+        check(lib().yr_hip_append_kv_paged(
+            _at(q), _at(k), _at(v), _at(out), _at(k_cache), _at(v_cache), _at(page_bounds), _at(cos), _at(sin), tdt,
+            npos, _at(q_norm), _at(k_norm), eps, _at(qo_indptr), _at(kv_indptr), _at(kv_indices), kv_indices.numel(),
+            _at(kv_len), T, batch, hq, hkv, D, page, P, strides, dt,
+            torch.cuda.current_stream(k.device).cuda_stream), "append_kv_paged")
+    return out
+
+
+def select_pages(q, page_bounds, kv_indptr, kv_indices, kv_len, page_size: int, top_pages: int, qo_indptr=None,
+                 first_pages: int = 1, last_pages: int = 1, max_kv_len: int | None = None, out=None):
+    """Pages that each row of q [T, Hq, D] attends to, per kv head: int32 [T, Hkv, top_pages], page
+    numbers within the sequence, ascending, -1 behind.
+
+    The first first_pages pages, the last last_pages (>= 1) visible ones, and the best of the others
+    by an upper bound of their scores from page_bounds [P, Hkv, 2, D] (append_kv_paged keeps it),
+    summed over the group's heads in 64 bits; ties take the lower page."""
+    _same_dtype(q, page_bounds)
+    dt = dtype_code(q.dtype)
+    _dense(q=q, page_bounds=page_bounds)
+    if q.dim() != 3 or page_bounds.dim() != 4 or page_bounds.shape[2] != 2 or page_bounds.shape[3] != q.shape[2]:
+        _fail("q must be [T, Hq, D], page_bounds [P, Hkv, 2, D]")
+    T, hq, D = q.shape
+    P, hkv = page_bounds.shape[:2]
+    batch = _page_table(T, kv_indptr, kv_indices, kv_len, qo_indptr)
+    out = _output(out, (T, hkv, top_pages), torch.int32, q.device)
+    _one_device(q, page_bounds, kv_indptr, kv_indices, kv_len, qo_indptr, out)
+    if T == 0:
+        return out
+    if max_kv_len is None:
+        max_kv_len = max(int(kv_len.max().item()), 1)
+    with _on(q.device):
+        check(lib().yr_hip_select_pages(
+            _at(q), _at(page_bounds), _at(qo_indptr), _at(kv_indptr), _at(kv_indices), kv_indices.numel(),
+            _at(kv_len), _at(out), T, batch, hq, hkv, D, page_size, P, max_kv_len, top_pages, first_pages, last_pages,
+            dt, torch.cuda.current_stream(q.device).cuda_stream), "select_pages")
+    return out
+
+
+def gqa_sparse_paged(q, k_cache, v_cache, kv_indptr, kv_indices, kv_len, pages, qo_indptr=None, out=None):
+    """Paged GQA attention over selected pages: row t of q [T, Hq, D] attends to the tokens at or
+    before its position in pages[t, h // (Hq / Hkv)] (int32 [T, Hkv, n], as select_pages gives them;
+    any order, negative, invisible and repeated entries count for nothing).  A row without a token is 0."""
+    _same_dtype(q, k_cache, v_cache)
+    dt = dtype_code(q.dtype)
+    _dense(q=q, k_cache=k_cache, v_cache=v_cache, pages=pages)
+    if q.dim() != 3 or k_cache.dim() != 4 or v_cache.shape != k_cache.shape or k_cache.shape[3] != q.shape[2]:
+        _fail("q must be [T, Hq, D], the caches [P, page, Hkv, D]")
+    T, hq, D = q.shape
+    P, page, hkv = k_cache.shape[:3]
+    batch = _page_table(T, kv_indptr, kv_indices, kv_len, qo_indptr)
+    if pages.dtype != torch.int32 or pages.dim() != 3 or tuple(pages.shape[:2]) != (T, hkv):
+        _fail(f"pages must be int32 [{T}, {hkv}, n]")
+    out = _output(out, q.shape, q.dtype, q.device)
+    _one_device(q, k_cache, v_cache, kv_indptr, kv_indices, kv_len, pages, qo_indptr, out)
+    if T == 0:
+        return out
+    with _on(q.device):
+        check(lib().yr_hip_gqa_sparse_paged(
+            _at(q), _at(k_cache), _at(v_cache), _at(qo_indptr), _at(kv_indptr), _at(kv_indices), kv_indices.numel(),
+            _at(kv_len), _at(pages), _at(out), T, batch, hq, hkv, D, page, P, pages.shape[2], dt,
+            torch.cuda.current_stream(q.device).cuda_stream), "gqa_sparse_paged")
+    return out
+
+
+class LogProbs(NamedTuple):
+    logprob: torch.Tensor      # [rows] fp32, of the given tokens
+    entropy: torch.Tensor      # [rows] fp32, nats
+    top_logprob: torch.Tensor  # [rows, top_n] fp32, descending
+    top_token: torch.Tensor    # [rows, top_n] int64, lowest first among equals
+
+
+def token_logprobs(logits, tokens, top_n: int = 0, n_valid: int | None = None) -> LogProbs:
+    """Log probabilities of tokens [rows] (int64) under softmax(logits[:, :n_valid]) (f16, bf16 or
+    fp32, rows contiguous), the rows' entropy, and the top_n (<= 64) most likely tokens.  A token outside
+    [0, n_valid) has NaN; NaN logits and rows of -inf alone give NaN numbers."""
+    if logits.dtype not in _DTYPE_ALL:
+        _fail(f"unsupported logits dtype {logits.dtype}")
+    if logits.dim() != 2 or (logits.numel() and logits.stride(1) != 1):
+        _fail("logits must be [rows, n] with contiguous rows")
+    rows, n = logits.shape
+    if tokens.dtype != torch.int64 or tuple(tokens.shape) != (rows,) or not tokens.is_contiguous():
+        _fail(f"tokens must be contiguous int64 [{rows}]")
+    _one_device(logits, tokens)
+    dev = logits.device
+    f32, i64 = {"dtype": torch.float32, "device": dev}, {"dtype": torch.int64, "device": dev}
+    res = LogProbs(torch.empty(rows, **f32), torch.empty(rows, **f32), torch.empty((rows, top_n), **f32),
+                   torch.empty((rows, top_n), **i64))
+    if rows == 0:
+        return res
+    with _on(dev):
+        check(lib().yr_hip_token_logprobs(
+            _at(logits), _at(tokens), _at(res.logprob), _at(res.entropy), _at(res.top_logprob), _at(res.top_token), rows, n,
+            n if n_valid is None else n_valid, logits.stride(0) if rows > 1 else n, top_n, _DTYPE_ALL[logits.dtype],
+            torch.cuda.current_stream(dev).cuda_stream), "token_logprobs")
+    return res
 
 
 def synth_fill(t: torch.Tensor, seed: int, std: float, offset: int = 0) -> torch.Tensor:
