@@ -211,9 +211,10 @@ int yr_hip_gqa_sparse_paged(const void* q, const void* k_cache, const void* v_ca
  * top_n: index -1, -inf) and make the row's numbers NaN, as does a row of -inf alone.
  * Sums in 64 bits over fp32 terms.  Next to yr_hip_argmax; no counterpart in
  * the reference. */
+size_t yr_hip_token_logprobs_workspace(int rows, int n_valid, int top_n, int dtype);
 int yr_hip_token_logprobs(const void* x, const int64_t* tokens, float* logprob, float* entropy, float* top_logprob,
                           int64_t* top_ids, int rows, int n, int n_valid, int64_t row_stride, int top_n, int dtype,
-                          void* stream);
+                          void* workspace, size_t workspace_bytes, void* stream);
 
 /* ------------------------------------------------------- kernel-graph operators */
 /* The operators of the reference's kernel graph (python/yirage/kernel.py:

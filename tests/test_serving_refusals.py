@@ -82,7 +82,7 @@ def test_sparse(change, text):
 
 def _logprobs(**change):
     a = dict(x=FAKE, tok=FAKE, lp=FAKE, h=FAKE, tlp=FAKE, tid=FAKE, rows=3, n=1000, nv=1000, stride=1000, top=5,
-             dt=_lib.DTYPE_F32, stream=None)
+             dt=_lib.DTYPE_F32, ws=FAKE, nb=1 << 30, stream=None)
     return _call("yr_hip_token_logprobs", a, **change)
 
 
@@ -90,11 +90,20 @@ def _logprobs(**change):
     (dict(x=None), "null"), (dict(tok=None), "null"), (dict(tlp=None), "null"), (dict(tid=None), "null"),
     (dict(rows=0), "bad shape"), (dict(n=0), "bad shape"), (dict(nv=0), "bad shape"), (dict(nv=1001), "bad shape"),
     (dict(stride=999), "bad shape"), (dict(top=-1), "top_n"), (dict(top=65), "top_n"), (dict(nv=4), "top_n"),
-    (dict(dt=_lib.DTYPE_I32), "dtype"),
+    (dict(dt=_lib.DTYPE_I32), "dtype"), (dict(x=ctypes.c_void_p(4098)), "aligned"), (dict(n=2 ** 30 + 1, stride=2 ** 31), "too many"),
 ])
 def test_logprobs(change, text):
     rc, msg = _logprobs(**change)
     assert rc == -1 and text in msg, msg
+
+
+def test_logprobs_workspace():
+    need = _lib.lib().yr_hip_token_logprobs_workspace(3, 100000, 5, _lib.DTYPE_F32)
+    assert need > 65536
+    for change in (dict(nb=need - 1), dict(ws=None)):
+        rc, msg = _logprobs(n=100000, nv=100000, stride=100000, **change)
+        assert rc == -3 and "workspace" in msg
+    assert _lib.lib().yr_hip_token_logprobs_workspace(4096, 100000, 5, _lib.DTYPE_F32) == 0
 
 
 # ------------------------------------------------------------------ wrappers

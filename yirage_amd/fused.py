@@ -183,6 +183,7 @@ def argmax(x, n_valid: int | None = None, out=None):
 # qo_indptr[b + 1) of the new tokens (qo_indptr None: one row each), the pages
 # kv_indices[kv_indptr[b] .. kv_indptr[b + 1]) and kv_len[b] tokens, the new ones
 # last.  Their kernels run on the tensors' device and its current stream.
+_TICKET_BYTES = 65536  # what a workspace has zeroed at rest
 _DTYPE_ALL = {**_TORCH_DT, torch.float32: _lib.DTYPE_F32}
 
 
@@ -210,6 +211,18 @@ def _dense(**ts):
     for name, t in ts.items():
         if t is not None and not t.is_contiguous():
             _fail(f"{name} must be contiguous (row-major)")
+
+
+def _scratch(nbytes: int, device):
+    """workspace(), but a captured call owns its scratch: the graph's pool keeps it,
+    tickets are cleared at every replay, and no two graphs meet in it."""
+    if nbytes == 0:
+        return None
+    if not torch.cuda.is_current_stream_capturing():
+        return workspace(nbytes, device)
+    ws = torch.empty(nbytes, dtype=torch.uint8, device=device)
+    ws[:_TICKET_BYTES].zero_()
+    return ws
 
 
 def _at(t):
@@ -386,10 +399,13 @@ def token_logprobs(logits, tokens, top_n: int = 0, n_valid: int | None = None) -
                    torch.empty((rows, top_n), **i64))
     if rows == 0:
         return res
+    dt, n_valid = _DTYPE_ALL[logits.dtype], n if n_valid is None else n_valid
     with _on(dev):
+        nb = lib().yr_hip_token_logprobs_workspace(rows, n_valid, top_n, dt)
+        ws = _scratch(nb, dev)
         check(lib().yr_hip_token_logprobs(
             _at(logits), _at(tokens), _at(res.logprob), _at(res.entropy), _at(res.top_logprob), _at(res.top_token), rows, n,
-            n if n_valid is None else n_valid, logits.stride(0) if rows > 1 else n, top_n, _DTYPE_ALL[logits.dtype],
+            n_valid, logits.stride(0) if rows > 1 else n, top_n, dt, _at(ws), nb,
             torch.cuda.current_stream(dev).cuda_stream), "token_logprobs")
     return res
 
