@@ -11,17 +11,18 @@
 // A row is split over up to 64 workgroups when there are few rows; their
 // records are joined by the one that arrives last.
 //
-// The top costs one comparison a tile: a wave compares the lanes' tile maxima
-// (formed for m anyway) with the worst key that can still be among its top, and
-// looks at single elements only where one beats it.  That bound starts as the
-// top-th largest of 64 lane maxima and moves whenever the wave's buffer of
-// candidates is reduced.  Keys order by value, then by the lower index, so the
-// result does not depend on the order in which candidates are found.
+// The top costs a few instructions a tile: a lane remembers its largest
+// exponent, and the top-th largest of the 64 lanes' is a bound that `top` values
+// reach.  Tiles with a lane at or above it are noted and looked at, those lanes
+// alone, when the pass is over and the bound of all waves is known.  Keys order by
+// value, then by the lower index, so the result does not depend on what else was noted.
 //
 // NaN values take no part in the top (as in argmax) and make the sums NaN; a
 // row of nothing but -inf has no distribution: NaN too.  A token outside
 // [0, n_valid) has log probability NaN.
-#include "yr_common.h"
+#include <type_traits>
+
+#include "attn_device.h"
 
 namespace yr {
 
@@ -43,7 +44,20 @@ constexpr int LP_WAVES = LP_THREADS / kWave;
 constexpr int LP_MAX_TOP = 64;    // a bound comes from 64 lane maxima
 constexpr int LP_BUF = 256;       // candidates a wave holds
 constexpr int LP_MAX_SPLITS = 64; // lists that one wave joins, a lane each
+constexpr int LP_HITS = 128;      // candidate tiles a wave notes (in the candidates' place)
 constexpr int LP_TARGET_WG = 1024;
+constexpr float kFar = 1e38f;     // |m| beyond which m log2 e may leave fp32
+
+// A tile with candidates: the lanes that have them, its first piece, its
+// largest exponent.
+struct LogprobHit {
+  uint64_t lanes;
+  int p0;
+  float high;
+};
+static_assert(LP_HITS * sizeof(LogprobHit) <= LP_BUF * sizeof(uint64_t), "the list shares the buffer");
+
+constexpr int LP_ITEMS = 512;     // (tile, lane) pairs a workgroup looks at
 
 // Order of a value and its index as one number: larger is better.  0: none.
 __device__ __forceinline__ uint64_t lp_key(float v, int i) {
@@ -82,6 +96,26 @@ __device__ __forceinline__ float wave_maxf(float v) {
   r = __builtin_amdgcn_permlane32_swap(__float_as_uint(v), __float_as_uint(v), false, false);
   return fmaxf(__uint_as_float(r[0]), __uint_as_float(r[1]));
 }
+// The larger of three, NaN left out (one instruction).
+__device__ __forceinline__ float max3(float a, float b, float c) {
+  float r;
+  asm("v_max3_f32 %0, %1, %2, %3" : "=v"(r) : "v"(a), "v"(b), "v"(c));
+  return r;
+}
+// (fmaxf(a, b) where a is not a signalling NaN: no instruction to make sure of that)
+__device__ __forceinline__ float max2(float a, float b) {
+  float r;
+  asm("v_max_f32 %0, %1, %2" : "=v"(r) : "v"(a), "v"(b));
+  return r;
+}
+// A value that is the same in all lanes, in a scalar register.
+__device__ __forceinline__ float uniform(float v) {
+  return __int_as_float(__builtin_amdgcn_readfirstlane(__float_as_int(v)));
+}
+__device__ __forceinline__ uint64_t uniform(uint64_t v) {
+  return (uint64_t)(uint32_t)__builtin_amdgcn_readfirstlane((int)(v >> 32)) << 32 |
+         (uint32_t)__builtin_amdgcn_readfirstlane((int)v);
+}
 __device__ __forceinline__ double wave_sum_d(double v) {
 #pragma unroll
   for (int o = 32; o > 0; o >>= 1) v += __shfl_xor(v, o, kWave);
@@ -90,6 +124,21 @@ __device__ __forceinline__ double wave_sum_d(double v) {
 __device__ __forceinline__ uint64_t lane_u64(uint64_t v, int l) {
   return (uint64_t)(uint32_t)__builtin_amdgcn_readlane((int)(v >> 32), l) << 32 |
          (uint32_t)__builtin_amdgcn_readlane((int)v, l);
+}
+
+// The top-th largest of the 64 lanes' values (top <= 64).
+__device__ __forceinline__ float lane_bound(float v, int top) {
+  if (top <= 8) {
+    for (int j = 1; j < top; j++) {
+      const uint64_t at = __ballot(v == wave_maxf(v));
+      if ((int)(threadIdx.x % kWave) == __builtin_ctzll(at | 1ull << 63)) v = -INFINITY;
+    }
+    return wave_maxf(v);
+  }
+  int r = 0;
+#pragma unroll 8
+  for (int l = 0; l < kWave; l++) r += __uint_as_float(__builtin_amdgcn_readlane(__float_as_uint(v), l)) > v;
+  return -wave_maxf(r < top ? -v : -INFINITY);
 }
 
 // How many of the 64 lanes' keys beat this lane's.
@@ -104,7 +153,14 @@ __device__ __forceinline__ int wave_rank(uint64_t k) {
 // buf[0, top) (0 where there are fewer).  Keys differ from one another.
 __device__ __forceinline__ void wave_top(uint64_t* buf, int count, int top) {
   const int lane = threadIdx.x % kWave;
-  if (count <= kWave) {
+  if (count <= kWave && top <= 8) {
+    uint64_t k = lane < count ? buf[lane] : 0;
+    for (int j = 0; j < top; j++) {
+      const uint64_t best = wave_max_key(k);
+      if (lane == 0) buf[j] = best;
+      if (k == best) k = 0;
+    }
+  } else if (count <= kWave) {
     const uint64_t k = lane < count ? buf[lane] : 0;
     const int r = wave_rank(k);
     if (lane < top) buf[lane] = 0;
@@ -125,14 +181,37 @@ __device__ __forceinline__ void wave_top(uint64_t* buf, int count, int top) {
   }
 }
 
-// Joins of (m, s, t): s and t relative to m (m = -inf: nothing yet, s = t = 0).
-__device__ __forceinline__ void lp_rescale(double& s, double& t, float from, float to) {
-  if (from == to) return;
-  if (from == -INFINITY) return;  // s = t = 0 (or NaN, which stays)
-  const double d = (double)from - (double)to, f = __expf((float)d);
+// The values of a 16-byte piece, and the largest of them (NaN left out).
+template <int DT>
+__device__ __forceinline__ void unpack_piece(uint4 w, float* v) {
+  if constexpr (DT == YR_DTYPE_F32) {
+    v[0] = __uint_as_float(w.x); v[1] = __uint_as_float(w.y); v[2] = __uint_as_float(w.z); v[3] = __uint_as_float(w.w);
+  } else {
+    v[0] = lo16<DT>(w.x); v[1] = hi16<DT>(w.x); v[2] = lo16<DT>(w.y); v[3] = hi16<DT>(w.y);
+    v[4] = lo16<DT>(w.z); v[5] = hi16<DT>(w.z); v[6] = lo16<DT>(w.w); v[7] = hi16<DT>(w.w);
+  }
+}
+template <int DT>
+__device__ __forceinline__ float piece_max(uint4 w) {
+  constexpr int EPP = DT == YR_DTYPE_F32 ? 4 : 8;
+  float v[EPP];
+  unpack_piece<DT>(w, v);
+  float m = v[0];
+#pragma unroll
+  for (int e = 1; e < EPP; e++) m = fmaxf(m, v[e]);
+  return m;
+}
+
+// s = sum 2^z and t = sum 2^z z, z relative to the exponent `from`, brought to `to`.
+__device__ __forceinline__ void lp_rescale(double& s, double& t, double from, double to) {
+  if (from == to || s == 0) return;  // (NaN stays)
+  const double d = from - to, f = __builtin_amdgcn_exp2f((float)d);
   t = f == 0 ? 0 * t : f * (t + d * s);
   s *= f;
 }
+
+// The exponent of e^m, exact in 64 bits up to the constant's rounding.
+__device__ __forceinline__ double lp_exponent(float m) { return (double)m * (double)kLog2e; }
 
 __device__ __forceinline__ void st_u64(uint64_t* p, uint64_t v) {
   __hip_atomic_store((YR_G uint64_t*)p, v, __ATOMIC_RELAXED, __HIP_MEMORY_SCOPE_AGENT);
@@ -141,18 +220,22 @@ __device__ __forceinline__ uint64_t ld_u64(const uint64_t* p) {
   return __hip_atomic_load((const YR_G uint64_t*)p, __ATOMIC_RELAXED, __HIP_MEMORY_SCOPE_AGENT);
 }
 
-template <int DT>
+// V: values per lane and tile
+template <int DT, int V>
 __global__ __launch_bounds__(LP_THREADS) void logprobs_kernel(LogprobArgs a) {
   constexpr int EPP = DT == YR_DTYPE_F32 ? 4 : 8;  // elements per 16-byte piece
-  constexpr int U = 32 / EPP;                      // pieces per lane and tile
+  constexpr int U = V / EPP;                       // pieces per lane and tile
   constexpr int ES = 16 / EPP;
+  constexpr int kTile = kWave * U, kStep = LP_WAVES * kTile;  // pieces
   __shared__ uint64_t s_buf[LP_WAVES][LP_BUF];
   extern __shared__ uint64_t s_list[];  // [splits][top]
-  __shared__ float s_m[LP_WAVES];
+  __shared__ int s_item[LP_ITEMS];  // first pieces of lanes with candidates
+  __shared__ int s_items, s_cands;
+  __shared__ float s_m[LP_WAVES], s_bound[LP_WAVES];
   __shared__ double s_s[LP_WAVES], s_t[LP_WAVES];
   const int row = blockIdx.x / a.splits, split = blockIdx.x % a.splits;
   const int tid = threadIdx.x, lane = tid % kWave, wave = __builtin_amdgcn_readfirstlane(tid / kWave);
-  const char* x = (const char*)a.x + (size_t)row * a.stride * ES;
+  const char* const x = (const char*)a.x + (size_t)row * a.stride * ES;
   auto at = [&](int i) __attribute__((always_inline)) -> float {
     if constexpr (DT == YR_DTYPE_F32) return gptr((const float*)x)[i];
     else return ld_elem<DT>(gptr((const uint16_t*)x)[i]);
@@ -169,120 +252,255 @@ __global__ __launch_bounds__(LP_THREADS) void logprobs_kernel(LogprobArgs a) {
   const int lead = (int)((uintptr_t)x & 15) / ES;
   const int np = (a.n + lead + EPP - 1) / EPP;
   const int p_begin = split * a.chunk, p_end = min(np, p_begin + a.chunk);
-  uint64_t* const buf = s_buf[wave];
-  float m = -INFINITY, bound = -INFINITY;  // bound: value of the worst key still wanted
-  uint64_t worst = 0;                      // keys above it are still wanted
-  int count = 0;
+  const int p_first = p_begin + wave * kTile;
+  // Piece p; -inf stands for what is not there: it adds nothing and is told
+  // apart by its index.
+  auto piece = [&](int p) __attribute__((always_inline)) -> uint4 {
+    constexpr uint32_t none = DT == DT_F16 ? 0xfc00fc00u : DT == DT_BF16 ? 0xff80ff80u : 0xff800000u;
+    const int i0 = p * EPP - lead;
+    if (p < p_end && i0 >= 0 && i0 + EPP <= a.n) return ldg16(x - lead * ES + (size_t)p * 16);
+    uint64_t f[2] = {(uint64_t)none << 32 | none, (uint64_t)none << 32 | none};
+    if (p < p_end) {  // the row's first or last piece
+#pragma unroll 1
+      for (int e = max(0, -i0); e < min(EPP, a.n - i0); e++) {
+        const int sh = 8 * ES * (e % (EPP / 2));
+        const uint64_t mask = (((uint64_t)1 << 8 * ES) - 1) << sh;
+        uint64_t bits;
+        if constexpr (DT == YR_DTYPE_F32) bits = gptr((const uint32_t*)x)[i0 + e];
+        else bits = gptr((const uint16_t*)x)[i0 + e];
+        if (e < EPP / 2) f[0] = (f[0] & ~mask) | bits << sh;
+        else f[1] = (f[1] & ~mask) | bits << sh;
+      }
+    }
+    return make_uint4((uint32_t)f[0], (uint32_t)(f[0] >> 32), (uint32_t)f[1], (uint32_t)(f[1] >> 32));
+  };
+  // A lane's pieces of tile p0.
+  auto load = [&](int p0, uint4* w) __attribute__((always_inline)) {
+    if ((p0 > 0 || lead == 0) && (p0 + kTile) * EPP - lead <= a.n && p0 + kTile <= p_end) {
+      const char* const tile = x - lead * ES + (size_t)p0 * 16;  // uniform
+#pragma unroll
+      for (int u = 0; u < U; u++) w[u] = ldg16(tile + (uint32_t)(16 * lane + 16 * kWave * u));
+    } else {
+#pragma unroll
+      for (int u = 0; u < U; u++) w[u] = piece(p0 + u * kWave + lane);
+    }
+  };
+
+  // ---- sums.  Terms are 2^z, z = x log2 e - c with c = m log2 e rounded: one
+  // fma each (m: the largest value so far, -inf: none yet).  s and t are
+  // relative to the exponent c and are brought to m log2 e itself at the end.
+  float m = -INFINITY, c = 0.f, zm = -INFINITY;  // zm: m's own z
   double s = 0, t = 0;
-  for (int p0 = p_begin + wave * (kWave * U); p0 < p_end; p0 += LP_WAVES * kWave * U) {
-    float v[U][EPP];
-    const bool inside = p0 > 0 && (p0 + kWave * U) * EPP - lead <= a.n && p0 + kWave * U <= p_end;  // uniform
-    if (inside || (lead == 0 && (p0 + kWave * U) * EPP <= a.n && p0 + kWave * U <= p_end)) {
-      uint4 w[U];
+  // Candidates for the top: tiles with a lane whose largest exponent z + c is
+  // at least `bound`, the top-th largest of the lanes' maxima.  z + c is off by
+  // rounding, by less than `slack` and 2^-18 of itself.
+  float high = -INFINITY, bound = -INFINITY, slack = 0.f;
+  int hits = 0, fresh = 0;  // entries; how many since the bound moved
+  LogprobHit* const hit = reinterpret_cast<LogprobHit*>(s_buf[wave]);
+  uint4 next[U];
+  if (p_first < p_end) load(p_first, next);
+  for (int p0 = p_first; p0 < p_end; p0 += kStep) {
+    uint4 w[U];
 #pragma unroll
-      for (int u = 0; u < U; u++) w[u] = ldg16(x + ((long long)(p0 + u * kWave + lane) * EPP - lead) * ES);
-#pragma unroll
-      for (int u = 0; u < U; u++) {
-        if constexpr (DT == YR_DTYPE_F32) {
-          v[u][0] = __uint_as_float(w[u].x); v[u][1] = __uint_as_float(w[u].y);
-          v[u][2] = __uint_as_float(w[u].z); v[u][3] = __uint_as_float(w[u].w);
-        } else {
-          v[u][0] = lo16<DT>(w[u].x); v[u][1] = hi16<DT>(w[u].x); v[u][2] = lo16<DT>(w[u].y); v[u][3] = hi16<DT>(w[u].y);
-          v[u][4] = lo16<DT>(w[u].z); v[u][5] = hi16<DT>(w[u].z); v[u][6] = lo16<DT>(w[u].w); v[u][7] = hi16<DT>(w[u].w);
-        }
-      }
-    } else {  // -inf stands for what is not there; it adds nothing and is told apart by its index below
+    for (int u = 0; u < U; u++) w[u] = next[u];
+    if (p0 + kStep < p_end) load(p0 + kStep, next);  // in flight while this tile is worked on
+    float z[U][EPP], mz;
+    auto exponents = [&]() __attribute__((always_inline)) {
 #pragma unroll
       for (int u = 0; u < U; u++) {
-        const int p = p0 + u * kWave + lane;
+        unpack_piece<DT>(w[u], z[u]);
 #pragma unroll
-        for (int e = 0; e < EPP; e++) {
-          const int i = p * EPP - lead + e;
-          v[u][e] = p < p_end && i >= 0 && i < a.n ? at(i) : -INFINITY;
-        }
+        for (int e = 0; e < EPP; e++) z[u][e] = fmaf(z[u][e], kLog2e, -c);
       }
-    }
-    float mx = -INFINITY;
+      // (of canonical values, unlike the unpacked ones: a maximum is one instruction)
+      mz = z[0][0];
 #pragma unroll
-    for (int u = 0; u < U; u++)
-#pragma unroll
-      for (int e = 0; e < EPP; e++) mx = fmaxf(mx, v[u][e]);
-    if (__ballot(mx > m)) {
-      const float to = wave_maxf(fmaxf(mx, m));
-      lp_rescale(s, t, m, to);
-      m = to;
+      for (int j = 1; j + 1 < U * EPP; j += 2) mz = max3(mz, z[j / EPP][j % EPP], z[(j + 1) / EPP][(j + 1) % EPP]);
+      mz = max2(mz, z[U - 1][EPP - 1]);
+    };
+    bool move = m == -INFINITY;
+    if (!move) {
+      exponents();
+      move = __ballot(mz > zm) != 0;
     }
-    const float ref = m == -INFINITY ? 0.f : m;
+    if (move) {  // a new maximum, or the first tile
+      float mx = -INFINITY;
+#pragma unroll
+      for (int u = 0; u < U; u++) mx = fmaxf(mx, piece_max<DT>(w[u]));
+      mx = uniform(wave_maxf(mx));
+      if (mx > m) {
+        const float was = c;
+        m = mx;
+        c = uniform(fminf(fmaxf(m, -2 * kFar), 2 * kFar) * kLog2e);
+        zm = uniform(fmaf(m, kLog2e, -c));
+        lp_rescale(s, t, was, c);
+        slack = fmaxf(slack, 0x1p-18f * fabsf(c));
+      }
+      exponents();
+    }
     float st = 0.f, tt = 0.f;
 #pragma unroll
     for (int u = 0; u < U; u++) {
       float es = 0.f;
 #pragma unroll
       for (int e = 0; e < EPP; e++) {
-        const float y = v[u][e] - ref, ex = __expf(y);
+        const float ex = __builtin_amdgcn_exp2f(z[u][e]);
         es += ex;
-        tt = fmaf(ex, fmaxf(y, -1e4f), tt);  // (0 * -inf is none)
+        tt = fmaf(ex, max2(z[u][e], -1e4f), tt);  // (0 * -inf is none)
       }
       st += es;
     }
     s += st;
     t += tt;
-
-    if (a.top > 0 && __ballot(mx >= bound)) {
-      // the elements' keys; 0: no element, NaN or not above `worst`
-      auto key_of = [&](int u, int e) __attribute__((always_inline)) -> uint64_t {
-        const int p = p0 + u * kWave + lane, i = p * EPP - lead + e;
-        const float f = v[u][e];
-        return p < p_end && i >= 0 && i < a.n && f == f ? lp_key(f, i) : 0;
-      };
-      if (worst == 0 || __popcll(__ballot(mx >= bound)) > 16) {
-        uint64_t k = 0;
-#pragma unroll
-        for (int u = 0; u < U; u++)
-#pragma unroll
-          for (int e = 0; e < EPP; e++) {
-            const uint64_t c = key_of(u, e);
-            k = c > k ? c : k;
+    if (a.top > 0) {
+      const float ex = mz + c;
+      high = max2(high, ex);
+      const uint64_t lanes = __ballot(!(ex < bound - slack));
+      if (lanes) {
+        if (hits == LP_HITS) {  // drop what the bound has passed
+          int kept = 0;
+          for (int i = 0; i < hits; i++) {
+            const LogprobHit h = hit[i];
+            if (!(h.high < bound - slack)) hit[kept++] = h;
           }
-        // `top` keys at least are as good as the top-th best lane's: keep it and what beats it
-        const int r = wave_rank(k);
-        const uint64_t hit = __ballot(k != 0 && r == a.top - 1);
-        if (hit) {
-          const uint64_t b = lane_u64(k, __builtin_ctzll(hit)) - 1;
-          if (b > worst) worst = b;
+          hits = kept < LP_HITS ? kept : LP_HITS + 1;  // too many: every tile is a candidate
+        }
+        if (hits < LP_HITS) {
+          const float th = uniform(wave_maxf(ex));
+          hit[hits++] = LogprobHit{lanes, p0, th};
+        }
+        if (++fresh > 2 || bound == -INFINITY) {
+          fresh = 0;
+          const float b = uniform(lane_bound(high, a.top));
+          const float lower = b - 0x1p-17f * fabsf(b) - slack;  // below what b stands for
+          if (lower > bound && lower < INFINITY) bound = lower;
         }
       }
-#pragma unroll
-      for (int u = 0; u < U; u++)
-#pragma unroll
-        for (int e = 0; e < EPP; e++) {
-          uint64_t k = key_of(u, e);
-          uint64_t take = __ballot(k > worst);
-          if (take) {
-            if (count + __popcll(take) > LP_BUF) {
-              wave_top(buf, count, a.top);
-              count = a.top;  // (the buffer was fuller than top)
-              const uint64_t b = buf[a.top - 1];
-              if (b > worst) worst = b;
-              take = __ballot(k > worst);
-            }
-            if (k > worst) buf[count + __popcll(take & ((1ull << lane) - 1))] = k;
-            count += __popcll(take);
-          }
-        }
-      bound = worst ? lp_value(worst) : -INFINITY;  // (one below a key: the same value, the next index)
     }
   }
-  if (a.top > 0) wave_top(buf, count, a.top);
+  if (fabsf(m) > kFar && m > -INFINITY) {
+    // m log2 e may have left fp32 (the type's lowest value as a mask, infinity):
+    // c was clamped and only m is right.  Once more, from x - m.
+    s = t = 0;
+    for (int p0 = p_first; p0 < p_end; p0 += kStep)
+#pragma unroll 1
+      for (int i = (p0 + lane) * EPP - lead; i < min((min(p0 + kTile, p_end)) * EPP - lead, a.n); i += 1) {
+        // lane's pieces p0 + lane, + 64, ...: their EPP elements, then the next piece
+        const int e = (i + lead) % EPP;
+        if (i >= 0) {
+          const float z = (at(i) - m) * kLog2e, ex = __builtin_amdgcn_exp2f(z);
+          s += ex;
+          t += ex * max2(z, -1e4f);
+        }
+        if (e == EPP - 1) i += (kWave - 1) * EPP;
+      }
+  } else if (m > -INFINITY) {
+    lp_rescale(s, t, c, lp_exponent(m));
+  }
   s = wave_sum_d(s);
   t = wave_sum_d(t);
   if (lane == 0) {
     s_m[wave] = m;
     s_s[wave] = s;
     s_t[wave] = t;
+    s_bound[wave] = bound;
+  }
+  if (tid == 0) s_items = s_cands = 0;
+  for (int i = tid; i < a.top; i += LP_THREADS) s_list[i] = 0;
+  __syncthreads();
+
+  // ---- the top.  What the lanes with candidates hold, at or above the bound of
+  // all waves, goes to one list of keys, and a key's place is the number that beat it.
+  if (a.top > 0) {
+#pragma unroll
+    for (int w = 0; w < LP_WAVES; w++) bound = fmaxf(bound, s_bound[w]);
+    bound = uniform(bound);
+    // the same bound for a value: x log2 e >= bound
+    const float b = bound * 0.693147180559945309f;
+    const float xb = bound > -INFINITY ? b - 0x1p-18f * fabsf(b) : -INFINITY;
+    const float least = bound - slack;
+    const uint64_t live = __ballot(!(high < least));
+    for (int j = 0; j < min(hits, LP_HITS); j++) {
+      const LogprobHit h = hit[j];
+      const uint64_t lanes = uniform(h.lanes) & live;
+      if (h.high < least || !lanes) continue;
+      int base = 0;
+      if (lane == 0) base = atomicAdd(&s_items, __popcll(lanes));
+      base = __builtin_amdgcn_readfirstlane(base) + __popcll(lanes & ((1ull << lane) - 1));
+      if (((lanes >> lane) & 1) && base < LP_ITEMS) s_item[base] = h.p0 + lane;
+    }
+    if (hits > LP_HITS && lane == 0) atomicAdd(&s_items, LP_ITEMS + 1);
+    __syncthreads();
+    const int items = s_items;
+    uint64_t* const cand = s_buf[0];
+    constexpr int kCands = LP_WAVES * LP_BUF;
+    if (items <= LP_ITEMS) {
+      for (int i = tid; i < items * U; i += LP_THREADS) {
+        const int p = s_item[i / U] + i % U * kWave;
+        float v[EPP];
+        unpack_piece<DT>(piece(p), v);
+#pragma unroll
+        for (int e = 0; e < EPP; e++) {
+          const int at = p * EPP - lead + e;
+          if (v[e] >= xb && p < p_end && at >= 0 && at < a.n) {
+            const int c = atomicAdd(&s_cands, 1);
+            if (c < kCands) cand[c] = lp_key(v[e], at);
+          }
+        }
+      }
+      __syncthreads();
+    }
+    const int cands = s_cands;
+    if (items <= LP_ITEMS && cands <= kCands) {
+      for (int i = tid; i < cands; i += LP_THREADS) {
+        const uint64_t k = cand[i];
+        int r = 0;
+        for (int j = 0; j < cands; j++) r += cand[j] > k;
+        if (r < a.top) s_list[r] = k;
+      }
+    } else {
+      // Too many: equal values in their thousands, as in a row that a mask has
+      // left nearly empty.  Each wave goes over its pieces once more, keeping
+      // its best keys; those above `worst` are still wanted.
+      uint64_t* const buf = s_buf[wave];
+      uint64_t worst = 0;
+      int count = 0;
+      __syncthreads();
+      for (int p0 = p_first; p0 < p_end; p0 += kStep)
+#pragma unroll 1
+        for (int u = 0; u < U; u++) {
+          const int i0 = (p0 + u * kWave + lane) * EPP - lead;
+          float v[EPP];
+          unpack_piece<DT>(piece(p0 + u * kWave + lane), v);
+#pragma unroll 1
+          for (int e = 0; e < EPP; e++) {
+            const float f = v[0];
+#pragma unroll
+            for (int i = 0; i + 1 < EPP; i++) v[i] = v[i + 1];
+            const int at = i0 + e;
+            const uint64_t k = f >= xb && p0 + u * kWave + lane < p_end && at >= 0 && at < a.n ? lp_key(f, at) : 0;
+            if (count + kWave > LP_BUF) {
+              wave_top(buf, count, a.top);
+              count = a.top;  // (the buffer was fuller than top)
+              worst = uniform(buf[a.top - 1]);
+            }
+            const uint64_t take = __ballot(k > worst);
+            if (k > worst) buf[count + __popcll(take & ((1ull << lane) - 1))] = k;
+            count += __popcll(take);
+          }
+        }
+      wave_top(buf, count, a.top);
+      __syncthreads();
+      for (int i = tid; i < LP_WAVES * a.top; i += LP_THREADS) {
+        const uint64_t k = s_buf[i / a.top][i % a.top];
+        int r = 0;
+        for (int j = 0; j < LP_WAVES * a.top; j++) r += s_buf[j / a.top][j % a.top] > k;
+        if (k && r < a.top) s_list[r] = k;
+      }
+    }
   }
   __syncthreads();
-  // ---- the waves' numbers and lists
+  // ---- the waves' numbers
   float M = -INFINITY;
 #pragma unroll
   for (int w = 0; w < LP_WAVES; w++) M = fmaxf(M, s_m[w]);
@@ -290,20 +508,9 @@ __global__ __launch_bounds__(LP_THREADS) void logprobs_kernel(LogprobArgs a) {
 #pragma unroll
   for (int w = 0; w < LP_WAVES; w++) {
     double sw = s_s[w], tw = s_t[w];
-    lp_rescale(sw, tw, s_m[w], M);
+    lp_rescale(sw, tw, lp_exponent(s_m[w]), lp_exponent(M));
     s += sw;
     t += tw;
-  }
-  // position of a key in the joined list: how many of every wave's keys beat it
-  for (int i = tid; i < a.top; i += LP_THREADS) s_list[i] = 0;
-  __syncthreads();
-  for (int i = tid; i < LP_WAVES * a.top; i += LP_THREADS) {
-    const uint64_t k = s_buf[i / a.top][i % a.top];
-    int r = 0;
-    for (int q = 0; q < a.top; q++)
-#pragma unroll
-      for (int w = 0; w < LP_WAVES; w++) r += s_buf[w][q] > k;
-    if (k && r < a.top) s_list[r] = k;
   }
   __syncthreads();
 
@@ -311,7 +518,7 @@ __global__ __launch_bounds__(LP_THREADS) void logprobs_kernel(LogprobArgs a) {
     const int rec_len = 3 + a.top;
     uint64_t* rec = a.records + (size_t)row * a.splits * rec_len;
     if (tid == 0) {
-      st_u64(rec + (size_t)split * rec_len, (uint64_t)__double_as_longlong((double)M));
+      st_u64(rec + (size_t)split * rec_len, (uint64_t)__double_as_longlong(lp_exponent(M)));
       st_u64(rec + (size_t)split * rec_len + 1, (uint64_t)__double_as_longlong(s));
       st_u64(rec + (size_t)split * rec_len + 2, (uint64_t)__double_as_longlong(t));
     }
@@ -327,8 +534,9 @@ __global__ __launch_bounds__(LP_THREADS) void logprobs_kernel(LogprobArgs a) {
       ss = __longlong_as_double((long long)ld_u64(rec + (size_t)lane * rec_len + 1));
       ts = __longlong_as_double((long long)ld_u64(rec + (size_t)lane * rec_len + 2));
     }
-    M = wave_maxf((float)ms);
-    lp_rescale(ss, ts, (float)ms, M);
+    // (a float times the constant: the division gives the float back)
+    M = wave_maxf((float)(ms / (double)kLog2e));
+    lp_rescale(ss, ts, ms, lp_exponent(M));
     s = wave_sum_d(ss);
     t = wave_sum_d(ts);
     // the splits' ordered lists: take the best head, `top` times
@@ -345,10 +553,11 @@ __global__ __launch_bounds__(LP_THREADS) void logprobs_kernel(LogprobArgs a) {
     if (lane < a.top) s_list[lane] = mine;  // (every head was read: the wave runs in step)
   }
   if (M == -INFINITY) s = t = NAN;  // no value at all
+  if (s < 1) s = 1;                 // the largest term alone, but for its rounding
   const double ls = log(s);
   if (tid == 0) {
     gptr(a.logprob)[row] = (float)((double)(given - M) - ls);
-    gptr(a.entropy)[row] = (float)(ls - t / s);
+    gptr(a.entropy)[row] = (float)(ls - t / s * 0.693147180559945309);
   }
   if (tid < a.top) {
     const uint64_t k = s_list[tid];
@@ -358,16 +567,23 @@ __global__ __launch_bounds__(LP_THREADS) void logprobs_kernel(LogprobArgs a) {
 }
 
 // A row is split until about LP_TARGET_WG workgroups run, each with one tile of
-// all its waves at least.
-static void logprobs_plan(int rows, int n, int dtype, int* splits, int* chunk) {
-  const int epp = dtype == YR_DTYPE_F32 ? 4 : 8, tile = LP_THREADS * 32 / epp;  // pieces
-  const int np = (n - 1) / epp + 2;  // a row off its boundary has one more
+// all its waves at least.  Where that leaves CUs idle the tiles are small (8
+// values a lane instead of 32).
+struct LogprobPlan {
+  int values, splits, chunk;
+};
+static LogprobPlan logprobs_plan(int rows, int n, int dtype) {
+  const int epp = dtype == YR_DTYPE_F32 ? 4 : 8;
+  const int np = (n - 1) / epp + 2;  // pieces; a row off its boundary has one more
+  LogprobPlan p;
+  p.values = (long long)rows * np < 256ll * LP_THREADS * 32 / epp ? 8 : 32;
+  const int tile = LP_THREADS * p.values / epp, most = (np + tile - 1) / tile;
   int sp = (LP_TARGET_WG + rows - 1) / rows;
   if (sp > LP_MAX_SPLITS) sp = LP_MAX_SPLITS;
-  const int most = (np + tile - 1) / tile;
   if (sp > most) sp = most;
-  *chunk = ((np + sp - 1) / sp + tile - 1) / tile * tile;
-  *splits = (np + *chunk - 1) / *chunk;
+  p.chunk = ((np + sp - 1) / sp + tile - 1) / tile * tile;
+  p.splits = (np + p.chunk - 1) / p.chunk;
+  return p;
 }
 
 }  // namespace yr
@@ -376,9 +592,8 @@ using namespace yr;
 
 extern "C" size_t yr_hip_token_logprobs_workspace(int rows, int n_valid, int top_n, int dtype) {
   if (rows <= 0 || n_valid <= 0 || top_n < 0) return 0;
-  int splits, chunk;
-  logprobs_plan(rows, n_valid, dtype, &splits, &chunk);
-  return splits > 1 ? kTicketBytes + (size_t)rows * splits * (3 + top_n) * sizeof(uint64_t) : 0;
+  const LogprobPlan p = logprobs_plan(rows, n_valid, dtype);
+  return p.splits > 1 ? kTicketBytes + (size_t)rows * p.splits * (3 + top_n) * sizeof(uint64_t) : 0;
 }
 
 extern "C" int yr_hip_token_logprobs(const void* x, const int64_t* tokens, float* logprob, float* entropy,
@@ -396,8 +611,9 @@ extern "C" int yr_hip_token_logprobs(const void* x, const int64_t* tokens, float
     return fail(YR_E_INVALID, "%s: dtype", nm);
   const int size = dtype == YR_DTYPE_F32 ? 4 : 2;
   if ((uintptr_t)x % size) return fail(YR_E_INVALID, "%s: logits must be aligned to their type", nm);
-  LogprobArgs a{x, tokens, logprob, entropy, top_logprob, top_ids, nullptr, nullptr, row_stride, n_valid, top_n, 1, 0};
-  logprobs_plan(rows, n_valid, dtype, &a.splits, &a.chunk);
+  const LogprobPlan p = logprobs_plan(rows, n_valid, dtype);
+  LogprobArgs a{x,       tokens,     logprob, entropy, top_logprob, top_ids, nullptr,
+                nullptr, row_stride, n_valid, top_n,   p.splits,    p.chunk};
   const size_t need = yr_hip_token_logprobs_workspace(rows, n_valid, top_n, dtype);
   if (need > workspace_bytes || (need && !workspace))
     return fail(YR_E_WORKSPACE, "%s: workspace %zu < %zu", nm, workspace_bytes, need);
@@ -407,12 +623,12 @@ extern "C" int yr_hip_token_logprobs(const void* x, const int64_t* tokens, float
   hipStream_t st = (hipStream_t)stream;
   const dim3 grid((unsigned)(rows * a.splits));
   const size_t lds = (size_t)a.splits * top_n * sizeof(uint64_t);
-  if (dtype == YR_DTYPE_F16)
-    hipLaunchKernelGGL((logprobs_kernel<YR_DTYPE_F16>), grid, dim3(LP_THREADS), lds, st, a);
-  else if (dtype == YR_DTYPE_BF16)
-    hipLaunchKernelGGL((logprobs_kernel<YR_DTYPE_BF16>), grid, dim3(LP_THREADS), lds, st, a);
-  else
-    hipLaunchKernelGGL((logprobs_kernel<YR_DTYPE_F32>), grid, dim3(LP_THREADS), lds, st, a);
+#define YR_LP(DT_, V_)                     \
+  if (dtype == DT_ && p.values == V_)      \
+    hipLaunchKernelGGL((logprobs_kernel<DT_, V_>), grid, dim3(LP_THREADS), lds, st, a);
+  YR_LP(YR_DTYPE_F16, 8) YR_LP(YR_DTYPE_F16, 32) YR_LP(YR_DTYPE_BF16, 8) YR_LP(YR_DTYPE_BF16, 32)
+  YR_LP(YR_DTYPE_F32, 8) YR_LP(YR_DTYPE_F32, 32)
+#undef YR_LP
   YR_CHECK_LAUNCH(nm);
   return YR_OK;
 }
