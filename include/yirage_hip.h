@@ -188,10 +188,12 @@ int yr_hip_append_kv_paged(const void* q, const void* k, const void* v, void* q_
  * lower page, a NaN sum or a missing page ranks last.
  * max_kv_len bounds kv_len (pages behind it are not seen); at most 16384 pages
  * of it.  No counterpart in the reference. */
+size_t yr_hip_select_pages_workspace(int rows, int hkv, int page_size, int max_kv_len);
 int yr_hip_select_pages(const void* q, const void* page_bounds, const int32_t* qo_indptr, const int32_t* kv_indptr,
                         const int32_t* kv_indices, int n_indices, const int32_t* kv_len, int32_t* pages, int rows,
                         int batch, int hq, int hkv, int d, int page_size, int num_pages, int max_kv_len,
-                        int top_pages, int first_pages, int last_pages, int dtype, void* stream);
+                        int top_pages, int first_pages, int last_pages, int dtype, void* workspace,
+                        size_t workspace_bytes, void* stream);
 
 /* out[t][h] = softmax(q[t][h] k^T / sqrt(d)) v over the tokens at or before row
  * t's position in the pages pages[t][h / (hq / hkv)][0 .. top_pages); hq / hkv

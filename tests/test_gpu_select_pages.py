@@ -36,7 +36,8 @@ def _reference(b, q, bounds, hkv, top, first, last, max_pages=1 << 30, ids_of=No
     ([900], [20], 14, 2, 128, 128, 20, 1, 1),       # fewer pages than asked for
     ([5000] * 3, [1] * 3, 2, 2, 64, 48, 3, 1, 2),   # nothing left to choose
     ([2500], [130], 8, 2, 128, 16, 33, 1, 1),
-    ([20000], [1], 4, 1, 64, 16, 400, 1, 1), ([5000, 4000], [33, 2], 8, 4, 128, 16, 16, 1, 1),
+    ([20000], [1], 4, 1, 64, 16, 400, 1, 1), ([16384], [1], 1, 1, 64, 1, 900, 1, 1), ([16384], [2], 2, 2, 64, 1, 16384, 1, 1),
+    ([16000, 9000], [1, 20], 2, 1, 64, 1, 8, 2, 2), ([5000, 4000], [33, 2], 8, 4, 128, 16, 16, 1, 1),
 ])
 def test_lists(lens, news, hq, hkv, d, page, top, first, last, dt):
     print("case", lens, news, hq, hkv, d, page, top, first, last, dt, flush=True)
@@ -51,7 +52,8 @@ def test_lists(lens, news, hq, hkv, d, page, top, first, last, dt):
     assert torch.equal(got.cpu(), ref)
     # the bound on the lengths may be larger than they are, or come from them
     again = F.select_pages(q.cuda(), bounds.cuda(), *b.args(), page_size=page, top_pages=top, qo_indptr=b.qo(),
-                           first_pages=first, last_pages=last, max_kv_len=max(lens) + 5 * page)
+                           first_pages=first, last_pages=last,
+                           max_kv_len=min(max(lens) + 5 * page, 16384 * page))
     assert torch.equal(again, got)
     none = F.select_pages(q.cuda(), bounds.cuda(), *b.args(), page_size=page, top_pages=top, qo_indptr=b.qo(),
                           first_pages=first, last_pages=last)

@@ -45,7 +45,7 @@ def test_append(change, text):
 
 def _select(**change):
     a = dict(q=FAKE, bounds=FAKE, qo=FAKE, ptr=FAKE, idx=FAKE, nidx=4, lens=FAKE, pages=FAKE, rows=5, batch=2, hq=32,
-             hkv=8, d=128, page=64, npages=4, maxlen=4096, top=8, first=1, last=1, dt=_lib.DTYPE_F16, stream=None)
+             hkv=8, d=128, page=64, npages=4, maxlen=4096, top=8, first=1, last=1, dt=_lib.DTYPE_F16, ws=FAKE, nb=1 << 30, stream=None)
     return _call("yr_hip_select_pages", a, **change)
 
 
@@ -60,6 +60,15 @@ def _select(**change):
 def test_select(change, text):
     rc, msg = _select(**change)
     assert rc == -1 and text in msg, msg
+
+
+def test_select_workspace():
+    need = _lib.lib().yr_hip_select_pages_workspace(5, 8, 64, 40000)
+    assert need == 65536 + 5 * 8 * 625 * 8
+    for change in (dict(nb=need - 1), dict(ws=None)):
+        rc, msg = _select(maxlen=40000, **change)
+        assert rc == -3 and "workspace" in msg
+    assert _lib.lib().yr_hip_select_pages_workspace(2048, 8, 64, 40000) == 0
 
 
 def _sparse(**change):

@@ -22,12 +22,16 @@ struct SelectArgs {
   const uint16_t* q;
   const uint16_t* bounds;  // [pages][hkv][2][D]
   int32_t* out;            // [rows][hkv][top]
-  int hq, hkv, max_pages, top, first, last;
+  uint64_t* keys;          // [rows][hkv][max_pages] where a row is split
+  uint32_t* tickets;       // [rows][hkv]
+  int hq, hkv, max_pages, top, first, last, splits, chunk;
 };
 
 constexpr int SEL_THREADS = 256;
 constexpr int SEL_WAVES = SEL_THREADS / kWave;
 constexpr int SEL_MAX_PAGES = 16384;  // 64-bit keys of one row in LDS: 128 of 160 KiB
+constexpr int SEL_TARGET_WG = 1024;
+constexpr int SEL_MIN_CHUNK = 64;     // pages per split at least
 
 // Whole-number order of a score: larger is better, -0 equals 0, NaN is last.
 __device__ __forceinline__ uint64_t score_key(double s) {
@@ -36,106 +40,178 @@ __device__ __forceinline__ uint64_t score_key(double s) {
   return b < 0 ? ~(uint64_t)b : (uint64_t)b | 0x8000000000000000ull;
 }
 
-// Writes the ascending list of a row: pages [0, f) and [n - l, n) and the `m`
-// best keys of [f, n - l), -1 behind.  Called by the whole workgroup.
-__device__ void choose(const uint64_t* key, int n, int f, int l, int m, int top, int32_t* out) {
-  __shared__ int s_hist[256];
-  __shared__ uint64_t s_lo;
-  __shared__ int s_need, s_done, s_cnt[SEL_WAVES][2];
-  const int tid = threadIdx.x, lane = tid % kWave, wave = tid / kWave;
-  const int c0 = f, c1 = n - l;  // candidates
-  // Radix selection, 8 bits at a time: `lo` is the m-th best key's known prefix,
-  // `need` how many of the keys with that prefix are still to be taken.
-  uint64_t lo = 0;
-  int need = m;
-  bool exact = false;  // `need` of the keys equal to lo, not all keys from lo on
-  if (m > 0 && m < c1 - c0) {
-    for (int shift = 56; shift >= 0; shift -= 8) {
-      for (int i = tid; i < 256; i += SEL_THREADS) s_hist[i] = 0;
-      __syncthreads();
-      for (int u = c0 + tid; u < c1; u += SEL_THREADS) {
-        const uint64_t k = key[u];
-        if (shift == 56 || (k >> (shift + 8)) == (lo >> (shift + 8))) atomicAdd(&s_hist[(int)(k >> shift) & 255], 1);
-      }
-      __syncthreads();
-      if (tid == 0) {
-        int left = need, bin = 255;
-        for (; bin > 0 && s_hist[bin] < left; bin--) left -= s_hist[bin];
-        s_lo = lo | ((uint64_t)bin << shift);
-        s_need = left;
-        s_done = s_hist[bin] == left;  // the whole bin is taken
-      }
-      __syncthreads();
-      lo = s_lo;
-      need = s_need;
-      const bool done = s_done;
-      __syncthreads();
-      if (done) break;
-      exact = shift == 0;
-    }
-  }
-  // ascending list
-  int at = 0, eq = 0;  // written so far, keys equal to lo seen so far
-  for (int u0 = 0; u0 < n; u0 += SEL_THREADS) {
-    const int u = u0 + tid;
-    const bool cand = u >= c0 && u < c1;
-    const uint64_t k = cand ? key[u] : 0;
-    const bool same = exact && cand && k == lo;
-    const uint64_t be = __ballot(same);
-    if (lane == 0) s_cnt[wave][0] = __popcll(be);
-    __syncthreads();
-    int before = eq, alle = 0;
-    for (int w = 0; w < SEL_WAVES; w++) {
-      if (w < wave) before += s_cnt[w][0];
-      alle += s_cnt[w][0];
-    }
-    before += __popcll(be & ((1ull << lane) - 1));
-    const bool take = u < n && (!cand || (m > 0 && (same ? before < need : k >= lo)));
-    const uint64_t bt = __ballot(take);
-    if (lane == 0) s_cnt[wave][1] = __popcll(bt);
-    __syncthreads();
-    int pos = at, all = 0;
-    for (int w = 0; w < SEL_WAVES; w++) {
-      if (w < wave) pos += s_cnt[w][1];
-      all += s_cnt[w][1];
-    }
-    pos += __popcll(bt & ((1ull << lane) - 1));
-    if (take && pos < top) gptr(out)[pos] = u;
-    at += all;
-    eq += alle;
-    __syncthreads();
-  }
-  for (int i = at + tid; i < top; i += SEL_THREADS) gptr(out)[i] = -1;
+template <int C>
+__device__ __forceinline__ uint32_t dpp_word(uint32_t v) {
+  return (uint32_t)__builtin_amdgcn_mov_dpp((int)v, C, 0xF, 0xF, false);
+}
+__device__ __forceinline__ uint32_t wave_or(uint32_t v) {
+  v |= dpp_word<0xB1>(v);
+  v |= dpp_word<0x4E>(v);
+  v |= dpp_word<0x141>(v);
+  v |= dpp_word<0x140>(v);
+  auto r = __builtin_amdgcn_permlane16_swap(v, v, false, false);
+  v = r[0] | r[1];
+  r = __builtin_amdgcn_permlane32_swap(v, v, false, false);
+  return r[0] | r[1];
+}
+template <int C>
+__device__ __forceinline__ double dpp_add(double v) {
+  const uint64_t b = (uint64_t)__double_as_longlong(v);
+  const uint64_t o = (uint64_t)dpp_word<C>((uint32_t)(b >> 32)) << 32 | dpp_word<C>((uint32_t)b);
+  return v + __longlong_as_double((long long)o);
+}
+// Sum over groups of 16 (8) lanes, every lane the same.
+template <int N>
+__device__ __forceinline__ double group_sum(double v) {
+  v = dpp_add<0x4E>(dpp_add<0xB1>(v));
+  v = dpp_add<0x141>(v);
+  return N == 16 ? dpp_add<0x140>(v) : v;
 }
 
+// Writes the ascending list of a row: pages [0, f) and [n - l, n) and the `m`
+// best keys of [f, n - l), -1 behind.  W waves work together (the whole
+// workgroup, or one wave by itself), the keys are in LDS.
+//
+// The m-th best key is found bit by bit: of the bits in which the keys differ,
+// from the highest, a bit is set when m keys at least reach the value with it.
+// That ends as soon as exactly m do, after about log2 n bits.
+template <int W>
+__device__ void choose(const uint64_t* key, int n, int f, int l, int m, int top, int32_t* out) {
+  __shared__ int s_cnt[2][SEL_WAVES];
+  __shared__ uint64_t s_diff[SEL_WAVES];
+  const int lane = threadIdx.x % kWave, wave = W == 1 ? 0 : threadIdx.x / kWave;
+  const int c0 = f, c1 = n - l;  // candidates
+  int turn = 0;
+  // sum of a count over the waves
+  auto all = [&](int c) __attribute__((always_inline)) -> int {
+    if constexpr (W == 1) return c;
+    if (lane == 0) s_cnt[turn][wave] = c;
+    __syncthreads();
+    int sum = 0;
+#pragma unroll
+    for (int w = 0; w < W; w++) sum += s_cnt[turn][w];
+    turn ^= 1;  // the next count goes elsewhere: one barrier each
+    return sum;
+  };
+  uint64_t bound = 0;  // keys from it on are taken ..
+  int equal = 0x7fffffff;  // .. of those equal to it only the first `equal`
+  if (m > 0 && m < c1 - c0) {
+    const uint64_t any = key[c0];
+    uint64_t diff = 0;
+    for (int u = c0 + wave * kWave + lane; u < c1; u += W * kWave) diff |= key[u] ^ any;
+    diff = (uint64_t)wave_or((uint32_t)(diff >> 32)) << 32 | wave_or((uint32_t)diff);
+    if constexpr (W > 1) {
+      if (lane == 0) s_diff[wave] = diff;
+      __syncthreads();
+#pragma unroll
+      for (int w = 0; w < W; w++) diff |= s_diff[w];
+    }
+    int bit = diff ? 63 - __builtin_clzll(diff) : -1;
+    bound = bit == 63 ? 0 : any & ~((2ull << (bit < 0 ? 0 : bit)) - 1);
+    if (bit < 0) bound = any;  // all the same
+    bool exact = false;
+    for (; bit >= 0 && !exact; bit--) {
+      const uint64_t cand = bound | 1ull << bit;
+      int c = 0;
+      for (int u0 = c0 + wave * kWave; u0 < c1; u0 += W * kWave) {
+        const int u = u0 + lane;
+        c += __popcll(__ballot(u < c1 && key[u] >= cand));
+      }
+      c = all(c);
+      if (c >= m) bound = cand;
+      exact = c == m;
+    }
+    if (!exact) {  // equal keys at the border: the first of them
+      int c = 0;
+      for (int u0 = c0 + wave * kWave; u0 < c1; u0 += W * kWave) {
+        const int u = u0 + lane;
+        c += __popcll(__ballot(u < c1 && key[u] > bound));
+      }
+      equal = m - all(c);
+    }
+  }
+  // ascending list; the waves take contiguous blocks of 64 pages in turn
+  int at = 0, eq = 0;  // written so far, keys equal to bound seen so far
+  for (int u0 = 0; u0 < n; u0 += W * kWave) {
+    const int u = u0 + wave * kWave + lane;
+    const bool cand = u >= c0 && u < c1;
+    const uint64_t k = cand ? key[u] : 0;
+    const bool same = cand && k == bound;
+    const uint64_t be = __ballot(same);
+    int before = eq, alle = __popcll(be);
+    if constexpr (W > 1) {
+      alle = all(alle);
+#pragma unroll
+      for (int w = 0; w < W; w++)
+        if (w < wave) before += s_cnt[turn ^ 1][w];
+    }
+    eq += alle;
+    before += __popcll(be & ((1ull << lane) - 1));
+    const bool take = u < n && (!cand || (m > 0 && (same ? before < equal : k > bound)));
+    const uint64_t bt = __ballot(take);
+    int pos = at, allt = __popcll(bt);
+    if constexpr (W > 1) {
+      allt = all(allt);
+#pragma unroll
+      for (int w = 0; w < W; w++)
+        if (w < wave) pos += s_cnt[turn ^ 1][w];
+    }
+    at += allt;
+    pos += __popcll(bt & ((1ull << lane) - 1));
+    if (take && pos < top) gptr(out)[pos] = u;
+  }
+  for (int i = at + wave * kWave + lane; i < top; i += W * kWave) gptr(out)[i] = -1;
+}
+
+// Pages of a row: visible and existing ones n, forced ones at the start (f) and
+// the end (l), and how many of the others are chosen (m).
+struct RowPages {
+  int n, f, l, m;
+};
+__device__ __forceinline__ RowPages row_pages(const SelectArgs& a, const SeqRows& s, int p) {
+  RowPages r;
+  r.n = p < 0 ? 0 : min(min(p / a.r.page + 1, s.npg), a.max_pages);
+  r.f = min(a.first, r.n);
+  r.l = min(a.last, r.n - r.f);
+  r.m = min(max(a.top - r.f - r.l, 0), r.n - r.f - r.l);
+  return r;
+}
+
+__device__ __forceinline__ void sel_store(uint64_t* p, uint64_t v) {
+  __hip_atomic_store((YR_G uint64_t*)p, v, __ATOMIC_RELAXED, __HIP_MEMORY_SCOPE_AGENT);
+}
+__device__ __forceinline__ uint64_t sel_load(const uint64_t* p) {
+  return __hip_atomic_load((const YR_G uint64_t*)p, __ATOMIC_RELAXED, __HIP_MEMORY_SCOPE_AGENT);
+}
+
+// One row and kv head, its pages split over `splits` workgroups; the last one
+// to arrive chooses.
 template <int DT, int D>
 __global__ __launch_bounds__(SEL_THREADS) void select_kernel(SelectArgs a) {
-  constexpr int LPP = D / 8, PPB = SEL_THREADS / LPP;  // lanes per page, pages per pass
+  constexpr int LPP = D / 8, PPB = SEL_THREADS / LPP, U = 4;  // lanes per page, pages per pass, passes in flight
   extern __shared__ uint64_t s_key[];
   __shared__ double s_q[2][D];
-  const int h = blockIdx.x % a.hkv, t = blockIdx.x / a.hkv, tid = threadIdx.x;
+  const int split = blockIdx.x % a.splits, pair = blockIdx.x / a.splits;
+  const int h = pair % a.hkv, t = pair / a.hkv, tid = threadIdx.x;
   const int b = seq_of_row(a.r, t);
   if (b < 0) return;
   const SeqRows s = seq_rows(a.r, b);
-  int32_t* out = a.out + ((size_t)t * a.hkv + h) * a.top;
-  const int p = s.len - s.n + (t - s.row0);
-  // visible pages that exist
-  const int n = p < 0 ? 0 : min(min(p / a.r.page + 1, s.npg), a.max_pages);
-  const int g = a.hq / a.hkv;
-  for (int d = tid; d < D; d += SEL_THREADS) {
-    double up = 0, down = 0;
-    for (int i = 0; i < g; i++) {
-      const double x = ld_elem<DT>(gptr(a.q)[((size_t)t * a.hq + (size_t)h * g + i) * D + d]);
-      up += x > 0 ? x : 0;
-      down += x < 0 ? x : 0;
+  int32_t* out = a.out + (size_t)pair * a.top;
+  const RowPages r = row_pages(a, s, s.len - s.n + (t - s.row0));
+  const bool scored = r.m > 0 && r.m < r.n - r.f - r.l;
+  if (scored) {
+    const int g = a.hq / a.hkv;
+    for (int d = tid; d < D; d += SEL_THREADS) {
+      double up = 0, down = 0;
+      for (int i = 0; i < g; i++) {
+        const double x = ld_elem<DT>(gptr(a.q)[((size_t)t * a.hq + (size_t)h * g + i) * D + d]);
+        up += x > 0 ? x : x != x ? x : 0;
+        down += x < 0 ? x : 0;
+      }
+      s_q[0][d] = down;
+      s_q[1][d] = up;
     }
-    s_q[0][d] = down;
-    s_q[1][d] = up;
-  }
-  __syncthreads();
-  const int f = min(a.first, n), l = min(a.last, n - f);
-  const int m = min(max(a.top - f - l, 0), n - f - l);
-  if (m > 0 && m < n - f - l) {
+    __syncthreads();
     const int j = tid % LPP;
     double qd[8], qu[8];
 #pragma unroll
@@ -143,40 +219,81 @@ __global__ __launch_bounds__(SEL_THREADS) void select_kernel(SelectArgs a) {
       qd[i] = s_q[0][8 * j + i];
       qu[i] = s_q[1][8 * j + i];
     }
-    for (int u0 = f; u0 < n - l; u0 += PPB) {
-      const int u = u0 + tid / LPP;
-      const int id = u < n - l ? page_id(a.r, s, u) : -1;
-      double sum = 0;
-      if (id >= 0) {
-        const uint16_t* bd = a.bounds + ((size_t)id * a.hkv + h) * 2 * D + 8 * j;
-        const uint4 mn = ldg16(bd), mx = ldg16(bd + D);
-        const uint32_t w0[4] = {mn.x, mn.y, mn.z, mn.w}, w1[4] = {mx.x, mx.y, mx.z, mx.w};
+    const int begin = max(split * a.chunk, r.f), end = min((split + 1) * a.chunk, r.n - r.l);
+    for (int u0 = begin; u0 < end; u0 += U * PPB) {
+      int id[U];
+      uint4 mn[U], mx[U];
 #pragma unroll
-        for (int i = 0; i < 4; i++) {
-          sum = fma(qd[2 * i], (double)lo16<DT>(w0[i]), sum);
-          sum = fma(qd[2 * i + 1], (double)hi16<DT>(w0[i]), sum);
-          sum = fma(qu[2 * i], (double)lo16<DT>(w1[i]), sum);
-          sum = fma(qu[2 * i + 1], (double)hi16<DT>(w1[i]), sum);
-        }
+      for (int i = 0; i < U; i++) {
+        const int u = u0 + i * PPB + tid / LPP;
+        id[i] = u < end ? page_id(a.r, s, u) : -1;
       }
 #pragma unroll
-      for (int o = 1; o < LPP; o <<= 1) sum += __shfl_xor(sum, o, kWave);
-      if (j == 0 && u < n - l) s_key[u] = id < 0 ? 0 : score_key(sum);
+      for (int i = 0; i < U; i++) {
+        // (a page that is not there reads page 0, unused)
+        const uint16_t* bd = a.bounds + ((size_t)max(id[i], 0) * a.hkv + h) * 2 * D + 8 * j;
+        mn[i] = ldg16(bd);
+        mx[i] = ldg16(bd + D);
+      }
+#pragma unroll
+      for (int i = 0; i < U; i++) {
+        const uint32_t w0[4] = {mn[i].x, mn[i].y, mn[i].z, mn[i].w}, w1[4] = {mx[i].x, mx[i].y, mx[i].z, mx[i].w};
+        double s0 = 0, s1 = 0;
+#pragma unroll
+        for (int e = 0; e < 4; e++) {
+          s0 = fma(qd[2 * e], (double)lo16<DT>(w0[e]), s0);
+          s1 = fma(qu[2 * e], (double)lo16<DT>(w1[e]), s1);
+          s0 = fma(qd[2 * e + 1], (double)hi16<DT>(w0[e]), s0);
+          s1 = fma(qu[2 * e + 1], (double)hi16<DT>(w1[e]), s1);
+        }
+        const double sum = group_sum<LPP>(s0 + s1);
+        const int u = u0 + i * PPB + tid / LPP;
+        if (j == 0 && u < end) {
+          const uint64_t k = id[i] < 0 ? 0 : score_key(sum);
+          if (a.splits > 1) sel_store(a.keys + (size_t)pair * a.max_pages + u, k);
+          else s_key[u] = k;
+        }
+      }
     }
+    if (a.splits > 1) {
+      if (!arrive_last(&a.tickets[pair], a.splits)) return;
+      for (int u = r.f + tid; u < r.n - r.l; u += SEL_THREADS) s_key[u] = sel_load(a.keys + (size_t)pair * a.max_pages + u);
+    }
+    __syncthreads();
+  } else if (split > 0) {
+    return;  // nothing to compare: the first workgroup writes the list
   }
-  __syncthreads();
-  choose(s_key, n, f, l, m, a.top, out);
+  choose<SEL_WAVES>(s_key, r.n, r.f, r.l, r.m, a.top, out);
 }
 
 }  // namespace yr
 
 using namespace yr;
 
+// Splits per row: enough workgroups to fill the chip, SEL_MIN_CHUNK pages each at least.
+static void select_plan(long long pairs, int max_pages, int* splits, int* chunk) {
+  long long sp = (SEL_TARGET_WG + pairs - 1) / pairs;
+  const int most = (max_pages + SEL_MIN_CHUNK - 1) / SEL_MIN_CHUNK;
+  if (sp > most) sp = most;
+  *chunk = (int)((max_pages + sp - 1) / sp);
+  *splits = (max_pages + *chunk - 1) / *chunk;
+}
+
+extern "C" size_t yr_hip_select_pages_workspace(int rows, int hkv, int page_size, int max_kv_len) {
+  if (rows <= 0 || hkv <= 0 || page_size <= 0 || max_kv_len <= 0) return 0;
+  int splits, chunk;
+  const long long pairs = (long long)rows * hkv;
+  const int max_pages = (max_kv_len - 1) / page_size + 1;
+  select_plan(pairs, max_pages, &splits, &chunk);
+  return splits > 1 ? kTicketBytes + (size_t)pairs * max_pages * sizeof(uint64_t) : 0;
+}
+
 extern "C" int yr_hip_select_pages(const void* q, const void* page_bounds, const int32_t* qo_indptr,
                                    const int32_t* kv_indptr, const int32_t* kv_indices, int n_indices,
                                    const int32_t* kv_len, int32_t* pages, int rows, int batch, int hq, int hkv, int d,
                                    int page_size, int num_pages, int max_kv_len, int top_pages, int first_pages,
-                                   int last_pages, int dtype, void* stream) {
+                                   int last_pages, int dtype, void* workspace, size_t workspace_bytes,
+                                   void* stream) {
   const char* nm = "yr_hip_select_pages";
   SelectArgs a;
   a.r = Ragged{qo_indptr, kv_indptr, kv_indices, kv_len, rows, batch, page_size, n_indices, num_pages};
@@ -201,11 +318,24 @@ extern "C" int yr_hip_select_pages(const void* q, const void* page_bounds, const
   a.top = top_pages;
   a.first = first_pages;
   a.last = last_pages;
+  select_plan((long long)rows * hkv, a.max_pages, &a.splits, &a.chunk);
+  const size_t need = yr_hip_select_pages_workspace(rows, hkv, page_size, max_kv_len);
+  if (need > workspace_bytes || (need && !workspace))
+    return fail(YR_E_WORKSPACE, "%s: workspace %zu < %zu", nm, workspace_bytes, need);
+  a.tickets = (uint32_t*)workspace;
+  a.keys = need ? (uint64_t*)((char*)workspace + kTicketBytes) : nullptr;
   const size_t lds = (size_t)a.max_pages * 8;
+  const dim3 grid((unsigned)(rows * hkv * a.splits));
   hipStream_t st = (hipStream_t)stream;
-#define YR_SEL(DT_, D_)                                                                                             \
-  if (dtype == DT_ && d == D_)                                                                                      \
-    hipLaunchKernelGGL((select_kernel<DT_, D_>), dim3((unsigned)(rows * hkv)), dim3(SEL_THREADS), lds, st, a);
+#define YR_SEL(DT_, D_)                                                                                              \
+  if (dtype == DT_ && d == D_) {                                                                                     \
+    if (lds > 60000) {                                                                                               \
+      const hipError_t e = hipFuncSetAttribute((const void*)select_kernel<DT_, D_>,                                  \
+                                               hipFuncAttributeMaxDynamicSharedMemorySize, (int)lds);                \
+      if (e != hipSuccess) return check_hip(e, nm);                                                                  \
+    }                                                                                                                \
+    hipLaunchKernelGGL((select_kernel<DT_, D_>), grid, dim3(SEL_THREADS), lds, st, a);                               \
+  }
   YR_SEL(DT_F16, 64) YR_SEL(DT_F16, 128) YR_SEL(DT_BF16, 64) YR_SEL(DT_BF16, 128)
 #undef YR_SEL
   YR_CHECK_LAUNCH(nm);

@@ -341,10 +341,12 @@ def select_pages(q, page_bounds, kv_indptr, kv_indices, kv_len, page_size: int, 
     if max_kv_len is None:
         max_kv_len = max(int(kv_len.max().item()), 1)
     with _on(q.device):
+        nb = lib().yr_hip_select_pages_workspace(T, hkv, page_size, max_kv_len)
+        ws = _scratch(nb, q.device)
         check(lib().yr_hip_select_pages(
             _at(q), _at(page_bounds), _at(qo_indptr), _at(kv_indptr), _at(kv_indices), kv_indices.numel(),
             _at(kv_len), _at(out), T, batch, hq, hkv, D, page_size, P, max_kv_len, top_pages, first_pages, last_pages,
-            dt, torch.cuda.current_stream(q.device).cuda_stream), "select_pages")
+            dt, _at(ws), nb, torch.cuda.current_stream(q.device).cuda_stream), "select_pages")
     return out
 
 
