@@ -61,6 +61,22 @@ __device__ __forceinline__ int page_id(const Ragged& r, const SeqRows& s, int u)
   return (unsigned)id < (unsigned)r.num_pages ? id : -1;
 }
 
+// Tile `tile` of a batch cut into tiles of up to `rows` rows of one sequence ->
+// {sequence (batch: none), its first row within the sequence}.  One thread.
+__device__ __forceinline__ void find_tile(const Ragged& r, int tile, int rows, int* out) {
+  int b = tile, left = 0;
+  if (r.qo_indptr) {
+    left = tile;
+    for (b = 0; b < r.batch; b++) {
+      const int n = (seq_rows(r, b).n + rows - 1) / rows;
+      if (left < n) break;
+      left -= n;
+    }
+  }
+  out[0] = b;
+  out[1] = left * rows;
+}
+
 // Host checks of the parts every such operator has.
 int ragged_check(const char* nm, const Ragged& r, int hq, int hkv, int d, int dtype);
 

@@ -17,6 +17,8 @@
 
 namespace yr {
 
+typedef double f64x4 __attribute__((ext_vector_type(4)));
+
 struct SelectArgs {
   Ragged r;
   const uint16_t* q;
@@ -30,6 +32,9 @@ struct SelectArgs {
 constexpr int SEL_THREADS = 256;
 constexpr int SEL_WAVES = SEL_THREADS / kWave;
 constexpr int SEL_MAX_PAGES = 16384;  // 64-bit keys of one row in LDS: 128 of 160 KiB
+constexpr int SEL_ROWS = 16;          // rows of a tile
+constexpr int SEL_TILE_PAGES = 1024;  // a tile's keys in LDS: as much
+constexpr int SEL_TILE_MIN = 4;       // rows per sequence from which tiles are taken
 constexpr int SEL_TARGET_WG = 1024;
 constexpr int SEL_MIN_CHUNK = 64;     // pages per split at least
 
@@ -70,17 +75,34 @@ __device__ __forceinline__ double group_sum(double v) {
 
 // Writes the ascending list of a row: pages [0, f) and [n - l, n) and the `m`
 // best keys of [f, n - l), -1 behind.  W waves work together (the whole
-// workgroup, or one wave by itself), the keys are in LDS.
+// workgroup, or one wave by itself); the keys are in LDS, and a lane holds those
+// of pages (i W + wave) 64 + lane, i < R, in registers (R = 0: more than 16; they
+// are read again each time).
 //
 // The m-th best key is found bit by bit: of the bits in which the keys differ,
 // from the highest, a bit is set when m keys at least reach the value with it.
 // That ends as soon as exactly m do, after about log2 n bits.
-template <int W>
-__device__ void choose(const uint64_t* key, int n, int f, int l, int m, int top, int32_t* out) {
+template <int W, int R>
+__device__ __forceinline__ void choose_from(const uint64_t* key, int n, int f, int l, int m, int top, int32_t* out) {
   __shared__ int s_cnt[2][SEL_WAVES];
   __shared__ uint64_t s_diff[SEL_WAVES];
-  const int lane = threadIdx.x % kWave, wave = W == 1 ? 0 : threadIdx.x / kWave;
+  const int lane = threadIdx.x % kWave, wave = W == 1 ? 0 : __builtin_amdgcn_readfirstlane(threadIdx.x / kWave);
   const int c0 = f, c1 = n - l;  // candidates
+  const int turns = R ? R : (n + W * kWave - 1) / (W * kWave);
+  uint64_t k[R ? R : 1];
+  // key i of this lane; 0 (never counted below) where there is no candidate
+  auto get = [&](int i) __attribute__((always_inline)) -> uint64_t {
+    if constexpr (R > 0) return k[i];
+    const int u = (i * W + wave) * kWave + lane;
+    return u >= c0 && u < c1 ? key[u] : 0;
+  };
+  if constexpr (R > 0) {
+#pragma unroll
+    for (int i = 0; i < R; i++) {
+      const int u = (i * W + wave) * kWave + lane;
+      k[i] = u >= c0 && u < c1 ? key[u] : 0;
+    }
+  }
   int turn = 0;
   // sum of a count over the waves
   auto all = [&](int c) __attribute__((always_inline)) -> int {
@@ -93,12 +115,27 @@ __device__ void choose(const uint64_t* key, int n, int f, int l, int m, int top,
     turn ^= 1;  // the next count goes elsewhere: one barrier each
     return sum;
   };
-  uint64_t bound = 0;  // keys from it on are taken ..
+  auto count = [&](uint64_t least) __attribute__((always_inline)) -> int {  // least > 0
+    int c = 0;
+    if constexpr (R > 0) {
+#pragma unroll
+      for (int i = 0; i < R; i++) c += __popcll(__ballot(k[i] >= least));
+    } else {
+#pragma unroll 4
+      for (int i = 0; i < turns; i++) c += __popcll(__ballot(get(i) >= least));
+    }
+    return all(c);
+  };
+  uint64_t bound = 0;      // keys from it on are taken ..
   int equal = 0x7fffffff;  // .. of those equal to it only the first `equal`
   if (m > 0 && m < c1 - c0) {
     const uint64_t any = key[c0];
     uint64_t diff = 0;
-    for (int u = c0 + wave * kWave + lane; u < c1; u += W * kWave) diff |= key[u] ^ any;
+#pragma unroll(R ? R : 4)
+    for (int i = 0; i < turns; i++) {
+      const int u = (i * W + wave) * kWave + lane;
+      if (u >= c0 && u < c1) diff |= get(i) ^ any;
+    }
     diff = (uint64_t)wave_or((uint32_t)(diff >> 32)) << 32 | wave_or((uint32_t)diff);
     if constexpr (W > 1) {
       if (lane == 0) s_diff[wave] = diff;
@@ -107,60 +144,58 @@ __device__ void choose(const uint64_t* key, int n, int f, int l, int m, int top,
       for (int w = 0; w < W; w++) diff |= s_diff[w];
     }
     int bit = diff ? 63 - __builtin_clzll(diff) : -1;
-    bound = bit == 63 ? 0 : any & ~((2ull << (bit < 0 ? 0 : bit)) - 1);
-    if (bit < 0) bound = any;  // all the same
+    bound = bit < 0 ? any : bit == 63 ? 0 : any & ~((2ull << bit) - 1);
     bool exact = false;
     for (; bit >= 0 && !exact; bit--) {
       const uint64_t cand = bound | 1ull << bit;
-      int c = 0;
-      for (int u0 = c0 + wave * kWave; u0 < c1; u0 += W * kWave) {
-        const int u = u0 + lane;
-        c += __popcll(__ballot(u < c1 && key[u] >= cand));
-      }
-      c = all(c);
+      const int c = count(cand);
       if (c >= m) bound = cand;
       exact = c == m;
     }
-    if (!exact) {  // equal keys at the border: the first of them
-      int c = 0;
-      for (int u0 = c0 + wave * kWave; u0 < c1; u0 += W * kWave) {
-        const int u = u0 + lane;
-        c += __popcll(__ballot(u < c1 && key[u] > bound));
-      }
-      equal = m - all(c);
-    }
+    if (!exact) equal = m - (bound == ~0ull ? 0 : count(bound + 1));  // equal keys at the border: the first of them
   }
-  // ascending list; the waves take contiguous blocks of 64 pages in turn
+  // ascending list; the waves take blocks of 64 pages in turn
   int at = 0, eq = 0;  // written so far, keys equal to bound seen so far
-  for (int u0 = 0; u0 < n; u0 += W * kWave) {
-    const int u = u0 + wave * kWave + lane;
+#pragma unroll(R ? R : 1)
+  for (int i = 0; i < turns; i++) {
+    const int u = (i * W + wave) * kWave + lane;
     const bool cand = u >= c0 && u < c1;
-    const uint64_t k = cand ? key[u] : 0;
-    const bool same = cand && k == bound;
+    const uint64_t key_u = get(i);
+    const bool same = cand && key_u == bound;
+    int before = eq;
     const uint64_t be = __ballot(same);
-    int before = eq, alle = __popcll(be);
-    if constexpr (W > 1) {
-      alle = all(alle);
+    if (equal != 0x7fffffff) {  // (uniform)
+      int alle = all(__popcll(be));
+      if constexpr (W > 1) {
 #pragma unroll
-      for (int w = 0; w < W; w++)
-        if (w < wave) before += s_cnt[turn ^ 1][w];
+        for (int w = 0; w < W; w++)
+          if (w < wave) before += s_cnt[turn ^ 1][w];
+      }
+      eq += alle;
+      before += __popcll(be & ((1ull << lane) - 1));
     }
-    eq += alle;
-    before += __popcll(be & ((1ull << lane) - 1));
-    const bool take = u < n && (!cand || (m > 0 && (same ? before < equal : k > bound)));
+    const bool take = u < n && (!cand || (m > 0 && (same ? before < equal : key_u > bound)));
     const uint64_t bt = __ballot(take);
-    int pos = at, allt = __popcll(bt);
+    int pos = at;
+    at += all(__popcll(bt));
     if constexpr (W > 1) {
-      allt = all(allt);
 #pragma unroll
       for (int w = 0; w < W; w++)
         if (w < wave) pos += s_cnt[turn ^ 1][w];
     }
-    at += allt;
     pos += __popcll(bt & ((1ull << lane) - 1));
     if (take && pos < top) gptr(out)[pos] = u;
   }
   for (int i = at + wave * kWave + lane; i < top; i += W * kWave) gptr(out)[i] = -1;
+}
+
+template <int W>
+__device__ __forceinline__ void choose(const uint64_t* key, int n, int f, int l, int m, int top, int32_t* out) {
+  const int turns = (n + W * kWave - 1) / (W * kWave);
+  if (turns <= 4) choose_from<W, 4>(key, n, f, l, m, top, out);
+  else if (turns <= 8) choose_from<W, 8>(key, n, f, l, m, top, out);
+  else if (turns <= 16) choose_from<W, 16>(key, n, f, l, m, top, out);
+  else choose_from<W, 0>(key, n, f, l, m, top, out);
 }
 
 // Pages of a row: visible and existing ones n, forced ones at the start (f) and
@@ -266,9 +301,102 @@ __global__ __launch_bounds__(SEL_THREADS) void select_kernel(SelectArgs a) {
   choose<SEL_WAVES>(s_key, r.n, r.f, r.l, r.m, a.top, out);
 }
 
+// Up to 16 rows of one sequence and one kv head: their scores are a product of
+// [16][2 D] by [2 D][pages] on the 64-bit matrix instruction 16x16x4, so the
+// bounds are read and converted once for all rows.  A lane holds its row's Q-
+// and Q+ for the dims 32 c + 8 (lane / 16) .. + 7 and loads the same dims of its
+// page, 16 bytes each: A and B only have to agree on the order of the products.
+// Bound by that instruction (64 cycles a SIMD per 16 x 16 x 4).
+template <int DT, int D>
+__global__ __launch_bounds__(SEL_THREADS) void select_tile_kernel(SelectArgs a) {
+  constexpr int C = D / 32;             // 16-byte pieces per lane of each bound
+  extern __shared__ uint64_t s_key[];   // [16][stride]
+  __shared__ int s_tile[2];
+  const int tid = threadIdx.x, lane = tid % kWave, wave = __builtin_amdgcn_readfirstlane(tid / kWave);
+  const int h = blockIdx.x % a.hkv, tile = blockIdx.x / a.hkv, stride = a.max_pages;
+  if (tid == 0) find_tile(a.r, tile, SEL_ROWS, s_tile);
+  __syncthreads();
+  const int b = s_tile[0], i0 = s_tile[1];
+  if (b >= a.r.batch) return;
+  const SeqRows s = seq_rows(a.r, b);
+  const int nt = min(SEL_ROWS, s.n - i0), t0 = s.row0 + i0, p0 = s.len - s.n + i0;
+  const RowPages last = row_pages(a, s, p0 + nt - 1);  // the row that sees most
+  const int g = a.hq / a.hkv, col = lane % 16, grp = lane / 16;
+  if (last.m > 0 && last.m < last.n - last.f - last.l) {
+    double down[C][8], up[C][8];
+    {
+      const uint16_t* q = a.q + ((size_t)(t0 + min(col, nt - 1)) * a.hq + (size_t)h * g) * D + 8 * grp;
+#pragma unroll
+      for (int c = 0; c < C; c++)
+#pragma unroll
+        for (int e = 0; e < 8; e++) down[c][e] = up[c][e] = 0;
+      for (int i = 0; i < g; i++)
+#pragma unroll
+        for (int c = 0; c < C; c++) {
+          const uint4 v = ldg16(q + (size_t)i * D + 32 * c);
+          const uint32_t w[4] = {v.x, v.y, v.z, v.w};
+#pragma unroll
+          for (int e = 0; e < 8; e++) {
+            const double x = e % 2 ? hi16<DT>(w[e / 2]) : lo16<DT>(w[e / 2]);
+            up[c][e] += x > 0 ? x : x != x ? x : 0;
+            down[c][e] += x < 0 ? x : 0;
+          }
+        }
+    }
+    // 16 pages a turn and wave; the next turn's bounds are on their way
+    auto fetch = [&](int u0, uint4* v) __attribute__((always_inline)) -> int {
+      const int u = u0 + col, id = u < last.n ? page_id(a.r, s, u) : -1;
+      const uint16_t* bd = a.bounds + ((size_t)max(id, 0) * a.hkv + h) * 2 * D + 8 * grp;
+#pragma unroll
+      for (int c = 0; c < C; c++) {
+        v[c] = ldg16(bd + 32 * c);
+        v[C + c] = ldg16(bd + D + 32 * c);
+      }
+      return id;
+    };
+    uint4 next[2 * C];
+    int id_next = fetch(16 * wave, next);
+    for (int u0 = 16 * wave; u0 < last.n; u0 += 16 * SEL_WAVES) {
+      uint4 v[2 * C];
+#pragma unroll
+      for (int c = 0; c < 2 * C; c++) v[c] = next[c];
+      const int id = id_next;
+      id_next = fetch(min(u0 + 16 * SEL_WAVES, last.n), next);
+      f64x4 acc[2] = {{0, 0, 0, 0}, {0, 0, 0, 0}};
+#pragma unroll
+      for (int c = 0; c < C; c++) {
+        const uint32_t w0[4] = {v[c].x, v[c].y, v[c].z, v[c].w};
+        const uint32_t w1[4] = {v[C + c].x, v[C + c].y, v[C + c].z, v[C + c].w};
+#pragma unroll
+        for (int e = 0; e < 8; e++) {
+          acc[0] = __builtin_amdgcn_mfma_f64_16x16x4f64(down[c][e], e % 2 ? hi16<DT>(w0[e / 2]) : lo16<DT>(w0[e / 2]),
+                                                        acc[0], 0, 0, 0);
+          acc[1] = __builtin_amdgcn_mfma_f64_16x16x4f64(up[c][e], e % 2 ? hi16<DT>(w1[e / 2]) : lo16<DT>(w1[e / 2]),
+                                                        acc[1], 0, 0, 0);
+        }
+      }
+      // result rows 4 i + grp, page col
+      if (u0 + col < last.n)
+#pragma unroll
+        for (int i = 0; i < 4; i++)
+          s_key[(4 * i + grp) * stride + u0 + col] = id < 0 ? 0 : score_key(acc[0][i] + acc[1][i]);
+    }
+  }
+  __syncthreads();
+  for (int i = wave; i < nt; i += SEL_WAVES) {
+    const RowPages r = row_pages(a, s, p0 + i);
+    choose<1>(s_key + (size_t)i * stride, r.n, r.f, r.l, r.m, a.top, a.out + ((size_t)(t0 + i) * a.hkv + h) * a.top);
+  }
+}
+
 }  // namespace yr
 
 using namespace yr;
+
+// Rows of the same sequence share their pages' bounds in a tile.
+static bool select_tiled(bool ragged, int rows, int batch, int max_pages) {
+  return ragged && rows >= SEL_TILE_MIN * (long long)batch && max_pages <= SEL_TILE_PAGES;
+}
 
 // Splits per row: enough workgroups to fill the chip, SEL_MIN_CHUNK pages each at least.
 static void select_plan(long long pairs, int max_pages, int* splits, int* chunk) {
@@ -286,6 +414,18 @@ extern "C" size_t yr_hip_select_pages_workspace(int rows, int hkv, int page_size
   const int max_pages = (max_kv_len - 1) / page_size + 1;
   select_plan(pairs, max_pages, &splits, &chunk);
   return splits > 1 ? kTicketBytes + (size_t)pairs * max_pages * sizeof(uint64_t) : 0;
+}
+
+// A launch with `lds` bytes of dynamic LDS.
+template <class K>
+static int select_launch(const char* nm, K kernel, unsigned grid, size_t lds, hipStream_t st, const SelectArgs& a) {
+  if (lds > 48 * 1024) {
+    const hipError_t e = hipFuncSetAttribute((const void*)kernel, hipFuncAttributeMaxDynamicSharedMemorySize, (int)lds);
+    if (e != hipSuccess) return check_hip(e, nm);
+  }
+  hipLaunchKernelGGL(kernel, dim3(grid), dim3(SEL_THREADS), lds, st, a);
+  YR_CHECK_LAUNCH(nm);
+  return YR_OK;
 }
 
 extern "C" int yr_hip_select_pages(const void* q, const void* page_bounds, const int32_t* qo_indptr,
@@ -324,20 +464,17 @@ extern "C" int yr_hip_select_pages(const void* q, const void* page_bounds, const
     return fail(YR_E_WORKSPACE, "%s: workspace %zu < %zu", nm, workspace_bytes, need);
   a.tickets = (uint32_t*)workspace;
   a.keys = need ? (uint64_t*)((char*)workspace + kTicketBytes) : nullptr;
-  const size_t lds = (size_t)a.max_pages * 8;
-  const dim3 grid((unsigned)(rows * hkv * a.splits));
+  const bool tiled = select_tiled(qo_indptr != nullptr, rows, batch, a.max_pages);
+  long long tiles = (long long)rows / SEL_ROWS + batch;  // at most, whatever the sequences' rows
+  if (tiles > rows) tiles = rows;
+  const size_t lds = (size_t)a.max_pages * 8 * (tiled ? SEL_ROWS : 1);
+  const unsigned grid = (unsigned)(tiled ? tiles * hkv : (long long)rows * hkv * a.splits);
   hipStream_t st = (hipStream_t)stream;
-#define YR_SEL(DT_, D_)                                                                                              \
-  if (dtype == DT_ && d == D_) {                                                                                     \
-    if (lds > 60000) {                                                                                               \
-      const hipError_t e = hipFuncSetAttribute((const void*)select_kernel<DT_, D_>,                                  \
-                                               hipFuncAttributeMaxDynamicSharedMemorySize, (int)lds);                \
-      if (e != hipSuccess) return check_hip(e, nm);                                                                  \
-    }                                                                                                                \
-    hipLaunchKernelGGL((select_kernel<DT_, D_>), grid, dim3(SEL_THREADS), lds, st, a);                               \
-  }
+#define YR_SEL(DT_, D_)                                                                        \
+  if (dtype == DT_ && d == D_)                                                                 \
+    return tiled ? select_launch(nm, select_tile_kernel<DT_, D_>, grid, lds, st, a)            \
+                 : select_launch(nm, select_kernel<DT_, D_>, grid, lds, st, a);
   YR_SEL(DT_F16, 64) YR_SEL(DT_F16, 128) YR_SEL(DT_BF16, 64) YR_SEL(DT_BF16, 128)
 #undef YR_SEL
-  YR_CHECK_LAUNCH(nm);
-  return YR_OK;
+  return fail(YR_E_INVALID, "%s: shape", nm);
 }

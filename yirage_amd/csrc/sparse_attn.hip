@@ -70,21 +70,7 @@ __global__ __launch_bounds__(SP_THREADS) void sparse_kernel(SparseArgs a) {
   const int G = a.hq / a.hkv, col = lane % 16, grp = lane / 16;
 
   // ---- the tile's sequence and rows
-  if (tid == 0) {
-    int b = tile, i0 = 0;
-    if (a.r.qo_indptr) {
-      int left = tile;
-      for (b = 0; b < a.r.batch; b++) {
-        const SeqRows s = seq_rows(a.r, b);
-        const int n = (s.n + a.tt - 1) / a.tt;
-        if (left < n) break;
-        left -= n;
-      }
-      i0 = left * a.tt;
-    }
-    s_tile[0] = b;
-    s_tile[1] = i0;
-  }
+  if (tid == 0) find_tile(a.r, tile, a.tt, s_tile);
   __syncthreads();
   const int b = s_tile[0], i0 = s_tile[1];
   if (b >= a.r.batch) return;
