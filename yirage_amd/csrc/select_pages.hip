@@ -33,6 +33,7 @@ constexpr int SEL_THREADS = 256;
 constexpr int SEL_WAVES = SEL_THREADS / kWave;
 constexpr int SEL_MAX_PAGES = 16384;  // 64-bit keys of one row in LDS: 128 of 160 KiB
 constexpr int SEL_ROWS = 16;          // rows of a tile
+constexpr int SEL_TILE_WAVES = 8;     // two a SIMD: 36 us for 512 rows of 512 pages, 43 with 4
 constexpr int SEL_TILE_PAGES = 1024;  // a tile's keys in LDS: as much
 constexpr int SEL_TILE_MIN = 4;       // rows per sequence from which tiles are taken
 constexpr int SEL_TARGET_WG = 1024;
@@ -238,10 +239,18 @@ __global__ __launch_bounds__(SEL_THREADS) void select_kernel(SelectArgs a) {
     const int g = a.hq / a.hkv;
     for (int d = tid; d < D; d += SEL_THREADS) {
       double up = 0, down = 0;
-      for (int i = 0; i < g; i++) {
-        const double x = ld_elem<DT>(gptr(a.q)[((size_t)t * a.hq + (size_t)h * g + i) * D + d]);
-        up += x > 0 ? x : x != x ? x : 0;
-        down += x < 0 ? x : 0;
+      const uint16_t* q = a.q + ((size_t)t * a.hq + (size_t)h * g) * D + d;
+      for (int i0 = 0; i0 < g; i0 += 4) {  // 4 loads in flight
+        uint32_t w[4];
+#pragma unroll
+        for (int i = 0; i < 4; i++) w[i] = gptr(q)[(size_t)min(i0 + i, g - 1) * D];
+#pragma unroll
+        for (int i = 0; i < 4; i++)
+          if (i0 + i < g) {
+            const double x = ld_elem<DT>(w[i]);
+            up += x > 0 ? x : x != x ? x : 0;
+            down += x < 0 ? x : 0;
+          }
       }
       s_q[0][d] = down;
       s_q[1][d] = up;
@@ -308,7 +317,7 @@ __global__ __launch_bounds__(SEL_THREADS) void select_kernel(SelectArgs a) {
 // page, 16 bytes each: A and B only have to agree on the order of the products.
 // Bound by that instruction (64 cycles a SIMD per 16 x 16 x 4).
 template <int DT, int D>
-__global__ __launch_bounds__(SEL_THREADS) void select_tile_kernel(SelectArgs a) {
+__global__ __launch_bounds__(SEL_TILE_WAVES * kWave) void select_tile_kernel(SelectArgs a) {
   constexpr int C = D / 32;             // 16-byte pieces per lane of each bound
   extern __shared__ uint64_t s_key[];   // [16][stride]
   __shared__ int s_tile[2];
@@ -356,12 +365,12 @@ __global__ __launch_bounds__(SEL_THREADS) void select_tile_kernel(SelectArgs a) 
     };
     uint4 next[2 * C];
     int id_next = fetch(16 * wave, next);
-    for (int u0 = 16 * wave; u0 < last.n; u0 += 16 * SEL_WAVES) {
+    for (int u0 = 16 * wave; u0 < last.n; u0 += 16 * SEL_TILE_WAVES) {
       uint4 v[2 * C];
 #pragma unroll
       for (int c = 0; c < 2 * C; c++) v[c] = next[c];
       const int id = id_next;
-      id_next = fetch(min(u0 + 16 * SEL_WAVES, last.n), next);
+      id_next = fetch(min(u0 + 16 * SEL_TILE_WAVES, last.n), next);
       f64x4 acc[2] = {{0, 0, 0, 0}, {0, 0, 0, 0}};
 #pragma unroll
       for (int c = 0; c < C; c++) {
@@ -383,7 +392,7 @@ __global__ __launch_bounds__(SEL_THREADS) void select_tile_kernel(SelectArgs a) 
     }
   }
   __syncthreads();
-  for (int i = wave; i < nt; i += SEL_WAVES) {
+  for (int i = wave; i < nt; i += SEL_TILE_WAVES) {
     const RowPages r = row_pages(a, s, p0 + i);
     choose<1>(s_key + (size_t)i * stride, r.n, r.f, r.l, r.m, a.top, a.out + ((size_t)(t0 + i) * a.hkv + h) * a.top);
   }
@@ -418,12 +427,12 @@ extern "C" size_t yr_hip_select_pages_workspace(int rows, int hkv, int page_size
 
 // A launch with `lds` bytes of dynamic LDS.
 template <class K>
-static int select_launch(const char* nm, K kernel, unsigned grid, size_t lds, hipStream_t st, const SelectArgs& a) {
+static int select_launch(const char* nm, K kernel, unsigned grid, int threads, size_t lds, hipStream_t st, const SelectArgs& a) {
   if (lds > 48 * 1024) {
     const hipError_t e = hipFuncSetAttribute((const void*)kernel, hipFuncAttributeMaxDynamicSharedMemorySize, (int)lds);
     if (e != hipSuccess) return check_hip(e, nm);
   }
-  hipLaunchKernelGGL(kernel, dim3(grid), dim3(SEL_THREADS), lds, st, a);
+  hipLaunchKernelGGL(kernel, dim3(grid), dim3(threads), lds, st, a);
   YR_CHECK_LAUNCH(nm);
   return YR_OK;
 }
@@ -472,8 +481,8 @@ extern "C" int yr_hip_select_pages(const void* q, const void* page_bounds, const
   hipStream_t st = (hipStream_t)stream;
 #define YR_SEL(DT_, D_)                                                                        \
   if (dtype == DT_ && d == D_)                                                                 \
-    return tiled ? select_launch(nm, select_tile_kernel<DT_, D_>, grid, lds, st, a)            \
-                 : select_launch(nm, select_kernel<DT_, D_>, grid, lds, st, a);
+    return tiled ? select_launch(nm, select_tile_kernel<DT_, D_>, grid, SEL_TILE_WAVES * kWave, lds, st, a) \
+                 : select_launch(nm, select_kernel<DT_, D_>, grid, SEL_THREADS, lds, st, a);
   YR_SEL(DT_F16, 64) YR_SEL(DT_F16, 128) YR_SEL(DT_BF16, 64) YR_SEL(DT_BF16, 128)
 #undef YR_SEL
   return fail(YR_E_INVALID, "%s: shape", nm);
