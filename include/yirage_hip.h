@@ -200,10 +200,13 @@ int yr_hip_select_pages(const void* q, const void* page_bounds, const int32_t* q
  * <= 16, top_pages <= 1024.  Entries in any order; negative, invisible, missing
  * and repeated ones count for nothing; a row without a token is 0.  The paged attention
  * of yr_hip_gqa_decode_paged on a selection; no counterpart in the reference. */
+size_t yr_hip_gqa_sparse_workspace(int rows, int batch, int ragged, int hq, int hkv, int d, int page_size,
+                                   int top_pages); /* ragged: a call with qo_indptr */
 int yr_hip_gqa_sparse_paged(const void* q, const void* k_cache, const void* v_cache, const int32_t* qo_indptr,
                             const int32_t* kv_indptr, const int32_t* kv_indices, int n_indices,
                             const int32_t* kv_len, const int32_t* pages, void* out, int rows, int batch, int hq,
-                            int hkv, int d, int page_size, int num_pages, int top_pages, int dtype, void* stream);
+                            int hkv, int d, int page_size, int num_pages, int top_pages, int dtype, void* workspace,
+                            size_t workspace_bytes, void* stream);
 
 /* Log probabilities of row-wise softmax over the first n_valid of n columns of
  * x (f16, bf16 or fp32; rows row_stride elements apart): logprob[r] of

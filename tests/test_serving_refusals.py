@@ -73,7 +73,7 @@ def test_select_workspace():
 
 def _sparse(**change):
     a = dict(q=FAKE, kc=FAKE, vc=FAKE, qo=FAKE, ptr=FAKE, idx=FAKE, nidx=4, lens=FAKE, pages=FAKE, out=FAKE, rows=5,
-             batch=2, hq=32, hkv=8, d=128, page=64, npages=4, top=8, dt=_lib.DTYPE_F16, stream=None)
+             batch=2, hq=32, hkv=8, d=128, page=64, npages=4, top=8, dt=_lib.DTYPE_F16, ws=FAKE, nb=1 << 30, stream=None)
     return _call("yr_hip_gqa_sparse_paged", a, **change)
 
 
@@ -81,12 +81,21 @@ def _sparse(**change):
     (dict(kc=None), "null"), (dict(out=None), "null"), (dict(pages=None), "null"), (dict(lens=None), "null"),
     (dict(d=256), "head_dim"), (dict(dt=_lib.DTYPE_F32), "dtype"), (dict(hq=136), "group size"), (dict(hq=0), "group size"),
     (dict(top=0), "top_pages"), (dict(top=1025), "top_pages"), (dict(page=0), "page size"), (dict(qo=None), "one row"),
-    (dict(top=1024, page=2 ** 20 + 1), "page size"), (dict(rows=2 ** 30), "too many"), (dict(vc=ODD), "aligned"),
+    (dict(top=1024, page=2 ** 20 + 1), "page size"), (dict(hq=2 ** 22, hkv=2 ** 20), "too many"), (dict(rows=2 ** 30), "too many"), (dict(vc=ODD), "aligned"),
     (dict(out=ODD), "aligned"),
 ])
 def test_sparse(change, text):
     rc, msg = _sparse(**change)
     assert rc == -1 and text in msg, msg
+
+
+def test_sparse_workspace():
+    need = _lib.lib().yr_hip_gqa_sparse_workspace(5, 2, 1, 32, 8, 128, 64, 8)
+    assert need > 65536
+    for change in (dict(nb=need - 1), dict(ws=None)):
+        rc, msg = _sparse(**change)
+        assert rc == -3 and "workspace" in msg
+    assert _lib.lib().yr_hip_gqa_sparse_workspace(64, 64, 0, 32, 8, 128, 64, 8) == 0
 
 
 def _logprobs(**change):

@@ -15,15 +15,17 @@
 // already the B operand of the second product (k slots 8 g + 4 j + i of lane
 // group g carry tokens 16 j + 4 g + i), while V^T comes from row-major V by
 // transposing reads in that same order.
+#include <type_traits>
+
 #include "attn_device.h"
 #include "ragged.h"
 
 namespace yr {
 
-constexpr int SP_WAVES = 8;
-constexpr int SP_THREADS = SP_WAVES * kWave;
-constexpr int SP_BLK = 32;           // tokens per wave block
-constexpr int SP_MAX_ENTRIES = 1024; // list entries of a tile
+constexpr int SP_BLK = 32;            // tokens per wave block
+constexpr int SP_MAX_ENTRIES = 1024;  // list entries of a tile
+constexpr int SP_TARGET_WG = 256;     // one per CU
+constexpr int SP_MIN_BLOCKS = 2;      // blocks per split at least
 
 struct SparseArgs {
   Ragged r;
@@ -32,7 +34,9 @@ struct SparseArgs {
   const uint16_t* vc;
   const int32_t* pages;   // [rows][hkv][top]
   uint16_t* out;
-  int hq, hkv, top, tt, tiles;  // tt: rows per tile
+  float* partial;         // [tiles][hkv][splits][tt G][D + 4]: O, m, l
+  uint32_t* tickets;      // [tiles][hkv]
+  int hq, hkv, top, tt, splits;  // tt: rows per tile
   float scale_log2;
 };
 
@@ -53,71 +57,42 @@ __device__ __forceinline__ int v_swz(int row) {
   return D == 128 ? ((row & 7) << 1) | ((row >> 3) & 1) : (row & 3) << 1;
 }
 
-template <int DT, int D>
-__global__ __launch_bounds__(SP_THREADS) void sparse_kernel(SparseArgs a) {
-  constexpr int RPI = 512 / D;         // rows per direct load (64 lanes of 16 bytes)
-  constexpr int NL = SP_BLK / RPI;     // loads per operand of a block
-  constexpr int CPR = D / 8;           // chunks per row
-  __shared__ __attribute__((aligned(16))) uint16_t s_k[SP_WAVES][SP_BLK * D];
-  __shared__ __attribute__((aligned(16))) uint16_t s_v[SP_WAVES][SP_BLK * D];
-  __shared__ float s_m[SP_WAVES][16], s_l[SP_WAVES][16];
-  __shared__ int s_cnt[SP_WAVES], s_tile[3];
-  __shared__ int s_u[SP_MAX_ENTRIES];  // page of each entry, -1: counts for nothing
-  __shared__ int l_u[SP_MAX_ENTRIES], l_id[SP_MAX_ENTRIES], l_mask[SP_MAX_ENTRIES];  // union: page, device page id, rows
+// NW waves; PG32: pages are a multiple of 32 tokens, so a block lies in one page
+// and its address is uniform (else the lanes work out one token's each).
+//
+// K and V go straight into the wave's LDS slots; its next K block is requested
+// as soon as this one's fragments are in registers and its next V block after
+// P V, so one of the two is always in flight.
+template <int DT, int D, int NW, bool PG32>
+__global__ __launch_bounds__(NW * kWave) void sparse_kernel(SparseArgs a) {
+  constexpr int T = NW * kWave;
+  constexpr int RPI = 512 / D;      // rows per direct load (64 lanes of 16 bytes)
+  constexpr int NL = SP_BLK / RPI;  // loads per operand of a block
+  constexpr int CPR = D / 8;        // chunks per row
+  __shared__ __attribute__((aligned(16))) uint16_t s_k[NW][SP_BLK * D];
+  __shared__ __attribute__((aligned(16))) uint16_t s_v[NW][SP_BLK * D];
+  __shared__ int l_u[SP_MAX_ENTRIES], l_id[SP_MAX_ENTRIES];  // union: page, device page id, rows
+  __shared__ uint16_t l_mask[SP_MAX_ENTRIES];
+  __shared__ float s_m[NW][16], s_l[NW][16];
+  __shared__ int s_cnt[NW], s_tile[2];
+  static_assert(SP_MAX_ENTRIES * 4 <= (int)sizeof(s_k), "the entries fit where K goes later");
+  int* const s_u = reinterpret_cast<int*>(&s_k[0][0]);  // page of each entry, -1: counts for nothing
   const int tid = threadIdx.x, lane = tid % kWave;
   const int wave = __builtin_amdgcn_readfirstlane(tid / kWave);
-  const int hk = blockIdx.x % a.hkv, tile = blockIdx.x / a.hkv;
+  const int split = blockIdx.x % a.splits, pair = blockIdx.x / a.splits;
+  const int hk = pair % a.hkv, tile = pair / a.hkv;
   const int G = a.hq / a.hkv, col = lane % 16, grp = lane / 16;
 
   // ---- the tile's sequence and rows
-  if (tid == 0) find_tile(a.r, tile, a.tt, s_tile);
-  __syncthreads();
-  const int b = s_tile[0], i0 = s_tile[1];
+  if (a.r.qo_indptr) {
+    if (tid == 0) find_tile(a.r, tile, a.tt, s_tile);
+    __syncthreads();
+  }
+  const int b = a.r.qo_indptr ? s_tile[0] : tile, i0 = a.r.qo_indptr ? s_tile[1] : 0;
   if (b >= a.r.batch) return;
   const SeqRows s = seq_rows(a.r, b);
   const int nt = min(a.tt, s.n - i0), t0 = s.row0 + i0, p0 = s.len - s.n + i0;  // rows, first row, its position
   const int pmax = p0 + nt - 1;
-
-  // ---- union of the rows' lists
-  const int E = nt * a.top;
-  for (int e = tid; e < E; e += SP_THREADS) {
-    const int i = e / a.top, p = p0 + i;
-    int u = gptr(a.pages)[((size_t)(t0 + i) * a.hkv + hk) * a.top + e % a.top];
-    if (u < 0 || p < 0 || u > p / a.r.page || page_id(a.r, s, u) < 0) u = -1;
-    s_u[e] = u;
-  }
-  __syncthreads();
-  int nsel = 0;
-  for (int e0 = 0; e0 < E; e0 += SP_THREADS) {
-    const int e = e0 + tid;
-    const int u = e < E ? s_u[e] : -1;
-    bool own = u >= 0;
-    int mask = 0;
-    if (own)
-      for (int i = 0; i < nt; i++)
-        for (int j = 0; j < a.top; j++)
-          if (s_u[i * a.top + j] == u) {
-            mask |= 1 << i;
-            if (i * a.top + j < e) own = false;
-          }
-    const uint64_t bal = __ballot(own);
-    if (lane == 0) s_cnt[wave] = __popcll(bal);
-    __syncthreads();
-    int at = nsel + __popcll(bal & ((1ull << lane) - 1));
-#pragma unroll
-    for (int w = 0; w < SP_WAVES; w++) {
-      if (w < wave) at += s_cnt[w];
-      nsel += s_cnt[w];
-    }
-    if (own) {
-      l_u[at] = u;
-      l_id[at] = page_id(a.r, s, u);
-      l_mask[at] = mask;
-    }
-    __syncthreads();
-  }
-  const int total = nsel * a.r.page;  // tokens of the union's pages
-  const int nblk = (total + SP_BLK - 1) / SP_BLK;
 
   // ---- this lane's query row: column col = row i of the tile, head g
   const int qi = col / G, qg = col % G;
@@ -129,6 +104,70 @@ __global__ __launch_bounds__(SP_THREADS) void sparse_kernel(SparseArgs a) {
     qf[st] = make_uint4(0, 0, 0, 0);
     if (qok) qf[st] = ldg16(a.q + ((size_t)(t0 + qi) * a.hq + (size_t)hk * G + qg) * D + 32 * st + 8 * grp);
   }
+
+  // ---- union of the rows' lists.  Ascending lists (the usual ones) are
+  // searched by halving, others entry by entry.
+  const int E = nt * a.top;
+  for (int e = tid; e < E; e += T) {
+    const int i = e / a.top, p = p0 + i;
+    int u = gptr(a.pages)[((size_t)(t0 + i) * a.hkv + hk) * a.top + e % a.top];
+    if (u < 0 || p < 0 || u > p / a.r.page || page_id(a.r, s, u) < 0) u = -1;
+    s_u[e] = u;
+  }
+  __syncthreads();
+  bool unordered = false;
+  for (int e = tid; e < E; e += T)
+    if (e % a.top) unordered |= s_u[e] >= 0 && (s_u[e - 1] < 0 || s_u[e] <= s_u[e - 1]);
+  const bool ordered = !__syncthreads_or(unordered);
+  int nsel = 0;
+  for (int e0 = 0; e0 < E; e0 += T) {
+    const int e = e0 + tid, mine = e / a.top;
+    const int u = e < E ? s_u[e] : -1;
+    bool own = u >= 0;
+    int mask = own ? 1 << mine : 0;
+    if (own && ordered) {
+      for (int i = 0; i < nt; i++) {
+        if (i == mine) continue;
+        const int* li = s_u + i * a.top;
+        int lo = 0, hi = a.top;  // first entry that is u, larger or none
+        while (lo < hi) {
+          const int mid = (lo + hi) / 2;
+          if ((unsigned)li[mid] < (unsigned)u) lo = mid + 1;
+          else hi = mid;
+        }
+        if (lo < a.top && li[lo] == u) {
+          mask |= 1 << i;
+          if (i < mine) own = false;
+        }
+      }
+    } else if (own) {
+      for (int j = 0; j < E; j++)
+        if (s_u[j] == u) {
+          mask |= 1 << (j / a.top);
+          if (j < e) own = false;
+        }
+    }
+    const uint64_t bal = __ballot(own);
+    if (lane == 0) s_cnt[wave] = __popcll(bal);
+    __syncthreads();
+    int at = nsel + __popcll(bal & ((1ull << lane) - 1));
+#pragma unroll
+    for (int w = 0; w < NW; w++) {
+      if (w < wave) at += s_cnt[w];
+      nsel += s_cnt[w];
+    }
+    if (own) {
+      l_u[at] = u;
+      l_id[at] = page_id(a.r, s, u);
+      l_mask[at] = (uint16_t)mask;
+    }
+    __syncthreads();
+  }
+  nsel = __builtin_amdgcn_readfirstlane(nsel);
+  const int total = nsel * a.r.page;  // tokens of the union's pages
+  const int nblk = (total + SP_BLK - 1) / SP_BLK;
+  const int per = (nblk + a.splits - 1) / a.splits;
+  const int blk0 = min(split * per, nblk), blk1 = min(blk0 + per, nblk);
 
   uint16_t* const ks = s_k[wave];
   uint16_t* const vs = s_v[wave];
@@ -148,22 +187,51 @@ __global__ __launch_bounds__(SP_THREADS) void sparse_kernel(SparseArgs a) {
   int j0 = 0, j1 = nt;
   bool exact = false;
   while (true) {
-    const int plim = p0 + j1 - 1, bits = ((1 << j1) - 1) & ~((1 << j0) - 1);
-    // element offset of virtual token j's row (of one that may be read where j is none)
-    auto row_of = [&](int j) __attribute__((always_inline)) -> size_t {
-      const int e = min(j / a.r.page, nsel - 1);
-      const int slot = max(min(j < total ? j % a.r.page : 0, pmax - l_u[e] * a.r.page), 0);
-      return ((size_t)l_id[e] * a.r.page + slot) * tok_stride + (size_t)hk * D;
+    const int bits = ((1 << j1) - 1) & ~((1 << j0) - 1);
+    // Tokens of a block: its first position, the rows that see its page and the
+    // address of its first row (PG32), or those of token lane % 32.
+    struct Block {
+      int pos, mask;
+      size_t off;
     };
-    auto issue = [&](int blk, auto is_k_c) __attribute__((always_inline)) {
+    auto block = [&](int blk) __attribute__((always_inline)) -> Block {
+      Block t;
+      const int j = blk * SP_BLK + (PG32 ? 0 : lane % SP_BLK);
+      const int e = min(j / a.r.page, nsel - 1), slot = j - e * a.r.page;  // (slot >= page behind the last page)
+      int u = l_u[e], id = l_id[e], mask = l_mask[e];
+      if constexpr (PG32) {
+        u = __builtin_amdgcn_readfirstlane(u);
+        id = __builtin_amdgcn_readfirstlane(id);
+        mask = __builtin_amdgcn_readfirstlane(mask);
+      }
+      t.pos = u * a.r.page + slot;
+      t.mask = j < total ? mask & bits : 0;
+      // what no row of the tile sees yet is not read: the page's last visible token stands in
+      const int at = PG32 ? slot : max(min(slot, min(pmax - u * a.r.page, a.r.page - 1)), 0);
+      t.off = ((size_t)id * a.r.page + at) * tok_stride + (size_t)hk * D;
+      return t;
+    };
+    auto issue = [&](const Block& t, auto is_k_c) __attribute__((always_inline)) {
       constexpr bool IS_K = decltype(is_k_c)::value;
-      const uint16_t* cache = IS_K ? a.kc : a.vc;
-      uint16_t* dst = IS_K ? ks : vs;
+      const uint16_t* const cache = IS_K ? a.kc : a.vc;
+      uint16_t* const dst = IS_K ? ks : vs;
 #pragma unroll
       for (int u = 0; u < NL; u++) {
         const int row = RPI * u + lane / CPR;
-        const int chunk = (lane % CPR) ^ (IS_K ? k_swz<D>(row) : v_swz<D>(row));
-        lds_load16(cache + row_of(blk * SP_BLK + row) + 8 * chunk, dst + RPI * u * D);
+        const int chunk = 8 * ((lane % CPR) ^ (IS_K ? k_swz<D>(row) : v_swz<D>(row)));
+        const uint16_t* src;
+        if constexpr (PG32) {
+          // rows that no row of the tile sees yet: the last visible one (in this page, maybe before the block)
+          if (pmax - t.pos >= SP_BLK - 1)  // (uniform)
+            src = reinterpret_cast<const uint16_t*>(reinterpret_cast<const char*>(cache + t.off) +
+                                                    2u * (uint32_t)(row * (int)tok_stride + chunk));
+          else
+            src = cache + t.off + (long long)min(row, pmax - t.pos) * (long long)tok_stride + chunk;
+        } else {
+          const uint32_t lo = (uint32_t)__shfl((int)(uint32_t)t.off, row), hi = (uint32_t)__shfl((int)(t.off >> 32), row);
+          src = cache + ((size_t)hi << 32 | lo) + chunk;
+        }
+        lds_load16(src, dst + RPI * u * D);
       }
     };
     float m_i = -INFINITY, l_i = 0.f;
@@ -171,19 +239,13 @@ __global__ __launch_bounds__(SP_THREADS) void sparse_kernel(SparseArgs a) {
 #pragma unroll
     for (int dt = 0; dt < D / 16; dt++) acc[dt] = f32x4{0.f, 0.f, 0.f, 0.f};
 
-    for (int blk = wave; blk < nblk; blk += SP_WAVES) {
-      issue(blk, std::true_type{});
-      issue(blk, std::false_type{});
-      asm volatile("s_waitcnt vmcnt(0)" ::: "memory");
-      if (exact) {
-#pragma unroll
-        for (int u = 0; u < NL; u++) {
-          const int j = blk * SP_BLK + RPI * u + lane / CPR, e = min(j / a.r.page, nsel - 1);
-          const bool see = j < total && (l_mask[e] & bits) && l_u[e] * a.r.page + j % a.r.page <= plim;
-          if (!see) *reinterpret_cast<uint4*>(vs + RPI * u * D + 8 * lane) = make_uint4(0, 0, 0, 0);
-        }
-        asm volatile("s_waitcnt lgkmcnt(0)" ::: "memory");
-      }
+    Block cur;
+    // LAST: there is no next block (a copy of its own: every path knows how many loads are in flight)
+    auto consume = [&](int blk, auto last_c) __attribute__((always_inline)) {
+      constexpr bool LAST = decltype(last_c)::value;
+      Block nxt;
+      if constexpr (!LAST) nxt = block(blk + NW);
+      asm volatile("s_waitcnt vmcnt(%0)" ::"n"(NL) : "memory");  // K has landed, V may be on its way
       f32x4 sc[2];
 #pragma unroll
       for (int n = 0; n < 2; n++) {
@@ -193,18 +255,39 @@ __global__ __launch_bounds__(SP_THREADS) void sparse_kernel(SparseArgs a) {
           c = mfma16<DT>(*reinterpret_cast<const uint4*>(&ks[koff[st] + 16 * n * D]), qf[st], c);
         sc[n] = c;
       }
-      // mask: tokens 16 n + 4 grp + i of the block
+      asm volatile("s_waitcnt lgkmcnt(0)" ::: "memory");  // every K fragment is in registers
+      if constexpr (!LAST) issue(nxt, std::true_type{});
+      // mask: this lane's tokens are 16 n + 4 grp + i
+      if constexpr (PG32) {
+        const bool row = (cur.mask >> qi) & 1;
+        if (cur.pos + SP_BLK - 1 <= p0 + j0) {  // (uniform) every row is behind the block
+          if (cur.mask != bits) {
+#pragma unroll
+            for (int n = 0; n < 2; n++)
+#pragma unroll
+              for (int i = 0; i < 4; i++) sc[n][i] = row ? sc[n][i] : -INFINITY;
+          }
+        } else {
+#pragma unroll
+          for (int n = 0; n < 2; n++)
+#pragma unroll
+            for (int i = 0; i < 4; i++)
+              sc[n][i] = row && cur.pos + 16 * n + 4 * grp + i <= qpos ? sc[n][i] : -INFINITY;
+        }
+      } else if (__ballot(cur.mask != bits || cur.pos > p0 + j0)) {
+#pragma unroll
+        for (int n = 0; n < 2; n++)
+#pragma unroll
+          for (int i = 0; i < 4; i++) {
+            const int mask = __shfl(cur.mask, 16 * n + 4 * grp + i), pos = __shfl(cur.pos, 16 * n + 4 * grp + i);
+            sc[n][i] = ((mask >> qi) & 1) && pos <= qpos ? sc[n][i] : -INFINITY;
+          }
+      }
       float mx = -INFINITY;
 #pragma unroll
       for (int n = 0; n < 2; n++)
 #pragma unroll
-        for (int i = 0; i < 4; i++) {
-          const int j = blk * SP_BLK + 16 * n + 4 * grp + i, e = min(j / a.r.page, nsel - 1);
-          const bool see = j < total && qok && qi >= j0 && qi < j1 && ((l_mask[e] >> qi) & 1) &&
-                           l_u[e] * a.r.page + j % a.r.page <= qpos;
-          sc[n][i] = see ? sc[n][i] : -INFINITY;
-          mx = fmaxf(mx, sc[n][i]);
-        }
+        for (int i = 0; i < 4; i++) mx = fmaxf(mx, sc[n][i]);
       mx = max_xor32(max_xor16(mx)) * a.scale_log2;
       if (__builtin_amdgcn_ballot_w64(mx > m_i + kLazy)) {
         const float mnew = mx > m_i + kLazy ? mx : m_i;
@@ -225,12 +308,37 @@ __global__ __launch_bounds__(SP_THREADS) void sparse_kernel(SparseArgs a) {
         }
       const uint4 pb = make_uint4(pack2<DT>(pv[0][0], pv[0][1]), pack2<DT>(pv[0][2], pv[0][3]),
                                   pack2<DT>(pv[1][0], pv[1][1]), pack2<DT>(pv[1][2], pv[1][3]));
+      if constexpr (!LAST) asm volatile("s_waitcnt vmcnt(%0)" ::"n"(NL) : "memory");  // V; the next K is on its way
+      else asm volatile("s_waitcnt vmcnt(0)" ::: "memory");
+      if (exact) {
+#pragma unroll
+        for (int u = 0; u < NL; u++) {
+          const int row = RPI * u + lane / CPR;
+          const int mask = PG32 ? cur.mask : __shfl(cur.mask, row), pos = PG32 ? cur.pos + row : __shfl(cur.pos, row);
+          if (!mask || pos > p0 + j0)
+            *reinterpret_cast<uint4*>(vs + RPI * u * D + 8 * lane) = make_uint4(0, 0, 0, 0);
+        }
+        asm volatile("s_waitcnt lgkmcnt(0)" ::: "memory");
+      }
 #pragma unroll
       for (int dt = 0; dt < D / 16; dt++) {
         const uint2 lo = lds_tr4(&vs[voff[dt]]), hi = lds_tr4(&vs[voff[dt] + 16 * D]);
         acc[dt] = mfma16<DT>(make_uint4(lo.x, lo.y, hi.x, hi.y), pb, acc[dt]);
       }
-      asm volatile("s_waitcnt lgkmcnt(0)" ::: "memory");  // every fragment is in registers
+      asm volatile("s_waitcnt lgkmcnt(0)" ::: "memory");  // every V fragment is in registers
+      if constexpr (!LAST) {
+        issue(nxt, std::false_type{});
+        cur = nxt;
+      }
+    };
+    // wave w takes blocks w, w + NW, .. of the split (a fixed order)
+    if (blk0 + wave < blk1) {
+      int blk = blk0 + wave;
+      cur = block(blk);
+      issue(cur, std::true_type{});
+      issue(cur, std::false_type{});
+      for (; blk + NW < blk1; blk += NW) consume(blk, std::false_type{});
+      consume(blk, std::true_type{});
     }
 
     // ---- the waves merge: O over each wave's own V slot
@@ -243,27 +351,32 @@ __global__ __launch_bounds__(SP_THREADS) void sparse_kernel(SparseArgs a) {
       s_l[wave][col] = l_i;
     }
     __syncthreads();
+    const int live = min(NW, blk1 - blk0);  // waves that had a block
     bool bad = false;
-    for (int idx = tid; idx < 16 * D / 4; idx += SP_THREADS) {
+    for (int idx = tid; idx < 16 * D / 4; idx += T) {
       const int row = idx / (D / 4), d0 = idx % (D / 4) * 4, i = row / G, g = row % G;
       if (i < j0 || i >= j1) continue;
       float M = -INFINITY, L = 0.f;
       f32x4 O = {0.f, 0.f, 0.f, 0.f};
-#pragma unroll
-      for (int w = 0; w < SP_WAVES; w++) M = fmaxf(M, s_m[w][row]);
-#pragma unroll
-      for (int w = 0; w < SP_WAVES; w++) {
+      for (int w = 0; w < live; w++) M = fmaxf(M, s_m[w][row]);
+      for (int w = 0; w < live; w++) {
         const float f = s_m[w][row] == -INFINITY ? 0.f : __builtin_amdgcn_exp2f(s_m[w][row] - M);
         const f32x4 v = *reinterpret_cast<const f32x4*>(reinterpret_cast<const float*>(s_v[w]) + row * D + d0);
         L += s_l[w][row] * f;
         O += v * f;
       }
-      const float inv = L > 0.f ? 1.f / L : 0.f;
-      O *= inv;
       const float sum = O[0] + O[1] + O[2] + O[3];
       bad |= !(fabsf(sum) < INFINITY);
-      *reinterpret_cast<uint2*>(a.out + ((size_t)(t0 + i) * a.hq + (size_t)hk * G + g) * D + d0) =
-          make_uint2(pack2<DT>(O[0], O[1]), pack2<DT>(O[2], O[3]));
+      if (a.splits == 1) {
+        const float inv = L > 0.f ? 1.f / L : 0.f;
+        O *= inv;
+        *reinterpret_cast<uint2*>(a.out + ((size_t)(t0 + i) * a.hq + (size_t)hk * G + g) * D + d0) =
+            make_uint2(pack2<DT>(O[0], O[1]), pack2<DT>(O[2], O[3]));
+      } else {
+        float* rec = a.partial + (((size_t)pair * a.splits + split) * a.tt * G + row) * (D + 4);
+        st_agent4(rec + d0, make_float4(O[0], O[1], O[2], O[3]));
+        if (d0 == 0) st_agent4(rec + D, make_float4(M, L, 0.f, 0.f));
+      }
     }
     const int again = __syncthreads_or(bad);
     if (!exact) {
@@ -277,17 +390,118 @@ __global__ __launch_bounds__(SP_THREADS) void sparse_kernel(SparseArgs a) {
       j1++;
     }
   }
+  if (a.splits == 1) return;
+
+  // ---- the splits meet in the workgroup that arrives last: a thread takes 4
+  // dims of one row over every SG-th split, 8 records in flight, and the SG
+  // parts meet in LDS (a fixed order)
+  if (!arrive_last(&a.tickets[pair], a.splits)) return;
+  constexpr int MU = 8;
+  const int rows = nt * G, items = rows * (D / 4);
+  const int SG = items * 2 <= T ? T / items : 1;
+  f32x4* const so = reinterpret_cast<f32x4*>(&s_v[0][0]);
+  float2* const sml = reinterpret_cast<float2*>(&s_k[0][0]);
+  for (int item0 = 0; item0 < items; item0 += T) {  // (one turn where SG > 1)
+    const int item = SG > 1 ? tid % items : item0 + tid, j = SG > 1 ? tid / items : 0;
+    const int row = item / (D / 4), d0 = item % (D / 4) * 4;
+    float M = -INFINITY, L = 0.f;
+    f32x4 O = {0.f, 0.f, 0.f, 0.f};
+    const bool work = item < items && j < SG;
+    if (work) {
+      const float* base = a.partial + ((size_t)pair * a.splits * a.tt * G + row) * (D + 4);
+      const size_t next = (size_t)a.tt * G * (D + 4);
+      for (int s0 = j; s0 < a.splits; s0 += SG * MU) {
+        float4 ml[MU], ov[MU];
+#pragma unroll
+        for (int u = 0; u < MU; u++) {
+          ml[u] = make_float4(-INFINITY, 0.f, 0.f, 0.f);
+          ov[u] = make_float4(0.f, 0.f, 0.f, 0.f);
+          if (s0 + u * SG < a.splits) {
+            ml[u] = ld_agent4(base + (size_t)(s0 + u * SG) * next + D);
+            ov[u] = ld_agent4(base + (size_t)(s0 + u * SG) * next + d0);
+          }
+        }
+        float mb = M;
+#pragma unroll
+        for (int u = 0; u < MU; u++) mb = fmaxf(mb, ml[u].x);
+        const float f0 = M == -INFINITY ? 0.f : __builtin_amdgcn_exp2f(M - mb);
+        L *= f0;
+        O *= f0;
+#pragma unroll
+        for (int u = 0; u < MU; u++) {
+          const float f = ml[u].x == -INFINITY ? 0.f : __builtin_amdgcn_exp2f(ml[u].x - mb);
+          L += ml[u].y * f;
+          O += f32x4{ov[u].x, ov[u].y, ov[u].z, ov[u].w} * f;
+        }
+        M = mb;
+      }
+    }
+    if (SG > 1) {
+      if (work) {
+        so[j * items + item] = O;
+        if (d0 == 0) sml[j * 16 + row] = make_float2(M, L);
+      }
+      __syncthreads();
+      if (!work || j > 0) return;
+      float mb = -INFINITY;
+      for (int u = 0; u < SG; u++) mb = fmaxf(mb, sml[u * 16 + row].x);
+      L = 0.f;
+      O = f32x4{0.f, 0.f, 0.f, 0.f};
+      for (int u = 0; u < SG; u++) {
+        const float2 v = sml[u * 16 + row];
+        const float f = v.x == -INFINITY ? 0.f : __builtin_amdgcn_exp2f(v.x - mb);
+        L += v.y * f;
+        O += so[u * items + item] * f;
+      }
+    }
+    if (work) {
+      const float inv = L > 0.f ? 1.f / L : 0.f;
+      O *= inv;
+      *reinterpret_cast<uint2*>(a.out + ((size_t)(t0 + row / G) * a.hq + (size_t)hk * G + row % G) * D + d0) =
+          make_uint2(pack2<DT>(O[0], O[1]), pack2<DT>(O[2], O[3]));
+    }
+  }
+}
+
+// Tiles, rows per tile and splits of a call.
+struct SparsePlan {
+  long long tiles;
+  int tt, splits, waves;
+};
+static SparsePlan sparse_plan(bool ragged, int rows, int batch, int hkv, int G, int page, int top) {
+  SparsePlan p;
+  p.tt = ragged ? 16 / G : 1;
+  if (p.tt > SP_MAX_ENTRIES / top) p.tt = SP_MAX_ENTRIES / top;
+  p.tiles = ragged ? (long long)rows / p.tt + batch : rows;
+  if (p.tiles > rows) p.tiles = rows;
+  const long long pairs = p.tiles * hkv, blocks = ((long long)p.tt * top * page + SP_BLK - 1) / SP_BLK;
+  long long sp = SP_TARGET_WG / pairs;
+  if (sp > blocks / SP_MIN_BLOCKS) sp = blocks / SP_MIN_BLOCKS;
+  if (pairs > kMaxTickets || sp < 1) sp = 1;
+  p.splits = (int)sp;
+  p.waves = pairs * sp > SP_TARGET_WG ? 4 : 8;
+  return p;
 }
 
 }  // namespace yr
 
 using namespace yr;
 
+extern "C" size_t yr_hip_gqa_sparse_workspace(int rows, int batch, int ragged, int hq, int hkv, int d, int page_size,
+                                              int top_pages) {
+  if (rows <= 0 || batch <= 0 || hkv <= 0 || hq < hkv || hq % hkv || hq / hkv > 16 || page_size <= 0 || top_pages < 1 ||
+      top_pages > SP_MAX_ENTRIES || d <= 0)
+    return 0;
+  const SparsePlan p = sparse_plan(ragged != 0, rows, batch, hkv, hq / hkv, page_size, top_pages);
+  if (p.splits == 1) return 0;
+  return kTicketBytes + (size_t)p.tiles * hkv * p.splits * p.tt * (hq / hkv) * (d + 4) * sizeof(float);
+}
+
 extern "C" int yr_hip_gqa_sparse_paged(const void* q, const void* k_cache, const void* v_cache,
                                        const int32_t* qo_indptr, const int32_t* kv_indptr, const int32_t* kv_indices,
                                        int n_indices, const int32_t* kv_len, const int32_t* pages, void* out, int rows,
                                        int batch, int hq, int hkv, int d, int page_size, int num_pages, int top_pages,
-                                       int dtype, void* stream) {
+                                       int dtype, void* workspace, size_t workspace_bytes, void* stream) {
   const char* nm = "yr_hip_gqa_sparse_paged";
   SparseArgs a;
   a.r = Ragged{qo_indptr, kv_indptr, kv_indices, kv_len, rows, batch, page_size, n_indices, num_pages};
@@ -308,20 +522,28 @@ extern "C" int yr_hip_gqa_sparse_paged(const void* q, const void* k_cache, const
   a.hq = hq;
   a.hkv = hkv;
   a.top = top_pages;
-  a.tt = qo_indptr ? 16 / G : 1;
-  if (a.tt > SP_MAX_ENTRIES / top_pages) a.tt = SP_MAX_ENTRIES / top_pages;
-  if ((long long)a.tt * top_pages * page_size > 0x7fffffff)
+  const SparsePlan p = sparse_plan(qo_indptr != nullptr, rows, batch, hkv, G, page_size, top_pages);
+  a.tt = p.tt;
+  a.splits = p.splits;
+  if ((long long)p.tt * top_pages * page_size > 0x7fffffff)
     return fail(YR_E_INVALID, "%s: %d pages of %d tokens a row are too many", nm, top_pages, page_size);
+  if (p.tiles * hkv * p.splits > 0x7fffffff) return fail(YR_E_INVALID, "%s: too many rows", nm);
+  if ((long long)hkv * d * 2 * SP_BLK > 0x7fffffff) return fail(YR_E_INVALID, "%s: too many heads", nm);
+  const size_t need = yr_hip_gqa_sparse_workspace(rows, batch, qo_indptr != nullptr, hq, hkv, d, page_size, top_pages);
+  if (need > workspace_bytes || (need && !workspace))
+    return fail(YR_E_WORKSPACE, "%s: workspace %zu < %zu", nm, workspace_bytes, need);
+  a.tickets = (uint32_t*)workspace;
+  a.partial = need ? (float*)((char*)workspace + kTicketBytes) : nullptr;
   a.scale_log2 = kLog2e / sqrtf((float)d);
-  long long tiles = qo_indptr ? (long long)rows / a.tt + batch : rows;
-  if (tiles > rows) tiles = rows;
-  if (tiles * hkv > 0x7fffffff) return fail(YR_E_INVALID, "%s: too many rows", nm);
-  a.tiles = (int)tiles;
+  const unsigned grid = (unsigned)(p.tiles * hkv * p.splits);
+  const bool pg32 = page_size % SP_BLK == 0;
   hipStream_t st = (hipStream_t)stream;
-#define YR_SP(DT_, D_)                                                                                             \
-  if (dtype == DT_ && d == D_)                                                                                     \
-    hipLaunchKernelGGL((sparse_kernel<DT_, D_>), dim3((unsigned)(tiles * hkv)), dim3(SP_THREADS), 0, st, a);
-  YR_SP(DT_F16, 64) YR_SP(DT_F16, 128) YR_SP(DT_BF16, 64) YR_SP(DT_BF16, 128)
+#define YR_SP(DT_, D_, W_, P_)                                                                              \
+  if (dtype == DT_ && d == D_ && p.waves == W_ && pg32 == P_)                                               \
+    hipLaunchKernelGGL((sparse_kernel<DT_, D_, W_, P_>), dim3(grid), dim3(W_ * kWave), 0, st, a);
+#define YR_SP2(DT_, D_) YR_SP(DT_, D_, 4, false) YR_SP(DT_, D_, 4, true) YR_SP(DT_, D_, 8, false) YR_SP(DT_, D_, 8, true)
+  YR_SP2(DT_F16, 64) YR_SP2(DT_F16, 128) YR_SP2(DT_BF16, 64) YR_SP2(DT_BF16, 128)
+#undef YR_SP2
 #undef YR_SP
   YR_CHECK_LAUNCH(nm);
   return YR_OK;

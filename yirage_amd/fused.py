@@ -369,10 +369,12 @@ def gqa_sparse_paged(q, k_cache, v_cache, kv_indptr, kv_indices, kv_len, pages, 
     if T == 0:
         return out
     with _on(q.device):
+        nb = lib().yr_hip_gqa_sparse_workspace(T, batch, qo_indptr is not None, hq, hkv, D, page, pages.shape[2])
+        ws = _scratch(nb, q.device)
         check(lib().yr_hip_gqa_sparse_paged(
             _at(q), _at(k_cache), _at(v_cache), _at(qo_indptr), _at(kv_indptr), _at(kv_indices), kv_indices.numel(),
             _at(kv_len), _at(pages), _at(out), T, batch, hq, hkv, D, page, P, pages.shape[2], dt,
-            torch.cuda.current_stream(q.device).cuda_stream), "gqa_sparse_paged")
+            _at(ws), nb, torch.cuda.current_stream(q.device).cuda_stream), "gqa_sparse_paged")
     return out
 
 
