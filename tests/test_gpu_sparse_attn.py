@@ -70,6 +70,9 @@ def _run(b, q, k, v, pages, **kw):
     ([400], [37], 2, 2, 64, 32, 5), ([260, 300], [20, 1], 16, 1, 64, 64, 3),  # 16 rows, one row
     ([300, 1], [50, 1], 7, 1, 128, 24, 8), ([640], [64], 16, 2, 128, 128, 2),
     ([200], [200], 12, 4, 128, 16, 3),                         # a whole prompt
+    ([700, 500], [300, 200], 16, 16, 64, 32, 3), ([400], [330], 16, 8, 128, 24, 4),  # more tiles than CUs
+    ([600], [520], 32, 8, 128, 64, 4), ([450, 300], [430, 290], 40, 8, 64, 16, 5),   # tiles of 16, 12 and 4 rows
+    ([300], [290], 64, 4, 128, 32, 3), ([200, 700], [1, 660], 28, 4, 64, 48, 6),
 ])
 def test_rows(lens, news, hq, hkv, d, page, top, dt):
     print("case", lens[:4], news[:4], hq, hkv, d, page, top, dt, flush=True)
@@ -104,23 +107,25 @@ def test_lists_with_what_counts_for_nothing(news, dt):
 
 
 @DTS
-@pytest.mark.parametrize("hq,page", [(2, 32), (8, 16), (4, 24)])
-def test_values_that_other_rows_see(hq, page, dt):
+@pytest.mark.parametrize("hq,page,before,rows,hkv", [(2, 32, 6, 14, 1), (8, 16, 6, 14, 1), (4, 24, 6, 14, 1),
+                                                     (32, 32, 20, 600, 8), (64, 24, 20, 300, 8)])
+def test_values_that_other_rows_see(hq, page, before, rows, hkv, dt):
     """A tile's rows read each other's pages: what a row did not choose or cannot see yet must
     not reach it, not even infinity or NaN."""
-    b = Batch([6 * page + 9], [14], page)
-    q, k, v, gen = _inputs(b, hq, 1, 64, dt, 8)
-    v[b.indices[1], 3, 0, 5] = float("inf")
-    v[b.indices[2], 2, 0, 7] = float("nan")
-    k[b.indices[3], 1, 0, 0] = float("nan")
+    b = Batch([max(before * page + 9, rows)], [rows], page)
+    q, k, v, gen = _inputs(b, hq, hkv, 64, dt, 8)
+    h = hkv - 1
+    v[b.indices[1], 3, h, 5] = float("inf")
+    v[b.indices[2], 2, h, 7] = float("nan")
+    k[b.indices[3], 1, h, 0] = float("nan")
     L = b.lens[0]
-    v[b.indices[(L - 3) // page], (L - 3) % page, 0, 9] = float("-inf")  # the third last token
-    pages = torch.full((b.rows, 1, 4), -1, dtype=torch.int32)
+    v[b.indices[(L - 3) // page], (L - 3) % page, h, 9] = float("-inf")  # the third last token
+    pages = torch.full((b.rows, hkv, 4), -1, dtype=torch.int32)
     for t in range(b.rows):
-        pages[t, 0, 0] = t % 6                    # one of six pages each
-        pages[t, 0, 1] = (L - b.rows + t) // page  # and its own
+        pages[t, :, 0] = t % 6                     # one of six pages each
+        pages[t, :, 1] = (L - b.rows + t) // page  # and its own
     out = _run(b, q, k, v, pages).cpu().double()
-    ref, tol = _reference(b, q, k, v, pages, 1)
+    ref, tol = _reference(b, q, k, v, pages, hkv)
     fin = ref.isfinite()
     assert torch.equal(out.isfinite(), fin)
     assert torch.equal(out.isnan(), ref.isnan())

@@ -57,6 +57,84 @@ __device__ __forceinline__ int v_swz(int row) {
   return D == 128 ? ((row & 7) << 1) | ((row >> 3) & 1) : (row & 3) << 1;
 }
 
+// Union of the lists of rows t0 .. t0 + nt - 1 (positions p0 ..) of kv head hk, in
+// page order: pages l_u, their device ids and the rows that chose them; returns
+// their number.  What counts for nothing (negative, not yet visible, missing,
+// repeated) is left out.  In page order, workgroups that run at the same time
+// pass over the same pages at about the same time, while those are in L2.
+//
+// A table of one mask per page is filled and read back where it fits into the
+// `cells` (even) 16-bit words at `table`, which hold nt * top ints at least.  A
+// single ascending list (a decode step's) needs none; otherwise every entry looks
+// for its like.  The whole workgroup of T.
+template <int T>
+__device__ __forceinline__ int build_union(const SparseArgs& a, const SeqRows& s, int nt, int t0, int p0, int hk,
+                                           uint32_t* table, int cells, int* l_u, int* l_id, uint16_t* l_mask, int* s_cnt) {
+  const int tid = threadIdx.x, lane = tid % kWave, wave = tid / kWave;
+  const int E = nt * a.top;
+  auto entry = [&](int e) __attribute__((always_inline)) -> int {
+    const int i = e / a.top, p = p0 + i;
+    const int u = gptr(a.pages)[((size_t)(t0 + i) * a.hkv + hk) * a.top + e % a.top];
+    return u < 0 || p < 0 || u > p / a.r.page || page_id(a.r, s, u) < 0 ? -1 : u;
+  };
+  // appends the workgroup's entries that are `own`, in thread order
+  int nsel = 0;
+  auto append = [&](bool own, int u, int mask) __attribute__((always_inline)) {
+    const uint64_t bal = __ballot(own);
+    if (lane == 0) s_cnt[wave] = __popcll(bal);
+    __syncthreads();
+    int at = nsel + __popcll(bal & ((1ull << lane) - 1));
+#pragma unroll
+    for (int w = 0; w < T / kWave; w++) {
+      if (w < wave) at += s_cnt[w];
+      nsel += s_cnt[w];
+    }
+    if (own) {
+      l_u[at] = u;
+      l_mask[at] = (uint16_t)mask;
+    }
+    __syncthreads();
+  };
+  const int pmax = p0 + nt - 1, n = pmax < 0 ? 0 : min(pmax / a.r.page + 1, s.npg);
+  if (nt > 1 && n <= cells) {
+    for (int i = tid; i < (n + 1) / 2; i += T) table[i] = 0;
+    __syncthreads();
+    for (int e = tid; e < E; e += T) {
+      const int u = entry(e);
+      if (u >= 0) atomicOr(&table[u / 2], 1u << (e / a.top + 16 * (u % 2)));
+    }
+    __syncthreads();
+    for (int u0 = 0; u0 < n; u0 += T) {
+      const int u = u0 + tid, mask = u < n ? table[u / 2] >> (16 * (u % 2)) & 0xffff : 0;
+      append(mask != 0, u, mask);
+    }
+  } else {
+    int* const s_u = reinterpret_cast<int*>(table);
+    for (int e = tid; e < E; e += T) s_u[e] = entry(e);
+    __syncthreads();
+    bool unordered = false;
+    for (int e = tid; e < E; e += T)
+      if (e % a.top) unordered |= s_u[e] >= 0 && (s_u[e - 1] < 0 || s_u[e] <= s_u[e - 1]);
+    const bool ordered = nt == 1 && !__syncthreads_or(unordered);
+    for (int e0 = 0; e0 < E; e0 += T) {
+      const int e = e0 + tid, u = e < E ? s_u[e] : -1;
+      bool own = u >= 0;
+      int mask = own ? 1 << (e / a.top) : 0;
+      if (own && !ordered)
+        for (int j = 0; j < E; j++)
+          if (s_u[j] == u) {
+            mask |= 1 << (j / a.top);
+            if (j < e) own = false;
+          }
+      append(own, u, mask);
+    }
+  }
+  nsel = __builtin_amdgcn_readfirstlane(nsel);
+  for (int e = tid; e < nsel; e += T) l_id[e] = page_id(a.r, s, l_u[e]);
+  __syncthreads();
+  return nsel;
+}
+
 // NW waves; PG32: pages are a multiple of 32 tokens, so a block lies in one page
 // and its address is uniform (else the lanes work out one token's each).
 //
@@ -76,7 +154,6 @@ __global__ __launch_bounds__(NW * kWave) void sparse_kernel(SparseArgs a) {
   __shared__ float s_m[NW][16], s_l[NW][16];
   __shared__ int s_cnt[NW], s_tile[2];
   static_assert(SP_MAX_ENTRIES * 4 <= (int)sizeof(s_k), "the entries fit where K goes later");
-  int* const s_u = reinterpret_cast<int*>(&s_k[0][0]);  // page of each entry, -1: counts for nothing
   const int tid = threadIdx.x, lane = tid % kWave;
   const int wave = __builtin_amdgcn_readfirstlane(tid / kWave);
   const int split = blockIdx.x % a.splits, pair = blockIdx.x / a.splits;
@@ -105,65 +182,8 @@ __global__ __launch_bounds__(NW * kWave) void sparse_kernel(SparseArgs a) {
     if (qok) qf[st] = ldg16(a.q + ((size_t)(t0 + qi) * a.hq + (size_t)hk * G + qg) * D + 32 * st + 8 * grp);
   }
 
-  // ---- union of the rows' lists.  Ascending lists (the usual ones) are
-  // searched by halving, others entry by entry.
-  const int E = nt * a.top;
-  for (int e = tid; e < E; e += T) {
-    const int i = e / a.top, p = p0 + i;
-    int u = gptr(a.pages)[((size_t)(t0 + i) * a.hkv + hk) * a.top + e % a.top];
-    if (u < 0 || p < 0 || u > p / a.r.page || page_id(a.r, s, u) < 0) u = -1;
-    s_u[e] = u;
-  }
-  __syncthreads();
-  bool unordered = false;
-  for (int e = tid; e < E; e += T)
-    if (e % a.top) unordered |= s_u[e] >= 0 && (s_u[e - 1] < 0 || s_u[e] <= s_u[e - 1]);
-  const bool ordered = !__syncthreads_or(unordered);
-  int nsel = 0;
-  for (int e0 = 0; e0 < E; e0 += T) {
-    const int e = e0 + tid, mine = e / a.top;
-    const int u = e < E ? s_u[e] : -1;
-    bool own = u >= 0;
-    int mask = own ? 1 << mine : 0;
-    if (own && ordered) {
-      for (int i = 0; i < nt; i++) {
-        if (i == mine) continue;
-        const int* li = s_u + i * a.top;
-        int lo = 0, hi = a.top;  // first entry that is u, larger or none
-        while (lo < hi) {
-          const int mid = (lo + hi) / 2;
-          if ((unsigned)li[mid] < (unsigned)u) lo = mid + 1;
-          else hi = mid;
-        }
-        if (lo < a.top && li[lo] == u) {
-          mask |= 1 << i;
-          if (i < mine) own = false;
-        }
-      }
-    } else if (own) {
-      for (int j = 0; j < E; j++)
-        if (s_u[j] == u) {
-          mask |= 1 << (j / a.top);
-          if (j < e) own = false;
-        }
-    }
-    const uint64_t bal = __ballot(own);
-    if (lane == 0) s_cnt[wave] = __popcll(bal);
-    __syncthreads();
-    int at = nsel + __popcll(bal & ((1ull << lane) - 1));
-#pragma unroll
-    for (int w = 0; w < NW; w++) {
-      if (w < wave) at += s_cnt[w];
-      nsel += s_cnt[w];
-    }
-    if (own) {
-      l_u[at] = u;
-      l_id[at] = page_id(a.r, s, u);
-      l_mask[at] = (uint16_t)mask;
-    }
-    __syncthreads();
-  }
-  nsel = __builtin_amdgcn_readfirstlane(nsel);
+  const int nsel = build_union<T>(a, s, nt, t0, p0, hk, reinterpret_cast<uint32_t*>(&s_k[0][0]), (int)sizeof(s_k) / 2, l_u,
+                                  l_id, l_mask, s_cnt);
   const int total = nsel * a.r.page;  // tokens of the union's pages
   const int nblk = (total + SP_BLK - 1) / SP_BLK;
   const int per = (nblk + a.splits - 1) / a.splits;
@@ -463,13 +483,245 @@ __global__ __launch_bounds__(NW * kWave) void sparse_kernel(SparseArgs a) {
   }
 }
 
+// Many rows: four groups of 16 query rows (a wave each, the rows of up to
+// 4 (16 / G) tokens) share one union.  Every 64-token block of it is loaded once
+// by the whole workgroup, the next one while this one is worked on, and a wave
+// skips the blocks that none of its rows chose.  Neighbouring rows choose much
+// alike (777 rows of 16 pages: 36 pages for 4 rows, 65 for 16).
+//
+// Lane l of every wave knows token l of a block: its row in the cache and which
+// rows of the tile see it.  A row's 64 tokens are then one ballot.
+// PG64: pages are a multiple of 64 tokens, a block lies in one page and its
+// address is uniform.
+constexpr int SW_BLK = 64, SW_WAVES = 4;
+
+template <int DT, int D, bool PG64>
+__global__ __launch_bounds__(SW_WAVES * kWave, 2) void sparse_wide_kernel(SparseArgs a) {
+  constexpr int T = SW_WAVES * kWave;
+  constexpr int RPI = T * 8 / D;    // rows per load instruction of the workgroup
+  constexpr int NL = SW_BLK / RPI;  // such loads per operand of a block
+  constexpr int CPR = D / 8;        // chunks per row
+  // separate objects: reads of one block do not wait for the loads that fill the other
+  __shared__ __attribute__((aligned(16))) uint16_t s_k0[SW_BLK * D], s_k1[SW_BLK * D];
+  __shared__ __attribute__((aligned(16))) uint16_t s_v0[SW_BLK * D], s_v1[SW_BLK * D];
+  __shared__ int l_u[SP_MAX_ENTRIES], l_id[SP_MAX_ENTRIES];  // union: page, device page id, rows
+  __shared__ uint16_t l_mask[SP_MAX_ENTRIES];
+  __shared__ int s_cnt[SW_WAVES], s_tile[2], s_bad;
+  static_assert(SP_MAX_ENTRIES * 4 <= (int)sizeof(s_k0), "the entries fit where K goes later");
+  const int tid = threadIdx.x, lane = tid % kWave;
+  const int wave = __builtin_amdgcn_readfirstlane(tid / kWave);
+  const int hk = blockIdx.x % a.hkv, tile = blockIdx.x / a.hkv;
+  const int G = a.hq / a.hkv, tb = 16 / G, col = lane % 16, grp = lane / 16;
+
+  if (tid == 0) {
+    find_tile(a.r, tile, a.tt, s_tile);
+    s_bad = 0;
+  }
+  __syncthreads();
+  const int b = s_tile[0], i0 = s_tile[1];
+  if (b >= a.r.batch) return;
+  const SeqRows s = seq_rows(a.r, b);
+  const int nt = min(a.tt, s.n - i0), t0 = s.row0 + i0, p0 = s.len - s.n + i0;  // rows, first row, its position
+  const int pmax = p0 + nt - 1;
+
+  // ---- this lane's query row: column col = row qi of the tile, head qg
+  const int qr = col / G, qi = wave * tb + qr, qg = col % G;
+  const bool qok = qr < tb && qi < nt;
+  uint4 qf[D / 32];
+#pragma unroll
+  for (int st = 0; st < D / 32; st++) {
+    qf[st] = make_uint4(0, 0, 0, 0);
+    if (qok) qf[st] = ldg16(a.q + ((size_t)(t0 + qi) * a.hq + (size_t)hk * G + qg) * D + 32 * st + 8 * grp);
+  }
+  const int nsel = build_union<T>(a, s, nt, t0, p0, hk, reinterpret_cast<uint32_t*>(s_k0), SW_BLK * D, l_u, l_id, l_mask,
+                                  s_cnt);
+  const int total = nsel * a.r.page, nblk = (total + SW_BLK - 1) / SW_BLK;
+  const int step_e = SW_BLK / a.r.page, step_s = SW_BLK % a.r.page;  // entries and slots from block to block
+
+  uint32_t koff[D / 32], voff[D / 16];
+#pragma unroll
+  for (int st = 0; st < D / 32; st++) koff[st] = col * D + 8 * ((4 * st + grp) ^ k_swz<D>(col));
+  {
+    const int r0 = 4 * grp + col / 4, qc = (col % 4) / 2, qh = 4 * (col % 2);
+#pragma unroll
+    for (int dt = 0; dt < D / 16; dt++) voff[dt] = r0 * D + 8 * ((2 * dt + qc) ^ v_swz<D>(r0)) + qh;
+  }
+  const size_t tok_stride = (size_t)a.hkv * D;
+
+  // Rows `bits` of the tile; exact: one row, with what it does not see zeroed (see sparse_kernel)
+  auto pass = [&](int bits, bool exact) __attribute__((always_inline)) {
+    const int mine = bits & (((1 << tb) - 1) << (wave * tb));  // this wave's rows
+    float m_i = -INFINITY, l_i = 0.f;
+    f32x4 acc[D / 16];
+#pragma unroll
+    for (int dt = 0; dt < D / 16; dt++) acc[dt] = f32x4{0.f, 0.f, 0.f, 0.f};
+    int e = lane / a.r.page, slot = lane % a.r.page, at = lane;  // this lane's token of the block to load
+    int vis = 0, vis_next = 0;  // rows that see this lane's token of the block at hand and of the next one
+    size_t off = 0;
+    int over = 0;  // (PG64) tokens of the block that some row of the tile sees, less one
+    auto inform = [&]() __attribute__((always_inline)) {
+      const int ec = min(e, nsel - 1);
+      int u = l_u[ec], id = l_id[ec], mask = l_mask[ec];
+      if constexpr (PG64) {
+        u = __builtin_amdgcn_readfirstlane(u);
+        id = __builtin_amdgcn_readfirstlane(id);
+        const int slot0 = __builtin_amdgcn_readfirstlane(slot);
+        over = pmax - (u * a.r.page + slot0);
+        off = ((size_t)id * a.r.page + slot0) * tok_stride + (size_t)hk * D;
+      } else {
+        off = ((size_t)id * a.r.page + min(slot, pmax - u * a.r.page)) * tok_stride + (size_t)hk * D;
+      }
+      // rows at positions p0 + i >= this token's
+      vis_next = at < total ? mask & bits & (-1 << min(max(u * a.r.page + slot - p0, 0), 16)) : 0;
+      e += step_e;
+      slot += step_s;
+      if (slot >= a.r.page) {
+        slot -= a.r.page;
+        e++;
+      }
+      at += SW_BLK;
+    };
+    auto issue = [&](uint16_t* kd, uint16_t* vd) __attribute__((always_inline)) {
+#pragma unroll
+      for (int u = 0; u < NL; u++) {
+        const int row = RPI * u + tid / CPR, c = lane % CPR;
+        // a wave's part of the instruction: 512 / D rows from here on
+        const int first = (RPI * u + wave * (512 / D)) * D, ck = 8 * (c ^ k_swz<D>(row)), cv = 8 * (c ^ v_swz<D>(row));
+        if (PG64 && over >= SW_BLK - 1) {  // (uniform)
+          const uint32_t o = (uint32_t)row * (uint32_t)tok_stride;
+          lds_load16(reinterpret_cast<const uint16_t*>(reinterpret_cast<const char*>(a.kc + off) + 2u * (o + ck)), kd + first);
+          lds_load16(reinterpret_cast<const uint16_t*>(reinterpret_cast<const char*>(a.vc + off) + 2u * (o + cv)), vd + first);
+        } else {
+          size_t o;
+          if constexpr (PG64) o = off + (long long)min(row, over) * (long long)tok_stride;  // (maybe before the block)
+          else o = (size_t)(uint32_t)__shfl((int)(off >> 32), row) << 32 | (uint32_t)__shfl((int)(uint32_t)off, row);
+          lds_load16(a.kc + o + ck, kd + first);
+          lds_load16(a.vc + o + cv, vd + first);
+        }
+      }
+    };
+    auto step = [&](int blk, const uint16_t* ks, uint16_t* vs, uint16_t* kn, uint16_t* vn) __attribute__((always_inline)) {
+      asm volatile("s_waitcnt vmcnt(0) lgkmcnt(0)" ::: "memory");
+      __builtin_amdgcn_s_barrier();  // the block has landed for every wave, and the one before is read out
+      asm volatile("" ::: "memory");
+      vis = vis_next;
+      if (blk + 1 < nblk) {
+        inform();
+        issue(kn, vn);
+      }
+      if (exact) {  // (rare)
+        asm volatile("s_waitcnt vmcnt(0)" ::: "memory");
+#pragma unroll
+        for (int u = 0; u < NL; u++)
+          if (!__shfl(vis, RPI * u + tid / CPR)) *reinterpret_cast<uint4*>(vs + RPI * u * D + 8 * tid) = make_uint4(0, 0, 0, 0);
+        __syncthreads();
+      }
+      if (!__ballot((vis & mine) != 0)) return;
+      const bool whole = !__ballot((vis & mine) != mine);
+      f32x4 sc[4];
+#pragma unroll
+      for (int n = 0; n < 4; n++) sc[n] = f32x4{0.f, 0.f, 0.f, 0.f};
+#pragma unroll
+      for (int st = 0; st < D / 32; st++)
+#pragma unroll
+        for (int n = 0; n < 4; n++)
+          sc[n] = mfma16<DT>(*reinterpret_cast<const uint4*>(&ks[koff[st] + 16 * n * D]), qf[st], sc[n]);
+      if (!whole) {
+        uint64_t seen = 0;  // tokens that this lane's row sees
+#pragma unroll
+        for (int i = 0; i < 4; i++) {
+          const uint64_t row = __ballot((vis >> (wave * tb + i)) & 1);
+          seen = qr == i ? row : seen;
+        }
+        const uint32_t lo = (uint32_t)seen >> (4 * grp), hi = (uint32_t)(seen >> 32) >> (4 * grp);
+#pragma unroll
+        for (int n = 0; n < 4; n++)
+#pragma unroll
+          for (int i = 0; i < 4; i++) sc[n][i] = (n < 2 ? lo : hi) >> (16 * (n % 2) + i) & 1 ? sc[n][i] : -INFINITY;
+      }
+      float mx = -INFINITY;
+#pragma unroll
+      for (int n = 0; n < 4; n++)
+#pragma unroll
+        for (int i = 0; i < 4; i++) mx = fmaxf(mx, sc[n][i]);
+      mx = max_xor32(max_xor16(mx)) * a.scale_log2;
+      if (__builtin_amdgcn_ballot_w64(mx > m_i + kLazy)) {
+        const float mnew = mx > m_i + kLazy ? mx : m_i;
+        const float alpha = m_i == -INFINITY ? 0.f : __builtin_amdgcn_exp2f(m_i - mnew);
+        m_i = mnew;
+        l_i *= alpha;
+#pragma unroll
+        for (int dt = 0; dt < D / 16; dt++) acc[dt] *= alpha;
+      }
+      const float mref = (m_i == -INFINITY ? 0.f : m_i) - kPBias<DT>;
+      uint4 pb[2];
+#pragma unroll
+      for (int m = 0; m < 2; m++) {
+        float pv[2][4];
+#pragma unroll
+        for (int n = 0; n < 2; n++)
+#pragma unroll
+          for (int i = 0; i < 4; i++) {
+            pv[n][i] = __builtin_amdgcn_exp2f(fmaf(sc[2 * m + n][i], a.scale_log2, -mref));
+            l_i += pv[n][i];
+          }
+        pb[m] = make_uint4(pack2<DT>(pv[0][0], pv[0][1]), pack2<DT>(pv[0][2], pv[0][3]), pack2<DT>(pv[1][0], pv[1][1]),
+                           pack2<DT>(pv[1][2], pv[1][3]));
+      }
+#pragma unroll
+      for (int m = 0; m < 2; m++)
+#pragma unroll
+        for (int dt = 0; dt < D / 16; dt++) {
+          const uint2 lo = lds_tr4(&vs[voff[dt] + 32 * m * D]), hi = lds_tr4(&vs[voff[dt] + (32 * m + 16) * D]);
+          acc[dt] = mfma16<DT>(make_uint4(lo.x, lo.y, hi.x, hi.y), pb[m], acc[dt]);
+        }
+    };
+    if (nblk > 0) {
+      inform();
+      issue(s_k0, s_v0);
+    }
+    for (int blk = 0; blk < nblk; blk += 2) {
+      step(blk, s_k0, s_v0, s_k1, s_v1);
+      if (blk + 1 < nblk) step(blk + 1, s_k1, s_v1, s_k0, s_v0);
+    }
+    l_i = add_xor32(add_xor16(l_i));
+    const float inv = l_i > 0.f ? 1.f / l_i : 0.f;
+    float sum = 0.f;
+    if (qok && (mine >> qi & 1)) {
+      uint16_t* const o = a.out + ((size_t)(t0 + qi) * a.hq + (size_t)hk * G + qg) * D + 4 * grp;
+#pragma unroll
+      for (int dt = 0; dt < D / 16; dt++) {
+        const f32x4 v = acc[dt] * inv;
+        sum += v[0] + v[1] + v[2] + v[3];
+        *reinterpret_cast<uint2*>(o + 16 * dt) = make_uint2(pack2<DT>(v[0], v[1]), pack2<DT>(v[2], v[3]));
+      }
+    }
+    if (!exact && !(fabsf(sum) < INFINITY)) atomicOr(&s_bad, 1 << qi);
+    __syncthreads();  // the blocks' slots are free again
+  };
+  pass((1 << nt) - 1, false);
+  for (int bad = s_bad; bad; bad &= bad - 1) pass(bad & -bad, true);
+}
+
 // Tiles, rows per tile and splits of a call.
 struct SparsePlan {
   long long tiles;
   int tt, splits, waves;
+  bool wide;
 };
 static SparsePlan sparse_plan(bool ragged, int rows, int batch, int hkv, int G, int page, int top) {
   SparsePlan p;
+  // four groups of rows to a tile where that leaves a workgroup per CU and the lists fit
+  const int wide_tt = SW_WAVES * (16 / G);
+  p.wide = ragged && G >= 4 && wide_tt * top <= SP_MAX_ENTRIES && (long long)rows / wide_tt * hkv >= SP_TARGET_WG;
+  if (p.wide) {
+    p.tt = wide_tt;
+    p.tiles = (long long)rows / p.tt + batch;
+    if (p.tiles > rows) p.tiles = rows;
+    p.splits = 1;
+    p.waves = SW_WAVES;
+    return p;
+  }
   p.tt = ragged ? 16 / G : 1;
   if (p.tt > SP_MAX_ENTRIES / top) p.tt = SP_MAX_ENTRIES / top;
   p.tiles = ragged ? (long long)rows / p.tt + batch : rows;
@@ -536,12 +788,17 @@ extern "C" int yr_hip_gqa_sparse_paged(const void* q, const void* k_cache, const
   a.partial = need ? (float*)((char*)workspace + kTicketBytes) : nullptr;
   a.scale_log2 = kLog2e / sqrtf((float)d);
   const unsigned grid = (unsigned)(p.tiles * hkv * p.splits);
-  const bool pg32 = page_size % SP_BLK == 0;
+  const bool pg32 = page_size % SP_BLK == 0 && !p.wide;
   hipStream_t st = (hipStream_t)stream;
 #define YR_SP(DT_, D_, W_, P_)                                                                              \
-  if (dtype == DT_ && d == D_ && p.waves == W_ && pg32 == P_)                                               \
+  if (dtype == DT_ && d == D_ && !p.wide && p.waves == W_ && pg32 == P_)                                    \
     hipLaunchKernelGGL((sparse_kernel<DT_, D_, W_, P_>), dim3(grid), dim3(W_ * kWave), 0, st, a);
-#define YR_SP2(DT_, D_) YR_SP(DT_, D_, 4, false) YR_SP(DT_, D_, 4, true) YR_SP(DT_, D_, 8, false) YR_SP(DT_, D_, 8, true)
+#define YR_SP2(DT_, D_)                                                                                     \
+  if (dtype == DT_ && d == D_ && p.wide && page_size % SW_BLK == 0)                                         \
+    hipLaunchKernelGGL((sparse_wide_kernel<DT_, D_, true>), dim3(grid), dim3(SW_WAVES * kWave), 0, st, a);  \
+  if (dtype == DT_ && d == D_ && p.wide && page_size % SW_BLK != 0)                                         \
+    hipLaunchKernelGGL((sparse_wide_kernel<DT_, D_, false>), dim3(grid), dim3(SW_WAVES * kWave), 0, st, a); \
+  YR_SP(DT_, D_, 4, false) YR_SP(DT_, D_, 4, true) YR_SP(DT_, D_, 8, false) YR_SP(DT_, D_, 8, true)
   YR_SP2(DT_F16, 64) YR_SP2(DT_F16, 128) YR_SP2(DT_BF16, 64) YR_SP2(DT_BF16, 128)
 #undef YR_SP2
 #undef YR_SP
