@@ -779,7 +779,8 @@ extern "C" int yr_hip_gqa_sparse_paged(const void* q, const void* k_cache, const
   a.splits = p.splits;
   if ((long long)p.tt * top_pages * page_size > 0x7fffffff)
     return fail(YR_E_INVALID, "%s: %d pages of %d tokens a row are too many", nm, top_pages, page_size);
-  if (p.tiles * hkv * p.splits > 0x7fffffff) return fail(YR_E_INVALID, "%s: too many rows", nm);
+  if ((long long)rows * hkv > 0x7fffffff || p.tiles * hkv * p.splits > 0x7fffffff)
+    return fail(YR_E_INVALID, "%s: too many rows", nm);
   if ((long long)hkv * d * 2 * SP_BLK > 0x7fffffff) return fail(YR_E_INVALID, "%s: too many heads", nm);
   const size_t need = yr_hip_gqa_sparse_workspace(rows, batch, qo_indptr != nullptr, hq, hkv, d, page_size, top_pages);
   if (need > workspace_bytes || (need && !workspace))

@@ -8,7 +8,6 @@ per-device cache that is zero-filled once at allocation.
 """
 from __future__ import annotations
 
-import contextlib
 import ctypes
 import struct
 from typing import NamedTuple
@@ -182,47 +181,60 @@ def argmax(x, n_valid: int | None = None, out=None):
 # Operators on a ragged batch: sequence b owns the rows qo_indptr[b] ..
 # qo_indptr[b + 1) of the new tokens (qo_indptr None: one row each), the pages
 # kv_indices[kv_indptr[b] .. kv_indptr[b + 1]) and kv_len[b] tokens, the new ones
-# last.  Their kernels run on the tensors' device and its current stream.
+# last.  Their kernels run on the tensors' device and its current stream.  A
+# decode step's calls are as short as their host side, so the checks below read
+# each property once.
 _TICKET_BYTES = 65536  # what a workspace has zeroed at rest
 _DTYPE_ALL = {**_TORCH_DT, torch.float32: _lib.DTYPE_F32}
+_Strides7 = ctypes.c_int64 * 7
 
 
 def _fail(msg: str):
     raise _lib.YirageHipError(f"hip backend: {msg}")
 
 
-def _on(device):
-    """Makes the tensors' device current for a launch."""
-    if torch.cuda.current_device() == device.index:
-        return contextlib.nullcontext()
-    return torch.cuda.device(device)
-
-
-def _one_device(x, *others):
-    dev = x.device
-    if dev.type != "cuda":
+def _one_device(*ts) -> int:
+    """Index of the one GPU that the tensors (or None) live on."""
+    index = ts[0].get_device()
+    for t in ts:
+        if t is not None and t.get_device() != index:
+            _fail(f"tensors on different devices ({t.device}, {ts[0].device})")
+    if index < 0:
         _fail("tensors must live on the GPU")
-    for t in others:
-        if t is not None and t.device != dev:
-            _fail(f"tensors on different devices ({t.device}, {dev})")
+    return index
 
 
-def _dense(**ts):
-    for name, t in ts.items():
+def _dense(*ts):
+    for t in ts:
         if t is not None and not t.is_contiguous():
-            _fail(f"{name} must be contiguous (row-major)")
+            _fail(f"caches, tables and inputs of shape {tuple(t.shape)} must be contiguous (row-major)")
 
 
-def _scratch(nbytes: int, device):
+def _launch(index: int, fn, what: str, *args):
+    """fn(*args) with the tensors' device current."""
+    if torch.cuda.current_device() == index:
+        rc = fn(*args)
+    else:
+        with torch.cuda.device(index):
+            rc = fn(*args)
+    if rc != _lib.YR_OK:
+        check(rc, what)
+
+
+def _scratch(nbytes: int, device, stream: int):
     """workspace(), but a captured call owns its scratch: the graph's pool keeps it,
     tickets are cleared at every replay, and no two graphs meet in it."""
     if nbytes == 0:
         return None
-    if not torch.cuda.is_current_stream_capturing():
-        return workspace(nbytes, device)
-    ws = torch.empty(nbytes, dtype=torch.uint8, device=device)
-    ws[:_TICKET_BYTES].zero_()
-    return ws
+    if torch.cuda.is_current_stream_capturing():
+        ws = torch.empty(nbytes, dtype=torch.uint8, device=device)
+        ws[:_TICKET_BYTES].zero_()
+        return ws.data_ptr()
+    ws = _ws_cache.get((device.index, stream))
+    if ws is None or ws.numel() < nbytes:
+        with torch.cuda.device(device):
+            ws = workspace(nbytes, device)
+    return ws.data_ptr()
 
 
 def _at(t):
@@ -231,24 +243,28 @@ def _at(t):
 
 def _page_table(rows, kv_indptr, kv_indices, kv_len, qo_indptr):
     """Checks of a ragged batch's tables -> batch size."""
-    for t in (kv_indptr, kv_indices, kv_len, qo_indptr):
-        if t is not None and (t.dtype != torch.int32 or t.dim() != 1):
-            _fail("page table tensors must be 1-D int32")
-    _dense(kv_indptr=kv_indptr, kv_indices=kv_indices, kv_len=kv_len, qo_indptr=qo_indptr)
+    i32 = torch.int32
+    if kv_indptr.dtype is not i32 or kv_indices.dtype is not i32 or kv_len.dtype is not i32:
+        _fail("page table tensors must be int32")
     batch = kv_len.numel()
-    if kv_indptr.numel() != batch + 1 or (qo_indptr is not None and qo_indptr.numel() != batch + 1):
-        _fail(f"kv_indptr and qo_indptr must have {batch + 1} entries (kv_len has {batch})")
-    if qo_indptr is None and rows != batch:
-        _fail(f"without qo_indptr every sequence has one row ({rows} rows, {batch} sequences)")
+    if kv_indptr.numel() != batch + 1:
+        _fail(f"kv_indptr must have {batch + 1} entries (kv_len has {batch})")
+    if qo_indptr is None:
+        if rows != batch:
+            _fail(f"without qo_indptr every sequence has one row ({rows} rows, {batch} sequences)")
+    elif qo_indptr.dtype is not i32 or qo_indptr.numel() != batch + 1:
+        _fail(f"qo_indptr must be int32 with {batch + 1} entries (kv_len has {batch})")
+    _dense(kv_indptr, kv_indices, kv_len, qo_indptr)
     return batch
 
 
-def _output(out, shape, dtype, device):
+def _output(out, shape, like):
+    """A result of like's dtype, or the caller's."""
     if out is None:
-        return torch.empty(shape, dtype=dtype, device=device)
-    if out.shape != torch.Size(shape) or out.dtype != dtype:
-        _fail(f"out must be {tuple(shape)} {dtype}, got {tuple(out.shape)} {out.dtype}")
-    _dense(out=out)
+        return torch.empty(shape, dtype=like.dtype, device=like.device)
+    if tuple(out.shape) != tuple(shape) or out.dtype is not like.dtype:
+        _fail(f"out must be {tuple(shape)} {like.dtype}, got {tuple(out.shape)} {out.dtype}")
+    _dense(out)
     return out
 
 
@@ -260,61 +276,67 @@ def append_kv_paged(k, v, k_cache, v_cache, kv_indptr, kv_indices, kv_len, q=Non
     kv_len counts the new tokens, so row i of a sequence's n rows has position kv_len - n + i.
     Keys and q are normalised per head (q_norm / k_norm [D]) and rotated (rotate-half, cos / sin
     [positions, D], fp32 or k's dtype), in fp32 with one rounding; a q row whose position lies
-    outside the tables is NaN and its key is not written.  page_bounds [P, Hkv, 2, D] keeps each page's smallest and
-    largest key per channel (what select_pages reads).  q is [T, Hq, D] or [T, Hkv, Hq / Hkv, D];
-    q, k and v may be slices of one projection (last dim contiguous, 16-byte aligned)."""
-    _same_dtype(k, v, k_cache, v_cache, q, q_norm, k_norm, page_bounds)
-    dt = dtype_code(k.dtype)
+    outside the tables is NaN and its key is not written.  page_bounds [P, Hkv, 2, D] keeps each
+    page's smallest and largest key per channel (what select_pages reads).  q is [T, Hq, D] or
+    [T, Hkv, Hq / Hkv, D]; q, k and v may be slices of one projection (last dim contiguous, 16-byte
+    aligned).  out may be q itself where that is contiguous.  D is 64 or 128."""
+    dtype = k.dtype
+    for t in (v, k_cache, v_cache, q, q_norm, k_norm, page_bounds):
+        if t is not None and t.dtype is not dtype:
+            _fail(f"operand dtype {t.dtype} differs from k's {dtype}")
+    dt = dtype_code(dtype)
     if k.dim() != 3 or v.shape != k.shape or k_cache.dim() != 4 or v_cache.shape != k_cache.shape:
         _fail("k and v must be [T, Hkv, D], the caches [P, page, Hkv, D]")
     T, hkv, D = k.shape
-    P, page = k_cache.shape[:2]
-    if tuple(k_cache.shape[2:]) != (hkv, D):
-        _fail(f"cache heads {tuple(k_cache.shape[2:])} differ from k's {(hkv, D)}")
+    P, page, h2, d2 = k_cache.shape
+    if h2 != hkv or d2 != D:
+        _fail(f"cache heads {(h2, d2)} differ from k's {(hkv, D)}")
     batch = _page_table(T, kv_indptr, kv_indices, kv_len, qo_indptr)
-    _dense(k_cache=k_cache, v_cache=v_cache, cos=cos, sin=sin, q_norm=q_norm, k_norm=k_norm, page_bounds=page_bounds)
+    _dense(k_cache, v_cache, cos, sin, q_norm, k_norm, page_bounds)
     if page_bounds is not None and tuple(page_bounds.shape) != (P, hkv, 2, D):
         _fail(f"page_bounds must be {(P, hkv, 2, D)}")
     for w in (q_norm, k_norm):
         if w is not None and tuple(w.shape) != (D,):
             _fail(f"norm weights must be [{D}]")
-    if (cos is None) != (sin is None):
-        _fail("cos and sin come together")
     tdt, npos = 0, 0
-    if cos is not None:
-        if cos.dim() != 2 or cos.shape[1] != D or sin.shape != cos.shape or sin.dtype != cos.dtype:
+    if cos is not None or sin is not None:
+        if cos is None or sin is None:
+            _fail("cos and sin come together")
+        if cos.dim() != 2 or cos.shape[1] != D or sin.shape != cos.shape or sin.dtype is not cos.dtype:
             _fail(f"cos and sin must be [positions, {D}] of one dtype")
-        if cos.dtype != k.dtype and cos.dtype != torch.float32:
-            _fail(f"tables must be float32 or {k.dtype}, got {cos.dtype}")
+        if cos.dtype is not dtype and cos.dtype is not torch.float32:
+            _fail(f"tables must be float32 or {dtype}, got {cos.dtype}")
         tdt, npos = _DTYPE_ALL[cos.dtype], cos.shape[0]
     hq, qs = 0, (0, 0, 0)
+    ks, vs = k.stride(), v.stride()
     if q is not None:
+        qs = q.stride()
         if q.dim() == 4:
             if q.shape[0] != T or q.shape[1] != hkv or q.shape[3] != D:
                 _fail(f"q must be [{T}, {hkv}, heads, {D}]")
-            hq, qs = hkv * q.shape[2], q.stride()[:3]
+            hq = hkv * q.shape[2]
         else:
             if q.dim() != 3 or q.shape[0] != T or q.shape[2] != D or q.shape[1] % hkv:
                 _fail(f"q must be [{T}, heads, {D}] with a multiple of {hkv} heads")
             hq = q.shape[1]
-            qs = (q.stride(0), q.stride(1) * (hq // hkv), q.stride(1))
-        out = _output(out, (T, hq, D), q.dtype, q.device)
+            qs = (qs[0], qs[1] * (hq // hkv), qs[1], qs[2])
+        if qs[3] != 1 and q.numel():
+            _fail("the last dim of q must be contiguous")
     elif out is not None or q_norm is not None:
         _fail("out and q_norm need q")
-    for t in (q, k, v):
-        if t is not None and t.numel() and t.stride(-1) != 1:
-            _fail("the last dim of q, k and v must be contiguous")
-    _one_device(k, v, k_cache, v_cache, kv_indptr, kv_indices, kv_len, q, cos, sin, q_norm, k_norm, qo_indptr,
-                page_bounds, out)
+    if (ks[2] != 1 or vs[2] != 1) and T:
+        _fail("the last dim of k and v must be contiguous")
+    if q is not None:
+        out = _output(out, (T, hq, D), q)
+    index = _one_device(k, v, k_cache, v_cache, kv_indptr, kv_indices, kv_len, q, cos, sin, q_norm, k_norm, qo_indptr,
+                        page_bounds, out)
     if T == 0:
         return out
-    strides = (ctypes.c_int64 * 7)(*qs, k.stride(0), k.stride(1), v.stride(0), v.stride(1))
-    with _on(k.device):
-        check(lib().yr_hip_append_kv_paged(
-            _at(q), _at(k), _at(v), _at(out), _at(k_cache), _at(v_cache), _at(page_bounds), _at(cos), _at(sin), tdt,
-            npos, _at(q_norm), _at(k_norm), eps, _at(qo_indptr), _at(kv_indptr), _at(kv_indices), kv_indices.numel(),
-            _at(kv_len), T, batch, hq, hkv, D, page, P, strides, dt,
-            torch.cuda.current_stream(k.device).cuda_stream), "append_kv_paged")
+    _launch(index, lib().yr_hip_append_kv_paged, "append_kv_paged", _at(q), k.data_ptr(), v.data_ptr(), _at(out),
+            k_cache.data_ptr(), v_cache.data_ptr(), _at(page_bounds), _at(cos), _at(sin), tdt, npos, _at(q_norm),
+            _at(k_norm), eps, _at(qo_indptr), kv_indptr.data_ptr(), kv_indices.data_ptr(), kv_indices.numel(),
+            kv_len.data_ptr(), T, batch, hq, hkv, D, page, P, _Strides7(qs[0], qs[1], qs[2], ks[0], ks[1], vs[0], vs[1]),
+            dt, torch._C._cuda_getCurrentRawStream(index))
     return out
 
 
@@ -325,28 +347,34 @@ def select_pages(q, page_bounds, kv_indptr, kv_indices, kv_len, page_size: int, 
 
     The first first_pages pages, the last last_pages (>= 1) visible ones, and the best of the others
     by an upper bound of their scores from page_bounds [P, Hkv, 2, D] (append_kv_paged keeps it),
-    summed over the group's heads in 64 bits; ties take the lower page."""
-    _same_dtype(q, page_bounds)
+    summed over the group's heads in 64 bits; ties take the lower page.  max_kv_len bounds kv_len
+    (None: its maximum, read on the host)."""
+    if page_bounds.dtype is not q.dtype:
+        _fail(f"page_bounds' dtype {page_bounds.dtype} differs from q's {q.dtype}")
     dt = dtype_code(q.dtype)
-    _dense(q=q, page_bounds=page_bounds)
+    _dense(q, page_bounds)
     if q.dim() != 3 or page_bounds.dim() != 4 or page_bounds.shape[2] != 2 or page_bounds.shape[3] != q.shape[2]:
         _fail("q must be [T, Hq, D], page_bounds [P, Hkv, 2, D]")
     T, hq, D = q.shape
-    P, hkv = page_bounds.shape[:2]
+    P, hkv, _, _ = page_bounds.shape
     batch = _page_table(T, kv_indptr, kv_indices, kv_len, qo_indptr)
-    out = _output(out, (T, hkv, top_pages), torch.int32, q.device)
-    _one_device(q, page_bounds, kv_indptr, kv_indices, kv_len, qo_indptr, out)
+    if top_pages < 1:
+        _fail("top_pages must be positive")
+    if out is None:
+        out = torch.empty((T, hkv, top_pages), dtype=torch.int32, device=q.device)
+    elif tuple(out.shape) != (T, hkv, top_pages) or out.dtype is not torch.int32 or not out.is_contiguous():
+        _fail(f"out must be contiguous int32 {(T, hkv, top_pages)}")
+    index = _one_device(q, page_bounds, kv_indptr, kv_indices, kv_len, qo_indptr, out)
     if T == 0:
         return out
     if max_kv_len is None:
         max_kv_len = max(int(kv_len.max().item()), 1)
-    with _on(q.device):
-        nb = lib().yr_hip_select_pages_workspace(T, hkv, page_size, max_kv_len)
-        ws = _scratch(nb, q.device)
-        check(lib().yr_hip_select_pages(
-            _at(q), _at(page_bounds), _at(qo_indptr), _at(kv_indptr), _at(kv_indices), kv_indices.numel(),
-            _at(kv_len), _at(out), T, batch, hq, hkv, D, page_size, P, max_kv_len, top_pages, first_pages, last_pages,
-            dt, _at(ws), nb, torch.cuda.current_stream(q.device).cuda_stream), "select_pages")
+    stream = torch._C._cuda_getCurrentRawStream(index)
+    nb = lib().yr_hip_select_pages_workspace(T, hkv, page_size, max_kv_len)
+    _launch(index, lib().yr_hip_select_pages, "select_pages", q.data_ptr(), page_bounds.data_ptr(), _at(qo_indptr),
+            kv_indptr.data_ptr(), kv_indices.data_ptr(), kv_indices.numel(), kv_len.data_ptr(), out.data_ptr(), T, batch,
+            hq, hkv, D, page_size, P, max_kv_len, top_pages, first_pages, last_pages, dt,
+            _scratch(nb, q.device, stream), nb, stream)
     return out
 
 
@@ -354,27 +382,28 @@ def gqa_sparse_paged(q, k_cache, v_cache, kv_indptr, kv_indices, kv_len, pages, 
     """Paged GQA attention over selected pages: row t of q [T, Hq, D] attends to the tokens at or
     before its position in pages[t, h // (Hq / Hkv)] (int32 [T, Hkv, n], as select_pages gives them;
     any order, negative, invisible and repeated entries count for nothing).  A row without a token is 0."""
-    _same_dtype(q, k_cache, v_cache)
+    if k_cache.dtype is not q.dtype or v_cache.dtype is not q.dtype:
+        _fail(f"cache dtypes {k_cache.dtype}, {v_cache.dtype} differ from q's {q.dtype}")
     dt = dtype_code(q.dtype)
-    _dense(q=q, k_cache=k_cache, v_cache=v_cache, pages=pages)
+    _dense(q, k_cache, v_cache, pages)
     if q.dim() != 3 or k_cache.dim() != 4 or v_cache.shape != k_cache.shape or k_cache.shape[3] != q.shape[2]:
         _fail("q must be [T, Hq, D], the caches [P, page, Hkv, D]")
     T, hq, D = q.shape
-    P, page, hkv = k_cache.shape[:3]
+    P, page, hkv, _ = k_cache.shape
     batch = _page_table(T, kv_indptr, kv_indices, kv_len, qo_indptr)
-    if pages.dtype != torch.int32 or pages.dim() != 3 or tuple(pages.shape[:2]) != (T, hkv):
+    if pages.dtype is not torch.int32 or pages.dim() != 3 or pages.shape[0] != T or pages.shape[1] != hkv:
         _fail(f"pages must be int32 [{T}, {hkv}, n]")
-    out = _output(out, q.shape, q.dtype, q.device)
-    _one_device(q, k_cache, v_cache, kv_indptr, kv_indices, kv_len, pages, qo_indptr, out)
+    top = pages.shape[2]
+    out = _output(out, (T, hq, D), q)
+    index = _one_device(q, k_cache, v_cache, kv_indptr, kv_indices, kv_len, pages, qo_indptr, out)
     if T == 0:
         return out
-    with _on(q.device):
-        nb = lib().yr_hip_gqa_sparse_workspace(T, batch, qo_indptr is not None, hq, hkv, D, page, pages.shape[2])
-        ws = _scratch(nb, q.device)
-        check(lib().yr_hip_gqa_sparse_paged(
-            _at(q), _at(k_cache), _at(v_cache), _at(qo_indptr), _at(kv_indptr), _at(kv_indices), kv_indices.numel(),
-            _at(kv_len), _at(pages), _at(out), T, batch, hq, hkv, D, page, P, pages.shape[2], dt,
-            _at(ws), nb, torch.cuda.current_stream(q.device).cuda_stream), "gqa_sparse_paged")
+    stream = torch._C._cuda_getCurrentRawStream(index)
+    nb = lib().yr_hip_gqa_sparse_workspace(T, batch, qo_indptr is not None, hq, hkv, D, page, top)
+    _launch(index, lib().yr_hip_gqa_sparse_paged, "gqa_sparse_paged", q.data_ptr(), k_cache.data_ptr(),
+            v_cache.data_ptr(), _at(qo_indptr), kv_indptr.data_ptr(), kv_indices.data_ptr(), kv_indices.numel(),
+            kv_len.data_ptr(), pages.data_ptr(), out.data_ptr(), T, batch, hq, hkv, D, page, P, top, dt,
+            _scratch(nb, q.device, stream), nb, stream)
     return out
 
 
@@ -389,28 +418,30 @@ def token_logprobs(logits, tokens, top_n: int = 0, n_valid: int | None = None) -
     """Log probabilities of tokens [rows] (int64) under softmax(logits[:, :n_valid]) (f16, bf16 or
     fp32, rows contiguous), the rows' entropy, and the top_n (<= 64) most likely tokens.  A token outside
     [0, n_valid) has NaN; NaN logits and rows of -inf alone give NaN numbers."""
-    if logits.dtype not in _DTYPE_ALL:
+    dt = _DTYPE_ALL.get(logits.dtype)
+    if dt is None:
         _fail(f"unsupported logits dtype {logits.dtype}")
-    if logits.dim() != 2 or (logits.numel() and logits.stride(1) != 1):
+    if logits.dim() != 2 or (logits.stride(1) != 1 and logits.shape[1] > 1):
         _fail("logits must be [rows, n] with contiguous rows")
     rows, n = logits.shape
-    if tokens.dtype != torch.int64 or tuple(tokens.shape) != (rows,) or not tokens.is_contiguous():
+    if tokens.dtype is not torch.int64 or tokens.dim() != 1 or tokens.shape[0] != rows or not tokens.is_contiguous():
         _fail(f"tokens must be contiguous int64 [{rows}]")
-    _one_device(logits, tokens)
-    dev = logits.device
-    f32, i64 = {"dtype": torch.float32, "device": dev}, {"dtype": torch.int64, "device": dev}
-    res = LogProbs(torch.empty(rows, **f32), torch.empty(rows, **f32), torch.empty((rows, top_n), **f32),
-                   torch.empty((rows, top_n), **i64))
+    index = _one_device(logits, tokens)
+    dev, n_valid, top_n = logits.device, n if n_valid is None else n_valid, int(top_n)
+    # one allocation: the ids first (8 bytes each), then the three fp32 results
+    flat = torch.empty(rows * (3 * max(top_n, 0) + 2), dtype=torch.float32, device=dev)
+    cut = rows * max(top_n, 0)
+    res = LogProbs(flat[3 * cut: 3 * cut + rows], flat[3 * cut + rows:], flat[2 * cut: 3 * cut].view(rows, -1) if cut else
+                   flat.new_empty((rows, 0)), flat[: 2 * cut].view(torch.int64).view(rows, -1) if cut else
+                   tokens.new_empty((rows, 0)))
     if rows == 0:
         return res
-    dt, n_valid = _DTYPE_ALL[logits.dtype], n if n_valid is None else n_valid
-    with _on(dev):
-        nb = lib().yr_hip_token_logprobs_workspace(rows, n_valid, top_n, dt)
-        ws = _scratch(nb, dev)
-        check(lib().yr_hip_token_logprobs(
-            _at(logits), _at(tokens), _at(res.logprob), _at(res.entropy), _at(res.top_logprob), _at(res.top_token), rows, n,
-            n_valid, logits.stride(0) if rows > 1 else n, top_n, dt, _at(ws), nb,
-            torch.cuda.current_stream(dev).cuda_stream), "token_logprobs")
+    stream = torch._C._cuda_getCurrentRawStream(index)
+    nb = lib().yr_hip_token_logprobs_workspace(rows, n_valid, top_n, dt)
+    at = flat.data_ptr()
+    _launch(index, lib().yr_hip_token_logprobs, "token_logprobs", logits.data_ptr(), tokens.data_ptr(), at + 12 * cut,
+            at + 12 * cut + 4 * rows, at + 8 * cut, at, rows, n, n_valid, logits.stride(0) if rows > 1 else n, top_n, dt,
+            _scratch(nb, dev, stream), nb, stream)
     return res
 
 
