@@ -82,11 +82,12 @@ __device__ __forceinline__ double group_sum(double v) {
 //
 // The m-th best key is found bit by bit: of the bits in which the keys differ,
 // from the highest, a bit is set when m keys at least reach the value with it.
-// That ends as soon as exactly m do, after about log2 n bits.
+// That ends as soon as exactly m do, after about log2 n bits.  Several waves take
+// two bits a step, which costs three counts and saves an exchange.
 template <int W, int R>
 __device__ __forceinline__ void choose_from(const uint64_t* key, int n, int f, int l, int m, int top, int32_t* out) {
-  __shared__ int s_cnt[2][SEL_WAVES];
-  __shared__ uint64_t s_diff[SEL_WAVES];
+  __shared__ uint64_t s_cnt[2][SEL_WAVES], s_diff[SEL_WAVES];
+  __shared__ int s_pos[kWave];
   const int lane = threadIdx.x % kWave, wave = W == 1 ? 0 : __builtin_amdgcn_readfirstlane(threadIdx.x / kWave);
   const int c0 = f, c1 = n - l;  // candidates
   const int turns = R ? R : (n + W * kWave - 1) / (W * kWave);
@@ -105,27 +106,34 @@ __device__ __forceinline__ void choose_from(const uint64_t* key, int n, int f, i
     }
   }
   int turn = 0;
-  // sum of a count over the waves
-  auto all = [&](int c) __attribute__((always_inline)) -> int {
+  // sums over the waves of three counts of up to 2^21, one barrier for all
+  auto all = [&](uint64_t c) __attribute__((always_inline)) -> uint64_t {
     if constexpr (W == 1) return c;
     if (lane == 0) s_cnt[turn][wave] = c;
     __syncthreads();
-    int sum = 0;
+    uint64_t sum = 0;
 #pragma unroll
     for (int w = 0; w < W; w++) sum += s_cnt[turn][w];
     turn ^= 1;  // the next count goes elsewhere: one barrier each
     return sum;
   };
-  auto count = [&](uint64_t least) __attribute__((always_inline)) -> int {  // least > 0
+  // how many keys reach a value > 0, or each of three
+  auto count = [&](uint64_t least) __attribute__((always_inline)) -> int {
     int c = 0;
-    if constexpr (R > 0) {
-#pragma unroll
-      for (int i = 0; i < R; i++) c += __popcll(__ballot(k[i] >= least));
-    } else {
-#pragma unroll 4
-      for (int i = 0; i < turns; i++) c += __popcll(__ballot(get(i) >= least));
+#pragma unroll(R ? R : 4)
+    for (int i = 0; i < turns; i++) c += __popcll(__ballot(get(i) >= least));
+    return (int)all(c);
+  };
+  auto count3 = [&](uint64_t x, uint64_t y, uint64_t z) __attribute__((always_inline)) -> uint64_t {
+    int cx = 0, cy = 0, cz = 0;
+#pragma unroll(R ? R : 4)
+    for (int i = 0; i < turns; i++) {
+      const uint64_t v = get(i);
+      cx += __popcll(__ballot(v >= x));
+      cy += __popcll(__ballot(v >= y));
+      cz += __popcll(__ballot(v >= z));
     }
-    return all(c);
+    return all((uint64_t)cx | (uint64_t)cy << 21 | (uint64_t)cz << 42);
   };
   uint64_t bound = 0;      // keys from it on are taken ..
   int equal = 0x7fffffff;  // .. of those equal to it only the first `equal`
@@ -147,15 +155,57 @@ __device__ __forceinline__ void choose_from(const uint64_t* key, int n, int f, i
     int bit = diff ? 63 - __builtin_clzll(diff) : -1;
     bound = bit < 0 ? any : bit == 63 ? 0 : any & ~((2ull << bit) - 1);
     bool exact = false;
-    for (; bit >= 0 && !exact; bit--) {
-      const uint64_t cand = bound | 1ull << bit;
-      const int c = count(cand);
-      if (c >= m) bound = cand;
-      exact = c == m;
+    if constexpr (W == 1) {
+      for (; bit >= 0 && !exact; bit--) {
+        const uint64_t cand = bound | 1ull << bit;
+        const int c = count(cand);
+        if (c >= m) bound = cand;
+        exact = c == m;
+      }
     }
-    if (!exact) equal = m - (bound == ~0ull ? 0 : count(bound + 1));  // equal keys at the border: the first of them
+    bit |= 1;  // pairs of bits: one above the differing ones comes out as all keys have it
+    for (bit--; W > 1 && bit >= 0 && !exact; bit -= 2) {
+      const uint64_t step = 1ull << bit, low = bound & ~(3 * step);
+      const uint64_t c = count3(low | step, low | 2 * step, low | 3 * step);
+      const int c1s = (int)(c & 0x1fffff), c2s = (int)(c >> 21 & 0x1fffff), c3s = (int)(c >> 42);
+      const int best = c3s >= m ? 3 : c2s >= m ? 2 : c1s >= m ? 1 : 0;
+      bound = low | best * step;
+      exact = (best == 3 ? c3s : best == 2 ? c2s : best == 1 ? c1s : -1) == m;
+    }
+    if (!exact) {  // equal keys at the border: the first of them
+      equal = m - (bound == ~0ull ? 0 : count(bound + 1));
+    }
   }
   // ascending list; the waves take blocks of 64 pages in turn
+  if constexpr (W > 1 && R > 0) {
+    if (equal == 0x7fffffff) {  // (uniform) no ties: one exchange of every block's count
+      uint64_t taken[R];
+      int mine = 0;  // lane i: block i's
+#pragma unroll
+      for (int i = 0; i < R; i++) {
+        const int u = (i * W + wave) * kWave + lane;
+        taken[i] = __ballot(u < n && (u < c0 || u >= c1 || (m > 0 && k[i] >= bound)));
+        mine = lane == i ? __popcll(taken[i]) : mine;
+      }
+      if (lane < R) s_pos[lane * W + wave] = mine;
+      __syncthreads();
+      int sum = lane < R * W ? s_pos[lane] : 0;  // up to and with block `lane`
+#pragma unroll
+      for (int o = 1; o < kWave; o <<= 1) {
+        const int v = __shfl_up(sum, o);
+        if (lane >= o) sum += v;
+      }
+#pragma unroll
+      for (int i = 0; i < R; i++) {
+        const int j = i * W + wave, base = j ? __builtin_amdgcn_readlane(sum, j - 1) : 0;
+        const int pos = base + __popcll(taken[i] & ((1ull << lane) - 1));
+        if ((taken[i] >> lane & 1) && pos < top) gptr(out)[pos] = j * kWave + lane;
+      }
+      const int all_taken = __builtin_amdgcn_readlane(sum, kWave - 1);
+      for (int i = all_taken + (int)threadIdx.x; i < top; i += W * kWave) gptr(out)[i] = -1;
+      return;
+    }
+  }
   int at = 0, eq = 0;  // written so far, keys equal to bound seen so far
 #pragma unroll(R ? R : 1)
   for (int i = 0; i < turns; i++) {
@@ -166,11 +216,11 @@ __device__ __forceinline__ void choose_from(const uint64_t* key, int n, int f, i
     int before = eq;
     const uint64_t be = __ballot(same);
     if (equal != 0x7fffffff) {  // (uniform)
-      int alle = all(__popcll(be));
+      const int alle = (int)all(__popcll(be));
       if constexpr (W > 1) {
 #pragma unroll
         for (int w = 0; w < W; w++)
-          if (w < wave) before += s_cnt[turn ^ 1][w];
+          if (w < wave) before += (int)s_cnt[turn ^ 1][w];
       }
       eq += alle;
       before += __popcll(be & ((1ull << lane) - 1));
@@ -178,11 +228,11 @@ __device__ __forceinline__ void choose_from(const uint64_t* key, int n, int f, i
     const bool take = u < n && (!cand || (m > 0 && (same ? before < equal : key_u > bound)));
     const uint64_t bt = __ballot(take);
     int pos = at;
-    at += all(__popcll(bt));
+    at += (int)all(__popcll(bt));
     if constexpr (W > 1) {
 #pragma unroll
       for (int w = 0; w < W; w++)
-        if (w < wave) pos += s_cnt[turn ^ 1][w];
+        if (w < wave) pos += (int)s_cnt[turn ^ 1][w];
     }
     pos += __popcll(bt & ((1ull << lane) - 1));
     if (take && pos < top) gptr(out)[pos] = u;
@@ -301,7 +351,15 @@ __global__ __launch_bounds__(SEL_THREADS) void select_kernel(SelectArgs a) {
     }
     if (a.splits > 1) {
       if (!arrive_last(&a.tickets[pair], a.splits)) return;
-      for (int u = r.f + tid; u < r.n - r.l; u += SEL_THREADS) s_key[u] = sel_load(a.keys + (size_t)pair * a.max_pages + u);
+      const uint64_t* const keys = a.keys + (size_t)pair * a.max_pages;
+      for (int u0 = r.f + tid; u0 < r.n - r.l; u0 += 8 * SEL_THREADS) {  // 8 loads in flight
+        uint64_t k[8];
+#pragma unroll
+        for (int i = 0; i < 8; i++) k[i] = sel_load(keys + min(u0 + i * SEL_THREADS, r.n - r.l - 1));
+#pragma unroll
+        for (int i = 0; i < 8; i++)
+          if (u0 + i * SEL_THREADS < r.n - r.l) s_key[u0 + i * SEL_THREADS] = k[i];
+      }
     }
     __syncthreads();
   } else if (split > 0) {
