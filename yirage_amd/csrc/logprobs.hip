@@ -149,6 +149,16 @@ __device__ __forceinline__ int wave_rank(uint64_t k) {
   return r;
 }
 
+// How many of the n keys at `list` (LDS) beat k; reads run 8 ahead.
+__device__ __forceinline__ int rank_in(const uint64_t* list, int n, uint64_t k) {
+  int r = 0, j = 0;
+  for (; j + 8 <= n; j += 8)
+#pragma unroll
+    for (int i = 0; i < 8; i++) r += list[j + i] > k;
+  for (; j < n; j++) r += list[j] > k;
+  return r;
+}
+
 // The `top` best of a wave's `count` keys in `buf`, in order, written back to
 // buf[0, top) (0 where there are fewer).  Keys differ from one another.
 __device__ __forceinline__ void wave_top(uint64_t* buf, int count, int top) {
@@ -228,7 +238,7 @@ __global__ __launch_bounds__(LP_THREADS) void logprobs_kernel(LogprobArgs a) {
   constexpr int ES = 16 / EPP;
   constexpr int kTile = kWave * U, kStep = LP_WAVES * kTile;  // pieces
   __shared__ uint64_t s_buf[LP_WAVES][LP_BUF];
-  extern __shared__ uint64_t s_list[];  // [splits][top]
+  extern __shared__ uint64_t s_list[];  // [top], then (splits > 1) the splits' candidates
   __shared__ int s_item[LP_ITEMS];  // first pieces of lanes with candidates
   __shared__ int s_items, s_cands;
   __shared__ float s_m[LP_WAVES], s_bound[LP_WAVES];
@@ -454,8 +464,7 @@ __global__ __launch_bounds__(LP_THREADS) void logprobs_kernel(LogprobArgs a) {
     if (items <= LP_ITEMS && cands <= kCands) {
       for (int i = tid; i < cands; i += LP_THREADS) {
         const uint64_t k = cand[i];
-        int r = 0;
-        for (int j = 0; j < cands; j++) r += cand[j] > k;
+        const int r = rank_in(cand, cands, k);
         if (r < a.top) s_list[r] = k;
       }
     } else {
@@ -494,7 +503,8 @@ __global__ __launch_bounds__(LP_THREADS) void logprobs_kernel(LogprobArgs a) {
       for (int i = tid; i < LP_WAVES * a.top; i += LP_THREADS) {
         const uint64_t k = s_buf[i / a.top][i % a.top];
         int r = 0;
-        for (int j = 0; j < LP_WAVES * a.top; j++) r += s_buf[j / a.top][j % a.top] > k;
+#pragma unroll
+        for (int w = 0; w < LP_WAVES; w++) r += rank_in(s_buf[w], a.top, k);
         if (k && r < a.top) s_list[r] = k;
       }
     }
@@ -524,33 +534,62 @@ __global__ __launch_bounds__(LP_THREADS) void logprobs_kernel(LogprobArgs a) {
     }
     for (int i = tid; i < a.top; i += LP_THREADS) st_u64(rec + (size_t)split * rec_len + 3 + i, s_list[i]);
     if (!arrive_last(&a.tickets[row], a.splits)) return;
-    for (int i = tid; i < a.splits * a.top; i += LP_THREADS)
-      s_list[i] = ld_u64(rec + (size_t)(i / a.top) * rec_len + 3 + i % a.top);
-    __syncthreads();
-    if (wave != 0) return;
+    // The splits' ordered lists.  `top` heads at least are as good as the top-th
+    // best head: what is below that is out, and the few others are ranked.
+    const int keys = a.splits * a.top;
+    uint64_t* const cand = s_list + a.top;  // (room for every key)
+    const bool listed = tid < a.splits;
     double ms = -INFINITY, ss = 0, ts = 0;
-    if (lane < a.splits) {
-      ms = __longlong_as_double((long long)ld_u64(rec + (size_t)lane * rec_len));
-      ss = __longlong_as_double((long long)ld_u64(rec + (size_t)lane * rec_len + 1));
-      ts = __longlong_as_double((long long)ld_u64(rec + (size_t)lane * rec_len + 2));
+    uint64_t head = 0;
+    if (listed) {
+      const uint64_t* const r = rec + (size_t)tid * rec_len;
+      ms = __longlong_as_double((long long)ld_u64(r));
+      ss = __longlong_as_double((long long)ld_u64(r + 1));
+      ts = __longlong_as_double((long long)ld_u64(r + 2));
+      if (a.top > 0) head = ld_u64(r + 3);
     }
-    // (a float times the constant: the division gives the float back)
-    M = wave_maxf((float)(ms / (double)kLog2e));
-    lp_rescale(ss, ts, ms, lp_exponent(M));
-    s = wave_sum_d(ss);
-    t = wave_sum_d(ts);
-    // the splits' ordered lists: take the best head, `top` times
-    int next = 0;
-    uint64_t head = lane < a.splits && a.top > 0 ? s_list[lane * a.top] : 0, mine = 0;
-    for (int k = 0; k < a.top; k++) {
-      const uint64_t best = wave_max_key(head);
-      if (lane == k) mine = best;
-      if (best && head == best) {
-        next++;
-        head = next < a.top ? s_list[lane * a.top + next] : 0;
+    constexpr int KU = 8;
+    uint64_t got[KU];  // the keys of this thread, i = tid + u threads (the others are read again below)
+#pragma unroll
+    for (int u = 0; u < KU; u++) {
+      const int i = tid + u * LP_THREADS;
+      got[u] = i < keys ? ld_u64(rec + (size_t)(i / a.top) * rec_len + 3 + i % a.top) : 0;
+    }
+    if (wave == 0) {
+      // (a float times the constant: the division gives the float back)
+      M = wave_maxf((float)(ms / (double)kLog2e));
+      lp_rescale(ss, ts, ms, lp_exponent(M));
+      s = wave_sum_d(ss);
+      t = wave_sum_d(ts);
+      if (a.top > 0) {
+        const float b = a.top <= a.splits ? lane_bound(head ? lp_value(head) : -INFINITY, a.top) : -INFINITY;
+        if (lane == 0) {
+          s_cands = 0;
+          s_bound[0] = b;
+        }
       }
     }
-    if (lane < a.top) s_list[lane] = mine;  // (every head was read: the wave runs in step)
+    for (int i = tid; i < a.top; i += LP_THREADS) s_list[i] = 0;
+    __syncthreads();
+    if (a.top > 0) {
+      const float b = s_bound[0];
+      auto take = [&](uint64_t k) __attribute__((always_inline)) {
+        if (k && lp_value(k) >= b) cand[atomicAdd(&s_cands, 1)] = k;
+      };
+#pragma unroll
+      for (int u = 0; u < KU; u++) take(got[u]);
+      for (int i = tid + KU * LP_THREADS; i < keys; i += LP_THREADS)
+        take(ld_u64(rec + (size_t)(i / a.top) * rec_len + 3 + i % a.top));
+      __syncthreads();
+      const int cands = s_cands;
+      for (int i = tid; i < cands; i += LP_THREADS) {
+        const uint64_t k = cand[i];
+        const int r = rank_in(cand, cands, k);
+        if (r < a.top) s_list[r] = k;
+      }
+      __syncthreads();
+    }
+    if (wave != 0) return;
   }
   if (M == -INFINITY) s = t = NAN;  // no value at all
   if (s < 1) s = 1;                 // the largest term alone, but for its rounding
@@ -622,7 +661,7 @@ extern "C" int yr_hip_token_logprobs(const void* x, const int64_t* tokens, float
   a.records = need ? (uint64_t*)((char*)workspace + kTicketBytes) : nullptr;
   hipStream_t st = (hipStream_t)stream;
   const dim3 grid((unsigned)(rows * a.splits));
-  const size_t lds = (size_t)a.splits * top_n * sizeof(uint64_t);
+  const size_t lds = (size_t)(a.splits > 1 ? a.splits + 1 : 1) * top_n * sizeof(uint64_t);
 #define YR_LP(DT_, V_)                     \
   if (dtype == DT_ && p.values == V_)      \
     hipLaunchKernelGGL((logprobs_kernel<DT_, V_>), grid, dim3(LP_THREADS), lds, st, a);
