@@ -25,7 +25,7 @@ namespace yr {
 constexpr int SP_BLK = 32;            // tokens per wave block
 constexpr int SP_MAX_ENTRIES = 1024;  // list entries of a tile
 constexpr int SP_TARGET_WG = 256;     // one per CU
-constexpr int SP_MIN_BLOCKS = 2;      // blocks per split at least
+constexpr int SP_MIN_BLOCKS = 4;      // blocks per split at least
 
 struct SparseArgs {
   Ragged r;
@@ -65,21 +65,22 @@ __device__ __forceinline__ int v_swz(int row) {
 //
 // A table of one mask per page is filled and read back where it fits into the
 // `cells` (even) 16-bit words at `table`, which hold nt * top ints at least.  A
-// single ascending list (a decode step's) needs none; otherwise every entry looks
-// for its like.  The whole workgroup of T.
+// single ascending list (a decode step's) is taken as it is; otherwise every entry
+// looks for its like.  The whole workgroup of T.
 template <int T>
 __device__ __forceinline__ int build_union(const SparseArgs& a, const SeqRows& s, int nt, int t0, int p0, int hk,
                                            uint32_t* table, int cells, int* l_u, int* l_id, uint16_t* l_mask, int* s_cnt) {
   const int tid = threadIdx.x, lane = tid % kWave, wave = tid / kWave;
   const int E = nt * a.top;
-  auto entry = [&](int e) __attribute__((always_inline)) -> int {
+  auto entry = [&](int e, int* id) __attribute__((always_inline)) -> int {
     const int i = e / a.top, p = p0 + i;
     const int u = gptr(a.pages)[((size_t)(t0 + i) * a.hkv + hk) * a.top + e % a.top];
-    return u < 0 || p < 0 || u > p / a.r.page || page_id(a.r, s, u) < 0 ? -1 : u;
+    *id = p < 0 || u > p / a.r.page ? -1 : page_id(a.r, s, u);
+    return *id < 0 ? -1 : u;
   };
   // appends the workgroup's entries that are `own`, in thread order
   int nsel = 0;
-  auto append = [&](bool own, int u, int mask) __attribute__((always_inline)) {
+  auto append = [&](bool own, int u, int mask, int id) __attribute__((always_inline)) {
     const uint64_t bal = __ballot(own);
     if (lane == 0) s_cnt[wave] = __popcll(bal);
     __syncthreads();
@@ -91,6 +92,7 @@ __device__ __forceinline__ int build_union(const SparseArgs& a, const SeqRows& s
     }
     if (own) {
       l_u[at] = u;
+      l_id[at] = id;
       l_mask[at] = (uint16_t)mask;
     }
     __syncthreads();
@@ -100,39 +102,44 @@ __device__ __forceinline__ int build_union(const SparseArgs& a, const SeqRows& s
     for (int i = tid; i < (n + 1) / 2; i += T) table[i] = 0;
     __syncthreads();
     for (int e = tid; e < E; e += T) {
-      const int u = entry(e);
+      int id;
+      const int u = entry(e, &id);
       if (u >= 0) atomicOr(&table[u / 2], 1u << (e / a.top + 16 * (u % 2)));
     }
     __syncthreads();
     for (int u0 = 0; u0 < n; u0 += T) {
       const int u = u0 + tid, mask = u < n ? table[u / 2] >> (16 * (u % 2)) & 0xffff : 0;
-      append(mask != 0, u, mask);
+      append(mask != 0, u, mask, mask ? page_id(a.r, s, u) : -1);
     }
+  } else if (nt == 1 && E <= T) {  // a decode step's: an entry a thread
+    int* const s_u = reinterpret_cast<int*>(table);
+    int id = -1;
+    const int u = tid < E ? entry(tid, &id) : -1;
+    s_u[tid] = u;
+    __syncthreads();
+    bool own = u >= 0;
+    if (__syncthreads_or(own && tid > 0 && (s_u[tid - 1] < 0 || u <= s_u[tid - 1])))  // not ascending: look for its like
+      for (int j = 0; own && j < tid; j++) own = s_u[j] != u;
+    append(own, u, 1, id);
   } else {
     int* const s_u = reinterpret_cast<int*>(table);
-    for (int e = tid; e < E; e += T) s_u[e] = entry(e);
+    int id;
+    for (int e = tid; e < E; e += T) s_u[e] = entry(e, &id);
     __syncthreads();
-    bool unordered = false;
-    for (int e = tid; e < E; e += T)
-      if (e % a.top) unordered |= s_u[e] >= 0 && (s_u[e - 1] < 0 || s_u[e] <= s_u[e - 1]);
-    const bool ordered = nt == 1 && !__syncthreads_or(unordered);
     for (int e0 = 0; e0 < E; e0 += T) {
       const int e = e0 + tid, u = e < E ? s_u[e] : -1;
       bool own = u >= 0;
-      int mask = own ? 1 << (e / a.top) : 0;
-      if (own && !ordered)
+      int mask = 0;
+      if (own)
         for (int j = 0; j < E; j++)
           if (s_u[j] == u) {
             mask |= 1 << (j / a.top);
             if (j < e) own = false;
           }
-      append(own, u, mask);
+      append(own, u, mask, own ? page_id(a.r, s, u) : -1);
     }
   }
-  nsel = __builtin_amdgcn_readfirstlane(nsel);
-  for (int e = tid; e < nsel; e += T) l_id[e] = page_id(a.r, s, l_u[e]);
-  __syncthreads();
-  return nsel;
+  return __builtin_amdgcn_readfirstlane(nsel);
 }
 
 // NW waves; PG32: pages are a multiple of 32 tokens, so a block lies in one page
