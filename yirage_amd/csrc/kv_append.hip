@@ -9,6 +9,15 @@
 //
 // All of it in fp32 from 16-bit inputs, rounded once to the cache's type; the
 // bounds are taken of the rounded keys, so they are exact.
+//
+// Bound by memory: every byte of q, k and v is read once and written once.  The
+// angles are what else there is to read, in fp32 four times a q row's bytes, so a
+// lane keeps them for 4 heads of its token (a row a lane: 97 us; two: 61; four
+// 54; eight 72 for registers).  A page's keys and bounds belong to one workgroup
+// and are reduced there, two channels a thread (a row's lanes alone: 88 us), and
+// the stores pass the caches (kept in them: 69 us).  12.3k rows of 32 and 8 heads
+// of 128 in bf16, 303 MB: 54 us, 5.6 TB/s, a copy of that size 58; 64 sequences'
+// new tokens 5.5 us, one's 4.
 #include "ragged.h"
 
 namespace yr {
@@ -27,14 +36,20 @@ struct AppendArgs {
   const uint16_t* q_norm;
   const uint16_t* k_norm;
   long long q_row, q_grp, q_head, k_row, k_head, v_row, v_head;  // strides in elements
-  int hq, hkv, max_pos, q_blocks, heads;  // heads: kv heads per cache workgroup
+  int hq, hkv, max_pos, q_blocks, q_chunks, heads;  // q_chunks per token; kv heads per cache workgroup
   float eps;
 };
 
 constexpr int AP_THREADS = 256;
+constexpr int AP_WAVES = AP_THREADS / kWave;
+constexpr int AP_Q = 4;  // q rows of a lane: they share its 32 angles
 
 // A row (one token's head) is D / 16 lanes; a lane holds 8 elements of each
 // half, so a rotated pair sits in one lane.
+// What is written is not read again here: stored past the caches.
+__device__ __forceinline__ void stg16_stream(uint16_t* p, uint4 v) {
+  __builtin_nontemporal_store(__builtin_bit_cast(yr_u32x4, v), (YR_G yr_u32x4*)p);
+}
 template <int DT>
 __device__ __forceinline__ void unpack8(uint4 v, float* x) {
   x[0] = lo16<DT>(v.x); x[1] = hi16<DT>(v.x); x[2] = lo16<DT>(v.y); x[3] = hi16<DT>(v.y);
@@ -57,33 +72,34 @@ __device__ __forceinline__ void table8(const void* t, size_t at, float* x) {
   }
 }
 
-// One lane's 16 elements of a row, normalised and rotated for position p.
+// One lane's angles at position p.
 template <int DT, int D, bool F32>
-__device__ __forceinline__ void norm_rotate(const AppendArgs& a, const uint16_t* w, uint4 lo, uint4 hi, int p, int l,
-                                            uint4* out) {
+__device__ __forceinline__ void angles(const AppendArgs& a, int p, int l, float* c, float* s) {
+  const size_t at = (size_t)p * D + 8 * l;
+  table8<DT, F32>(a.cos, at, c);
+  table8<DT, F32>(a.cos, at + D / 2, c + 8);
+  table8<DT, F32>(a.sin, at, s);
+  table8<DT, F32>(a.sin, at + D / 2, s + 8);
+}
+
+// One lane's 16 elements of a row, normalised by the weights w and rotated.
+template <int DT, int D>
+__device__ __forceinline__ void norm_rotate(bool norm, bool rotate, float eps, const float* w, const float* c,
+                                            const float* s, uint4 lo, uint4 hi, uint4* out) {
   float x[16];
   unpack8<DT>(lo, x);
   unpack8<DT>(hi, x + 8);
-  if (w) {
+  if (norm) {
     float ss = 0.f;
 #pragma unroll
     for (int i = 0; i < 16; i++) ss = fmaf(x[i], x[i], ss);
 #pragma unroll
     for (int o = 1; o < D / 16; o <<= 1) ss += __shfl_xor(ss, o, kWave);
-    const float f = 1.f / sqrtf(ss * (1.f / D) + a.eps);
-    float wv[16];
-    unpack8<DT>(ldg16(w + 8 * l), wv);
-    unpack8<DT>(ldg16(w + D / 2 + 8 * l), wv + 8);
+    const float f = 1.f / sqrtf(ss * (1.f / D) + eps);
 #pragma unroll
-    for (int i = 0; i < 16; i++) x[i] = x[i] * f * wv[i];
+    for (int i = 0; i < 16; i++) x[i] = x[i] * f * w[i];
   }
-  if (a.cos) {
-    float c[16], s[16];
-    const size_t at = (size_t)p * D + 8 * l;
-    table8<DT, F32>(a.cos, at, c);
-    table8<DT, F32>(a.cos, at + D / 2, c + 8);
-    table8<DT, F32>(a.sin, at, s);
-    table8<DT, F32>(a.sin, at + D / 2, s + 8);
+  if (rotate) {
 #pragma unroll
     for (int i = 0; i < 8; i++) {
       const float u = x[i], t = x[i + 8];
@@ -97,56 +113,86 @@ __device__ __forceinline__ void norm_rotate(const AppendArgs& a, const uint16_t*
 
 template <int DT, int D, bool F32>
 __global__ __launch_bounds__(AP_THREADS) void append_kernel(AppendArgs a) {
-  constexpr int LPR = D / 16, RPP = AP_THREADS / LPR;  // lanes per row, rows per pass
-  const int tid = threadIdx.x, l = tid % LPR, slot = tid / LPR;
+  constexpr int LPR = D / 16, RPW = kWave / LPR, RPP = AP_THREADS / LPR;  // lanes per row, rows per wave and per pass
+  const int tid = threadIdx.x, lane = tid % kWave, wave = __builtin_amdgcn_readfirstlane(tid / kWave);
+  const int l = tid % LPR, slot = tid / LPR;
   const Ragged& r = a.r;
 
-  // ---- q: rows of (token, head)
+  // ---- q: a wave takes AP_Q * RPW heads of one token
   if ((int)blockIdx.x < a.q_blocks) {
-    const long long i = (long long)blockIdx.x * RPP + slot;
-    const int t = (int)(i / a.hq), h = (int)(i % a.hq), g = a.hq / a.hkv;
+    const long long i = (long long)blockIdx.x * AP_WAVES + wave;
+    const int t = (int)(i / a.q_chunks), h0 = (int)(i % a.q_chunks) * AP_Q * RPW + lane / LPR, g = a.hq / a.hkv;
     if (t >= r.rows) return;
+    uint4 x[AP_Q][2];
+#pragma unroll
+    for (int j = 0; j < AP_Q; j++) {
+      const int h = min(h0 + j * RPW, a.hq - 1);
+      const uint16_t* src = a.q + t * a.q_row + (h / g) * a.q_grp + (h % g) * a.q_head + 8 * l;
+      x[j][0] = ldg16(src);
+      x[j][1] = ldg16(src + D / 2);
+    }
+    float w[16], c[16], sn[16];
+    if (a.q_norm) {
+      unpack8<DT>(ldg16(a.q_norm + 8 * l), w);
+      unpack8<DT>(ldg16(a.q_norm + D / 2 + 8 * l), w + 8);
+    }
     const int b = seq_of_row(r, t);
     if (b < 0) return;
     const SeqRows s = seq_rows(r, b);
     const int p = s.len - s.n + (t - s.row0);
-    const uint16_t* src = a.q + t * a.q_row + (h / g) * a.q_grp + (h % g) * a.q_head + 8 * l;
-    uint4 y[2];
-    if (a.cos && (unsigned)p >= (unsigned)a.max_pos) {  // no angle for this position: a loud answer
-      const uint32_t nan2 = pack2<DT>(NAN, NAN);
-      y[0] = y[1] = make_uint4(nan2, nan2, nan2, nan2);
-    } else {
-      norm_rotate<DT, D, F32>(a, a.q_norm, ldg16(src), ldg16(src + D / 2), p, l, y);
+    const bool lost = a.cos && (unsigned)p >= (unsigned)a.max_pos;  // no angle for this position: a loud answer
+    if (a.cos && !lost) angles<DT, D, F32>(a, p, l, c, sn);
+#pragma unroll
+    for (int j = 0; j < AP_Q; j++) {
+      const int h = h0 + j * RPW;
+      if (h0 - lane / LPR + j * RPW >= a.hq) break;  // (uniform)
+      uint4 y[2];
+      norm_rotate<DT, D>(a.q_norm, a.cos, a.eps, w, c, sn, x[j][0], x[j][1], y);
+      if (lost) {
+        const uint32_t nan2 = pack2<DT>(NAN, NAN);
+        y[0] = y[1] = make_uint4(nan2, nan2, nan2, nan2);
+      }
+      if (h < a.hq) {
+        uint16_t* dst = a.q_out + ((size_t)t * a.hq + h) * D + 8 * l;
+        stg16_stream(dst, y[0]);
+        stg16_stream(dst + D / 2, y[1]);
+      }
     }
-    uint16_t* dst = a.q_out + ((size_t)t * a.hq + h) * D + 8 * l;
-    stg16(dst, y[0]);
-    stg16(dst + D / 2, y[1]);
     return;
   }
 
   // ---- k, v and bounds: one page of one sequence, a.heads kv heads
   const int groups = (a.hkv + a.heads - 1) / a.heads;
   const int item = (blockIdx.x - a.q_blocks) / groups, h0 = (blockIdx.x - a.q_blocks) % groups * a.heads;
-  __shared__ int s_item[2];
-  if (tid == 0) {
-    int left = item, b = 0, u = -1;
-    for (; b < r.batch; b++) {
-      const SeqRows s = seq_rows(r, b);
-      const int p0 = max(s.len - s.n, 0);
-      const int pages = s.len > p0 ? (s.len - 1) / r.page - p0 / r.page + 1 : 0;
-      if (left < pages) {
-        u = p0 / r.page + left;
+  int b = item, u = 0;
+  if (r.qo_indptr) {  // 64 sequences at a time, each wave for itself
+    int left = item;
+    for (b = 0; b < r.batch; b += kWave) {
+      int pages = 0, p0 = 0;
+      if (b + lane < r.batch) {
+        const SeqRows s = seq_rows(r, b + lane);
+        p0 = max(s.len - s.n, 0);
+        pages = s.len > p0 ? (s.len - 1) / r.page - p0 / r.page + 1 : 0;
+      }
+      int sum = pages;
+#pragma unroll
+      for (int o = 1; o < kWave; o <<= 1) {
+        const int v = __shfl_up(sum, o);
+        if (lane >= o) sum += v;
+      }
+      const uint64_t past = __ballot(sum > left);
+      if (past) {
+        const int i = __builtin_ctzll(past);
+        b += i;
+        u = __builtin_amdgcn_readlane(p0 / r.page + left - (sum - pages), i);
         break;
       }
-      left -= pages;
+      left -= __builtin_amdgcn_readlane(sum, kWave - 1);
     }
-    s_item[0] = b;
-    s_item[1] = u;
+    if (b >= r.batch) return;
   }
-  __syncthreads();
-  const int b = s_item[0], u = s_item[1];
-  if (u < 0) return;
   const SeqRows s = seq_rows(r, b);
+  if (!r.qo_indptr) u = max(s.len - 1, 0) / r.page;
   const int id = page_id(r, s, u);
   if (id < 0) return;
   const int first = s.len - s.n;  // position of the sequence's first new row
@@ -154,6 +200,16 @@ __global__ __launch_bounds__(AP_THREADS) void append_kernel(AppendArgs a) {
   const int pos1 = min(min(s.len, (u + 1) * r.page), a.cos ? a.max_pos : 0x7fffffff);  // none without an angle
   if (pos0 >= pos1) return;
   const int hh = slot % a.heads, h = h0 + hh, step = RPP / a.heads;
+  // the thread's word of the page's bounds, two channels (a head's first D / 2 words
+  // are minima), as the tokens before left it
+  const int word = tid % D;
+  const bool low = word < D / 2;
+  uint32_t* bd = nullptr;
+  uint32_t old = low ? pack2<DT>(INFINITY, INFINITY) : pack2<DT>(-INFINITY, -INFINITY);
+  if (a.bounds && tid / D < a.heads && h0 + tid / D < a.hkv) {
+    bd = (uint32_t*)(a.bounds + ((size_t)id * a.hkv + h0 + tid / D) * 2 * D) + word;
+    if (pos0 > u * r.page) old = gptr(bd)[0];
+  }
   float mn[16], mx[16];
 #pragma unroll
   for (int i = 0; i < 16; i++) {
@@ -161,18 +217,26 @@ __global__ __launch_bounds__(AP_THREADS) void append_kernel(AppendArgs a) {
     mx[i] = -INFINITY;
   }
   if (h < a.hkv) {
+    float w[16];
+    if (a.k_norm) {
+      unpack8<DT>(ldg16(a.k_norm + 8 * l), w);
+      unpack8<DT>(ldg16(a.k_norm + D / 2 + 8 * l), w + 8);
+    }
     for (int p = pos0 + slot / a.heads; p < pos1; p += step) {
       const long long t = s.row0 + (p - first);
       const uint16_t* ks = a.k + t * a.k_row + h * a.k_head + 8 * l;
       const uint16_t* vs = a.v + t * a.v_row + h * a.v_head + 8 * l;
       const uint4 v0 = ldg16(vs), v1 = ldg16(vs + D / 2);
+      const uint4 k0 = ldg16(ks), k1 = ldg16(ks + D / 2);
+      float c[16], sn[16];
+      if (a.cos) angles<DT, D, F32>(a, p, l, c, sn);
       uint4 y[2];
-      norm_rotate<DT, D, F32>(a, a.k_norm, ldg16(ks), ldg16(ks + D / 2), p, l, y);
+      norm_rotate<DT, D>(a.k_norm, a.cos, a.eps, w, c, sn, k0, k1, y);
       const size_t dst = (((size_t)id * r.page + (p - u * r.page)) * a.hkv + h) * D + 8 * l;
-      stg16(a.kc + dst, y[0]);
-      stg16(a.kc + dst + D / 2, y[1]);
-      stg16(a.vc + dst, v0);
-      stg16(a.vc + dst + D / 2, v1);
+      stg16_stream(a.kc + dst, y[0]);
+      stg16_stream(a.kc + dst + D / 2, y[1]);
+      stg16_stream(a.vc + dst, v0);
+      stg16_stream(a.vc + dst + D / 2, v1);
       float x[16];
       unpack8<DT>(y[0], x);
       unpack8<DT>(y[1], x + 8);
@@ -185,39 +249,23 @@ __global__ __launch_bounds__(AP_THREADS) void append_kernel(AppendArgs a) {
   }
   if (!a.bounds) return;
   __shared__ uint4 s_b[RPP][4][LPR];
-  s_b[slot][0][l] = pack8<DT>(mn);
-  s_b[slot][1][l] = pack8<DT>(mn + 8);
-  s_b[slot][2][l] = pack8<DT>(mx);
-  s_b[slot][3][l] = pack8<DT>(mx + 8);
+  const int slots = min(RPP, (pos1 - pos0) * a.heads);
+  if (slot < slots) {
+    s_b[slot][0][l] = pack8<DT>(mn);
+    s_b[slot][1][l] = pack8<DT>(mn + 8);
+    s_b[slot][2][l] = pack8<DT>(mx);
+    s_b[slot][3][l] = pack8<DT>(mx + 8);
+  }
   __syncthreads();
-  if (slot >= a.heads || h >= a.hkv) return;
-  for (int o = slot + a.heads; o < RPP; o += a.heads) {
-    float x[16];
-    unpack8<DT>(s_b[o][0][l], x);
-    unpack8<DT>(s_b[o][1][l], x + 8);
-#pragma unroll
-    for (int i = 0; i < 16; i++) mn[i] = fminf(mn[i], x[i]);
-    unpack8<DT>(s_b[o][2][l], x);
-    unpack8<DT>(s_b[o][3][l], x + 8);
-#pragma unroll
-    for (int i = 0; i < 16; i++) mx[i] = fmaxf(mx[i], x[i]);
+  float e0 = lo16<DT>(old), e1 = hi16<DT>(old);
+  const uint32_t* const rows = (const uint32_t*)s_b + word;
+#pragma unroll 8
+  for (int o = tid / D; o < slots; o += a.heads) {
+    const uint32_t x = rows[o * D];
+    e0 = low ? fminf(e0, lo16<DT>(x)) : fmaxf(e0, lo16<DT>(x));
+    e1 = low ? fminf(e1, hi16<DT>(x)) : fmaxf(e1, hi16<DT>(x));
   }
-  uint16_t* bd = a.bounds + ((size_t)id * a.hkv + h) * 2 * D + 8 * l;
-  if (pos0 > u * r.page) {  // the page held tokens already
-    float x[16];
-    unpack8<DT>(ldg16(bd), x);
-    unpack8<DT>(ldg16(bd + D / 2), x + 8);
-#pragma unroll
-    for (int i = 0; i < 16; i++) mn[i] = fminf(mn[i], x[i]);
-    unpack8<DT>(ldg16(bd + D), x);
-    unpack8<DT>(ldg16(bd + D + D / 2), x + 8);
-#pragma unroll
-    for (int i = 0; i < 16; i++) mx[i] = fmaxf(mx[i], x[i]);
-  }
-  stg16(bd, pack8<DT>(mn));
-  stg16(bd + D / 2, pack8<DT>(mn + 8));
-  stg16(bd + D, pack8<DT>(mx));
-  stg16(bd + D + D / 2, pack8<DT>(mx + 8));
+  if (bd) gptr(bd)[0] = pack2<DT>(e0, e1);
 }
 
 int ragged_check(const char* nm, const Ragged& r, int hq, int hkv, int d, int dtype) {
@@ -281,15 +329,17 @@ extern "C" int yr_hip_append_kv_paged(const void* q, const void* k, const void* 
   a.hkv = hkv;
   a.max_pos = max_pos;
   a.eps = eps;
-  const int rpp = AP_THREADS / (d / 16);
-  const long long qb = q ? ((long long)rows * hq + rpp - 1) / rpp : 0;
+  const int rpp = AP_THREADS / (d / 16), chunk = AP_Q * kWave / (d / 16);
+  a.q_chunks = ((q ? hq : 1) + chunk - 1) / chunk;
+  const long long qb = q ? ((long long)rows * a.q_chunks + AP_WAVES - 1) / AP_WAVES : 0;
   // pages that new rows can touch: each sequence's span, at most one per row
   long long items = (long long)rows / page_size + 2ll * batch;
   if (items > rows) items = rows;
-  // kv heads per workgroup: as many as leave every row slot a token of the page
+  // kv heads per workgroup: as many as leave every row slot a token of the page and
+  // each thread one word of the bounds
   const int tokens = qo_indptr ? (int)((rows + batch - 1) / batch < page_size ? (rows + batch - 1) / batch : page_size) : 1;
   a.heads = 1;
-  while (a.heads < hkv && a.heads * tokens < rpp && a.heads < rpp) a.heads *= 2;
+  while (a.heads < hkv && a.heads * tokens < rpp && a.heads < AP_THREADS / d) a.heads *= 2;
   const long long blocks = qb + items * ((hkv + a.heads - 1) / a.heads);
   if (blocks > 0x7fffffff) return fail(YR_E_INVALID, "%s: too many rows", nm);
   a.q_blocks = (int)qb;
