@@ -122,3 +122,15 @@ def test_small_entropies_and_probabilities(dt):
     _check(x, tok, 2, got)
     p1 = torch.log1p(39999 * torch.exp(-x[:, 31111].double()))
     assert ((got.logprob.cpu().double() + p1).abs() <= 2.0 ** -20 * p1 + 2.0 ** -24 * 40).all()
+
+
+@DTS
+def test_top_64_of_a_row_over_64_workgroups(dt):
+    """Parts of a row that hold fewer numbers than are asked for."""
+    gen = torch.Generator().manual_seed(5)
+    x = torch.randn((3, 140001), generator=gen).to(dt)
+    x[1, 70:] = -math.inf
+    x[2, : 139990] = math.nan
+    tok = torch.tensor([7, 69, 139999])
+    for r in range(3):  # a row a call, so that each is split as far as it goes
+        _check(x[r: r + 1], tok[r: r + 1], 64, F.token_logprobs(x[r: r + 1].cuda(), tok[r: r + 1].cuda(), top_n=64))

@@ -126,19 +126,20 @@ __device__ __forceinline__ uint64_t lane_u64(uint64_t v, int l) {
          (uint32_t)__builtin_amdgcn_readlane((int)v, l);
 }
 
-// The top-th largest of the 64 lanes' values (top <= 64).
+// A bound that `top` of the 64 lanes' values reach (top <= 64, no NaN), and no
+// other lane's where values differ: their order as whole numbers, found bit by bit
+// until exactly `top` reach what is set.
 __device__ __forceinline__ float lane_bound(float v, int top) {
-  if (top <= 8) {
-    for (int j = 1; j < top; j++) {
-      const uint64_t at = __ballot(v == wave_maxf(v));
-      if ((int)(threadIdx.x % kWave) == __builtin_ctzll(at | 1ull << 63)) v = -INFINITY;
-    }
-    return wave_maxf(v);
+  if (top == 1) return wave_maxf(v);
+  const uint32_t b = __float_as_uint(v), k = b ^ ((uint32_t)((int)b >> 31) | 0x80000000u);
+  uint32_t least = 0;
+  for (int bit = 31; bit >= 0; bit--) {
+    const int n = __popcll(__ballot(k >= (least | 1u << bit)));
+    if (n >= top) least |= 1u << bit;
+    if (n == top) break;
   }
-  int r = 0;
-#pragma unroll 8
-  for (int l = 0; l < kWave; l++) r += __uint_as_float(__builtin_amdgcn_readlane(__float_as_uint(v), l)) > v;
-  return -wave_maxf(r < top ? -v : -INFINITY);
+  if (least < 0x007fffffu) return -INFINITY;  // (all 64 reach it: numbers before that one are NaN)
+  return __uint_as_float(least & 0x80000000u ? least ^ 0x80000000u : ~least);
 }
 
 // How many of the 64 lanes' keys beat this lane's.
@@ -268,7 +269,7 @@ __global__ __launch_bounds__(LP_THREADS) void logprobs_kernel(LogprobArgs a) {
   auto piece = [&](int p) __attribute__((always_inline)) -> uint4 {
     constexpr uint32_t none = DT == DT_F16 ? 0xfc00fc00u : DT == DT_BF16 ? 0xff80ff80u : 0xff800000u;
     const int i0 = p * EPP - lead;
-    if (p < p_end && i0 >= 0 && i0 + EPP <= a.n) return ldg16(x - lead * ES + (size_t)p * 16);
+    if (p < p_end && i0 >= 0 && i0 + EPP <= a.n) return ldg16_stream(x - lead * ES + (size_t)p * 16);
     uint64_t f[2] = {(uint64_t)none << 32 | none, (uint64_t)none << 32 | none};
     if (p < p_end) {  // the row's first or last piece
 #pragma unroll 1
@@ -289,7 +290,7 @@ __global__ __launch_bounds__(LP_THREADS) void logprobs_kernel(LogprobArgs a) {
     if ((p0 > 0 || lead == 0) && (p0 + kTile) * EPP - lead <= a.n && p0 + kTile <= p_end) {
       const char* const tile = x - lead * ES + (size_t)p0 * 16;  // uniform
 #pragma unroll
-      for (int u = 0; u < U; u++) w[u] = ldg16(tile + (uint32_t)(16 * lane + 16 * kWave * u));
+      for (int u = 0; u < U; u++) w[u] = ldg16_stream(tile + (uint32_t)(16 * lane + 16 * kWave * u));
     } else {
 #pragma unroll
       for (int u = 0; u < U; u++) w[u] = piece(p0 + u * kWave + lane);
@@ -534,9 +535,11 @@ __global__ __launch_bounds__(LP_THREADS) void logprobs_kernel(LogprobArgs a) {
     }
     for (int i = tid; i < a.top; i += LP_THREADS) st_u64(rec + (size_t)split * rec_len + 3 + i, s_list[i]);
     if (!arrive_last(&a.tickets[row], a.splits)) return;
-    // The splits' ordered lists.  `top` heads at least are as good as the top-th
-    // best head: what is below that is out, and the few others are ranked.
-    const int keys = a.splits * a.top;
+    // The splits' ordered lists.  Where `some` of them have their deep-th key at or
+    // above a bound, deep * some >= top keys are: what is below the bound is out,
+    // and the few others are ranked.
+    const int keys = a.splits * a.top, deep = (a.top + a.splits - 1) / a.splits;
+    const int some = deep ? (a.top + deep - 1) / deep : 0;
     uint64_t* const cand = s_list + a.top;  // (room for every key)
     const bool listed = tid < a.splits;
     double ms = -INFINITY, ss = 0, ts = 0;
@@ -546,15 +549,18 @@ __global__ __launch_bounds__(LP_THREADS) void logprobs_kernel(LogprobArgs a) {
       ms = __longlong_as_double((long long)ld_u64(r));
       ss = __longlong_as_double((long long)ld_u64(r + 1));
       ts = __longlong_as_double((long long)ld_u64(r + 2));
-      if (a.top > 0) head = ld_u64(r + 3);
+      if (a.top > 0) head = ld_u64(r + 2 + deep);
     }
-    constexpr int KU = 8;
-    uint64_t got[KU];  // the keys of this thread, i = tid + u threads (the others are read again below)
+    constexpr int KU = 8;  // keys of a thread in flight
+    uint64_t got[KU];
+    auto fetch = [&](int i0) __attribute__((always_inline)) {
 #pragma unroll
-    for (int u = 0; u < KU; u++) {
-      const int i = tid + u * LP_THREADS;
-      got[u] = i < keys ? ld_u64(rec + (size_t)(i / a.top) * rec_len + 3 + i % a.top) : 0;
-    }
+      for (int u = 0; u < KU; u++) {
+        const int i = i0 + u * LP_THREADS;
+        got[u] = i < keys ? ld_u64(rec + (size_t)(i / a.top) * rec_len + 3 + i % a.top) : 0;
+      }
+    };
+    fetch(tid);
     if (wave == 0) {
       // (a float times the constant: the division gives the float back)
       M = wave_maxf((float)(ms / (double)kLog2e));
@@ -562,7 +568,7 @@ __global__ __launch_bounds__(LP_THREADS) void logprobs_kernel(LogprobArgs a) {
       s = wave_sum_d(ss);
       t = wave_sum_d(ts);
       if (a.top > 0) {
-        const float b = a.top <= a.splits ? lane_bound(head ? lp_value(head) : -INFINITY, a.top) : -INFINITY;
+        const float b = lane_bound(head ? lp_value(head) : -INFINITY, some);
         if (lane == 0) {
           s_cands = 0;
           s_bound[0] = b;
@@ -573,13 +579,14 @@ __global__ __launch_bounds__(LP_THREADS) void logprobs_kernel(LogprobArgs a) {
     __syncthreads();
     if (a.top > 0) {
       const float b = s_bound[0];
-      auto take = [&](uint64_t k) __attribute__((always_inline)) {
-        if (k && lp_value(k) >= b) cand[atomicAdd(&s_cands, 1)] = k;
-      };
+      for (int i = tid;;) {
 #pragma unroll
-      for (int u = 0; u < KU; u++) take(got[u]);
-      for (int i = tid + KU * LP_THREADS; i < keys; i += LP_THREADS)
-        take(ld_u64(rec + (size_t)(i / a.top) * rec_len + 3 + i % a.top));
+        for (int u = 0; u < KU; u++)
+          if (got[u] && lp_value(got[u]) >= b) cand[atomicAdd(&s_cands, 1)] = got[u];
+        i += KU * LP_THREADS;
+        if (i >= keys) break;
+        fetch(i);
+      }
       __syncthreads();
       const int cands = s_cands;
       for (int i = tid; i < cands; i += LP_THREADS) {
