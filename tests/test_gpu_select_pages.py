@@ -112,3 +112,57 @@ def test_missing_pages_and_short_bounds(news):
     assert torch.equal(got[: b.news[0]].cpu(), _reference(b, q[: b.rows], bounds, 2, 6, 1, 1)[: b.news[0]])
     assert int(got[b.news[0]: b.news[0] + b.news[1]].max()) < 30 - int(ptr[1])  # the second sequence lost pages
     assert (got[b.news[0] + b.news[1]: b.rows] == -1).all()                     # the third all of them
+
+
+# Rows enough for tiles of them (the ones above are mostly taken row by row).
+
+
+@pytest.mark.parametrize("dt", [torch.float16, torch.bfloat16], ids=["f16", "bf16"])
+@pytest.mark.parametrize("lens,news,hq,hkv,d,page,top,first,last", [
+    ([4800], [350], 4, 1, 64, 16, 33, 1, 1), ([900, 5000, 40], [300, 420, 40], 14, 2, 128, 16, 16, 1, 2),
+    ([2200], [450], 2, 2, 64, 1, 40, 2, 3),          # 8 rows a tile
+    ([300, 3900], [200, 330], 4, 4, 128, 1, 20, 1, 1),  # 4 rows a tile
+    ([9000], [400], 4, 4, 64, 16, 130, 3, 4),        # more pages taken than a wave has lanes
+    ([6000], [700], 16, 2, 128, 64, 8, 0, 1), ([1000], [600], 8, 8, 64, 16, 60, 1, 1),
+])
+def test_tiles(lens, news, hq, hkv, d, page, top, first, last, dt):
+    test_lists(lens, news, hq, hkv, d, page, top, first, last, dt)
+
+
+@pytest.mark.parametrize("dt", [torch.float16, torch.bfloat16], ids=["f16", "bf16"])
+@pytest.mark.parametrize("top", [20, 100])
+@pytest.mark.parametrize("kind", ["kinds", "zeros", "groups", "all alike", "special", "scales", "small"])
+def test_tiles_near_the_border(kind, top, dt):
+    """Scores that fp32 cannot tell apart, equal ones, and rows beyond its range."""
+    print("case", kind, top, dt, flush=True)
+    d, page, n, rows = 64, 16, 300, 360
+    b = Batch([n * page], [rows], page)
+    gen = torch.Generator().manual_seed(top)
+    q = torch.randn((b.rows, 2, d), generator=gen).to(dt)
+    ids = torch.from_numpy(b.indices).long()
+    bounds = torch.zeros((b.pool, 1, 2, d))
+    base = lambda k: torch.randn((k, 1, 2, d), generator=gen).sort(2).values
+    if kind == "kinds":
+        bounds[ids] = base(4)[torch.arange(n) % 4]
+    elif kind == "zeros":
+        bounds[ids[::2]] = -0.0
+    elif kind in ("groups", "all alike"):  # groups of 20 (of all) that differ in one tiny channel
+        bounds[ids] = base(15 if kind == "groups" else 1).repeat_interleave(20 if kind == "groups" else n, 0)
+        tiny = 2.0 ** -24 if dt is torch.float16 else 2.0 ** -30
+        bounds[ids, 0, 1, 5] = (torch.randint(0, 9, (n,), generator=gen) * tiny).float()
+    elif kind == "special":
+        bounds[ids] = base(n)
+        bounds[ids[10:20], 0, 1, 3] = float("inf")
+        bounds[ids[30:40], 0, 0, 3] = float("-inf")
+        bounds[ids[50:60], 0, 0, 7] = float("nan")
+    elif kind == "scales":  # (what f16 cannot hold is infinite or zero)
+        bounds[ids] = base(n)
+        q = (q.float() * 10.0 ** torch.linspace(-36, 36, rows)[:, None, None]).to(dt)
+        q[::50] = 0
+    else:                   # bounds and q at the bottom of the type's range
+        bounds[ids] = base(n) * (2.0 ** -20 if dt is torch.float16 else 2.0 ** -130)
+        q = (q.float() * 2.0 ** -16).to(dt)
+    bounds = bounds.to(dt)
+    got = F.select_pages(q.cuda(), bounds.cuda(), *b.args(), page_size=page, top_pages=top, qo_indptr=b.qo(),
+                         max_kv_len=n * page)
+    assert torch.equal(got.cpu(), _reference(b, q, bounds, 1, top, 1, 1))

@@ -17,7 +17,7 @@
 
 namespace yr {
 
-typedef double f64x4 __attribute__((ext_vector_type(4)));
+typedef uint32_t u32x2 __attribute__((ext_vector_type(2)));
 
 struct SelectArgs {
   Ragged r;
@@ -26,16 +26,15 @@ struct SelectArgs {
   int32_t* out;            // [rows][hkv][top]
   uint64_t* keys;          // [rows][hkv][max_pages] where a row is split
   uint32_t* tickets;       // [rows][hkv]
-  int hq, hkv, max_pages, top, first, last, splits, chunk;
+  int hq, hkv, max_pages, top, first, last, splits, chunk, tile;  // tile: rows
 };
 
 constexpr int SEL_THREADS = 256;
 constexpr int SEL_WAVES = SEL_THREADS / kWave;
 constexpr int SEL_MAX_PAGES = 16384;  // 64-bit keys of one row in LDS: 128 of 160 KiB
 constexpr int SEL_ROWS = 16;          // rows of a tile
-constexpr int SEL_TILE_WAVES = 8;     // two a SIMD: 36 us for 512 rows of 512 pages, 43 with 4
-constexpr int SEL_TILE_PAGES = 1024;  // a tile's keys in LDS: as much
-constexpr int SEL_TILE_MIN = 4;       // rows per sequence from which tiles are taken
+constexpr int SEL_TILE_WAVES = 16;    // a row's list each: 512 rows of 512 pages 21 us, 23 with 8
+constexpr int SEL_TILE_PAGES = 4096;  // a tile's keys in LDS: as much, 4 rows at least
 constexpr int SEL_TARGET_WG = 1024;
 constexpr int SEL_MIN_CHUNK = 64;     // pages per split at least
 
@@ -270,6 +269,21 @@ __device__ __forceinline__ uint64_t sel_load(const uint64_t* p) {
   return __hip_atomic_load((const YR_G uint64_t*)p, __ATOMIC_RELAXED, __HIP_MEMORY_SCOPE_AGENT);
 }
 
+// A lane's part of a page's score: 8 channels.
+template <int DT>
+__device__ __forceinline__ double page_dot(const double* down, const double* up, uint4 mn, uint4 mx) {
+  const uint32_t w0[4] = {mn.x, mn.y, mn.z, mn.w}, w1[4] = {mx.x, mx.y, mx.z, mx.w};
+  double s0 = 0, s1 = 0;
+#pragma unroll
+  for (int e = 0; e < 4; e++) {
+    s0 = fma(down[2 * e], (double)lo16<DT>(w0[e]), s0);
+    s1 = fma(up[2 * e], (double)lo16<DT>(w1[e]), s1);
+    s0 = fma(down[2 * e + 1], (double)hi16<DT>(w0[e]), s0);
+    s1 = fma(up[2 * e + 1], (double)hi16<DT>(w1[e]), s1);
+  }
+  return s0 + s1;
+}
+
 // One row and kv head, its pages split over `splits` workgroups; the last one
 // to arrive chooses.
 template <int DT, int D>
@@ -331,16 +345,7 @@ __global__ __launch_bounds__(SEL_THREADS) void select_kernel(SelectArgs a) {
       }
 #pragma unroll
       for (int i = 0; i < U; i++) {
-        const uint32_t w0[4] = {mn[i].x, mn[i].y, mn[i].z, mn[i].w}, w1[4] = {mx[i].x, mx[i].y, mx[i].z, mx[i].w};
-        double s0 = 0, s1 = 0;
-#pragma unroll
-        for (int e = 0; e < 4; e++) {
-          s0 = fma(qd[2 * e], (double)lo16<DT>(w0[e]), s0);
-          s1 = fma(qu[2 * e], (double)lo16<DT>(w1[e]), s1);
-          s0 = fma(qd[2 * e + 1], (double)hi16<DT>(w0[e]), s0);
-          s1 = fma(qu[2 * e + 1], (double)hi16<DT>(w1[e]), s1);
-        }
-        const double sum = group_sum<LPP>(s0 + s1);
+        const double sum = group_sum<LPP>(page_dot<DT>(qd, qu, mn[i], mx[i]));
         const int u = u0 + i * PPB + tid / LPP;
         if (j == 0 && u < end) {
           const uint64_t k = id[i] < 0 ? 0 : score_key(sum);
@@ -368,57 +373,341 @@ __global__ __launch_bounds__(SEL_THREADS) void select_kernel(SelectArgs a) {
   choose<SEL_WAVES>(s_key, r.n, r.f, r.l, r.m, a.top, out);
 }
 
-// Up to 16 rows of one sequence and one kv head: their scores are a product of
-// [16][2 D] by [2 D][pages] on the 64-bit matrix instruction 16x16x4, so the
-// bounds are read and converted once for all rows.  A lane holds its row's Q-
-// and Q+ for the dims 32 c + 8 (lane / 16) .. + 7 and loads the same dims of its
-// page, 16 bytes each: A and B only have to agree on the order of the products.
-// Bound by that instruction (64 cycles a SIMD per 16 x 16 x 4).
+// Memory that a wave's lanes wrote, before they read each other's.
+__device__ __forceinline__ void wave_sync() {
+  __builtin_amdgcn_fence(__ATOMIC_ACQ_REL, "wavefront");
+  __builtin_amdgcn_wave_barrier();
+}
+// Order of an fp32 score; 0 stands for none.
+__device__ __forceinline__ uint32_t rough_key(float s) {
+  const uint32_t b = __float_as_uint(s);
+  return b ^ ((uint32_t)((int)b >> 31) | 0x80000000u);
+}
+__device__ __forceinline__ float rough_score(uint32_t k) {
+  return __uint_as_float(k & 0x80000000u ? k ^ 0x80000000u : ~k);
+}
+template <int C>
+__device__ __forceinline__ uint32_t dpp_max(uint32_t v) {
+  return max(v, dpp_word<C>(v));
+}
+__device__ __forceinline__ uint32_t wave_max(uint32_t v) {
+  v = dpp_max<0x140>(dpp_max<0x141>(dpp_max<0x4E>(dpp_max<0xB1>(v))));
+  auto r = __builtin_amdgcn_permlane16_swap(v, v, false, false);
+  v = max(r[0], r[1]);
+  r = __builtin_amdgcn_permlane32_swap(v, v, false, false);
+  return max(r[0], r[1]);
+}
+
+// Exact scores by one wave: D / 8 lanes a page, 8 channels each.
+template <int DT, int D>
+struct ExactRow {
+  static constexpr int LPP = D / 8, PP = kWave / LPP, U = 2;  // lanes per page, pages per pass, passes in flight
+  double down[8], up[8];
+  // row t, kv head h
+  __device__ __forceinline__ void load(const SelectArgs& a, int t, int h) {
+    const int g = a.hq / a.hkv;
+    const uint16_t* q = a.q + ((size_t)t * a.hq + (size_t)h * g) * D + 8 * (threadIdx.x % LPP);
+#pragma unroll
+    for (int e = 0; e < 8; e++) down[e] = up[e] = 0;
+#pragma unroll 4
+    for (int i = 0; i < g; i++) {
+      const uint4 v = ldg16(q + (size_t)i * D);
+      const uint32_t w[4] = {v.x, v.y, v.z, v.w};
+#pragma unroll
+      for (int e = 0; e < 8; e++) {
+        const double x = e % 2 ? hi16<DT>(w[e / 2]) : lo16<DT>(w[e / 2]);
+        up[e] += x > 0 ? x : x != x ? x : 0;
+        down[e] += x < 0 ? x : 0;
+      }
+    }
+  }
+  // keys of the pages page(0) .. page(n - 1) -> out[i]
+  template <class F>
+  __device__ __forceinline__ void keys(const SelectArgs& a, const SeqRows& s, int h, int n, F page, uint64_t* out) {
+    const int lane = threadIdx.x % kWave, j = lane % LPP;
+    for (int i0 = 0; i0 < n; i0 += U * PP) {
+      int id[U];
+      uint4 mn[U], mx[U];
+#pragma unroll
+      for (int k = 0; k < U; k++) {
+        const int i = i0 + k * PP + lane / LPP;
+        id[k] = i < n ? page_id(a.r, s, page(i)) : -1;
+      }
+#pragma unroll
+      for (int k = 0; k < U; k++) {
+        const uint16_t* bd = a.bounds + ((size_t)max(id[k], 0) * a.hkv + h) * 2 * D + 8 * j;
+        mn[k] = ldg16(bd);
+        mx[k] = ldg16(bd + D);
+      }
+#pragma unroll
+      for (int k = 0; k < U; k++) {
+        const double sum = group_sum<LPP>(page_dot<DT>(down, up, mn[k], mx[k]));
+        const int i = i0 + k * PP + lane / LPP;
+        if (j == 0 && i < n) out[i] = id[k] < 0 ? 0 : score_key(sum);
+      }
+    }
+  }
+};
+
+// A wave's border among a row's scores: get(i), i < turns, gives a lane's keys
+// (0: none), page(i) the pages they belong to, in order.  With A the m-th best
+// score, a page more than 2 err above A is in and one more than 2 err below it is
+// out.  Between, where there is a choice, the pages are scored exactly and their
+// keys in `key` (LDS) become the verdict, for the caller to read again.  Returns
+// the key from which on pages are in; 0: more than 64 of them are too close.
+template <int DT, int D, int R, class Get, class Page>
+__device__ __forceinline__ uint32_t rough_border(const SelectArgs& a, const SeqRows& s, int m, int t, int h, float err,
+                                                 int turns, uint32_t any, Get get, Page page, uint32_t* key, int* list,
+                                                 uint64_t* exact, bool* settled) {
+  const int lane = threadIdx.x % kWave;
+  uint32_t diff = 0;
+#pragma unroll(R ? R : 4)
+  for (int i = 0; i < turns; i++) diff |= get(i) ? get(i) ^ any : 0;
+  diff = wave_or(diff);
+  int bit = diff ? 31 - __builtin_clz(diff) : -1;
+  uint32_t bound = bit < 0 ? any : bit == 31 ? 0 : any & ~((2u << bit) - 1);
+  for (bool split = false; bit >= 0 && !split; bit--) {
+    const uint32_t cand = bound | 1u << bit;
+    int c = 0;
+#pragma unroll(R ? R : 4)
+    for (int i = 0; i < turns; i++) c += __popcll(__ballot(get(i) >= cand));
+    if (c >= m) bound = cand;
+    split = c == m;
+  }
+  // the worst of those at `bound` or above, which is A, and the best below it
+  uint32_t least = 0, next = 0;
+  int reach = 0;
+#pragma unroll(R ? R : 4)
+  for (int i = 0; i < turns; i++) {
+    const uint32_t v = get(i);
+    reach += __popcll(__ballot(v >= bound));
+    least = max(least, v >= bound ? ~v : 0);
+    next = max(next, v < bound ? v : 0);
+  }
+  bound = ~wave_max(least);
+  next = wave_max(next);
+  const float A = rough_score(bound), low = A - 2 * err, high = A + 2 * err;
+  if (reach == m && !(next && rough_score(next) >= low)) return bound;
+  *settled = true;
+  int n = 0, in = 0;
+#pragma unroll(R ? R : 4)
+  for (int i = 0; i < turns; i++) {
+    const uint32_t k = get(i);
+    const float v = rough_score(k);
+    const bool sure = k && v > high, band = k && v >= low && !sure;
+    const uint64_t b = __ballot(band);
+    in += __popcll(__ballot(sure));
+    const int at = n + __popcll(b & ((1ull << lane) - 1));
+    if (band && at < kWave) list[at] = page(i);
+    n += __popcll(b);
+  }
+  if (n > kWave) return 0;
+  wave_sync();
+  ExactRow<DT, D> row;
+  row.load(a, t, h);
+  row.keys(a, s, h, n, [&](int i) { return list[i]; }, exact);
+  wave_sync();
+  if (lane < n) {
+    const uint64_t mine = exact[lane];
+    int rank = 0;
+    for (int i = 0; i < n; i++) rank += exact[i] > mine || (exact[i] == mine && i < lane);
+    key[list[lane]] = rank < m - in ? ~0u : 1u;  // (1: below every score)
+  }
+  wave_sync();
+  return bound;
+}
+
+// The list of a row whose scores' keys at `key` (LDS, written over) are within err
+// of the exact ones, by one wave; R of the keys a lane in registers (0: read
+// again).  False: too many are too close.
+template <int DT, int D, int R>
+__device__ __forceinline__ bool choose_rough(const SelectArgs& a, const SeqRows& s, const RowPages& r, int t, int h, float err,
+                                             uint32_t* key, int* list, uint64_t* exact, int32_t* out) {
+  const int lane = threadIdx.x % kWave, c0 = r.f, c1 = r.n - r.l;
+  const int turns = R ? R : (r.n + kWave - 1) / kWave;
+  uint32_t k[R ? R : 1];
+  auto read = [&](int i) __attribute__((always_inline)) -> uint32_t {
+    const int u = i * kWave + lane;
+    return u >= c0 && u < c1 ? key[u] : 0;
+  };
+  auto get = [&](int i) __attribute__((always_inline)) -> uint32_t {
+    if constexpr (R > 0) return k[i];
+    return read(i);
+  };
+  auto keep = [&]() __attribute__((always_inline)) {
+#pragma unroll
+    for (int i = 0; i < R; i++) k[i] = read(i);
+  };
+  keep();
+  uint32_t bound = 0;
+  if (r.m > 0 && r.m < c1 - c0) {
+    if (r.m <= kWave) {
+      // The m-th best of the lanes' best keys bounds A from below, and few pages
+      // are above it: up to 64 of them go to a list, and the rest is done there.
+      uint32_t best = 0, least = 0;
+#pragma unroll(R ? R : 4)
+      for (int i = 0; i < turns; i++) best = max(best, get(i));
+      if (c1 - c0 > kWave)  // (fewer: all of them)
+        for (int bit = 31; bit >= 0; bit--) {
+          const int c = __popcll(__ballot(best >= (least | 1u << bit)));
+          if (c >= r.m) least |= 1u << bit;
+          if (c == r.m) break;
+        }
+      const float from = rough_score(least) - 2.125f * err;
+      int n = 0;
+#pragma unroll(R ? R : 4)
+      for (int i = 0; i < turns; i++) {
+        const uint32_t v = get(i);
+        const bool near = v && !(rough_score(v) < from);  // (least may stand for NaN: all of them)
+        const uint64_t b = __ballot(near);
+        const int at = n + __popcll(b & ((1ull << lane) - 1));
+        if (near && at < kWave) list[at] = i * kWave + lane;
+        n += __popcll(b);
+      }
+      if (n <= kWave) {
+        wave_sync();
+        const int mine = lane < n ? list[lane] : 0;
+        uint32_t v = lane < n ? key[mine] : 0;
+        wave_sync();
+        bool settled = false;
+        bound = rough_border<DT, D, 1>(a, s, r.m, t, h, err, 1, __builtin_amdgcn_readfirstlane(v),
+                                       [&](int) { return v; }, [&](int) { return mine; }, key, list, exact, &settled);
+        if (settled) v = lane < n ? key[mine] : 0;
+        const uint64_t b = __ballot(v >= bound && lane < n);
+        const int taken = __popcll(b);  // m
+        if (b >> lane & 1) gptr(out)[r.f + __popcll(b & ((1ull << lane) - 1))] = mine;
+        for (int i = lane; i < a.top - taken; i += kWave) {
+          const int j = i < r.f ? i : i + taken;
+          gptr(out)[j] = i < r.f ? i : i - r.f < r.l ? c1 + i - r.f : -1;
+        }
+        return true;
+      }
+    }
+    bool settled = false;
+    bound = rough_border<DT, D, R>(a, s, r.m, t, h, err, turns, key[c0], get, [&](int i) { return i * kWave + lane; }, key,
+                                   list, exact, &settled);
+    if (bound == 0) return false;
+    if (settled) keep();
+  }
+  int at = 0;
+#pragma unroll(R ? R : 4)
+  for (int i = 0; i < turns; i++) {
+    const int u = i * kWave + lane;
+    const bool take = u < r.n && (u < c0 || u >= c1 || (r.m > 0 && get(i) >= bound));
+    const uint64_t b = __ballot(take);
+    const int pos = at + __popcll(b & ((1ull << lane) - 1));
+    if (take && pos < a.top) gptr(out)[pos] = u;
+    at += __popcll(b);
+  }
+  for (int i = at + lane; i < a.top; i += kWave) gptr(out)[i] = -1;
+  return true;
+}
+
+// Up to 16 rows of one sequence and one kv head.  Their scores are a product of
+// [16][2 D] by [2 D][pages] on the 16-bit matrix instruction: Q- and Q+ (fp32) as
+// the sum of three bf16 parts, or of two f16 parts after a scaling by row, against
+// the bounds as they come from memory.  (In fp32 on 16x16x4 the loop takes 15
+// instead of 10 us at 512 rows of 512 pages, on the 64-bit one 24.)
+//
+// The list is that of the exact scores all the same: products of the parts are
+// exact, and a score's error is at most that of adding up D products in each of two
+// sums, a step of fp32 each (half of one if the instruction rounds to nearest), of
+// Q's own g terms, of the parts' rest and of joining the sums, all relative to
+// sum |Q| |bound| <= |Q| |bound| (Euclidean norms, the largest of any page).  Pages
+// nearer to the border than that allows are scored in 64 bits, as are all of a row
+// with numbers too large, too small or not finite.
+//
+// 512 rows of 512 pages, 8 kv heads of 128: 21 us, of which Q 3, the scores 10, a
+// row's list for each wave 5.
 template <int DT, int D>
 __global__ __launch_bounds__(SEL_TILE_WAVES * kWave) void select_tile_kernel(SelectArgs a) {
-  constexpr int C = D / 32;             // 16-byte pieces per lane of each bound
-  extern __shared__ uint64_t s_key[];   // [16][stride]
+  constexpr int C = D / 32;                   // 16-byte pieces per lane of each bound
+  constexpr int L = DT == DT_F16 ? 2 : 3;     // parts of Q
+  constexpr float kPart = DT == DT_F16 ? 2048.f : 1.f;
+  constexpr int QS = 2 * D + 8;               // a row of Q- and Q+ (padded: rows start in other banks)
+  extern __shared__ uint64_t s_key[];         // [tile][stride], fp32 keys in the first half of each row's
   __shared__ int s_tile[2];
+  __shared__ uint32_t s_odd, s_norm;          // rows that need 64 bits throughout, the largest squared norm of a page
+  __shared__ float s_q2[SEL_ROWS], s_scale[SEL_ROWS];  // squared norms of Q, what its parts were divided by
+  struct Lists {
+    uint64_t exact[kWave];
+    int list[kWave];
+  };
+  __shared__ union __attribute__((aligned(16))) {
+    uint16_t q[L][SEL_ROWS][QS];
+    Lists w[SEL_TILE_WAVES];  // after the scores
+  } s_u;
   const int tid = threadIdx.x, lane = tid % kWave, wave = __builtin_amdgcn_readfirstlane(tid / kWave);
   const int h = blockIdx.x % a.hkv, tile = blockIdx.x / a.hkv, stride = a.max_pages;
-  if (tid == 0) find_tile(a.r, tile, SEL_ROWS, s_tile);
+  if (tid == 0) {
+    find_tile(a.r, tile, a.tile, s_tile);
+    s_odd = s_norm = 0;
+  }
   __syncthreads();
-  const int b = s_tile[0], i0 = s_tile[1];
+  const int b = __builtin_amdgcn_readfirstlane(s_tile[0]), i0 = __builtin_amdgcn_readfirstlane(s_tile[1]);
   if (b >= a.r.batch) return;
   const SeqRows s = seq_rows(a.r, b);
-  const int nt = min(SEL_ROWS, s.n - i0), t0 = s.row0 + i0, p0 = s.len - s.n + i0;
+  const int nt = min(a.tile, s.n - i0), t0 = s.row0 + i0, p0 = s.len - s.n + i0;
   const RowPages last = row_pages(a, s, p0 + nt - 1);  // the row that sees most
   const int g = a.hq / a.hkv, col = lane % 16, grp = lane / 16;
   if (last.m > 0 && last.m < last.n - last.f - last.l) {
-    double down[C][8], up[C][8];
-    {
-      const uint16_t* q = a.q + ((size_t)(t0 + min(col, nt - 1)) * a.hq + (size_t)h * g) * D + 8 * grp;
+    // Q and its parts, 4 channels of each sign a thread, a row in D / 4 lanes of a wave
+    for (int i = tid; i < SEL_ROWS * (D / 4); i += SEL_TILE_WAVES * kWave) {
+      const int row = i / (D / 4), d = i % (D / 4) * 4;
+      const uint16_t* q = a.q + ((size_t)(t0 + min(row, nt - 1)) * a.hq + (size_t)h * g) * D + d;
+      float x[8] = {};  // Q-, Q+
+#pragma unroll 4
+      for (int j = 0; j < g; j++) {
+        const u32x2 v = *(const YR_G u32x2*)(q + (size_t)j * D);
+        const float y[4] = {lo16<DT>(v.x), hi16<DT>(v.x), lo16<DT>(v.y), hi16<DT>(v.y)};
 #pragma unroll
-      for (int c = 0; c < C; c++)
+        for (int e = 0; e < 4; e++) {
+          x[4 + e] += y[e] > 0 ? y[e] : y[e] != y[e] ? y[e] : 0;
+          x[e] += y[e] < 0 ? y[e] : 0;
+        }
+      }
+      float q2 = 0, most = 0;
 #pragma unroll
-        for (int e = 0; e < 8; e++) down[c][e] = up[c][e] = 0;
-      for (int i = 0; i < g; i++)
+      for (int e = 0; e < 8; e++) {
+        q2 = fmaf(x[e], x[e], q2);
+        most = fmaxf(most, fabsf(x[e]));
+      }
 #pragma unroll
-        for (int c = 0; c < C; c++) {
-          const uint4 v = ldg16(q + (size_t)i * D + 32 * c);
-          const uint32_t w[4] = {v.x, v.y, v.z, v.w};
+      for (int o = 1; o < D / 4; o <<= 1) {
+        q2 += __shfl_xor(q2, o);
+        most = fmaxf(most, __shfl_xor(most, o));
+      }
+      // f16 parts of numbers up to 2^15
+      const int up = DT == DT_F16 && most > 0 && most < INFINITY ? 15 - (ilogbf(most) + 1) : 0;
+      if (d == 0) {
+        s_q2[row] = q2;
+        s_scale[row] = ldexpf(1.f, -up);
+      }
 #pragma unroll
-          for (int e = 0; e < 8; e++) {
-            const double x = e % 2 ? hi16<DT>(w[e / 2]) : lo16<DT>(w[e / 2]);
-            up[c][e] += x > 0 ? x : x != x ? x : 0;
-            down[c][e] += x < 0 ? x : 0;
-          }
+      for (int e = 0; e < 8; e++) x[e] = ldexpf(x[e], up);
+#pragma unroll
+      for (int part = 0; part < L; part++)
+#pragma unroll
+        for (int e = 0; e < 8; e += 4) {
+          const u32x2 w = {pack2<DT>(x[e], x[e + 1]), pack2<DT>(x[e + 2], x[e + 3])};
+          *(u32x2*)&s_u.q[part][row][(e ? D : 0) + d] = w;
+          const float y[4] = {lo16<DT>(w.x), hi16<DT>(w.x), lo16<DT>(w.y), hi16<DT>(w.y)};
+#pragma unroll
+          for (int j = 0; j < 4; j++) x[e + j] = (x[e + j] - y[j]) * kPart;
         }
     }
+    __syncthreads();
+    float scale[4];
+#pragma unroll
+    for (int i = 0; i < 4; i++) scale[i] = s_scale[4 * grp + i];
+    float norm = 0;
+    uint32_t odd = 0;
     // 16 pages a turn and wave; the next turn's bounds are on their way
     auto fetch = [&](int u0, uint4* v) __attribute__((always_inline)) -> int {
       const int u = u0 + col, id = u < last.n ? page_id(a.r, s, u) : -1;
       const uint16_t* bd = a.bounds + ((size_t)max(id, 0) * a.hkv + h) * 2 * D + 8 * grp;
 #pragma unroll
-      for (int c = 0; c < C; c++) {
-        v[c] = ldg16(bd + 32 * c);
-        v[C + c] = ldg16(bd + D + 32 * c);
-      }
+      for (int c = 0; c < 2 * C; c++) v[c] = ldg16(bd + c / C * D + c % C * 32);
       return id;
     };
     uint4 next[2 * C];
@@ -427,32 +716,73 @@ __global__ __launch_bounds__(SEL_TILE_WAVES * kWave) void select_tile_kernel(Sel
       uint4 v[2 * C];
 #pragma unroll
       for (int c = 0; c < 2 * C; c++) v[c] = next[c];
-      const int id = id_next;
-      id_next = fetch(min(u0 + 16 * SEL_TILE_WAVES, last.n), next);
-      f64x4 acc[2] = {{0, 0, 0, 0}, {0, 0, 0, 0}};
+      const int u = u0 + col, id = id_next;
+      if (u0 + 16 * SEL_TILE_WAVES < last.n) id_next = fetch(u0 + 16 * SEL_TILE_WAVES, next);
+      f32x4 acc[L][2] = {};
+      float b2 = 0;
+      int row = col;  // (hidden: 96 registers of Q would not fit, so it is read from LDS each turn)
+      asm volatile("" : "+v"(row));
 #pragma unroll
-      for (int c = 0; c < C; c++) {
-        const uint32_t w0[4] = {v[c].x, v[c].y, v[c].z, v[c].w};
-        const uint32_t w1[4] = {v[C + c].x, v[C + c].y, v[C + c].z, v[C + c].w};
+      for (int c = 0; c < 2 * C; c++) {
 #pragma unroll
-        for (int e = 0; e < 8; e++) {
-          acc[0] = __builtin_amdgcn_mfma_f64_16x16x4f64(down[c][e], e % 2 ? hi16<DT>(w0[e / 2]) : lo16<DT>(w0[e / 2]),
-                                                        acc[0], 0, 0, 0);
-          acc[1] = __builtin_amdgcn_mfma_f64_16x16x4f64(up[c][e], e % 2 ? hi16<DT>(w1[e / 2]) : lo16<DT>(w1[e / 2]),
-                                                        acc[1], 0, 0, 0);
+        for (int part = 0; part < L; part++) {
+          const uint4 q = *(const uint4*)&s_u.q[part][row][c / C * D + c % C * 32 + 8 * grp];
+          acc[part][c / C] = mfma16<DT>(q, v[c], acc[part][c / C]);
+        }
+        const uint32_t w[4] = {v[c].x, v[c].y, v[c].z, v[c].w};
+#pragma unroll
+        for (int e = 0; e < 4; e++) {
+          b2 = fmaf(lo16<DT>(w[e]), lo16<DT>(w[e]), b2);
+          b2 = fmaf(hi16<DT>(w[e]), hi16<DT>(w[e]), b2);
         }
       }
-      // result rows 4 i + grp, page col
-      if (u0 + col < last.n)
+      b2 += __shfl_xor(b2, 16);
+      b2 += __shfl_xor(b2, 32);
+      if (u < last.n) {
+        norm = fmaxf(norm, b2);
+        if (id < 0 || !(b2 < INFINITY)) odd = 0xffff;
+        // result rows 4 grp + i, page col
 #pragma unroll
-        for (int i = 0; i < 4; i++)
-          s_key[(4 * i + grp) * stride + u0 + col] = id < 0 ? 0 : score_key(acc[0][i] + acc[1][i]);
+        for (int i = 0; i < 4; i++) {
+          float sum = acc[L - 1][0][i] + acc[L - 1][1][i];
+#pragma unroll
+          for (int part = L - 2; part >= 0; part--) sum = fmaf(sum, 1.f / kPart, acc[part][0][i] + acc[part][1][i]);
+          sum *= scale[i];
+          if (!(fabsf(sum) < INFINITY)) odd |= 1u << (4 * grp + i);
+          if (4 * grp + i < nt) reinterpret_cast<uint32_t*>(s_key + (size_t)(4 * grp + i) * stride)[u] = rough_key(sum);
+        }
+      }
     }
+    if (odd) atomicOr(&s_odd, odd);
+    norm = __uint_as_float(wave_max(__float_as_uint(norm)));
+    if (lane == 0) atomicMax(&s_norm, __float_as_uint(norm));
   }
   __syncthreads();
   for (int i = wave; i < nt; i += SEL_TILE_WAVES) {
     const RowPages r = row_pages(a, s, p0 + i);
-    choose<1>(s_key + (size_t)i * stride, r.n, r.f, r.l, r.m, a.top, a.out + ((size_t)(t0 + i) * a.hkv + h) * a.top);
+    int32_t* const out = a.out + ((size_t)(t0 + i) * a.hkv + h) * a.top;
+    uint64_t* const key = s_key + (size_t)i * stride;
+    const bool scored = r.m > 0 && r.m < r.n - r.f - r.l;
+    const float b2 = __uint_as_float(s_norm), q2 = s_q2[i];
+    bool done = !scored;
+    if (!scored || (!(s_odd >> i & 1) && b2 > 1e-30f && b2 < 1e30f && q2 > 1e-30f && q2 < 1e30f)) {
+      const float err = scored ? (float)(D + 8 + g) * (0x1p-23f * (1.f + 1.f / 32)) * (sqrtf(b2) * sqrtf(q2)) : 0.f;
+      uint32_t* const rough = reinterpret_cast<uint32_t*>(key);
+      int* const list = s_u.w[wave].list;
+      uint64_t* const exact = s_u.w[wave].exact;
+      const int turns = (r.n + kWave - 1) / kWave;
+      done = turns <= 4    ? choose_rough<DT, D, 4>(a, s, r, t0 + i, h, err, rough, list, exact, out)
+             : turns <= 8  ? choose_rough<DT, D, 8>(a, s, r, t0 + i, h, err, rough, list, exact, out)
+             : turns <= 16 ? choose_rough<DT, D, 16>(a, s, r, t0 + i, h, err, rough, list, exact, out)
+                           : choose_rough<DT, D, 0>(a, s, r, t0 + i, h, err, rough, list, exact, out);
+    }
+    if (!done) {
+      ExactRow<DT, D> row;
+      row.load(a, t0 + i, h);
+      row.keys(a, s, h, r.n, [](int i) { return i; }, key);
+      wave_sync();
+      choose_from<1, 0>(key, r.n, r.f, r.l, r.m, a.top, out);
+    }
   }
 }
 
@@ -460,9 +790,24 @@ __global__ __launch_bounds__(SEL_TILE_WAVES * kWave) void select_tile_kernel(Sel
 
 using namespace yr;
 
-// Rows of the same sequence share their pages' bounds in a tile.
-static bool select_tiled(bool ragged, int rows, int batch, int max_pages) {
-  return ragged && rows >= SEL_TILE_MIN * (long long)batch && max_pages <= SEL_TILE_PAGES;
+// Rows of a tile: as many as have room for their keys.
+static int select_tile_rows(int max_pages) {
+  int tile = SEL_ROWS;
+  while (tile > 1 && tile * max_pages > SEL_MAX_PAGES) tile /= 2;
+  return tile;
+}
+
+// Rows of the same sequence share their pages' bounds in a tile, but a tile is one
+// workgroup's work, and a row by itself spreads over the chip.  As measured (8 kv
+// heads of 128) tiles take 12 us and 1 us for 57 pages, once per 256 of them, and
+// rows 12 us and 1 us for 18200 pages of all rows and heads:
+//   one sequence of 1024 pages, 16 rows 30 and 21 us, 64 rows 30 and 44; 512 rows of
+//   512 pages 21 and 100, of 2048 94 and 334; 32 rows of 8 sequences, 512 pages, 20
+//   and 20; 4 rows of 64 sequences, 128 pages, 31 and 22.
+static bool select_tiled(bool ragged, long long tiles, long long pairs, int hkv, int max_pages) {
+  if (!ragged || max_pages > SEL_TILE_PAGES) return false;
+  const long long rounds = (tiles * hkv + 255) / 256;
+  return rounds * (684 + max_pages) < 684 + pairs * max_pages / 319;
 }
 
 // Splits per row: enough workgroups to fill the chip, SEL_MIN_CHUNK pages each at least.
@@ -531,10 +876,11 @@ extern "C" int yr_hip_select_pages(const void* q, const void* page_bounds, const
     return fail(YR_E_WORKSPACE, "%s: workspace %zu < %zu", nm, workspace_bytes, need);
   a.tickets = (uint32_t*)workspace;
   a.keys = need ? (uint64_t*)((char*)workspace + kTicketBytes) : nullptr;
-  const bool tiled = select_tiled(qo_indptr != nullptr, rows, batch, a.max_pages);
-  long long tiles = (long long)rows / SEL_ROWS + batch;  // at most, whatever the sequences' rows
+  a.tile = select_tile_rows(a.max_pages);
+  long long tiles = (long long)rows / a.tile + batch;  // at most, whatever the sequences' rows
   if (tiles > rows) tiles = rows;
-  const size_t lds = (size_t)a.max_pages * 8 * (tiled ? SEL_ROWS : 1);
+  const bool tiled = select_tiled(qo_indptr != nullptr, tiles, (long long)rows * hkv, hkv, a.max_pages);
+  const size_t lds = (size_t)a.max_pages * 8 * (tiled ? a.tile : 1);
   const unsigned grid = (unsigned)(tiled ? tiles * hkv : (long long)rows * hkv * a.splits);
   hipStream_t st = (hipStream_t)stream;
 #define YR_SEL(DT_, D_)                                                                        \
