@@ -261,7 +261,7 @@ def _page_table(rows, kv_indptr, kv_indices, kv_len, qo_indptr):
 def _output(out, shape, like):
     """A result of like's dtype, or the caller's."""
     if out is None:
-        return torch.empty(shape, dtype=like.dtype, device=like.device)
+        return like.new_empty(shape)
     if tuple(out.shape) != tuple(shape) or out.dtype is not like.dtype:
         _fail(f"out must be {tuple(shape)} {like.dtype}, got {tuple(out.shape)} {out.dtype}")
     _dense(out)
@@ -427,13 +427,18 @@ def token_logprobs(logits, tokens, top_n: int = 0, n_valid: int | None = None) -
     if tokens.dtype is not torch.int64 or tokens.dim() != 1 or tokens.shape[0] != rows or not tokens.is_contiguous():
         _fail(f"tokens must be contiguous int64 [{rows}]")
     index = _one_device(logits, tokens)
-    dev, n_valid, top_n = logits.device, n if n_valid is None else n_valid, int(top_n)
+    n_valid, top_n = n if n_valid is None else n_valid, int(top_n)
     # one allocation: the ids first (8 bytes each), then the three fp32 results
-    flat = torch.empty(rows * (3 * max(top_n, 0) + 2), dtype=torch.float32, device=dev)
     cut = rows * max(top_n, 0)
-    res = LogProbs(flat[3 * cut: 3 * cut + rows], flat[3 * cut + rows:], flat[2 * cut: 3 * cut].view(rows, -1) if cut else
-                   flat.new_empty((rows, 0)), flat[: 2 * cut].view(torch.int64).view(rows, -1) if cut else
-                   tokens.new_empty((rows, 0)))
+    if logits.dtype is torch.float32:
+        flat = logits.new_empty(3 * cut + 2 * rows)
+    else:
+        flat = torch.empty(3 * cut + 2 * rows, dtype=torch.float32, device=logits.device)
+    ids, tops, lp, ent = flat.split_with_sizes((2 * cut, cut, rows, rows))
+    if cut:
+        res = LogProbs(lp, ent, tops.view(rows, top_n), ids.view(torch.int64).view(rows, top_n))
+    else:
+        res = LogProbs(lp, ent, tops.view(rows, 0), tokens.new_empty((rows, 0)))
     if rows == 0:
         return res
     stream = torch._C._cuda_getCurrentRawStream(index)
@@ -441,7 +446,7 @@ def token_logprobs(logits, tokens, top_n: int = 0, n_valid: int | None = None) -
     at = flat.data_ptr()
     _launch(index, lib().yr_hip_token_logprobs, "token_logprobs", logits.data_ptr(), tokens.data_ptr(), at + 12 * cut,
             at + 12 * cut + 4 * rows, at + 8 * cut, at, rows, n, n_valid, logits.stride(0) if rows > 1 else n, top_n, dt,
-            _scratch(nb, dev, stream), nb, stream)
+            _scratch(nb, logits.device, stream), nb, stream)
     return res
 
 
