@@ -15,6 +15,11 @@
 // already the B operand of the second product (k slots 8 g + 4 j + i of lane
 // group g carry tokens 16 j + 4 g + i), while V^T comes from row-major V by
 // transposing reads in that same order.
+//
+// A decode step is bound by memory and its chain of dependent loads: 32 rows of 128
+// pages of 16, 8 kv heads of 64 (134 MB) 25 us, 5.3 TB/s; one row of 32 pages of 64,
+// d = 128, 12 us, of which the lists 3, the blocks 3, the merges of waves and splits
+// 6.  Many rows are bound by issuing loads and by the softmax between products.
 #include <type_traits>
 
 #include "attn_device.h"
@@ -22,10 +27,11 @@
 
 namespace yr {
 
+constexpr int SP_WAVES = 4;           // (8: 32 rows of 64 pages of 16, d = 128: 26.1 for 25.4 us; 64 of 16 22.1 for 16.4)
 constexpr int SP_BLK = 32;            // tokens per wave block
 constexpr int SP_MAX_ENTRIES = 1024;  // list entries of a tile
-constexpr int SP_TARGET_WG = 256;     // one per CU
-constexpr int SP_MIN_BLOCKS = 4;      // blocks per split at least
+constexpr int SP_TARGET_WG = 256;     // one per CU (512: 4 rows of 32 pages of 64 17.6 us for 14.2, 32 of 64 of 16 30.3 for 25.1)
+constexpr int SP_MIN_BLOCKS = 4;      // blocks per split at least (1 row of 32 pages of 64: 2 16.7 us, 4 13.3, 8 12.4; of 8 pages 10.8, 10.4, 11.4)
 
 struct SparseArgs {
   Ragged r;
@@ -142,24 +148,24 @@ __device__ __forceinline__ int build_union(const SparseArgs& a, const SeqRows& s
   return __builtin_amdgcn_readfirstlane(nsel);
 }
 
-// NW waves; PG32: pages are a multiple of 32 tokens, so a block lies in one page
+// PG32: pages are a multiple of 32 tokens, so a block lies in one page
 // and its address is uniform (else the lanes work out one token's each).
 //
 // K and V go straight into the wave's LDS slots; its next K block is requested
 // as soon as this one's fragments are in registers and its next V block after
 // P V, so one of the two is always in flight.
-template <int DT, int D, int NW, bool PG32>
-__global__ __launch_bounds__(NW * kWave) void sparse_kernel(SparseArgs a) {
-  constexpr int T = NW * kWave;
+template <int DT, int D, bool PG32>
+__global__ __launch_bounds__(SP_WAVES * kWave) void sparse_kernel(SparseArgs a) {
+  constexpr int T = SP_WAVES * kWave;
   constexpr int RPI = 512 / D;      // rows per direct load (64 lanes of 16 bytes)
   constexpr int NL = SP_BLK / RPI;  // loads per operand of a block
   constexpr int CPR = D / 8;        // chunks per row
-  __shared__ __attribute__((aligned(16))) uint16_t s_k[NW][SP_BLK * D];
-  __shared__ __attribute__((aligned(16))) uint16_t s_v[NW][SP_BLK * D];
+  __shared__ __attribute__((aligned(16))) uint16_t s_k[SP_WAVES][SP_BLK * D];
+  __shared__ __attribute__((aligned(16))) uint16_t s_v[SP_WAVES][SP_BLK * D];
   __shared__ int l_u[SP_MAX_ENTRIES], l_id[SP_MAX_ENTRIES];  // union: page, device page id, rows
   __shared__ uint16_t l_mask[SP_MAX_ENTRIES];
-  __shared__ float s_m[NW][16], s_l[NW][16];
-  __shared__ int s_cnt[NW], s_tile[2];
+  __shared__ float s_m[SP_WAVES][16], s_l[SP_WAVES][16];
+  __shared__ int s_cnt[SP_WAVES], s_tile[2];
   static_assert(SP_MAX_ENTRIES * 4 <= (int)sizeof(s_k), "the entries fit where K goes later");
   const int tid = threadIdx.x, lane = tid % kWave;
   const int wave = __builtin_amdgcn_readfirstlane(tid / kWave);
@@ -271,7 +277,7 @@ __global__ __launch_bounds__(NW * kWave) void sparse_kernel(SparseArgs a) {
     auto consume = [&](int blk, auto last_c) __attribute__((always_inline)) {
       constexpr bool LAST = decltype(last_c)::value;
       Block nxt;
-      if constexpr (!LAST) nxt = block(blk + NW);
+      if constexpr (!LAST) nxt = block(blk + SP_WAVES);
       asm volatile("s_waitcnt vmcnt(%0)" ::"n"(NL) : "memory");  // K has landed, V may be on its way
       f32x4 sc[2];
 #pragma unroll
@@ -358,13 +364,13 @@ __global__ __launch_bounds__(NW * kWave) void sparse_kernel(SparseArgs a) {
         cur = nxt;
       }
     };
-    // wave w takes blocks w, w + NW, .. of the split (a fixed order)
+    // wave w takes blocks w, w + SP_WAVES, .. of the split (a fixed order)
     if (blk0 + wave < blk1) {
       int blk = blk0 + wave;
       cur = block(blk);
       issue(cur, std::true_type{});
       issue(cur, std::false_type{});
-      for (; blk + NW < blk1; blk += NW) consume(blk, std::false_type{});
+      for (; blk + SP_WAVES < blk1; blk += SP_WAVES) consume(blk, std::false_type{});
       consume(blk, std::true_type{});
     }
 
@@ -378,7 +384,7 @@ __global__ __launch_bounds__(NW * kWave) void sparse_kernel(SparseArgs a) {
       s_l[wave][col] = l_i;
     }
     __syncthreads();
-    const int live = min(NW, blk1 - blk0);  // waves that had a block
+    const int live = min(SP_WAVES, blk1 - blk0);  // waves that had a block
     bool bad = false;
     for (int idx = tid; idx < 16 * D / 4; idx += T) {
       const int row = idx / (D / 4), d0 = idx % (D / 4) * 4, i = row / G, g = row % G;
@@ -713,12 +719,15 @@ __global__ __launch_bounds__(SW_WAVES * kWave, 2) void sparse_wide_kernel(Sparse
 // Tiles, rows per tile and splits of a call.
 struct SparsePlan {
   long long tiles;
-  int tt, splits, waves;
+  int tt, splits;
   bool wide;
 };
 static SparsePlan sparse_plan(bool ragged, int rows, int batch, int hkv, int G, int page, int top) {
   SparsePlan p;
-  // four groups of rows to a tile where that leaves a workgroup per CU and the lists fit
+  // Four groups of rows to a tile where that leaves a workgroup per CU and the lists
+  // fit (8 kv heads of 4: 777 rows of 16 pages of 64 122 us, one group to a tile 131;
+  // 2048 rows 230 and 272, of 64 pages of 16 320 and 439, d = 64 161 and 185; pages
+  // at random, which rows do not share, 474 and 418).
   const int wide_tt = SW_WAVES * (16 / G);
   p.wide = ragged && G >= 4 && wide_tt * top <= SP_MAX_ENTRIES && (long long)rows / wide_tt * hkv >= SP_TARGET_WG;
   if (p.wide) {
@@ -726,7 +735,6 @@ static SparsePlan sparse_plan(bool ragged, int rows, int batch, int hkv, int G, 
     p.tiles = (long long)rows / p.tt + batch;
     if (p.tiles > rows) p.tiles = rows;
     p.splits = 1;
-    p.waves = SW_WAVES;
     return p;
   }
   p.tt = ragged ? 16 / G : 1;
@@ -738,7 +746,6 @@ static SparsePlan sparse_plan(bool ragged, int rows, int batch, int hkv, int G, 
   if (sp > blocks / SP_MIN_BLOCKS) sp = blocks / SP_MIN_BLOCKS;
   if (pairs > kMaxTickets || sp < 1) sp = 1;
   p.splits = (int)sp;
-  p.waves = pairs * sp > SP_TARGET_WG ? 4 : 8;
   return p;
 }
 
@@ -798,15 +805,15 @@ extern "C" int yr_hip_gqa_sparse_paged(const void* q, const void* k_cache, const
   const unsigned grid = (unsigned)(p.tiles * hkv * p.splits);
   const bool pg32 = page_size % SP_BLK == 0 && !p.wide;
   hipStream_t st = (hipStream_t)stream;
-#define YR_SP(DT_, D_, W_, P_)                                                                              \
-  if (dtype == DT_ && d == D_ && !p.wide && p.waves == W_ && pg32 == P_)                                    \
-    hipLaunchKernelGGL((sparse_kernel<DT_, D_, W_, P_>), dim3(grid), dim3(W_ * kWave), 0, st, a);
+#define YR_SP(DT_, D_, P_)                                                                                  \
+  if (dtype == DT_ && d == D_ && !p.wide && pg32 == P_)                                                     \
+    hipLaunchKernelGGL((sparse_kernel<DT_, D_, P_>), dim3(grid), dim3(SP_WAVES * kWave), 0, st, a);
 #define YR_SP2(DT_, D_)                                                                                     \
   if (dtype == DT_ && d == D_ && p.wide && page_size % SW_BLK == 0)                                         \
     hipLaunchKernelGGL((sparse_wide_kernel<DT_, D_, true>), dim3(grid), dim3(SW_WAVES * kWave), 0, st, a);  \
   if (dtype == DT_ && d == D_ && p.wide && page_size % SW_BLK != 0)                                         \
     hipLaunchKernelGGL((sparse_wide_kernel<DT_, D_, false>), dim3(grid), dim3(SW_WAVES * kWave), 0, st, a); \
-  YR_SP(DT_, D_, 4, false) YR_SP(DT_, D_, 4, true) YR_SP(DT_, D_, 8, false) YR_SP(DT_, D_, 8, true)
+  YR_SP(DT_, D_, false) YR_SP(DT_, D_, true)
   YR_SP2(DT_F16, 64) YR_SP2(DT_F16, 128) YR_SP2(DT_BF16, 64) YR_SP2(DT_BF16, 128)
 #undef YR_SP2
 #undef YR_SP
