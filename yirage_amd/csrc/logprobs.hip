@@ -20,6 +20,10 @@
 // NaN values take no part in the top (as in argmax) and make the sums NaN; a
 // row of nothing but -inf has no distribution: NaN too.  A token outside
 // [0, n_valid) has log probability NaN.
+//
+// Bound by memory for many rows (2048 of 128256 in bf16, 525 MB, top 5: 95 us, 5.5
+// TB/s; without a top 83), by the chain of loads, waves, splits and ranks for few
+// (one row 12 us, 64 of 50000 14).
 #include <type_traits>
 
 #include "attn_device.h"
@@ -45,7 +49,8 @@ constexpr int LP_MAX_TOP = 64;    // a bound comes from 64 lane maxima
 constexpr int LP_BUF = 256;       // candidates a wave holds
 constexpr int LP_MAX_SPLITS = 64; // lists that one wave joins, a lane each
 constexpr int LP_HITS = 128;      // candidate tiles a wave notes (in the candidates' place)
-constexpr int LP_TARGET_WG = 1024;
+constexpr int LP_VALUES = 32;     // values per lane and tile (8: 16 rows of 128256 23.5 for 14.6 us, 1 row 11.9 for 12.0)
+constexpr int LP_TARGET_WG = 1024; // (512: 256 rows of 32000 16.1 for 15.9 us; 2048: of 128256 34.7 for 26.6)
 constexpr float kFar = 1e38f;     // |m| beyond which m log2 e may leave fp32
 
 // A tile with candidates: the lanes that have them, its first piece, its
@@ -231,11 +236,10 @@ __device__ __forceinline__ uint64_t ld_u64(const uint64_t* p) {
   return __hip_atomic_load((const YR_G uint64_t*)p, __ATOMIC_RELAXED, __HIP_MEMORY_SCOPE_AGENT);
 }
 
-// V: values per lane and tile
-template <int DT, int V>
+template <int DT>
 __global__ __launch_bounds__(LP_THREADS) void logprobs_kernel(LogprobArgs a) {
   constexpr int EPP = DT == YR_DTYPE_F32 ? 4 : 8;  // elements per 16-byte piece
-  constexpr int U = V / EPP;                       // pieces per lane and tile
+  constexpr int U = LP_VALUES / EPP;                       // pieces per lane and tile
   constexpr int ES = 16 / EPP;
   constexpr int kTile = kWave * U, kStep = LP_WAVES * kTile;  // pieces
   __shared__ uint64_t s_buf[LP_WAVES][LP_BUF];
@@ -612,21 +616,20 @@ __global__ __launch_bounds__(LP_THREADS) void logprobs_kernel(LogprobArgs a) {
   }
 }
 
-// A row is split until about LP_TARGET_WG workgroups run, each with one tile of
-// all its waves at least.  Where that leaves CUs idle the tiles are small (8
-// values a lane instead of 32).
+// A row is split while LP_TARGET_WG workgroups or fewer run, each with one tile of
+// all its waves at least (1000 rows of 128256 whole 60 us, in two 64).
 struct LogprobPlan {
-  int values, splits, chunk;
+  int splits, chunk;
 };
 static LogprobPlan logprobs_plan(int rows, int n, int dtype) {
   const int epp = dtype == YR_DTYPE_F32 ? 4 : 8;
   const int np = (n - 1) / epp + 2;  // pieces; a row off its boundary has one more
   LogprobPlan p;
-  p.values = (long long)rows * np < 256ll * LP_THREADS * 32 / epp ? 8 : 32;
-  const int tile = LP_THREADS * p.values / epp, most = (np + tile - 1) / tile;
-  int sp = (LP_TARGET_WG + rows - 1) / rows;
+  const int tile = LP_THREADS * LP_VALUES / epp, most = (np + tile - 1) / tile;
+  int sp = LP_TARGET_WG / rows;
   if (sp > LP_MAX_SPLITS) sp = LP_MAX_SPLITS;
   if (sp > most) sp = most;
+  if (sp < 1) sp = 1;
   p.chunk = ((np + sp - 1) / sp + tile - 1) / tile * tile;
   p.splits = (np + p.chunk - 1) / p.chunk;
   return p;
@@ -669,11 +672,9 @@ extern "C" int yr_hip_token_logprobs(const void* x, const int64_t* tokens, float
   hipStream_t st = (hipStream_t)stream;
   const dim3 grid((unsigned)(rows * a.splits));
   const size_t lds = (size_t)(a.splits > 1 ? a.splits + 1 : 1) * top_n * sizeof(uint64_t);
-#define YR_LP(DT_, V_)                     \
-  if (dtype == DT_ && p.values == V_)      \
-    hipLaunchKernelGGL((logprobs_kernel<DT_, V_>), grid, dim3(LP_THREADS), lds, st, a);
-  YR_LP(YR_DTYPE_F16, 8) YR_LP(YR_DTYPE_F16, 32) YR_LP(YR_DTYPE_BF16, 8) YR_LP(YR_DTYPE_BF16, 32)
-  YR_LP(YR_DTYPE_F32, 8) YR_LP(YR_DTYPE_F32, 32)
+#define YR_LP(DT_) \
+  if (dtype == DT_) hipLaunchKernelGGL((logprobs_kernel<DT_>), grid, dim3(LP_THREADS), lds, st, a);
+  YR_LP(YR_DTYPE_F16) YR_LP(YR_DTYPE_BF16) YR_LP(YR_DTYPE_F32)
 #undef YR_LP
   YR_CHECK_LAUNCH(nm);
   return YR_OK;
