@@ -29,14 +29,13 @@ struct SelectArgs {
   int hq, hkv, max_pages, top, first, last, splits, chunk, tile;  // tile: rows
 };
 
-constexpr int SEL_THREADS = 256;
-constexpr int SEL_WAVES = SEL_THREADS / kWave;
+constexpr int SEL_WAVES = 8;          // of a workgroup, or
+constexpr int SEL_MANY = 16;          // where there is work enough
 constexpr int SEL_MAX_PAGES = 16384;  // 64-bit keys of one row in LDS: 128 of 160 KiB
 constexpr int SEL_ROWS = 16;          // rows of a tile
 constexpr int SEL_TILE_WAVES = 16;    // a row's list each: 512 rows of 512 pages 21 us, 23 with 8
 constexpr int SEL_TILE_PAGES = 4096;  // a tile's keys in LDS: as much, 4 rows at least
-constexpr int SEL_TARGET_WG = 1024;
-constexpr int SEL_MIN_CHUNK = 64;     // pages per split at least
+constexpr int SEL_MIN_CHUNK = 128;    // pages per split at least
 
 // Whole-number order of a score: larger is better, -0 equals 0, NaN is last.
 __device__ __forceinline__ uint64_t score_key(double s) {
@@ -85,7 +84,7 @@ __device__ __forceinline__ double group_sum(double v) {
 // two bits a step, which costs three counts and saves an exchange.
 template <int W, int R>
 __device__ __forceinline__ void choose_from(const uint64_t* key, int n, int f, int l, int m, int top, int32_t* out) {
-  __shared__ uint64_t s_cnt[2][SEL_WAVES], s_diff[SEL_WAVES];
+  __shared__ uint64_t s_cnt[2][W], s_diff[W];
   __shared__ int s_pos[kWave];
   const int lane = threadIdx.x % kWave, wave = W == 1 ? 0 : __builtin_amdgcn_readfirstlane(threadIdx.x / kWave);
   const int c0 = f, c1 = n - l;  // candidates
@@ -176,7 +175,7 @@ __device__ __forceinline__ void choose_from(const uint64_t* key, int n, int f, i
     }
   }
   // ascending list; the waves take blocks of 64 pages in turn
-  if constexpr (W > 1 && R > 0) {
+  if constexpr (W > 1 && R > 0 && R * W <= kWave) {
     if (equal == 0x7fffffff) {  // (uniform) no ties: one exchange of every block's count
       uint64_t taken[R];
       int mine = 0;  // lane i: block i's
@@ -242,7 +241,8 @@ __device__ __forceinline__ void choose_from(const uint64_t* key, int n, int f, i
 template <int W>
 __device__ __forceinline__ void choose(const uint64_t* key, int n, int f, int l, int m, int top, int32_t* out) {
   const int turns = (n + W * kWave - 1) / (W * kWave);
-  if (turns <= 4) choose_from<W, 4>(key, n, f, l, m, top, out);
+  if (turns <= 1) choose_from<W, 1>(key, n, f, l, m, top, out);
+  else if (turns <= 4) choose_from<W, 4>(key, n, f, l, m, top, out);
   else if (turns <= 8) choose_from<W, 8>(key, n, f, l, m, top, out);
   else if (turns <= 16) choose_from<W, 16>(key, n, f, l, m, top, out);
   else choose_from<W, 0>(key, n, f, l, m, top, out);
@@ -285,10 +285,13 @@ __device__ __forceinline__ double page_dot(const double* down, const double* up,
 }
 
 // One row and kv head, its pages split over `splits` workgroups; the last one
-// to arrive chooses.
-template <int DT, int D>
-__global__ __launch_bounds__(SEL_THREADS) void select_kernel(SelectArgs a) {
-  constexpr int LPP = D / 8, PPB = SEL_THREADS / LPP, U = 4;  // lanes per page, pages per pass, passes in flight
+// to arrive chooses.  Bound by memory where there are rows enough (32 of 1024 pages,
+// 8 kv heads of 128, 105 MB: 27 us, of which the scores 20), else by the chain of
+// page id, bounds, tickets, keys and steps of the border (one of 2048 pages 13 us).
+template <int DT, int D, int W>
+__global__ __launch_bounds__(W * kWave) void select_kernel(SelectArgs a) {
+  constexpr int T = W * kWave;
+  constexpr int LPP = D / 8, PPB = T / LPP, U = 4;  // lanes per page, pages per pass, passes in flight
   extern __shared__ uint64_t s_key[];
   __shared__ double s_q[2][D];
   const int split = blockIdx.x % a.splits, pair = blockIdx.x / a.splits;
@@ -301,7 +304,7 @@ __global__ __launch_bounds__(SEL_THREADS) void select_kernel(SelectArgs a) {
   const bool scored = r.m > 0 && r.m < r.n - r.f - r.l;
   if (scored) {
     const int g = a.hq / a.hkv;
-    for (int d = tid; d < D; d += SEL_THREADS) {
+    for (int d = tid; d < D; d += T) {
       double up = 0, down = 0;
       const uint16_t* q = a.q + ((size_t)t * a.hq + (size_t)h * g) * D + d;
       for (int i0 = 0; i0 < g; i0 += 4) {  // 4 loads in flight
@@ -357,20 +360,20 @@ __global__ __launch_bounds__(SEL_THREADS) void select_kernel(SelectArgs a) {
     if (a.splits > 1) {
       if (!arrive_last(&a.tickets[pair], a.splits)) return;
       const uint64_t* const keys = a.keys + (size_t)pair * a.max_pages;
-      for (int u0 = r.f + tid; u0 < r.n - r.l; u0 += 8 * SEL_THREADS) {  // 8 loads in flight
+      for (int u0 = r.f + tid; u0 < r.n - r.l; u0 += 8 * T) {  // 8 loads in flight
         uint64_t k[8];
 #pragma unroll
-        for (int i = 0; i < 8; i++) k[i] = sel_load(keys + min(u0 + i * SEL_THREADS, r.n - r.l - 1));
+        for (int i = 0; i < 8; i++) k[i] = sel_load(keys + min(u0 + i * T, r.n - r.l - 1));
 #pragma unroll
         for (int i = 0; i < 8; i++)
-          if (u0 + i * SEL_THREADS < r.n - r.l) s_key[u0 + i * SEL_THREADS] = k[i];
+          if (u0 + i * T < r.n - r.l) s_key[u0 + i * T] = k[i];
       }
     }
     __syncthreads();
   } else if (split > 0) {
     return;  // nothing to compare: the first workgroup writes the list
   }
-  choose<SEL_WAVES>(s_key, r.n, r.f, r.l, r.m, a.top, out);
+  choose<W>(s_key, r.n, r.f, r.l, r.m, a.top, out);
 }
 
 // Memory that a wave's lanes wrote, before they read each other's.
@@ -810,22 +813,33 @@ static bool select_tiled(bool ragged, long long tiles, long long pairs, int hkv,
   return rounds * (684 + max_pages) < 684 + pairs * max_pages / 319;
 }
 
-// Splits per row: enough workgroups to fill the chip, SEL_MIN_CHUNK pages each at least.
-static void select_plan(long long pairs, int max_pages, int* splits, int* chunk) {
-  long long sp = (SEL_TARGET_WG + pairs - 1) / pairs;
+// Waves per workgroup and splits per row: as many as run at once, 16 waves a CU.
+// A workgroup of 16 where that lets every row and head have one for itself, and for
+// rows whose keys would not fit into the registers of 8 waves otherwise (8 kv heads
+// of 128; rows, pages, us with 16 and 8 waves): 18 1024 23.8 25.0; 32 256 13.1 15.2;
+// 32 1024 26.9 32.6; 4 6144 36.2 42.4; 8 8192 56 64; but 1 2048 17.4 13.2; 16 1024
+// 22.5 22.2; 40 1024 43.1 38.2; 128 512 61 44.  One split more than run at once, 24
+// rows of 1024 pages: 38.3 for 24.4.
+struct SelectPlan {
+  int waves, splits, chunk;
+};
+static SelectPlan select_plan(long long pairs, int max_pages) {
+  SelectPlan p;
+  p.waves = (pairs > 128 && pairs <= 256) || max_pages >= 6144 ? SEL_MANY : SEL_WAVES;
+  const long long target = 256 * 16 / p.waves;
+  long long sp = target > pairs ? target / pairs : 1;
   const int most = (max_pages + SEL_MIN_CHUNK - 1) / SEL_MIN_CHUNK;
   if (sp > most) sp = most;
-  *chunk = (int)((max_pages + sp - 1) / sp);
-  *splits = (max_pages + *chunk - 1) / *chunk;
+  p.chunk = (int)((max_pages + sp - 1) / sp);
+  p.splits = (max_pages + p.chunk - 1) / p.chunk;
+  return p;
 }
 
 extern "C" size_t yr_hip_select_pages_workspace(int rows, int hkv, int page_size, int max_kv_len) {
   if (rows <= 0 || hkv <= 0 || page_size <= 0 || max_kv_len <= 0) return 0;
-  int splits, chunk;
   const long long pairs = (long long)rows * hkv;
   const int max_pages = (max_kv_len - 1) / page_size + 1;
-  select_plan(pairs, max_pages, &splits, &chunk);
-  return splits > 1 ? kTicketBytes + (size_t)pairs * max_pages * sizeof(uint64_t) : 0;
+  return select_plan(pairs, max_pages).splits > 1 ? kTicketBytes + (size_t)pairs * max_pages * sizeof(uint64_t) : 0;
 }
 
 // A launch with `lds` bytes of dynamic LDS.
@@ -870,7 +884,9 @@ extern "C" int yr_hip_select_pages(const void* q, const void* page_bounds, const
   a.top = top_pages;
   a.first = first_pages;
   a.last = last_pages;
-  select_plan((long long)rows * hkv, a.max_pages, &a.splits, &a.chunk);
+  const SelectPlan p = select_plan((long long)rows * hkv, a.max_pages);
+  a.splits = p.splits;
+  a.chunk = p.chunk;
   const size_t need = yr_hip_select_pages_workspace(rows, hkv, page_size, max_kv_len);
   if (need > workspace_bytes || (need && !workspace))
     return fail(YR_E_WORKSPACE, "%s: workspace %zu < %zu", nm, workspace_bytes, need);
@@ -886,7 +902,9 @@ extern "C" int yr_hip_select_pages(const void* q, const void* page_bounds, const
 #define YR_SEL(DT_, D_)                                                                        \
   if (dtype == DT_ && d == D_)                                                                 \
     return tiled ? select_launch(nm, select_tile_kernel<DT_, D_>, grid, SEL_TILE_WAVES * kWave, lds, st, a) \
-                 : select_launch(nm, select_kernel<DT_, D_>, grid, SEL_THREADS, lds, st, a);
+           : p.waves == SEL_MANY                                                               \
+               ? select_launch(nm, select_kernel<DT_, D_, SEL_MANY>, grid, SEL_MANY * kWave, lds, st, a)   \
+               : select_launch(nm, select_kernel<DT_, D_, SEL_WAVES>, grid, SEL_WAVES * kWave, lds, st, a);
   YR_SEL(DT_F16, 64) YR_SEL(DT_F16, 128) YR_SEL(DT_BF16, 64) YR_SEL(DT_BF16, 128)
 #undef YR_SEL
   return fail(YR_E_INVALID, "%s: shape", nm);
