@@ -29,8 +29,6 @@ struct SelectArgs {
   int hq, hkv, max_pages, top, first, last, splits, chunk, tile;  // tile: rows
 };
 
-constexpr int SEL_WAVES = 8;          // of a workgroup, or
-constexpr int SEL_MANY = 16;          // where there is work enough
 constexpr int SEL_MAX_PAGES = 16384;  // 64-bit keys of one row in LDS: 128 of 160 KiB
 constexpr int SEL_ROWS = 16;          // rows of a tile
 constexpr int SEL_TILE_WAVES = 16;    // a row's list each: 512 rows of 512 pages 21 us, 23 with 8
@@ -813,19 +811,24 @@ static bool select_tiled(bool ragged, long long tiles, long long pairs, int hkv,
   return rounds * (684 + max_pages) < 684 + pairs * max_pages / 319;
 }
 
-// Waves per workgroup and splits per row: as many as run at once, 16 waves a CU.
-// A workgroup of 16 where that lets every row and head have one for itself, and for
-// rows whose keys would not fit into the registers of 8 waves otherwise (8 kv heads
-// of 128; rows, pages, us with 16 and 8 waves): 18 1024 23.8 25.0; 32 256 13.1 15.2;
-// 32 1024 26.9 32.6; 4 6144 36.2 42.4; 8 8192 56 64; but 1 2048 17.4 13.2; 16 1024
-// 22.5 22.2; 40 1024 43.1 38.2; 128 512 61 44.  One split more than run at once, 24
-// rows of 1024 pages: 38.3 for 24.4.
+// Waves per workgroup and splits per row: as many as run at once, 16 waves a CU (one
+// split more, 24 rows of 1024 pages: 38.3 us for 24.4).  Times with 8 kv heads of 128:
+//   16 waves where every row and head then has a workgroup for itself at once, and
+//   for rows whose keys would not fit into the registers of 8: 18 rows of 1024 pages
+//   23.8 (8 waves 25.0), 32 of 256 13.1 (15.2), 32 of 1024 26.9 (32.6), 4 of 6144 36.2
+//   (42.4), 8 of 8192 56 (64); but 1 of 2048 17.4 (13.2), 40 of 1024 43.1 (38.2);
+//   4 waves for more rows than 8 of them run at once, and for few pages: 64 rows of
+//   64 pages 8.3 (8 waves 10.1), 128 of 64 10.4 (17.5), 256 of 128 27.6 (37.4), 128
+//   of 512 41.7 (44.3); but 64 of 256 19.8 (17.1).
 struct SelectPlan {
   int waves, splits, chunk;
 };
 static SelectPlan select_plan(long long pairs, int max_pages) {
   SelectPlan p;
-  p.waves = (pairs > 128 && pairs <= 256) || max_pages >= 6144 ? SEL_MANY : SEL_WAVES;
+  p.waves = max_pages >= 6144                 ? 16
+            : max_pages <= 64 || pairs > 512  ? 4
+            : pairs > 128 && pairs <= 256     ? 16
+                                              : 8;
   const long long target = 256 * 16 / p.waves;
   long long sp = target > pairs ? target / pairs : 1;
   const int most = (max_pages + SEL_MIN_CHUNK - 1) / SEL_MIN_CHUNK;
@@ -902,9 +905,9 @@ extern "C" int yr_hip_select_pages(const void* q, const void* page_bounds, const
 #define YR_SEL(DT_, D_)                                                                        \
   if (dtype == DT_ && d == D_)                                                                 \
     return tiled ? select_launch(nm, select_tile_kernel<DT_, D_>, grid, SEL_TILE_WAVES * kWave, lds, st, a) \
-           : p.waves == SEL_MANY                                                               \
-               ? select_launch(nm, select_kernel<DT_, D_, SEL_MANY>, grid, SEL_MANY * kWave, lds, st, a)   \
-               : select_launch(nm, select_kernel<DT_, D_, SEL_WAVES>, grid, SEL_WAVES * kWave, lds, st, a);
+           : p.waves == 4 ? select_launch(nm, select_kernel<DT_, D_, 4>, grid, 4 * kWave, lds, st, a)      \
+           : p.waves == 8 ? select_launch(nm, select_kernel<DT_, D_, 8>, grid, 8 * kWave, lds, st, a)      \
+                          : select_launch(nm, select_kernel<DT_, D_, 16>, grid, 16 * kWave, lds, st, a);
   YR_SEL(DT_F16, 64) YR_SEL(DT_F16, 128) YR_SEL(DT_BF16, 64) YR_SEL(DT_BF16, 128)
 #undef YR_SEL
   return fail(YR_E_INVALID, "%s: shape", nm);
