@@ -800,15 +800,15 @@ static int select_tile_rows(int max_pages) {
 
 // Rows of the same sequence share their pages' bounds in a tile, but a tile is one
 // workgroup's work, and a row by itself spreads over the chip.  As measured (8 kv
-// heads of 128) tiles take 12 us and 1 us for 57 pages, once per 256 of them, and
-// rows 12 us and 1 us for 18200 pages of all rows and heads:
-//   one sequence of 1024 pages, 16 rows 30 and 21 us, 64 rows 30 and 44; 512 rows of
-//   512 pages 21 and 100, of 2048 94 and 334; 32 rows of 8 sequences, 512 pages, 20
-//   and 20; 4 rows of 64 sequences, 128 pages, 31 and 22.
+// heads of 128) tiles take 10 us and 1 us for 57 pages, once per 256 of them, and
+// rows 8 us and 1 us for 19400 pages of all rows and heads.  Tiles and rows, us: one
+// sequence of 1024 pages, 16 rows 30 and 22, 32 rows 28 and 23, 48 rows 28 and 35; 512
+// rows of 512 pages 21 and 98, of 2048 93 and 333; 8 rows of 8 sequences, 512 pages,
+// 18 and 20; 16 of 4, 128 pages, 12.4 and 10.1; 4 of 64, 128 pages, 30 and 19.
 static bool select_tiled(bool ragged, long long tiles, long long pairs, int hkv, int max_pages) {
   if (!ragged || max_pages > SEL_TILE_PAGES) return false;
   const long long rounds = (tiles * hkv + 255) / 256;
-  return rounds * (684 + max_pages) < 684 + pairs * max_pages / 319;
+  return rounds * (570 + max_pages) < 456 + pairs * max_pages / 340;
 }
 
 // Waves per workgroup and splits per row: as many as run at once, 16 waves a CU (one
