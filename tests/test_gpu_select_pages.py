@@ -119,7 +119,7 @@ def test_missing_pages_and_short_bounds(news):
 
 @pytest.mark.parametrize("dt", [torch.float16, torch.bfloat16], ids=["f16", "bf16"])
 @pytest.mark.parametrize("lens,news,hq,hkv,d,page,top,first,last", [
-    ([4800], [350], 4, 1, 64, 16, 33, 1, 1), ([900, 5000, 40], [300, 420, 40], 14, 2, 128, 16, 16, 1, 2),
+    ([4800], [700], 4, 1, 64, 16, 33, 1, 1), ([900, 5000, 40], [300, 420, 40], 14, 2, 128, 16, 16, 1, 2),
     ([2200], [450], 2, 2, 64, 1, 40, 2, 3),          # 8 rows a tile
     ([300, 3900], [200, 330], 4, 4, 128, 1, 20, 1, 1),  # 4 rows a tile
     ([9000], [400], 4, 4, 64, 16, 130, 3, 4),        # more pages taken than a wave has lanes
@@ -135,7 +135,7 @@ def test_tiles(lens, news, hq, hkv, d, page, top, first, last, dt):
 def test_tiles_near_the_border(kind, top, dt):
     """Scores that fp32 cannot tell apart, equal ones, and rows beyond its range."""
     print("case", kind, top, dt, flush=True)
-    d, page, n, rows = 64, 16, 300, 360
+    d, page, n, rows = 64, 16, 300, 700
     b = Batch([n * page], [rows], page)
     gen = torch.Generator().manual_seed(top)
     q = torch.randn((b.rows, 2, d), generator=gen).to(dt)
