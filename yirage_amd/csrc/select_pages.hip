@@ -402,7 +402,7 @@ __device__ __forceinline__ uint32_t wave_max(uint32_t v) {
 // Exact scores by one wave: D / 8 lanes a page, 8 channels each.
 template <int DT, int D>
 struct ExactRow {
-  static constexpr int LPP = D / 8, PP = kWave / LPP, U = 2;  // lanes per page, pages per pass, passes in flight
+  static constexpr int LPP = D / 8, PP = kWave / LPP;  // lanes per page, pages per pass
   double down[8], up[8];
   // row t, kv head h
   __device__ __forceinline__ void load(const SelectArgs& a, int t, int h) {
@@ -426,26 +426,11 @@ struct ExactRow {
   template <class F>
   __device__ __forceinline__ void keys(const SelectArgs& a, const SeqRows& s, int h, int n, F page, uint64_t* out) {
     const int lane = threadIdx.x % kWave, j = lane % LPP;
-    for (int i0 = 0; i0 < n; i0 += U * PP) {
-      int id[U];
-      uint4 mn[U], mx[U];
-#pragma unroll
-      for (int k = 0; k < U; k++) {
-        const int i = i0 + k * PP + lane / LPP;
-        id[k] = i < n ? page_id(a.r, s, page(i)) : -1;
-      }
-#pragma unroll
-      for (int k = 0; k < U; k++) {
-        const uint16_t* bd = a.bounds + ((size_t)max(id[k], 0) * a.hkv + h) * 2 * D + 8 * j;
-        mn[k] = ldg16(bd);
-        mx[k] = ldg16(bd + D);
-      }
-#pragma unroll
-      for (int k = 0; k < U; k++) {
-        const double sum = group_sum<LPP>(page_dot<DT>(down, up, mn[k], mx[k]));
-        const int i = i0 + k * PP + lane / LPP;
-        if (j == 0 && i < n) out[i] = id[k] < 0 ? 0 : score_key(sum);
-      }
+    for (int i0 = 0; i0 < n; i0 += PP) {
+      const int i = i0 + lane / LPP, id = i < n ? page_id(a.r, s, page(i)) : -1;
+      const uint16_t* bd = a.bounds + ((size_t)max(id, 0) * a.hkv + h) * 2 * D + 8 * j;
+      const double sum = group_sum<LPP>(page_dot<DT>(down, up, ldg16(bd), ldg16(bd + D)));
+      if (j == 0 && i < n) out[i] = id < 0 ? 0 : score_key(sum);
     }
   }
 };
