@@ -248,24 +248,27 @@ __global__ __launch_bounds__(SP_WAVES * kWave) void sparse_kernel(SparseArgs a) 
       constexpr bool IS_K = decltype(is_k_c)::value;
       const uint16_t* const cache = IS_K ? a.kc : a.vc;
       uint16_t* const dst = IS_K ? ks : vs;
+      auto rows = [&](auto whole_c) __attribute__((always_inline)) {
 #pragma unroll
-      for (int u = 0; u < NL; u++) {
-        const int row = RPI * u + lane / CPR;
-        const int chunk = 8 * ((lane % CPR) ^ (IS_K ? k_swz<D>(row) : v_swz<D>(row)));
-        const uint16_t* src;
-        if constexpr (PG32) {
-          // rows that no row of the tile sees yet: the last visible one (in this page, maybe before the block)
-          if (pmax - t.pos >= SP_BLK - 1)  // (uniform)
+        for (int u = 0; u < NL; u++) {
+          const int row = RPI * u + lane / CPR;
+          const int chunk = 8 * ((lane % CPR) ^ (IS_K ? k_swz<D>(row) : v_swz<D>(row)));
+          const uint16_t* src;
+          if constexpr (decltype(whole_c)::value) {
             src = reinterpret_cast<const uint16_t*>(reinterpret_cast<const char*>(cache + t.off) +
                                                     2u * (uint32_t)(row * (int)tok_stride + chunk));
-          else
+          } else if constexpr (PG32) {
+            // rows that no row of the tile sees yet: the last visible one (in this page, maybe before the block)
             src = cache + t.off + (long long)min(row, pmax - t.pos) * (long long)tok_stride + chunk;
-        } else {
-          const uint32_t lo = (uint32_t)__shfl((int)(uint32_t)t.off, row), hi = (uint32_t)__shfl((int)(t.off >> 32), row);
-          src = cache + ((size_t)hi << 32 | lo) + chunk;
+          } else {
+            const uint32_t lo = (uint32_t)__shfl((int)(uint32_t)t.off, row), hi = (uint32_t)__shfl((int)(t.off >> 32), row);
+            src = cache + ((size_t)hi << 32 | lo) + chunk;
+          }
+          lds_load16(src, dst + RPI * u * D);
         }
-        lds_load16(src, dst + RPI * u * D);
-      }
+      };
+      if (PG32 && pmax - t.pos >= SP_BLK - 1) rows(std::true_type{});  // (uniform)
+      else rows(std::false_type{});
     };
     float m_i = -INFINITY, l_i = 0.f;
     f32x4 acc[D / 16];
@@ -595,23 +598,27 @@ __global__ __launch_bounds__(SW_WAVES * kWave, 2) void sparse_wide_kernel(Sparse
       at += SW_BLK;
     };
     auto issue = [&](uint16_t* kd, uint16_t* vd) __attribute__((always_inline)) {
+      auto rows = [&](auto whole_c) __attribute__((always_inline)) {
 #pragma unroll
-      for (int u = 0; u < NL; u++) {
-        const int row = RPI * u + tid / CPR, c = lane % CPR;
-        // a wave's part of the instruction: 512 / D rows from here on
-        const int first = (RPI * u + wave * (512 / D)) * D, ck = 8 * (c ^ k_swz<D>(row)), cv = 8 * (c ^ v_swz<D>(row));
-        if (PG64 && over >= SW_BLK - 1) {  // (uniform)
-          const uint32_t o = (uint32_t)row * (uint32_t)tok_stride;
-          lds_load16(reinterpret_cast<const uint16_t*>(reinterpret_cast<const char*>(a.kc + off) + 2u * (o + ck)), kd + first);
-          lds_load16(reinterpret_cast<const uint16_t*>(reinterpret_cast<const char*>(a.vc + off) + 2u * (o + cv)), vd + first);
-        } else {
-          size_t o;
-          if constexpr (PG64) o = off + (long long)min(row, over) * (long long)tok_stride;  // (maybe before the block)
-          else o = (size_t)(uint32_t)__shfl((int)(off >> 32), row) << 32 | (uint32_t)__shfl((int)(uint32_t)off, row);
-          lds_load16(a.kc + o + ck, kd + first);
-          lds_load16(a.vc + o + cv, vd + first);
+        for (int u = 0; u < NL; u++) {
+          const int row = RPI * u + tid / CPR, c = lane % CPR;
+          // a wave's part of the instruction: 512 / D rows from here on
+          const int first = (RPI * u + wave * (512 / D)) * D, ck = 8 * (c ^ k_swz<D>(row)), cv = 8 * (c ^ v_swz<D>(row));
+          if constexpr (decltype(whole_c)::value) {
+            const uint32_t o = (uint32_t)row * (uint32_t)tok_stride;
+            lds_load16(reinterpret_cast<const uint16_t*>(reinterpret_cast<const char*>(a.kc + off) + 2u * (o + ck)), kd + first);
+            lds_load16(reinterpret_cast<const uint16_t*>(reinterpret_cast<const char*>(a.vc + off) + 2u * (o + cv)), vd + first);
+          } else {
+            size_t o;
+            if constexpr (PG64) o = off + (long long)min(row, over) * (long long)tok_stride;  // (maybe before the block)
+            else o = (size_t)(uint32_t)__shfl((int)(off >> 32), row) << 32 | (uint32_t)__shfl((int)(uint32_t)off, row);
+            lds_load16(a.kc + o + ck, kd + first);
+            lds_load16(a.vc + o + cv, vd + first);
+          }
         }
-      }
+      };
+      if (PG64 && over >= SW_BLK - 1) rows(std::true_type{});  // (uniform)
+      else rows(std::false_type{});
     };
     auto step = [&](int blk, const uint16_t* ks, uint16_t* vs, uint16_t* kn, uint16_t* vn) __attribute__((always_inline)) {
       asm volatile("s_waitcnt vmcnt(0) lgkmcnt(0)" ::: "memory");
