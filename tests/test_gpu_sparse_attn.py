@@ -167,3 +167,21 @@ def test_padded_rows_are_left_alone():
     ref, tol = _reference(b, q[:8], k, v, pages[:8], 2)
     assert ((out[:8].cpu().double() - ref).abs() <= tol).all()
     assert (out[8:] == 5).all()
+
+
+# Rows enough for four groups of them to a tile.
+
+
+@DTS
+@pytest.mark.parametrize("lens,news,hq,hkv,d,page,top", [
+    ([1100], [1010], 32, 8, 128, 64, 4), ([400, 360], [390, 310], 40, 8, 64, 16, 5), ([300], [250], 128, 8, 64, 64, 3),
+    ([600, 500], [560, 440], 28, 4, 128, 48, 6), ([1010], [1010], 32, 8, 64, 128, 2),
+])
+def test_rows_of_wide_tiles(lens, news, hq, hkv, d, page, top, dt):
+    test_rows(lens, news, hq, hkv, d, page, top, dt)
+
+
+@DTS
+@pytest.mark.parametrize("hq,page,before,rows,hkv", [(64, 24, 20, 480, 8), (32, 64, 20, 1000, 8)])
+def test_values_that_other_rows_of_wide_tiles_see(hq, page, before, rows, hkv, dt):
+    test_values_that_other_rows_see(hq, page, before, rows, hkv, dt)

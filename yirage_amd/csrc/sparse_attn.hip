@@ -731,12 +731,15 @@ struct SparsePlan {
 };
 static SparsePlan sparse_plan(bool ragged, int rows, int batch, int hkv, int G, int page, int top) {
   SparsePlan p;
-  // Four groups of rows to a tile where that leaves a workgroup per CU and the lists
-  // fit (8 kv heads of 4: 777 rows of 16 pages of 64 122 us, one group to a tile 131;
-  // 2048 rows 230 and 272, of 64 pages of 16 320 and 439, d = 64 161 and 185; pages
-  // at random, which rows do not share, 474 and 418).
+  // Four groups of rows to a tile where its workgroups, two a CU, fill their rounds
+  // well enough and the lists fit.  One group to a tile loads shared pages again, in
+  // any number of workgroups, and works out every token's address unless pages are a
+  // multiple of 32 (8 kv heads of 4, d = 128; rows, pages, us with four groups and one):
+  // 777 16 of 64 121 111; 777 16 of 16 57 77; 1200 16 of 64 174 140; 2048 16 of 64 224
+  // 242, 64 of 16 319 455, 32 of 32 269 248; 2048 of 8 heads, d = 64, 158 177.
   const int wide_tt = SW_WAVES * (16 / G);
-  p.wide = ragged && G >= 4 && wide_tt * top <= SP_MAX_ENTRIES && (long long)rows / wide_tt * hkv >= SP_TARGET_WG;
+  const long long wide = ((long long)rows + wide_tt - 1) / wide_tt * hkv, slots = (wide + 511) / 512 * 512;
+  p.wide = ragged && G >= 4 && wide_tt * top <= SP_MAX_ENTRIES && 100 * slots < wide * (page % SP_BLK ? 140 : 108);
   if (p.wide) {
     p.tt = wide_tt;
     p.tiles = (long long)rows / p.tt + batch;
