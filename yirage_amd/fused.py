@@ -212,7 +212,7 @@ def _dense(*ts):
 
 def _launch(index: int, fn, what: str, *args):
     """fn(*args) with the tensors' device current."""
-    if torch.cuda.current_device() == index:
+    if torch._C._cuda_getDevice() == index:
         rc = fn(*args)
     else:
         with torch.cuda.device(index):
@@ -281,44 +281,51 @@ def append_kv_paged(k, v, k_cache, v_cache, kv_indptr, kv_indices, kv_len, q=Non
     [T, Hkv, Hq / Hkv, D]; q, k and v may be slices of one projection (last dim contiguous, 16-byte
     aligned).  out may be q itself where that is contiguous.  D is 64 or 128."""
     dtype = k.dtype
-    for t in (v, k_cache, v_cache, q, q_norm, k_norm, page_bounds):
+    dt = dtype_code(dtype)
+    for t in (v, q):
         if t is not None and t.dtype is not dtype:
             _fail(f"operand dtype {t.dtype} differs from k's {dtype}")
-    dt = dtype_code(dtype)
-    if k.dim() != 3 or v.shape != k.shape or k_cache.dim() != 4 or v_cache.shape != k_cache.shape:
+    for t in (k_cache, v_cache, page_bounds, q_norm, k_norm):
+        if t is not None and (t.dtype is not dtype or not t.is_contiguous()):
+            if t.dtype is not dtype:
+                _fail(f"operand dtype {t.dtype} differs from k's {dtype}")
+            _dense(t)
+    kshape, cshape = k.shape, k_cache.shape
+    if len(kshape) != 3 or v.shape != kshape or len(cshape) != 4 or v_cache.shape != cshape:
         _fail("k and v must be [T, Hkv, D], the caches [P, page, Hkv, D]")
-    T, hkv, D = k.shape
-    P, page, h2, d2 = k_cache.shape
+    T, hkv, D = kshape
+    P, page, h2, d2 = cshape
     if h2 != hkv or d2 != D:
         _fail(f"cache heads {(h2, d2)} differ from k's {(hkv, D)}")
     batch = _page_table(T, kv_indptr, kv_indices, kv_len, qo_indptr)
-    _dense(k_cache, v_cache, cos, sin, q_norm, k_norm, page_bounds)
-    if page_bounds is not None and tuple(page_bounds.shape) != (P, hkv, 2, D):
+    if page_bounds is not None and page_bounds.shape != (P, hkv, 2, D):
         _fail(f"page_bounds must be {(P, hkv, 2, D)}")
     for w in (q_norm, k_norm):
-        if w is not None and tuple(w.shape) != (D,):
+        if w is not None and w.shape != (D,):
             _fail(f"norm weights must be [{D}]")
     tdt, npos = 0, 0
     if cos is not None or sin is not None:
         if cos is None or sin is None:
             _fail("cos and sin come together")
-        if cos.dim() != 2 or cos.shape[1] != D or sin.shape != cos.shape or sin.dtype is not cos.dtype:
+        tshape, ttype = cos.shape, cos.dtype
+        if len(tshape) != 2 or tshape[1] != D or sin.shape != tshape or sin.dtype is not ttype:
             _fail(f"cos and sin must be [positions, {D}] of one dtype")
-        if cos.dtype is not dtype and cos.dtype is not torch.float32:
-            _fail(f"tables must be float32 or {dtype}, got {cos.dtype}")
-        tdt, npos = _DTYPE_ALL[cos.dtype], cos.shape[0]
+        if ttype is not dtype and ttype is not torch.float32:
+            _fail(f"tables must be float32 or {dtype}, got {ttype}")
+        _dense(cos, sin)
+        tdt, npos = _DTYPE_ALL[ttype], tshape[0]
     hq, qs = 0, (0, 0, 0)
     ks, vs = k.stride(), v.stride()
     if q is not None:
-        qs = q.stride()
-        if q.dim() == 4:
-            if q.shape[0] != T or q.shape[1] != hkv or q.shape[3] != D:
+        qs, qshape = q.stride(), q.shape
+        if len(qshape) == 4:
+            if qshape[0] != T or qshape[1] != hkv or qshape[3] != D:
                 _fail(f"q must be [{T}, {hkv}, heads, {D}]")
-            hq = hkv * q.shape[2]
+            hq = hkv * qshape[2]
         else:
-            if q.dim() != 3 or q.shape[0] != T or q.shape[2] != D or q.shape[1] % hkv:
+            if len(qshape) != 3 or qshape[0] != T or qshape[2] != D or qshape[1] % hkv:
                 _fail(f"q must be [{T}, heads, {D}] with a multiple of {hkv} heads")
-            hq = q.shape[1]
+            hq = qshape[1]
             qs = (qs[0], qs[1] * (hq // hkv), qs[1], qs[2])
         if qs[3] != 1 and q.numel():
             _fail("the last dim of q must be contiguous")
@@ -353,15 +360,16 @@ def select_pages(q, page_bounds, kv_indptr, kv_indices, kv_len, page_size: int, 
         _fail(f"page_bounds' dtype {page_bounds.dtype} differs from q's {q.dtype}")
     dt = dtype_code(q.dtype)
     _dense(q, page_bounds)
-    if q.dim() != 3 or page_bounds.dim() != 4 or page_bounds.shape[2] != 2 or page_bounds.shape[3] != q.shape[2]:
+    qshape, bshape = q.shape, page_bounds.shape
+    if len(qshape) != 3 or len(bshape) != 4 or bshape[2] != 2 or bshape[3] != qshape[2]:
         _fail("q must be [T, Hq, D], page_bounds [P, Hkv, 2, D]")
-    T, hq, D = q.shape
-    P, hkv, _, _ = page_bounds.shape
+    T, hq, D = qshape
+    P, hkv, _, _ = bshape
     batch = _page_table(T, kv_indptr, kv_indices, kv_len, qo_indptr)
     if top_pages < 1:
         _fail("top_pages must be positive")
     if out is None:
-        out = torch.empty((T, hkv, top_pages), dtype=torch.int32, device=q.device)
+        out = kv_len.new_empty((T, hkv, top_pages))  # (int32, q's device: checked here and below)
     elif tuple(out.shape) != (T, hkv, top_pages) or out.dtype is not torch.int32 or not out.is_contiguous():
         _fail(f"out must be contiguous int32 {(T, hkv, top_pages)}")
     index = _one_device(q, page_bounds, kv_indptr, kv_indices, kv_len, qo_indptr, out)
@@ -386,15 +394,16 @@ def gqa_sparse_paged(q, k_cache, v_cache, kv_indptr, kv_indices, kv_len, pages, 
         _fail(f"cache dtypes {k_cache.dtype}, {v_cache.dtype} differ from q's {q.dtype}")
     dt = dtype_code(q.dtype)
     _dense(q, k_cache, v_cache, pages)
-    if q.dim() != 3 or k_cache.dim() != 4 or v_cache.shape != k_cache.shape or k_cache.shape[3] != q.shape[2]:
+    qshape, cshape, pshape = q.shape, k_cache.shape, pages.shape
+    if len(qshape) != 3 or len(cshape) != 4 or v_cache.shape != cshape or cshape[3] != qshape[2]:
         _fail("q must be [T, Hq, D], the caches [P, page, Hkv, D]")
-    T, hq, D = q.shape
-    P, page, hkv, _ = k_cache.shape
+    T, hq, D = qshape
+    P, page, hkv, _ = cshape
     batch = _page_table(T, kv_indptr, kv_indices, kv_len, qo_indptr)
-    if pages.dtype is not torch.int32 or pages.dim() != 3 or pages.shape[0] != T or pages.shape[1] != hkv:
+    if pages.dtype is not torch.int32 or len(pshape) != 3 or pshape[0] != T or pshape[1] != hkv:
         _fail(f"pages must be int32 [{T}, {hkv}, n]")
-    top = pages.shape[2]
-    out = _output(out, (T, hq, D), q)
+    top = pshape[2]
+    out = torch.empty_like(q) if out is None else _output(out, qshape, q)
     index = _one_device(q, k_cache, v_cache, kv_indptr, kv_indices, kv_len, pages, qo_indptr, out)
     if T == 0:
         return out
