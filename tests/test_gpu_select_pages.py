@@ -166,3 +166,31 @@ def test_tiles_near_the_border(kind, top, dt):
     got = F.select_pages(q.cuda(), bounds.cuda(), *b.args(), page_size=page, top_pages=top, qo_indptr=b.qo(),
                          max_kv_len=n * page)
     assert torch.equal(got.cpu(), _reference(b, q, bounds, 1, top, 1, 1))
+
+
+def test_tiles_with_missing_pages_and_rows_left_alone():
+    """Ids outside the pool rank last, max_kv_len hides what lies behind, rows behind the last
+    sequence are left as they were, two streams at once."""
+    dt, d, page, rows = torch.bfloat16, 64, 16, 600
+    b = Batch([4800, 700], [rows, 100], page)
+    gen = torch.Generator().manual_seed(9)
+    q = torch.randn((b.rows + 5, 4, d), generator=gen).to(dt)
+    bounds = torch.randn((b.pool, 2, 2, d), generator=gen).sort(2).values.to(dt)
+    whole = b.indices.copy()
+    b.indices[3:9] = [-1, b.pool, 1 << 30, -5, b.pool + 1, -(1 << 31)]
+    ref = _reference(b, q[: b.rows], bounds, 2, 20, 1, 1, max_pages=280)
+    bad = b.args()
+    b.indices = whole
+    ref2 = _reference(b, q[: b.rows], bounds, 2, 20, 1, 1)
+    good, qd, bd, streams, outs = b.args(), q.cuda(), bounds.cuda(), [torch.cuda.Stream() for _ in range(2)], []
+    torch.cuda.synchronize()
+    for i in range(4):
+        with torch.cuda.stream(streams[i % 2]):
+            out = torch.full((b.rows + 5, 2, 20), 99, dtype=torch.int32, device="cuda")
+            table, most = (bad, 280 * page) if i % 2 else (good, 4800)
+            F.select_pages(qd, bd, *table, page_size=page, top_pages=20, qo_indptr=b.qo(), max_kv_len=most, out=out)
+            outs.append(out)
+    torch.cuda.synchronize()
+    for i, out in enumerate(outs):
+        assert torch.equal(out[: b.rows].cpu(), ref if i % 2 else ref2), i
+        assert (out[b.rows:] == 99).all()

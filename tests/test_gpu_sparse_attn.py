@@ -185,3 +185,21 @@ def test_rows_of_wide_tiles(lens, news, hq, hkv, d, page, top, dt):
 @pytest.mark.parametrize("hq,page,before,rows,hkv", [(64, 24, 20, 480, 8), (32, 64, 20, 1000, 8)])
 def test_values_that_other_rows_of_wide_tiles_see(hq, page, before, rows, hkv, dt):
     test_values_that_other_rows_see(hq, page, before, rows, hkv, dt)
+
+
+@DTS
+def test_wide_tiles_with_lists_that_count_for_nothing(dt):
+    """Any order, the same page twice, pages not yet visible, behind the table, outside the pool."""
+    b = Batch([900, 300], [390, 100], 24)
+    b.indices[4] = -1
+    b.indices[b.kv_ptr[1] + 2] = b.pool + 7
+    q, k, v, gen = _inputs(b, 64, 8, 64, dt, 3)
+    pages = torch.randint(-2, 45, (b.rows, 8, 12), generator=gen, dtype=torch.int32)
+    pages[:, :, 5], pages[:, :, 6] = pages[:, :, 0], 2 ** 31 - 1
+    pages[0, 1] = -1                      # an empty list
+    pages[b.news[0], 0] = 2               # a page outside the pool alone
+    out = torch.full((b.rows, 64, 64), 9.0, dtype=dt, device="cuda")
+    assert _run(b, q, k, v, pages, out=out) is out
+    ref, tol = _reference(b, q, k, v, pages, 8)
+    assert ((out.cpu().double() - ref).abs() <= tol).all()
+    assert (out[0, 8:16] == 0).all() and (out[b.news[0], :8] == 0).all()
