@@ -194,3 +194,20 @@ def test_tiles_with_missing_pages_and_rows_left_alone():
     for i, out in enumerate(outs):
         assert torch.equal(out[: b.rows].cpu(), ref if i % 2 else ref2), i
         assert (out[b.rows:] == 99).all()
+
+
+@pytest.mark.parametrize("dt", [torch.float16, torch.bfloat16], ids=["f16", "bf16"])
+@pytest.mark.parametrize("offset,spread", [(2.0, 0.5), (8.0, 0.1), (64.0, 0.25), (500.0, 1.0)])
+def test_tiles_of_scores_that_cancel(offset, spread, dt):
+    """Keys around a common value: sums of large terms of both signs, close to one another."""
+    print("case", offset, spread, dt, flush=True)
+    d, page, n, rows = 128, 16, 260, 720
+    b = Batch([n * page], [rows], page)
+    gen = torch.Generator().manual_seed(int(offset))
+    q = torch.randn((b.rows, 3, d), generator=gen).to(dt)
+    sign = torch.randint(0, 2, (1, 1, 1, d), generator=gen) * 2 - 1
+    bounds = (offset * sign + spread * torch.randn((b.pool, 1, 2, d), generator=gen)).sort(2).values.to(dt)
+    for top in (9, 40):
+        got = F.select_pages(q.cuda(), bounds.cuda(), *b.args(), page_size=page, top_pages=top, qo_indptr=b.qo(),
+                             max_kv_len=n * page)
+        assert torch.equal(got.cpu(), _reference(b, q, bounds, 1, top, 1, 1))
