@@ -186,7 +186,7 @@ def argmax(x, n_valid: int | None = None, out=None):
 # each property once.
 _TICKET_BYTES = 65536  # what a workspace has zeroed at rest
 _DTYPE_ALL = {**_TORCH_DT, torch.float32: _lib.DTYPE_F32}
-_Strides7 = ctypes.c_int64 * 7
+_pack7 = struct.Struct("7q").pack  # seven int64 in memory, as a pointer argument takes them
 
 
 def _fail(msg: str):
@@ -334,16 +334,18 @@ def append_kv_paged(k, v, k_cache, v_cache, kv_indptr, kv_indices, kv_len, q=Non
     if (ks[2] != 1 or vs[2] != 1) and T:
         _fail("the last dim of k and v must be contiguous")
     if q is not None:
-        out = _output(out, (T, hq, D), q)
+        out = q.new_empty((T, hq, D)) if out is None else _output(out, (T, hq, D), q)
     index = _one_device(k, v, k_cache, v_cache, kv_indptr, kv_indices, kv_len, q, cos, sin, q_norm, k_norm, qo_indptr,
                         page_bounds, out)
     if T == 0:
         return out
-    _launch(index, lib().yr_hip_append_kv_paged, "append_kv_paged", _at(q), k.data_ptr(), v.data_ptr(), _at(out),
-            k_cache.data_ptr(), v_cache.data_ptr(), _at(page_bounds), _at(cos), _at(sin), tdt, npos, _at(q_norm),
-            _at(k_norm), eps, _at(qo_indptr), kv_indptr.data_ptr(), kv_indices.data_ptr(), kv_indices.numel(),
-            kv_len.data_ptr(), T, batch, hq, hkv, D, page, P, _Strides7(qs[0], qs[1], qs[2], ks[0], ks[1], vs[0], vs[1]),
-            dt, torch._C._cuda_getCurrentRawStream(index))
+    _launch(index, lib().yr_hip_append_kv_paged, "append_kv_paged", None if q is None else q.data_ptr(), k.data_ptr(),
+            v.data_ptr(), None if q is None else out.data_ptr(), k_cache.data_ptr(), v_cache.data_ptr(),
+            None if page_bounds is None else page_bounds.data_ptr(), None if cos is None else cos.data_ptr(),
+            None if cos is None else sin.data_ptr(), tdt, npos, None if q_norm is None else q_norm.data_ptr(),
+            None if k_norm is None else k_norm.data_ptr(), eps, None if qo_indptr is None else qo_indptr.data_ptr(),
+            kv_indptr.data_ptr(), kv_indices.data_ptr(), kv_indices.numel(), kv_len.data_ptr(), T, batch, hq, hkv, D, page,
+            P, _pack7(qs[0], qs[1], qs[2], ks[0], ks[1], vs[0], vs[1]), dt, torch._C._cuda_getCurrentRawStream(index))
     return out
 
 
