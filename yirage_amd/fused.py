@@ -223,18 +223,21 @@ def _launch(index: int, fn, what: str, *args):
 
 def _scratch(nbytes: int, device, stream: int):
     """workspace(), but a captured call owns its scratch: the graph's pool keeps it,
-    tickets are cleared at every replay, and no two graphs meet in it."""
+    tickets are cleared at every replay, and no two graphs meet in it.  The caller
+    holds the tensor until its launch has returned: another thread's larger call on the
+    same stream may replace the cache's entry at any time, and a block that nothing
+    holds is the allocator's again."""
     if nbytes == 0:
         return None
     if torch.cuda.is_current_stream_capturing():
         ws = torch.empty(nbytes, dtype=torch.uint8, device=device)
         ws[:_TICKET_BYTES].zero_()
-        return ws.data_ptr()
+        return ws
     ws = _ws_cache.get((device.index, stream))
     if ws is None or ws.numel() < nbytes:
         with torch.cuda.device(device):
             ws = workspace(nbytes, device)
-    return ws.data_ptr()
+    return ws
 
 
 def _at(t):
@@ -381,10 +384,11 @@ def select_pages(q, page_bounds, kv_indptr, kv_indices, kv_len, page_size: int, 
         max_kv_len = max(int(kv_len.max().item()), 1)
     stream = torch._C._cuda_getCurrentRawStream(index)
     nb = lib().yr_hip_select_pages_workspace(T, hkv, page_size, max_kv_len)
+    ws = _scratch(nb, q.device, stream)
     _launch(index, lib().yr_hip_select_pages, "select_pages", q.data_ptr(), page_bounds.data_ptr(), _at(qo_indptr),
             kv_indptr.data_ptr(), kv_indices.data_ptr(), kv_indices.numel(), kv_len.data_ptr(), out.data_ptr(), T, batch,
             hq, hkv, D, page_size, P, max_kv_len, top_pages, first_pages, last_pages, dt,
-            _scratch(nb, q.device, stream), nb, stream)
+            _at(ws), nb, stream)
     return out
 
 
@@ -411,10 +415,11 @@ def gqa_sparse_paged(q, k_cache, v_cache, kv_indptr, kv_indices, kv_len, pages, 
         return out
     stream = torch._C._cuda_getCurrentRawStream(index)
     nb = lib().yr_hip_gqa_sparse_workspace(T, batch, qo_indptr is not None, hq, hkv, D, page, top)
+    ws = _scratch(nb, q.device, stream)
     _launch(index, lib().yr_hip_gqa_sparse_paged, "gqa_sparse_paged", q.data_ptr(), k_cache.data_ptr(),
             v_cache.data_ptr(), _at(qo_indptr), kv_indptr.data_ptr(), kv_indices.data_ptr(), kv_indices.numel(),
             kv_len.data_ptr(), pages.data_ptr(), out.data_ptr(), T, batch, hq, hkv, D, page, P, top, dt,
-            _scratch(nb, q.device, stream), nb, stream)
+            _at(ws), nb, stream)
     return out
 
 
@@ -454,10 +459,11 @@ def token_logprobs(logits, tokens, top_n: int = 0, n_valid: int | None = None) -
         return res
     stream = torch._C._cuda_getCurrentRawStream(index)
     nb = lib().yr_hip_token_logprobs_workspace(rows, n_valid, top_n, dt)
+    ws = _scratch(nb, logits.device, stream)
     at = flat.data_ptr()
     _launch(index, lib().yr_hip_token_logprobs, "token_logprobs", logits.data_ptr(), tokens.data_ptr(), at + 12 * cut,
             at + 12 * cut + 4 * rows, at + 8 * cut, at, rows, n, n_valid, logits.stride(0) if rows > 1 else n, top_n, dt,
-            _scratch(nb, logits.device, stream), nb, stream)
+            _at(ws), nb, stream)
     return res
 
 
