@@ -51,7 +51,10 @@ constexpr int LP_MAX_SPLITS = 64; // lists that one wave joins, a lane each
 constexpr int LP_HITS = 128;      // candidate tiles a wave notes (in the candidates' place)
 constexpr int LP_VALUES = 32;     // values per lane and tile (8: 16 rows of 128256 23.5 for 14.6 us, 1 row 11.9 for 12.0)
 constexpr int LP_TARGET_WG = 1024; // (512: 256 rows of 32000 16.1 for 15.9 us; 2048: of 128256 34.7 for 26.6)
-constexpr float kFar = 1e38f;     // |m| beyond which m log2 e may leave fp32
+// |m| beyond which one fma an exponent does not do: c's step is 1/8 here, so m's own exponent
+// m log2 e - c is at most 1/16 off 0 and costs no bits; from 2^31 on it may reach 128, where 2^z
+// leaves fp32, and near the type's end c itself does.
+constexpr float kFar = 0x1p20f;
 
 // A tile with candidates: the lanes that have them, its first piece, its
 // largest exponent.
@@ -304,7 +307,11 @@ __global__ __launch_bounds__(LP_THREADS) void logprobs_kernel(LogprobArgs a) {
   // ---- sums.  Terms are 2^z, z = x log2 e - c with c = m log2 e rounded: one
   // fma each (m: the largest value so far, -inf: none yet).  s and t are
   // relative to the exponent c and are brought to m log2 e itself at the end.
+  // Where m is far off (a mask of -1e9 or the type's lowest value, infinity) z is
+  // (x - m) log2 e, exact next to m whatever its size, and they are relative to
+  // m log2 e itself.
   float m = -INFINITY, c = 0.f, zm = -INFINITY;  // zm: m's own z
+  bool far = false;
   double s = 0, t = 0;
   // Candidates for the top: tiles with a lane whose largest exponent z + c is
   // at least `bound`, the top-th largest of the lanes' maxima.  z + c is off by
@@ -319,8 +326,26 @@ __global__ __launch_bounds__(LP_THREADS) void logprobs_kernel(LogprobArgs a) {
 #pragma unroll
     for (int u = 0; u < U; u++) w[u] = next[u];
     if (p0 + kStep < p_end) load(p0 + kStep, next);  // in flight while this tile is worked on
-    float z[U][EPP], mz;
+    float z[U][EPP], mz, ex;  // mz: the largest; ex: its value's own exponent
+    auto largest = [&]() __attribute__((always_inline)) -> float {
+      float mx = -INFINITY;
+#pragma unroll
+      for (int u = 0; u < U; u++) mx = fmaxf(mx, piece_max<DT>(w[u]));
+      return mx;
+    };
     auto exponents = [&]() __attribute__((always_inline)) {
+      if (far) {  // (uniform)
+#pragma unroll
+        for (int u = 0; u < U; u++) {
+          unpack_piece<DT>(w[u], z[u]);
+#pragma unroll
+          for (int e = 0; e < EPP; e++) z[u][e] = (z[u][e] - m) * kLog2e;
+        }
+        const float mx = largest();
+        mz = (mx - m) * kLog2e;
+        ex = mx * kLog2e;
+        return;
+      }
 #pragma unroll
       for (int u = 0; u < U; u++) {
         unpack_piece<DT>(w[u], z[u]);
@@ -332,6 +357,7 @@ __global__ __launch_bounds__(LP_THREADS) void logprobs_kernel(LogprobArgs a) {
 #pragma unroll
       for (int j = 1; j + 1 < U * EPP; j += 2) mz = max3(mz, z[j / EPP][j % EPP], z[(j + 1) / EPP][(j + 1) % EPP]);
       mz = max2(mz, z[U - 1][EPP - 1]);
+      ex = mz + c;
     };
     bool move = m == -INFINITY;
     if (!move) {
@@ -339,17 +365,15 @@ __global__ __launch_bounds__(LP_THREADS) void logprobs_kernel(LogprobArgs a) {
       move = __ballot(mz > zm) != 0;
     }
     if (move) {  // a new maximum, or the first tile
-      float mx = -INFINITY;
-#pragma unroll
-      for (int u = 0; u < U; u++) mx = fmaxf(mx, piece_max<DT>(w[u]));
-      mx = uniform(wave_maxf(mx));
+      const float mx = uniform(wave_maxf(largest()));
       if (mx > m) {
-        const float was = c;
+        const double was = far ? lp_exponent(m) : (double)c;
         m = mx;
-        c = uniform(fminf(fmaxf(m, -2 * kFar), 2 * kFar) * kLog2e);
-        zm = uniform(fmaf(m, kLog2e, -c));
-        lp_rescale(s, t, was, c);
-        slack = fmaxf(slack, 0x1p-18f * fabsf(c));
+        far = fabsf(m) > kFar;
+        c = uniform(m * kLog2e);
+        zm = far ? 0.f : uniform(fmaf(m, kLog2e, -c));
+        lp_rescale(s, t, was, far ? lp_exponent(m) : (double)c);
+        if (!far) slack = fmaxf(slack, 0x1p-18f * fabsf(c));
       }
       exponents();
     }
@@ -359,16 +383,15 @@ __global__ __launch_bounds__(LP_THREADS) void logprobs_kernel(LogprobArgs a) {
       float es = 0.f;
 #pragma unroll
       for (int e = 0; e < EPP; e++) {
-        const float ex = __builtin_amdgcn_exp2f(z[u][e]);
-        es += ex;
-        tt = fmaf(ex, max2(z[u][e], -1e4f), tt);  // (0 * -inf is none)
+        const float p = __builtin_amdgcn_exp2f(z[u][e]);
+        es += p;
+        tt = fmaf(p, max2(z[u][e], -1e4f), tt);  // (0 * -inf is none)
       }
       st += es;
     }
     s += st;
     t += tt;
     if (a.top > 0) {
-      const float ex = mz + c;
       high = max2(high, ex);
       const uint64_t lanes = __ballot(!(ex < bound - slack));
       if (lanes) {
@@ -393,25 +416,7 @@ __global__ __launch_bounds__(LP_THREADS) void logprobs_kernel(LogprobArgs a) {
       }
     }
   }
-  if (fabsf(m) > kFar && m > -INFINITY) {
-    // m log2 e may have left fp32 (the type's lowest value as a mask, infinity):
-    // c was clamped and only m is right.  Once more, from x - m.
-    s = t = 0;
-    for (int p0 = p_first; p0 < p_end; p0 += kStep)
-#pragma unroll 1
-      for (int i = (p0 + lane) * EPP - lead; i < min((min(p0 + kTile, p_end)) * EPP - lead, a.n); i += 1) {
-        // lane's pieces p0 + lane, + 64, ...: their EPP elements, then the next piece
-        const int e = (i + lead) % EPP;
-        if (i >= 0) {
-          const float z = (at(i) - m) * kLog2e, ex = __builtin_amdgcn_exp2f(z);
-          s += ex;
-          t += ex * max2(z, -1e4f);
-        }
-        if (e == EPP - 1) i += (kWave - 1) * EPP;
-      }
-  } else if (m > -INFINITY) {
-    lp_rescale(s, t, c, lp_exponent(m));
-  }
+  if (!far && m > -INFINITY) lp_rescale(s, t, c, lp_exponent(m));
   s = wave_sum_d(s);
   t = wave_sum_d(t);
   if (lane == 0) {
