@@ -54,6 +54,17 @@ struct SparseArgs {
 template <int DT>
 constexpr float kPBias = DT == DT_F16 ? 7.f : 0.f;
 
+// An exponent is one fma, score log2 e / sqrt(D) less the running maximum, a rounded
+// number: the largest comes out as that rounding, a 16th at most up to here.  Beyond,
+// where it reaches 8 (2^27) P would leave f16's range, at 128 (2^31) fp32's, so there
+// the product is rounded like the maximum before they are subtracted.
+constexpr float kFarScore = 0x1p20f;
+__device__ __forceinline__ float far_exponent(float score, float scale, float m) {
+  float x = score * scale;
+  asm volatile("" : "+v"(x));  // (no fma)
+  return fabsf(m) > kFarScore ? x - m : fmaf(score, scale, -m);
+}
+
 // 16-byte chunk permutations of an LDS row of D elements.  K fragments read one
 // chunk column of 16 consecutive rows, transposing V reads a chunk pair of 4
 // consecutive rows: any 8 lanes of either hit 8 chunks apart modulo 128 bytes.
@@ -272,6 +283,7 @@ __global__ __launch_bounds__(SP_WAVES * kWave) void sparse_kernel(SparseArgs a) 
       else rows(std::false_type{});
     };
     float m_i = -INFINITY, l_i = 0.f;
+    bool far = false;  // some row's m_i is beyond kFarScore
     f32x4 acc[D / 16];
 #pragma unroll
     for (int dt = 0; dt < D / 16; dt++) acc[dt] = f32x4{0.f, 0.f, 0.f, 0.f};
@@ -330,17 +342,27 @@ __global__ __launch_bounds__(SP_WAVES * kWave) void sparse_kernel(SparseArgs a) 
         const float mnew = mx > m_i + kLazy ? mx : m_i;
         const float alpha = m_i == -INFINITY ? 0.f : __builtin_amdgcn_exp2f(m_i - mnew);
         m_i = mnew;
+        far = __builtin_amdgcn_ballot_w64(fabsf(m_i) > kFarScore && m_i > -INFINITY) != 0;
         l_i *= alpha;
 #pragma unroll
         for (int dt = 0; dt < D / 16; dt++) acc[dt] *= alpha;
       }
-      const float mref = (m_i == -INFINITY ? 0.f : m_i) - kPBias<DT>;
+      float mref = m_i == -INFINITY ? 0.f : m_i, scale = a.scale_log2;
+      if (far) {  // (uniform; a row goes by its own maximum, so its weights agree)
+#pragma unroll
+        for (int n = 0; n < 2; n++)
+#pragma unroll
+          for (int i = 0; i < 4; i++) sc[n][i] = far_exponent(sc[n][i], scale, mref);
+        mref = 0.f;
+        scale = 1.f;
+      }
+      mref -= kPBias<DT>;
       float pv[2][4];
 #pragma unroll
       for (int n = 0; n < 2; n++)
 #pragma unroll
         for (int i = 0; i < 4; i++) {
-          pv[n][i] = __builtin_amdgcn_exp2f(fmaf(sc[n][i], a.scale_log2, -mref));
+          pv[n][i] = __builtin_amdgcn_exp2f(fmaf(sc[n][i], scale, -mref));
           l_i += pv[n][i];
         }
       const uint4 pb = make_uint4(pack2<DT>(pv[0][0], pv[0][1]), pack2<DT>(pv[0][2], pv[0][3]),
@@ -571,6 +593,7 @@ __global__ __launch_bounds__(SW_WAVES * kWave, 2) void sparse_wide_kernel(Sparse
   auto pass = [&](int bits, bool exact) __attribute__((always_inline)) {
     const int mine = bits & (((1 << tb) - 1) << (wave * tb));  // this wave's rows
     float m_i = -INFINITY, l_i = 0.f;
+    bool far = false;  // some row's m_i is beyond kFarScore
     f32x4 acc[D / 16];
 #pragma unroll
     for (int dt = 0; dt < D / 16; dt++) acc[dt] = f32x4{0.f, 0.f, 0.f, 0.f};
@@ -672,11 +695,21 @@ __global__ __launch_bounds__(SW_WAVES * kWave, 2) void sparse_wide_kernel(Sparse
         const float mnew = mx > m_i + kLazy ? mx : m_i;
         const float alpha = m_i == -INFINITY ? 0.f : __builtin_amdgcn_exp2f(m_i - mnew);
         m_i = mnew;
+        far = __builtin_amdgcn_ballot_w64(fabsf(m_i) > kFarScore && m_i > -INFINITY) != 0;
         l_i *= alpha;
 #pragma unroll
         for (int dt = 0; dt < D / 16; dt++) acc[dt] *= alpha;
       }
-      const float mref = (m_i == -INFINITY ? 0.f : m_i) - kPBias<DT>;
+      float mref = m_i == -INFINITY ? 0.f : m_i, scale = a.scale_log2;
+      if (far) {  // (uniform; a row goes by its own maximum, so its weights agree)
+#pragma unroll
+        for (int n = 0; n < 4; n++)
+#pragma unroll
+          for (int i = 0; i < 4; i++) sc[n][i] = far_exponent(sc[n][i], scale, mref);
+        mref = 0.f;
+        scale = 1.f;
+      }
+      mref -= kPBias<DT>;
       uint4 pb[2];
 #pragma unroll
       for (int m = 0; m < 2; m++) {
@@ -685,7 +718,7 @@ __global__ __launch_bounds__(SW_WAVES * kWave, 2) void sparse_wide_kernel(Sparse
         for (int n = 0; n < 2; n++)
 #pragma unroll
           for (int i = 0; i < 4; i++) {
-            pv[n][i] = __builtin_amdgcn_exp2f(fmaf(sc[2 * m + n][i], a.scale_log2, -mref));
+            pv[n][i] = __builtin_amdgcn_exp2f(fmaf(sc[2 * m + n][i], scale, -mref));
             l_i += pv[n][i];
           }
         pb[m] = make_uint4(pack2<DT>(pv[0][0], pv[0][1]), pack2<DT>(pv[0][2], pv[0][3]), pack2<DT>(pv[1][0], pv[1][1]),
