@@ -189,6 +189,9 @@ int yr_hip_append_kv_paged(const void* q, const void* k, const void* v, void* q_
  * max_kv_len bounds kv_len (pages behind it are not seen); at most 16384 pages
  * of it.  No counterpart in the reference. */
 size_t yr_hip_select_pages_workspace(int rows, int hkv, int page_size, int max_kv_len);
+/* The kernel a call runs on (host only; `ragged`: with qo_indptr): plan3 = {rows of a
+ * sequence per tile (0: row by row), waves per workgroup, splits per row}. */
+int yr_hip_select_pages_plan(int rows, int batch, int ragged, int hkv, int page_size, int max_kv_len, int* plan3);
 int yr_hip_select_pages(const void* q, const void* page_bounds, const int32_t* qo_indptr, const int32_t* kv_indptr,
                         const int32_t* kv_indices, int n_indices, const int32_t* kv_len, int32_t* pages, int rows,
                         int batch, int hq, int hkv, int d, int page_size, int num_pages, int max_kv_len,
@@ -202,6 +205,9 @@ int yr_hip_select_pages(const void* q, const void* page_bounds, const int32_t* q
  * of yr_hip_gqa_decode_paged on a selection; no counterpart in the reference. */
 size_t yr_hip_gqa_sparse_workspace(int rows, int batch, int ragged, int hq, int hkv, int d, int page_size,
                                    int top_pages); /* ragged: a call with qo_indptr */
+/* The kernel a call runs on (host only): plan3 = {rows of a sequence per tile, 1
+ * where four groups of them share a union of pages, splits of a tile's blocks}. */
+int yr_hip_gqa_sparse_plan(int rows, int batch, int ragged, int hq, int hkv, int page_size, int top_pages, int* plan3);
 int yr_hip_gqa_sparse_paged(const void* q, const void* k_cache, const void* v_cache, const int32_t* qo_indptr,
                             const int32_t* kv_indptr, const int32_t* kv_indices, int n_indices,
                             const int32_t* kv_len, const int32_t* pages, void* out, int rows, int batch, int hq,

@@ -68,8 +68,10 @@ SIGNATURES = {
     "yr_hip_argmax": (_I, [_P, _P, _I, _I, _I, _I, _P]),
     "yr_hip_append_kv_paged": (_I, [_P] * 9 + [_I, _I, _P, _P, _F, _P, _P, _P, _I, _P] + [_I] * 7 + [_P, _I, _P]),
     "yr_hip_select_pages_workspace": (_SZ, [_I] * 4),
+    "yr_hip_select_pages_plan": (_I, [_I] * 6 + [_P]),
     "yr_hip_select_pages": (_I, [_P] * 5 + [_I, _P, _P] + [_I] * 12 + [_P, _SZ, _P]),
     "yr_hip_gqa_sparse_workspace": (_SZ, [_I] * 8),
+    "yr_hip_gqa_sparse_plan": (_I, [_I] * 7 + [_P]),
     "yr_hip_gqa_sparse_paged": (_I, [_P] * 6 + [_I, _P, _P, _P] + [_I] * 9 + [_P, _SZ, _P]),
     "yr_hip_token_logprobs_workspace": (_SZ, [_I] * 4),
     "yr_hip_token_logprobs": (_I, [_P] * 6 + [_I, _I, _I, ctypes.c_int64, _I, _I, _P, _SZ, _P]),

@@ -797,6 +797,14 @@ static bool select_tiled(bool ragged, long long tiles, long long pairs, int hkv,
   return rounds * (570 + max_pages) < 456 + pairs * max_pages / 340;
 }
 
+// Rows per tile of a call and its tiles at most, whatever the sequences' rows; 0: row by row.
+static int select_tile_plan(bool ragged, int rows, int batch, int hkv, int max_pages, long long* tiles) {
+  const int tile = select_tile_rows(max_pages);
+  *tiles = (long long)rows / tile + batch;
+  if (*tiles > rows) *tiles = rows;
+  return select_tiled(ragged, *tiles, (long long)rows * hkv, hkv, max_pages) ? tile : 0;
+}
+
 // Waves per workgroup and splits per row: as many as run at once, 16 waves a CU (one
 // split more, 24 rows of 1024 pages: 38.3 us for 24.4).  Times with 8 kv heads of 128:
 //   16 waves where every row and head then has a workgroup for itself at once, and
@@ -829,6 +837,20 @@ extern "C" size_t yr_hip_select_pages_workspace(int rows, int hkv, int page_size
   const long long pairs = (long long)rows * hkv;
   const int max_pages = (max_kv_len - 1) / page_size + 1;
   return select_plan(pairs, max_pages).splits > 1 ? kTicketBytes + (size_t)pairs * max_pages * sizeof(uint64_t) : 0;
+}
+
+extern "C" int yr_hip_select_pages_plan(int rows, int batch, int ragged, int hkv, int page_size, int max_kv_len, int* plan3) {
+  const char* nm = "yr_hip_select_pages_plan";
+  if (!plan3 || rows <= 0 || batch <= 0 || hkv <= 0 || page_size <= 0 || max_kv_len <= 0 ||
+      (max_kv_len - 1) / page_size >= SEL_MAX_PAGES)
+    return fail(YR_E_INVALID, "%s: shape", nm);
+  const int max_pages = (max_kv_len - 1) / page_size + 1;
+  const SelectPlan p = select_plan((long long)rows * hkv, max_pages);
+  long long tiles;
+  plan3[0] = select_tile_plan(ragged != 0, rows, batch, hkv, max_pages, &tiles);
+  plan3[1] = plan3[0] ? SEL_TILE_WAVES : p.waves;
+  plan3[2] = plan3[0] ? 1 : p.splits;
+  return YR_OK;
 }
 
 // A launch with `lds` bytes of dynamic LDS.
@@ -881,10 +903,9 @@ extern "C" int yr_hip_select_pages(const void* q, const void* page_bounds, const
     return fail(YR_E_WORKSPACE, "%s: workspace %zu < %zu", nm, workspace_bytes, need);
   a.tickets = (uint32_t*)workspace;
   a.keys = need ? (uint64_t*)((char*)workspace + kTicketBytes) : nullptr;
-  a.tile = select_tile_rows(a.max_pages);
-  long long tiles = (long long)rows / a.tile + batch;  // at most, whatever the sequences' rows
-  if (tiles > rows) tiles = rows;
-  const bool tiled = select_tiled(qo_indptr != nullptr, tiles, (long long)rows * hkv, hkv, a.max_pages);
+  long long tiles;
+  a.tile = select_tile_plan(qo_indptr != nullptr, rows, batch, hkv, a.max_pages, &tiles);
+  const bool tiled = a.tile > 0;
   const size_t lds = (size_t)a.max_pages * 8 * (tiled ? a.tile : 1);
   const unsigned grid = (unsigned)(tiled ? tiles * hkv : (long long)rows * hkv * a.splits);
   hipStream_t st = (hipStream_t)stream;

@@ -809,6 +809,18 @@ extern "C" size_t yr_hip_gqa_sparse_workspace(int rows, int batch, int ragged, i
   return kTicketBytes + (size_t)p.tiles * hkv * p.splits * p.tt * (hq / hkv) * (d + 4) * sizeof(float);
 }
 
+extern "C" int yr_hip_gqa_sparse_plan(int rows, int batch, int ragged, int hq, int hkv, int page_size, int top_pages, int* plan3) {
+  const char* nm = "yr_hip_gqa_sparse_plan";
+  if (!plan3 || rows <= 0 || batch <= 0 || hkv <= 0 || hq < hkv || hq % hkv || hq / hkv > 16 || page_size <= 0 ||
+      top_pages < 1 || top_pages > SP_MAX_ENTRIES)
+    return fail(YR_E_INVALID, "%s: shape", nm);
+  const SparsePlan p = sparse_plan(ragged != 0, rows, batch, hkv, hq / hkv, page_size, top_pages);
+  plan3[0] = p.tt;
+  plan3[1] = p.wide;
+  plan3[2] = p.splits;
+  return YR_OK;
+}
+
 extern "C" int yr_hip_gqa_sparse_paged(const void* q, const void* k_cache, const void* v_cache,
                                        const int32_t* qo_indptr, const int32_t* kv_indptr, const int32_t* kv_indices,
                                        int n_indices, const int32_t* kv_len, const int32_t* pages, void* out, int rows,
