@@ -110,7 +110,7 @@ size_t yr_hip_linear_workspace(int batch, int k, int n, int dtype, int w_layout)
  * q[batch][hq][d]; k_cache/v_cache[num_pages][page_size][hkv][d];
  * sequence b owns pages kv_indices[kv_indptr[b] .. kv_indptr[b+1]) and has
  * kv_len[b] tokens; out[batch][hq][d] = softmax(q k^T / sqrt(d)) v with kv
- * head h / (hq / hkv).  Replaces the attention part of the MPK paged
+ * head h / (hq / hkv); 0 where every score is -inf.  Replaces the attention part of the MPK paged
  * attention task (tasks/ampere/multitoken_paged_attention_4_16.cuh:40-656)
  * and the superoptimize GQA customized ops
  * (demo/reference_mugraphs/group_query_attention.py:10-34). */
@@ -165,8 +165,8 @@ int yr_hip_argmax(const void* x, int64_t* out, int rows, int n, int n_valid, int
  * tables cos / sin [max_pos][d] in fp32 or dtype, NULL: not), all in fp32 with one
  * rounding.  A key whose position lies outside the tables is not written, its q row
  * becomes NaN.  page_bounds[num_pages][hkv][2][d] (NULL: none) keeps the
- * smallest and largest stored key per channel of each page: it starts anew when
- * slot 0 of the page is written and grows otherwise.  strides7 = {q row, q kv group, q head in the group, k row, k head,
+ * smallest and largest stored key per channel of each page (NaN left out): it starts
+ * anew when slot 0 of the page is written and grows otherwise.  strides7 = {q row, q kv group, q head in the group, k row, k head,
  * v row, v head} in elements, multiples of 8; the last dim is contiguous.
  * q_out may be q where the layouts agree.  No two sequences may write one page in one call.
  * The append, RoPE and qk-norm part of the MPK paged attention task
@@ -201,8 +201,9 @@ int yr_hip_select_pages(const void* q, const void* page_bounds, const int32_t* q
 /* out[t][h] = softmax(q[t][h] k^T / sqrt(d)) v over the tokens at or before row
  * t's position in the pages pages[t][h / (hq / hkv)][0 .. top_pages); hq / hkv
  * <= 16, top_pages <= 1024.  Entries in any order; negative, invisible, missing
- * and repeated ones count for nothing; a row without a token is 0.  The paged attention
- * of yr_hip_gqa_decode_paged on a selection; no counterpart in the reference. */
+ * and repeated ones count for nothing; a row without a token is 0, as is one whose
+ * scores are all -inf.  Softmax statistics are fp32; the weights are rounded to dtype
+ * before they meet v.  The paged attention of yr_hip_gqa_decode_paged on a selection; no counterpart in the reference. */
 size_t yr_hip_gqa_sparse_workspace(int rows, int batch, int ragged, int hq, int hkv, int d, int page_size,
                                    int top_pages); /* ragged: a call with qo_indptr */
 /* The kernel a call runs on (host only): plan3 = {rows of a sequence per tile, 1

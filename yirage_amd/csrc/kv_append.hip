@@ -16,7 +16,7 @@
 // 54; eight 72 for registers).  A page's keys and bounds belong to one workgroup
 // and are reduced there, two channels a thread (a row's lanes alone: 88 us), and
 // the stores pass the caches (kept in them: 69 us).  12.3k rows of 32 and 8 heads
-// of 128 in bf16, 303 MB: 54 us, 5.6 TB/s, a copy of that size 58; 64 sequences'
+// of 128 in bf16, 307 MB: 54 us, 5.6 TB/s, a copy of that size 58; 64 sequences'
 // new tokens 5.5 us, one's 4.
 #include "ragged.h"
 

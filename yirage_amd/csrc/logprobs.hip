@@ -21,9 +21,9 @@
 // row of nothing but -inf has no distribution: NaN too.  A token outside
 // [0, n_valid) has log probability NaN.
 //
-// Bound by memory for many rows (2048 of 128256 in bf16, 525 MB, top 5: 95 us, 5.5
+// Bound by memory for many rows (2048 of 128256 in bf16, 525 MB, top 5: 97 us, 5.4
 // TB/s; without a top 83), by the chain of loads, waves, splits and ranks for few
-// (one row 12 us, 64 of 50000 14).
+// (one row 13 us, 64 of 50001 13).
 #include <type_traits>
 
 #include "attn_device.h"

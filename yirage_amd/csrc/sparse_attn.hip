@@ -20,7 +20,8 @@
 // pages of 16, 8 kv heads of 64 (134 MB) 25 us, 5.3 TB/s; one row of 32 pages of 64,
 // d = 128, 12 us, of which the lists 3, the blocks 3, the merges of waves and splits
 // 6.  Many rows are bound by what moves from L2 to LDS: 777 rows of 16 pages of 64, 8
-// kv heads of 4 heads of 128, 107 us, 1.8 GB of unions, 17 TB/s.
+// kv heads of 4 heads of 128, 107 us, 1.8 GB of unions, 17 TB/s.  (Repeated inputs, one
+// call after another.)
 #include <type_traits>
 
 #include "attn_device.h"
@@ -47,7 +48,9 @@ struct SparseArgs {
   float scale_log2;
 };
 
-// P is stored in 16 bits for the second product.  f16's normal range ends at
+// P is rounded to 16 bits for the second product, the row sum is not: half a step of
+// each weight, against the result's own half step (fp32 products would take 8 times
+// the matrix instructions).  f16's normal range ends at
 // 2^-14: weights carry a factor 2^7 there (cancelled by the row sum, at most
 // 2^15 with the lazy maximum's slack of 2^8), so a weight loses bits only below
 // 2^-21 of the largest and vanishes below 2^-32.
@@ -82,9 +85,11 @@ __device__ __forceinline__ int v_swz(int row) {
 // pass over the same pages at about the same time, while those are in L2.
 //
 // A table of one mask per page is filled and read back where it fits into the
-// `cells` (even) 16-bit words at `table`, which hold nt * top ints at least.  A
-// single ascending list (a decode step's) is taken as it is; otherwise every entry
-// looks for its like.  The whole workgroup of T.
+// `cells` (even) 16-bit words at `table`, which hold nt * top ints at least; that costs
+// a turn with two barriers per T pages.  A single row's ascending list of up to T
+// entries (a decode step's) is taken as it is; otherwise every entry looks for its like
+// among all (one row, pages of 16: 256 entries 16 us, 512 78, 1024 257).  The whole
+// workgroup of T.
 template <int T>
 __device__ __forceinline__ int build_union(const SparseArgs& a, const SeqRows& s, int nt, int t0, int p0, int hk,
                                            uint32_t* table, int cells, int* l_u, int* l_id, uint16_t* l_mask, int* s_cnt) {
@@ -528,7 +533,7 @@ __global__ __launch_bounds__(SP_WAVES * kWave) void sparse_kernel(SparseArgs a) 
 // skips the blocks that none of its rows chose.  Neighbouring rows choose much
 // alike (777 rows of 16 pages: 36 pages for 4 rows, 65 for 16).  Bound by the slowest
 // wave between two barriers: 1024 workgroups (2048 rows of 16 pages of 64, 8 kv heads
-// of 4 heads of 128) take 224 us, MFMA busy for a tenth of it.
+// of 4 heads of 128) take 207 us, MFMA busy for a tenth of it.
 //
 // Lane l of every wave knows token l of a block: its row in the cache and which
 // rows of the tile see it.  A row's 64 tokens are then one ballot.
@@ -771,8 +776,10 @@ static SparsePlan sparse_plan(bool ragged, int rows, int batch, int hkv, int G, 
   // well enough and the lists fit.  One group to a tile loads shared pages again, in
   // any number of workgroups, and works out every token's address unless pages are a
   // multiple of 32 (8 kv heads of 4, d = 128; rows, pages, us with four groups and one):
-  // 777 16 of 64 121 111; 777 16 of 16 57 77; 1200 16 of 64 174 140; 2048 16 of 64 224
-  // 242, 64 of 16 319 455, 32 of 32 269 248; 2048 of 8 heads, d = 64, 158 177.
+  // 256 16 of 64 98 37; 777 16 of 64 120 107; 777 16 of 16 53 74; 1200 16 of 64 177 141;
+  // 2048 16 of 64 207 219, 64 of 16 260 394, 32 of 32 255 225; 2048 of 8 heads, d = 64, 161
+  // 167.  Rows of many sequences, whose last tiles are not full, come out alike: up to 4
+  // rows in each of 256, 16 of 64 316 357, 16 of 16 153 206.
   const int wide_tt = SW_WAVES * (16 / G);
   const long long wide = ((long long)rows + wide_tt - 1) / wide_tt * hkv, slots = (wide + 511) / 512 * 512;
   p.wide = ragged && G >= 4 && wide_tt * top <= SP_MAX_ENTRIES && 100 * slots < wide * (page % SP_BLK ? 140 : 108);

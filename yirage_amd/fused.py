@@ -280,7 +280,7 @@ def append_kv_paged(k, v, k_cache, v_cache, kv_indptr, kv_indices, kv_len, q=Non
     Keys and q are normalised per head (q_norm / k_norm [D]) and rotated (rotate-half, cos / sin
     [positions, D], fp32 or k's dtype), in fp32 with one rounding; a q row whose position lies
     outside the tables is NaN and its key is not written.  page_bounds [P, Hkv, 2, D] keeps each
-    page's smallest and largest key per channel (what select_pages reads).  q is [T, Hq, D] or
+    page's smallest and largest key per channel, NaN left out (what select_pages reads).  q is [T, Hq, D] or
     [T, Hkv, Hq / Hkv, D]; q, k and v may be slices of one projection (last dim contiguous, 16-byte
     aligned).  out may be q itself where that is contiguous.  D is 64 or 128."""
     dtype = k.dtype
@@ -395,7 +395,8 @@ def select_pages(q, page_bounds, kv_indptr, kv_indices, kv_len, page_size: int, 
 def gqa_sparse_paged(q, k_cache, v_cache, kv_indptr, kv_indices, kv_len, pages, qo_indptr=None, out=None):
     """Paged GQA attention over selected pages: row t of q [T, Hq, D] attends to the tokens at or
     before its position in pages[t, h // (Hq / Hkv)] (int32 [T, Hkv, n], as select_pages gives them;
-    any order, negative, invisible and repeated entries count for nothing).  A row without a token is 0."""
+    any order, negative, invisible and repeated entries count for nothing).  A row without a token, or
+    whose scores are all -inf, is 0.  Lists of up to 256 pages are the fast ones."""
     if k_cache.dtype is not q.dtype or v_cache.dtype is not q.dtype:
         _fail(f"cache dtypes {k_cache.dtype}, {v_cache.dtype} differ from q's {q.dtype}")
     dt = dtype_code(q.dtype)
