@@ -1,6 +1,7 @@
 """The serving operators' scratch lives until their launch has returned, whatever
 another thread does to the cache of workspaces in between.  On the CPU: the library
 and the stream are stand-ins."""
+import contextlib
 import gc
 import weakref
 
@@ -66,7 +67,7 @@ def test_scratch_outlives_a_replaced_cache_entry(call, capturing, monkeypatch):
 
     def during(address):
         # another thread's larger call on the same stream takes the entry over
-        F._ws_cache[key] = torch.zeros(4 * NB, dtype=torch.uint8)
+        F._scratch_cache[key] = torch.zeros(4 * NB, dtype=torch.uint8)
         gc.collect()
         assert [p for _, p in made] == [address]
         assert made[0][0]() is not None, "the scratch was freed before the launch"
@@ -78,8 +79,27 @@ def test_scratch_outlives_a_replaced_cache_entry(call, capturing, monkeypatch):
     monkeypatch.setattr(torch._C, "_cuda_getCurrentRawStream", lambda i: STREAM, raising=False)
     monkeypatch.setattr(torch.cuda, "is_current_stream_capturing", lambda: capturing)
     monkeypatch.setattr(torch, "empty", allocate)
-    monkeypatch.setattr(F, "_ws_cache", {})
+    monkeypatch.setattr(F, "_scratch_cache", {})
     if not capturing:
-        F._ws_cache[key] = torch.empty(NB, dtype=torch.uint8)
+        F._scratch_cache[key] = torch.empty(NB, dtype=torch.uint8)
     call()
     assert lib.launches == 1
+
+
+@pytest.mark.parametrize("call", [_select, _sparse, _logprobs])
+def test_the_other_operators_workspace_stays(call, monkeypatch):
+    """A graph may have its address: a call that needs more takes memory of its own."""
+    lib = Library(lambda address: None)
+    monkeypatch.setattr(F, "lib", lambda: lib)
+    monkeypatch.setattr(F, "_one_device", lambda *ts: 0)
+    monkeypatch.setattr(torch._C, "_cuda_getDevice", lambda: 0, raising=False)
+    monkeypatch.setattr(torch._C, "_cuda_getCurrentRawStream", lambda i: STREAM, raising=False)
+    monkeypatch.setattr(torch.cuda, "is_current_stream_capturing", lambda: False)
+    monkeypatch.setattr(torch.cuda, "current_stream", lambda d=None: type("Stream", (), {"cuda_stream": STREAM}))
+    monkeypatch.setattr(torch.cuda, "device", lambda d: contextlib.nullcontext())
+    mine = torch.empty(NB - 1, dtype=torch.uint8)
+    monkeypatch.setattr(F, "_ws_cache", {(None, STREAM): mine})
+    monkeypatch.setattr(F, "_scratch_cache", {}, raising=False)
+    call()
+    assert lib.launches == 1
+    assert F.workspace(NB - 1, "cpu") is mine

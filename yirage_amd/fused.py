@@ -185,6 +185,7 @@ def argmax(x, n_valid: int | None = None, out=None):
 # decode step's calls are as short as their host side, so the checks below read
 # each property once.
 _TICKET_BYTES = 65536  # what a workspace has zeroed at rest
+_scratch_cache: dict = {}
 _DTYPE_ALL = {**_TORCH_DT, torch.float32: _lib.DTYPE_F32}
 _pack7 = struct.Struct("7q").pack  # seven int64 in memory, as a pointer argument takes them
 
@@ -222,21 +223,24 @@ def _launch(index: int, fn, what: str, *args):
 
 
 def _scratch(nbytes: int, device, stream: int):
-    """workspace(), but a captured call owns its scratch: the graph's pool keeps it,
-    tickets are cleared at every replay, and no two graphs meet in it.  The caller
-    holds the tensor until its launch has returned: another thread's larger call on the
-    same stream may replace the cache's entry at any time, and a block that nothing
-    holds is the allocator's again."""
+    """Zero-filled scratch of one device and stream.  It is not workspace()'s: these calls ask
+    for much more, and an entry that they replaced there could be one that a captured
+    graph of the other operators has the address of.  A captured call owns its scratch: the
+    graph's pool keeps it, tickets are cleared at every replay, and no two graphs meet in
+    it.  The caller holds the tensor until its launch has returned: another thread's larger
+    call on the same stream may replace the cache's entry at any time, and a block that
+    nothing holds is the allocator's again."""
     if nbytes == 0:
         return None
     if torch.cuda.is_current_stream_capturing():
         ws = torch.empty(nbytes, dtype=torch.uint8, device=device)
         ws[:_TICKET_BYTES].zero_()
         return ws
-    ws = _ws_cache.get((device.index, stream))
+    key = (device.index, stream)
+    ws = _scratch_cache.get(key)
     if ws is None or ws.numel() < nbytes:
-        with torch.cuda.device(device):
-            ws = workspace(nbytes, device)
+        with torch.cuda.device(device):  # (allocated and cleared on its stream)
+            ws = _scratch_cache[key] = torch.zeros(max(nbytes, 1 << 20), dtype=torch.uint8, device=device)
     return ws
 
 
