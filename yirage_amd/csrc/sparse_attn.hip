@@ -58,9 +58,10 @@ template <int DT>
 constexpr float kPBias = DT == DT_F16 ? 7.f : 0.f;
 
 // An exponent is one fma, score log2 e / sqrt(D) less the running maximum, a rounded
-// number: the largest comes out as that rounding, a 16th at most up to here.  Beyond,
-// where it reaches 8 (2^27) P would leave f16's range, at 128 (2^31) fp32's, so there
-// the product is rounded like the maximum before they are subtracted.
+// number: the largest comes out as that rounding, a 16th at most up to here.  From
+// 2^24 on it may be 1 and more, and P, up to 2^15 with its factor and slack, would leave
+// f16's range, from 2^31 on fp32's; so beyond this the product is rounded like the
+// maximum before they are subtracted (777 rows of 16 pages of 64: 1 % for the branch).
 constexpr float kFarScore = 0x1p20f;
 __device__ __forceinline__ float far_exponent(float score, float scale, float m) {
   float x = score * scale;
