@@ -1,17 +1,18 @@
 """Drafting over a paged key-value cache in 8 bits, as measurable cases: appending
-rotated keys and values as e4m3 with a scale per token and head, attention of single
-tokens, trees of drafted tokens and chunks of prompts over such a cache (or one in
-16 bits), reading the cache back, and keeping the accepted path of a tree.
+rotated keys and values as e4m3 with a power of two per token and head (codes that
+float lose nothing to a scale without a fraction), attention of single tokens, trees
+of drafted tokens and chunks of prompts over such a cache (or one in 16 bits), reading
+the cache back, and keeping the accepted path of a tree.
 
 Sizes are those of a Llama-3-8B-shaped model (32 / 8 heads of 128, pages of 64) and
 generic ones around them; draw() spreads lengths, page sizes, head counts, head dims
 and types.
 
-Layouts: caches [pages, page, kv heads, d], scales [pages, kv heads, page] in fp32,
+Layouts: caches [pages, page, kv heads, d], scales [pages, page, kv heads] in e8m0,
 rows of a ragged batch back to back (sequence b: rows qo_indptr[b] .. qo_indptr[b + 1],
-its last kv_len[b] - new ones in front of them in the cache), page table and lengths
-int32 as for the paged decode.  tree_mask[row, j]: whether a row sees new token j of
-its sequence; tokens before the new ones are always seen.
+which are the last of its kv_len[b] tokens), page table and lengths int32 as for the
+paged decode.  tree_mask[row, j]: whether a row sees new token j of its sequence;
+tokens before the new ones are always seen.
 """
 import math
 
@@ -21,9 +22,9 @@ import torch
 own = False  # True: run() calls this package's operators; False: their plain forms
 
 DTYPES = {"f16": torch.float16, "bf16": torch.bfloat16}
-E4M3 = torch.float8_e4m3fn
-LARGEST = 448.0  # of e4m3
-LEAST = 2.0 ** -100  # the smallest magnitude that a scale goes by
+E4M3, E8M0 = torch.float8_e4m3fn, torch.float8_e8m0fnu
+LARGEST = 448.0  # of e4m3: 0.875 * 2^9
+LEAST = -126  # the smallest scale's exponent
 THETA = 500000.0
 EPS = 1e-6
 DEVICE = "cuda"
@@ -171,8 +172,7 @@ def _codes(gen, shape):
 
 
 def _scales(gen, shape):
-    pool, page, hkv, _ = shape
-    return (1 + torch.rand((pool, hkv, page), device=DEVICE, generator=gen)) / 225
+    return torch.randint(118, 121, shape[:3], dtype=torch.uint8, device=DEVICE, generator=gen).view(E8M0)
 
 
 def _tables(case):
@@ -247,8 +247,15 @@ def _rotate(x, weight, cos, sin):
 
 
 def _quantise(x):
-    scale = x.abs().amax(-1).clamp(min=LEAST) / LARGEST
-    return (x / scale[..., None]).clamp(-LARGEST, LARGEST).to(E4M3), scale
+    """Codes, and the smallest power of two that leaves none beyond the largest."""
+    m, e = torch.frexp(x.abs().amax(-1))  # m * 2^e, m in [0.5, 1) or 0
+    e = torch.where(m == 0, LEAST, (e - 9 + (m > 0.875)).clamp(min=LEAST))
+    return (x * _power((127 - e).to(torch.uint8))[..., None]).to(E4M3), (e + 127).to(torch.uint8)
+
+
+def _power(scale):
+    """The power of two that a scale in e8m0 (or its bits) stands for."""
+    return (scale.view(torch.uint8).int() << 23).view(torch.float32)
 
 
 def _append(s):
@@ -260,7 +267,7 @@ def _append(s):
     ids, slot = _slot(s, seq, pos)
     s["k_cache"].view(torch.uint8)[ids, slot] = k.view(torch.uint8)
     s["v_cache"].view(torch.uint8)[ids, slot] = v.view(torch.uint8)
-    s["k_scale"][ids, :, slot], s["v_scale"][ids, :, slot] = ks, vs
+    s["k_scale"].view(torch.uint8)[ids, slot], s["v_scale"].view(torch.uint8)[ids, slot] = ks, vs
     return _rotate(s["q"], s["q_norm"], cos, sin).to(s["q"].dtype), s["k_cache"], s["v_cache"], s["k_scale"], s["v_scale"]
 
 
@@ -271,7 +278,7 @@ def _padded(s, name):
     ids = ids[(ptr[:-1, None] + torch.arange(most, device=DEVICE)).clamp(max=ids.numel() - 1)]
     x = s[name + "_cache"]
     if x.dtype == E4M3:
-        x = x.view(torch.uint8)[ids].view(E4M3).float() * s[name + "_scale"][ids].transpose(2, 3)[..., None]
+        x = x.view(torch.uint8)[ids].view(E4M3).float() * _power(s[name + "_scale"])[ids][..., None]
     else:
         x = x[ids].float()
     return x.flatten(1, 2).transpose(1, 2).contiguous()
@@ -306,7 +313,7 @@ def _read(s):
     seq = torch.searchsorted(s["out_indptr"][1:].long(), row, right=True)
     ids, slot = _slot(s, seq, row - s["out_indptr"].long()[seq])
     dt = DTYPES[s["case"]["dtype"]]
-    return tuple((s[n + "_cache"].view(torch.uint8)[ids, slot].view(E4M3).float() * s[n + "_scale"][ids, :, slot][..., None]).to(dt)
+    return tuple((s[n + "_cache"].view(torch.uint8)[ids, slot].view(E4M3).float() * _power(s[n + "_scale"])[ids, slot][..., None]).to(dt)
                  for n in ("k", "v"))
 
 
@@ -315,12 +322,10 @@ def _keep(s):
     first = lens - (s["qo_indptr"][1:] - s["qo_indptr"][:-1]).long()
     seq, to = (path >= 0).nonzero(as_tuple=True)
     src, dst = _slot(s, seq, first[seq] + path[seq, to]), _slot(s, seq, first[seq] + to)
-    for n in ("k", "v"):
-        x = s[n + "_cache"]
-        x = x.view(torch.uint8) if x.dtype == E4M3 else x
-        x[dst] = x[src]
-        if s[n + "_scale"] is not None:
-            s[n + "_scale"][dst[0], :, dst[1]] = s[n + "_scale"][src[0], :, src[1]]
+    for n in ("k_cache", "v_cache", "k_scale", "v_scale"):
+        if s[n] is not None:
+            x = s[n].view(torch.uint8) if s[n].itemsize == 1 else s[n]
+            x[dst] = x[src]
     if s["bounds"] is not None:
         k = s["k_cache"][dst]
         at = dst[0][:, None, None].expand(k.shape)
@@ -369,7 +374,7 @@ def run(s):
 def work(case):
     hkv, d = case["hkv"], case["d"]
     lens, news = _lengths(case)
-    size = 2 * d if case.get("cache") == "16" else d + 4  # of a token's head in the cache, its scale included
+    size = 2 * d if case.get("cache") == "16" else d + 1  # of a token's head in the cache, its scale included
     if case["op"] == "read":
         return {"bytes": int(lens.sum()) * 2 * hkv * (size + 2 * d), "flops": 2 * int(lens.sum()) * hkv * d}
     if case["op"] == "keep":
@@ -401,7 +406,7 @@ def _values(s, name, ids):
     if x.dtype != E4M3:
         return x[ids].double().flatten(0, 1)
     codes = x.view(torch.uint8)[ids].view(E4M3).double()
-    return (codes * s[name + "_scale"][ids].double().permute(0, 2, 1)[..., None]).flatten(0, 1)
+    return (codes * s[name + "_scale"].double()[ids][..., None]).flatten(0, 1)
 
 
 def exact(case, seed):
@@ -414,16 +419,16 @@ def exact(case, seed):
     if case["op"] == "append":
         # the codes before their rounding to 8 bits
         q = torch.empty(s["q"].shape, dtype=torch.float64, device=DEVICE)
-        caches = [s["k_cache"].float().double(), s["v_cache"].float().double(), s["k_scale"].double(), s["v_scale"].double()]
+        caches = [s[n].float().double() for n in ("k_cache", "v_cache", "k_scale", "v_scale")]
         for b, ids in enumerate(pages):
             r, token = slice(starts[b], starts[b + 1]), torch.arange(lens[b] - news[b], lens[b], device=DEVICE)
             at = token if s["positions"] is None else s["positions"][r].long()
             q[r] = _exact_rotate(s["q"][r], s["q_norm"], s["cos"][at], s["sin"][at])
             new = (_exact_rotate(s["k"][r], s["k_norm"], s["cos"][at], s["sin"][at]), s["v"][r].double())
             for x, cache, scale in zip(new, caches[:2], caches[2:]):
-                step = torch.maximum(x.amax(-1), -x.amin(-1)).clamp(min=LEAST) / LARGEST
+                step = torch.exp2(torch.ceil(torch.log2(torch.maximum(x.amax(-1), -x.amin(-1)) / LARGEST)).clamp(min=LEAST))
                 cache[ids[token // page], token % page] = x / step[..., None]
-                scale[ids[token // page], :, token % page] = step
+                scale[ids[token // page], token % page] = step
         return q, *caches
     if case["op"] == "read":
         return tuple(torch.cat([_values(s, n, ids)[:m] for ids, m in zip(pages, lens)]) for n in ("k", "v"))
@@ -435,11 +440,9 @@ def exact(case, seed):
             path = [p for p in path if p >= 0]
             for to, frm in enumerate(path):
                 (u, i), (w, j) = divmod(base + frm, page), divmod(base + to, page)
-                for x in out[:2]:
-                    x[ids[w], j] = x[ids[u], i]
-                for x in out[2:4]:
+                for x in out[:4]:
                     if x is not None:
-                        x[ids[w], :, j] = x[ids[u], :, i]
+                        x[ids[w], j] = x[ids[u], i]
                 if out[4] is not None:
                     key = out[0][ids[w], j]
                     out[4][ids[w]] = torch.stack([torch.minimum(out[4][ids[w], :, 0], key), torch.maximum(out[4][ids[w], :, 1], key)], 1)
