@@ -33,6 +33,7 @@ extern "C" {
 #define YR_E_TIMEOUT (-6)     /* persistent kernel watchdog fired */
 
 /* dtypes: values mirror yirage::type::DataType (include/yirage/type.h:84-120) */
+#define YR_DTYPE_E4M3 930 /* 8-bit cache codes (OCP e4m3fn) */
 #define YR_DTYPE_F16 940
 #define YR_DTYPE_BF16 941
 #define YR_DTYPE_F32 950
@@ -178,6 +179,69 @@ int yr_hip_append_kv_paged(const void* q, const void* k, const void* v, void* q_
                            const int32_t* kv_indptr, const int32_t* kv_indices, int n_indices, const int32_t* kv_len,
                            int rows, int batch, int hq, int hkv, int d, int page_size, int num_pages,
                            const int64_t* strides7, int dtype, void* stream);
+
+/* The same with the rows' table rows given: row t is rotated by positions[t] (a drafted
+ * token's depth in its tree, behind the tokens before it) and still written to its place. */
+int yr_hip_append_kv_paged_at(const void* q, const void* k, const void* v, void* q_out, void* k_cache, void* v_cache,
+                              void* page_bounds, const void* cos_table, const void* sin_table, int table_dtype,
+                              int max_pos, const void* q_norm, const void* k_norm, float eps, const int32_t* positions,
+                              const int32_t* qo_indptr, const int32_t* kv_indptr, const int32_t* kv_indices,
+                              int n_indices, const int32_t* kv_len, int rows, int batch, int hq, int hkv, int d,
+                              int page_size, int num_pages, const int64_t* strides7, int dtype, void* stream);
+
+/* The append into a cache in 8 bits: k_cache / v_cache[num_pages][page_size][hkv][d] hold
+ * e4m3 codes, k_scale / v_scale[num_pages][page_size][hkv] a power of two per token and
+ * head in e8m0 (byte e stands for 2^(e - 127), 255 for NaN), the smallest from 2^-126 on
+ * under which the largest magnitude is at most 448.  value = code * scale, rounded once from
+ * fp32; a head with a NaN or an infinity has scale NaN and codes 0.  positions (NULL: none) as
+ * above.  No page bounds.  No counterpart in the reference, as the next three. */
+int yr_hip_append_kv_paged_fp8(const void* q, const void* k, const void* v, void* q_out, void* k_cache, void* v_cache,
+                               void* k_scale, void* v_scale, const void* cos_table, const void* sin_table,
+                               int table_dtype, int max_pos, const void* q_norm, const void* k_norm, float eps,
+                               const int32_t* positions, const int32_t* qo_indptr, const int32_t* kv_indptr,
+                               const int32_t* kv_indices, int n_indices, const int32_t* kv_len, int rows, int batch,
+                               int hq, int hkv, int d, int page_size, int num_pages, const int64_t* strides7, int dtype,
+                               void* stream);
+
+/* Reads such a cache back: row out_indptr[b] + i of k_out / v_out[rows][hkv][d] (f16 or
+ * bf16) is token i of sequence b, 0 where the sequence has no such token or its page is
+ * missing. */
+int yr_hip_read_kv_paged_fp8(const void* k_cache, const void* v_cache, const void* k_scale, const void* v_scale,
+                             const int32_t* kv_indptr, const int32_t* kv_indices, int n_indices, const int32_t* kv_len,
+                             const int32_t* out_indptr, void* k_out, void* v_out, int rows, int batch, int hkv, int d,
+                             int page_size, int num_pages, int dtype, void* stream);
+
+/* out[t][h] = softmax(q[t][h] k^T / sqrt(d)) v over the tokens before the sequence's new
+ * ones and, of the new ones, those up to row t's own or, with tree_mask (bytes, row t at
+ * tree_mask + t * mask_row, mask_cols of them), those j with tree_mask[t][j] != 0 (none
+ * from mask_cols on).  The cache is of dtype (scales NULL) or YR_DTYPE_E4M3 with its scales;
+ * hq / hkv <= 16.  A row without a token, or whose scores are all -inf, is 0.
+ * max_kv_len, about the largest kv_len, decides how finely the work is split; it does not
+ * limit what is seen.  Softmax statistics are fp32; the weights are rounded to dtype before they
+ * meet v (to bf16 with a cache in 8 bits). */
+size_t yr_hip_gqa_tree_workspace(int rows, int batch, int ragged, int hq, int hkv, int d, int max_kv_len,
+                                 int cache_dtype); /* ragged: a call with qo_indptr */
+/* The kernel a call runs on (host only): plan3 = {groups of 16 columns (rows times heads of a kv
+ * head) of a wave, rows of a sequence per tile, splits of a tile's tokens}. */
+int yr_hip_gqa_tree_plan(int rows, int batch, int ragged, int hq, int hkv, int d, int max_kv_len, int cache_dtype,
+                         int* plan3);
+int yr_hip_gqa_tree_paged(const void* q, const void* k_cache, const void* v_cache, const void* k_scale,
+                          const void* v_scale, const void* tree_mask, int64_t mask_row, int mask_cols,
+                          const int32_t* qo_indptr, const int32_t* kv_indptr, const int32_t* kv_indices, int n_indices,
+                          const int32_t* kv_len, void* out, int rows, int batch, int hq, int hkv, int d, int page_size,
+                          int num_pages, int max_kv_len, int cache_dtype, int dtype, void* workspace,
+                          size_t workspace_bytes, void* stream);
+
+/* Moves the accepted path of each sequence's drafted tokens to the front of its new slots:
+ * slot kv_len[b] - n + j takes what slot kv_len[b] - n + path[b][j] held, n the sequence's
+ * new tokens (by qo_indptr; NULL: 1).  path[batch][depth] ascends; the first entry that does
+ * not, is negative or not below n ends it.  len_out[b] = kv_len[b] - n + entries.  dtype is the
+ * cache's: f16 or bf16 (scales NULL; page_bounds, or NULL, grow to hold the kept keys) or
+ * YR_DTYPE_E4M3 (with scales, without bounds). */
+int yr_hip_keep_kv_paged(void* k_cache, void* v_cache, void* k_scale, void* v_scale, void* page_bounds,
+                         const int32_t* path, int depth, const int32_t* qo_indptr, const int32_t* kv_indptr,
+                         const int32_t* kv_indices, int n_indices, const int32_t* kv_len, int32_t* len_out, int batch,
+                         int hkv, int d, int page_size, int num_pages, int dtype, void* stream);
 
 /* pages[rows][hkv][top_pages] = for each row and kv head the first first_pages
  * pages of the sequence, the last last_pages (>= 1) visible ones and those of

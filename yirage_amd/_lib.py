@@ -12,7 +12,7 @@ _HERE = os.path.dirname(os.path.abspath(__file__))
 LIB_PATH = os.path.join(_HERE, "libyirage_hip.so")
 
 YR_OK = 0
-DTYPE_F16, DTYPE_BF16, DTYPE_F32, DTYPE_I32, DTYPE_I64 = 940, 941, 950, 955, 965
+DTYPE_E4M3, DTYPE_F16, DTYPE_BF16, DTYPE_F32, DTYPE_I32, DTYPE_I64 = 930, 940, 941, 950, 955, 965
 W_NK, W_KN = 0, 1
 (OP_RMSNORM_LINEAR, OP_GATED_MLP, OP_GQA_PREFILL, OP_LINEAR, OP_GQA_DECODE, OP_ATTENTION, OP_MATMUL, OP_UNARY,
  OP_BINARY, OP_REDUCTION, OP_RMSNORM, OP_PACK, OP_COPY_ND, OP_REDUCTION_MAX, OP_EWISE, OP_TB_PROGRAM) = range(1, 17)
@@ -67,6 +67,13 @@ SIGNATURES = {
     "yr_hip_gqa_prefill": (_I, [_P, _P, _P, _P, _I, _I, _I, _I, _I, _I, _I, _P]),
     "yr_hip_argmax": (_I, [_P, _P, _I, _I, _I, _I, _P]),
     "yr_hip_append_kv_paged": (_I, [_P] * 9 + [_I, _I, _P, _P, _F, _P, _P, _P, _I, _P] + [_I] * 7 + [_P, _I, _P]),
+    "yr_hip_append_kv_paged_at": (_I, [_P] * 9 + [_I, _I, _P, _P, _F, _P, _P, _P, _P, _I, _P] + [_I] * 7 + [_P, _I, _P]),
+    "yr_hip_append_kv_paged_fp8": (_I, [_P] * 10 + [_I, _I, _P, _P, _F, _P, _P, _P, _P, _I, _P] + [_I] * 7 + [_P, _I, _P]),
+    "yr_hip_read_kv_paged_fp8": (_I, [_P] * 6 + [_I] + [_P] * 4 + [_I] * 7 + [_P]),
+    "yr_hip_keep_kv_paged": (_I, [_P] * 6 + [_I] + [_P] * 3 + [_I, _P, _P] + [_I] * 6 + [_P]),
+    "yr_hip_gqa_tree_workspace": (_SZ, [_I] * 8),
+    "yr_hip_gqa_tree_plan": (_I, [_I] * 8 + [_P]),
+    "yr_hip_gqa_tree_paged": (_I, [_P] * 6 + [ctypes.c_int64, _I, _P, _P, _P, _I, _P, _P] + [_I] * 10 + [_P, _SZ, _P]),
     "yr_hip_select_pages_workspace": (_SZ, [_I] * 4),
     "yr_hip_select_pages_plan": (_I, [_I] * 6 + [_P]),
     "yr_hip_select_pages": (_I, [_P] * 5 + [_I, _P, _P] + [_I] * 12 + [_P, _SZ, _P]),

@@ -18,7 +18,7 @@
 // the stores pass the caches (kept in them: 69 us).  12.3k rows of 32 and 8 heads
 // of 128 in bf16, 307 MB: 54 us, 5.6 TB/s, a copy of that size 58; 64 sequences'
 // new tokens 5.5 us, one's 4.
-#include "ragged.h"
+#include "kv_rows.h"
 
 namespace yr {
 
@@ -35,6 +35,7 @@ struct AppendArgs {
   const void* sin;
   const uint16_t* q_norm;
   const uint16_t* k_norm;
+  const int32_t* positions;  // [rows]: whose angles a row takes (AT)
   long long q_row, q_grp, q_head, k_row, k_head, v_row, v_head;  // strides in elements
   int hq, hkv, max_pos, q_blocks, q_chunks, heads;  // q_chunks per token; kv heads per cache workgroup
   float eps;
@@ -44,74 +45,8 @@ constexpr int AP_THREADS = 256;
 constexpr int AP_WAVES = AP_THREADS / kWave;
 constexpr int AP_Q = 4;  // q rows of a lane: they share its 32 angles
 
-// A row (one token's head) is D / 16 lanes; a lane holds 8 elements of each
-// half, so a rotated pair sits in one lane.
-// What is written is not read again here: stored past the caches.
-__device__ __forceinline__ void stg16_stream(uint16_t* p, uint4 v) {
-  __builtin_nontemporal_store(__builtin_bit_cast(yr_u32x4, v), (YR_G yr_u32x4*)p);
-}
-template <int DT>
-__device__ __forceinline__ void unpack8(uint4 v, float* x) {
-  x[0] = lo16<DT>(v.x); x[1] = hi16<DT>(v.x); x[2] = lo16<DT>(v.y); x[3] = hi16<DT>(v.y);
-  x[4] = lo16<DT>(v.z); x[5] = hi16<DT>(v.z); x[6] = lo16<DT>(v.w); x[7] = hi16<DT>(v.w);
-}
-template <int DT>
-__device__ __forceinline__ uint4 pack8(const float* x) {
-  return make_uint4(pack2<DT>(x[0], x[1]), pack2<DT>(x[2], x[3]), pack2<DT>(x[4], x[5]), pack2<DT>(x[6], x[7]));
-}
-
-// 8 table entries at `at`
-template <int DT, bool F32>
-__device__ __forceinline__ void table8(const void* t, size_t at, float* x) {
-  if constexpr (F32) {
-    const uint4 a = ldg16((const float*)t + at), b = ldg16((const float*)t + at + 4);
-    x[0] = __uint_as_float(a.x); x[1] = __uint_as_float(a.y); x[2] = __uint_as_float(a.z); x[3] = __uint_as_float(a.w);
-    x[4] = __uint_as_float(b.x); x[5] = __uint_as_float(b.y); x[6] = __uint_as_float(b.z); x[7] = __uint_as_float(b.w);
-  } else {
-    unpack8<DT>(ldg16((const uint16_t*)t + at), x);
-  }
-}
-
-// One lane's angles at position p.
-template <int DT, int D, bool F32>
-__device__ __forceinline__ void angles(const AppendArgs& a, int p, int l, float* c, float* s) {
-  const size_t at = (size_t)p * D + 8 * l;
-  table8<DT, F32>(a.cos, at, c);
-  table8<DT, F32>(a.cos, at + D / 2, c + 8);
-  table8<DT, F32>(a.sin, at, s);
-  table8<DT, F32>(a.sin, at + D / 2, s + 8);
-}
-
-// One lane's 16 elements of a row, normalised by the weights w and rotated.
-template <int DT, int D>
-__device__ __forceinline__ void norm_rotate(bool norm, bool rotate, float eps, const float* w, const float* c,
-                                            const float* s, uint4 lo, uint4 hi, uint4* out) {
-  float x[16];
-  unpack8<DT>(lo, x);
-  unpack8<DT>(hi, x + 8);
-  if (norm) {
-    float ss = 0.f;
-#pragma unroll
-    for (int i = 0; i < 16; i++) ss = fmaf(x[i], x[i], ss);
-#pragma unroll
-    for (int o = 1; o < D / 16; o <<= 1) ss += __shfl_xor(ss, o, kWave);
-    const float f = 1.f / sqrtf(ss * (1.f / D) + eps);
-#pragma unroll
-    for (int i = 0; i < 16; i++) x[i] = x[i] * f * w[i];
-  }
-  if (rotate) {
-#pragma unroll
-    for (int i = 0; i < 8; i++) {
-      const float u = x[i], t = x[i + 8];
-      x[i] = u * c[i] - t * s[i];
-      x[i + 8] = t * c[i + 8] + u * s[i + 8];
-    }
-  }
-  out[0] = pack8<DT>(x);
-  out[1] = pack8<DT>(x + 8);
-}
-
-template <int DT, int D, bool F32>
+// AT: rows are rotated by `positions` (drafted tokens by their depth in a tree), not by their place.
+template <int DT, int D, bool F32, bool AT>
 __global__ __launch_bounds__(AP_THREADS) void append_kernel(AppendArgs a) {
   constexpr int LPR = D / 16, RPW = kWave / LPR, RPP = AP_THREADS / LPR;  // lanes per row, rows per wave and per pass
   const int tid = threadIdx.x, lane = tid % kWave, wave = __builtin_amdgcn_readfirstlane(tid / kWave);
@@ -139,9 +74,9 @@ __global__ __launch_bounds__(AP_THREADS) void append_kernel(AppendArgs a) {
     const int b = seq_of_row(r, t);
     if (b < 0) return;
     const SeqRows s = seq_rows(r, b);
-    const int p = s.len - s.n + (t - s.row0);
+    const int p = AT ? gptr(a.positions)[t] : s.len - s.n + (t - s.row0);
     const bool lost = a.cos && (unsigned)p >= (unsigned)a.max_pos;  // no angle for this position: a loud answer
-    if (a.cos && !lost) angles<DT, D, F32>(a, p, l, c, sn);
+    if (a.cos && !lost) angles<DT, D, F32>(a.cos, a.sin, p, l, c, sn);
 #pragma unroll
     for (int j = 0; j < AP_Q; j++) {
       const int h = h0 + j * RPW;
@@ -197,7 +132,7 @@ __global__ __launch_bounds__(AP_THREADS) void append_kernel(AppendArgs a) {
   if (id < 0) return;
   const int first = s.len - s.n;  // position of the sequence's first new row
   const int pos0 = max(max(first, 0), u * r.page);
-  const int pos1 = min(min(s.len, (u + 1) * r.page), a.cos ? a.max_pos : 0x7fffffff);  // none without an angle
+  const int pos1 = min(min(s.len, (u + 1) * r.page), a.cos && !AT ? a.max_pos : 0x7fffffff);  // none without an angle
   if (pos0 >= pos1) return;
   const int hh = slot % a.heads, h = h0 + hh, step = RPP / a.heads;
   // the thread's word of the page's bounds, two channels (a head's first D / 2 words
@@ -224,12 +159,14 @@ __global__ __launch_bounds__(AP_THREADS) void append_kernel(AppendArgs a) {
     }
     for (int p = pos0 + slot / a.heads; p < pos1; p += step) {
       const long long t = s.row0 + (p - first);
+      const int at = AT ? gptr(a.positions)[t] : p;
+      if (AT && (unsigned)at >= (unsigned)a.max_pos) continue;
       const uint16_t* ks = a.k + t * a.k_row + h * a.k_head + 8 * l;
       const uint16_t* vs = a.v + t * a.v_row + h * a.v_head + 8 * l;
       const uint4 v0 = ldg16(vs), v1 = ldg16(vs + D / 2);
       const uint4 k0 = ldg16(ks), k1 = ldg16(ks + D / 2);
       float c[16], sn[16];
-      if (a.cos) angles<DT, D, F32>(a, p, l, c, sn);
+      if (a.cos) angles<DT, D, F32>(a.cos, a.sin, at, l, c, sn);
       uint4 y[2];
       norm_rotate<DT, D>(a.k_norm, a.cos, a.eps, w, c, sn, k0, k1, y);
       const size_t dst = (((size_t)id * r.page + (p - u * r.page)) * a.hkv + h) * D + 8 * l;
@@ -284,13 +221,12 @@ int ragged_check(const char* nm, const Ragged& r, int hq, int hkv, int d, int dt
 
 using namespace yr;
 
-extern "C" int yr_hip_append_kv_paged(const void* q, const void* k, const void* v, void* q_out, void* k_cache,
-                                      void* v_cache, void* page_bounds, const void* cos_table, const void* sin_table,
-                                      int table_dtype, int max_pos, const void* q_norm, const void* k_norm, float eps,
-                                      const int32_t* qo_indptr, const int32_t* kv_indptr, const int32_t* kv_indices,
-                                      int n_indices, const int32_t* kv_len, int rows, int batch, int hq, int hkv, int d,
-                                      int page_size, int num_pages, const int64_t* strides7, int dtype, void* stream) {
-  const char* nm = "yr_hip_append_kv_paged";
+static int append_paged(const char* nm, const void* q, const void* k, const void* v, void* q_out, void* k_cache,
+                        void* v_cache, void* page_bounds, const void* cos_table, const void* sin_table, int table_dtype,
+                        int max_pos, const void* q_norm, const void* k_norm, float eps, const int32_t* positions,
+                        const int32_t* qo_indptr, const int32_t* kv_indptr, const int32_t* kv_indices, int n_indices,
+                        const int32_t* kv_len, int rows, int batch, int hq, int hkv, int d, int page_size, int num_pages,
+                        const int64_t* strides7, int dtype, void* stream) {
   AppendArgs a;
   a.r = Ragged{qo_indptr, kv_indptr, kv_indices, kv_len, rows, batch, page_size, n_indices, num_pages};
   if (!k || !v || !k_cache || !v_cache || !strides7) return fail(YR_E_INVALID, "%s: null pointer", nm);
@@ -318,6 +254,7 @@ extern "C" int yr_hip_append_kv_paged(const void* q, const void* k, const void* 
   a.sin = sin_table;
   a.q_norm = (const uint16_t*)q_norm;
   a.k_norm = (const uint16_t*)k_norm;
+  a.positions = positions;
   a.q_row = strides7[0];
   a.q_grp = strides7[1];
   a.q_head = strides7[2];
@@ -345,12 +282,39 @@ extern "C" int yr_hip_append_kv_paged(const void* q, const void* k, const void* 
   a.q_blocks = (int)qb;
   const bool f32 = table_dtype == YR_DTYPE_F32;
   hipStream_t st = (hipStream_t)stream;
-#define YR_AP(DT_, D_, F_)                                                                                     \
-  if (dtype == DT_ && d == D_ && f32 == F_)                                                                    \
-    hipLaunchKernelGGL((append_kernel<DT_, D_, F_>), dim3((unsigned)blocks), dim3(AP_THREADS), 0, st, a);
+#define YR_AP(DT_, D_, F_)                                                                                        \
+  if (dtype == DT_ && d == D_ && f32 == F_ && !positions)                                                         \
+    hipLaunchKernelGGL((append_kernel<DT_, D_, F_, false>), dim3((unsigned)blocks), dim3(AP_THREADS), 0, st, a);  \
+  if (dtype == DT_ && d == D_ && f32 == F_ && positions)                                                          \
+    hipLaunchKernelGGL((append_kernel<DT_, D_, F_, true>), dim3((unsigned)blocks), dim3(AP_THREADS), 0, st, a);
   YR_AP(DT_F16, 64, false) YR_AP(DT_F16, 64, true) YR_AP(DT_F16, 128, false) YR_AP(DT_F16, 128, true)
   YR_AP(DT_BF16, 64, false) YR_AP(DT_BF16, 64, true) YR_AP(DT_BF16, 128, false) YR_AP(DT_BF16, 128, true)
 #undef YR_AP
   YR_CHECK_LAUNCH(nm);
   return YR_OK;
+}
+
+extern "C" int yr_hip_append_kv_paged(const void* q, const void* k, const void* v, void* q_out, void* k_cache,
+                                      void* v_cache, void* page_bounds, const void* cos_table, const void* sin_table,
+                                      int table_dtype, int max_pos, const void* q_norm, const void* k_norm, float eps,
+                                      const int32_t* qo_indptr, const int32_t* kv_indptr, const int32_t* kv_indices,
+                                      int n_indices, const int32_t* kv_len, int rows, int batch, int hq, int hkv, int d,
+                                      int page_size, int num_pages, const int64_t* strides7, int dtype, void* stream) {
+  return append_paged("yr_hip_append_kv_paged", q, k, v, q_out, k_cache, v_cache, page_bounds, cos_table, sin_table,
+                      table_dtype, max_pos, q_norm, k_norm, eps, nullptr, qo_indptr, kv_indptr, kv_indices, n_indices,
+                      kv_len, rows, batch, hq, hkv, d, page_size, num_pages, strides7, dtype, stream);
+}
+
+extern "C" int yr_hip_append_kv_paged_at(const void* q, const void* k, const void* v, void* q_out, void* k_cache,
+                                         void* v_cache, void* page_bounds, const void* cos_table, const void* sin_table,
+                                         int table_dtype, int max_pos, const void* q_norm, const void* k_norm, float eps,
+                                         const int32_t* positions, const int32_t* qo_indptr, const int32_t* kv_indptr,
+                                         const int32_t* kv_indices, int n_indices, const int32_t* kv_len, int rows,
+                                         int batch, int hq, int hkv, int d, int page_size, int num_pages,
+                                         const int64_t* strides7, int dtype, void* stream) {
+  const char* nm = "yr_hip_append_kv_paged_at";
+  if (!positions || !cos_table) return fail(YR_E_INVALID, "%s: positions choose rows of the tables: both are needed", nm);
+  return append_paged(nm, q, k, v, q_out, k_cache, v_cache, page_bounds, cos_table, sin_table, table_dtype, max_pos, q_norm,
+                      k_norm, eps, positions, qo_indptr, kv_indptr, kv_indices, n_indices, kv_len, rows, batch, hq, hkv, d,
+                      page_size, num_pages, strides7, dtype, stream);
 }

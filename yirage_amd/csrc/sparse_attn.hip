@@ -48,27 +48,6 @@ struct SparseArgs {
   float scale_log2;
 };
 
-// P is rounded to 16 bits for the second product, the row sum is not: half a step of
-// each weight, against the result's own half step (fp32 products would take 8 times
-// the matrix instructions).  f16's normal range ends at
-// 2^-14: weights carry a factor 2^7 there (cancelled by the row sum, at most
-// 2^15 with the lazy maximum's slack of 2^8), so a weight loses bits only below
-// 2^-21 of the largest and vanishes below 2^-32.
-template <int DT>
-constexpr float kPBias = DT == DT_F16 ? 7.f : 0.f;
-
-// An exponent is one fma, score log2 e / sqrt(D) less the running maximum, a rounded
-// number: the largest comes out as that rounding, a 16th at most up to here.  From
-// 2^24 on it may be 1 and more, and P, up to 2^15 with its factor and slack, would leave
-// f16's range, from 2^31 on fp32's; so beyond this the product is rounded like the
-// maximum before they are subtracted (777 rows of 16 pages of 64: 1 % for the branch).
-constexpr float kFarScore = 0x1p20f;
-__device__ __forceinline__ float far_exponent(float score, float scale, float m) {
-  float x = score * scale;
-  asm volatile("" : "+v"(x));  // (no fma)
-  return fabsf(m) > kFarScore ? x - m : fmaf(score, scale, -m);
-}
-
 // 16-byte chunk permutations of an LDS row of D elements.  K fragments read one
 // chunk column of 16 consecutive rows, transposing V reads a chunk pair of 4
 // consecutive rows: any 8 lanes of either hit 8 chunks apart modulo 128 bytes.

@@ -276,7 +276,7 @@ def _output(out, shape, like):
 
 
 def append_kv_paged(k, v, k_cache, v_cache, kv_indptr, kv_indices, kv_len, q=None, cos=None, sin=None, q_norm=None,
-                    k_norm=None, eps: float = 1e-6, qo_indptr=None, page_bounds=None, out=None):
+                    k_norm=None, eps: float = 1e-6, qo_indptr=None, page_bounds=None, out=None, positions=None):
     """Writes new tokens k, v [T, Hkv, D] into the paged caches [P, page, Hkv, D]; returns q as the
     attention reads it, [T, Hq, D] (None without q).
 
@@ -286,7 +286,9 @@ def append_kv_paged(k, v, k_cache, v_cache, kv_indptr, kv_indices, kv_len, q=Non
     outside the tables is NaN and its key is not written.  page_bounds [P, Hkv, 2, D] keeps each
     page's smallest and largest key per channel, NaN left out (what select_pages reads).  q is [T, Hq, D] or
     [T, Hkv, Hq / Hkv, D]; q, k and v may be slices of one projection (last dim contiguous, 16-byte
-    aligned).  out may be q itself where that is contiguous.  D is 64 or 128."""
+    aligned).  out may be q itself where that is contiguous.  D is 64 or 128.  positions [T] (int32) are
+    the rows of the tables that rows take instead of their own place's: a drafted token's is its depth in
+    the tree behind the tokens before it."""
     dtype = k.dtype
     dt = dtype_code(dtype)
     for t in (v, q):
@@ -344,6 +346,17 @@ def append_kv_paged(k, v, k_cache, v_cache, kv_indptr, kv_indices, kv_len, q=Non
         out = q.new_empty((T, hq, D)) if out is None else _output(out, (T, hq, D), q)
     index = _one_device(k, v, k_cache, v_cache, kv_indptr, kv_indices, kv_len, q, cos, sin, q_norm, k_norm, qo_indptr,
                         page_bounds, out)
+    if positions is not None:
+        _positions(positions, T, cos)
+        _one_device(k, positions)
+        if T:
+            _launch(index, lib().yr_hip_append_kv_paged_at, "append_kv_paged", _at(q), k.data_ptr(), v.data_ptr(),
+                    None if q is None else out.data_ptr(), k_cache.data_ptr(), v_cache.data_ptr(), _at(page_bounds),
+                    cos.data_ptr(), sin.data_ptr(), tdt, npos, _at(q_norm), _at(k_norm), eps, positions.data_ptr(),
+                    _at(qo_indptr), kv_indptr.data_ptr(), kv_indices.data_ptr(), kv_indices.numel(), kv_len.data_ptr(), T,
+                    batch, hq, hkv, D, page, P, _pack7(qs[0], qs[1], qs[2], ks[0], ks[1], vs[0], vs[1]), dt,
+                    torch._C._cuda_getCurrentRawStream(index))
+        return out
     if T == 0:
         return out
     _launch(index, lib().yr_hip_append_kv_paged, "append_kv_paged", None if q is None else q.data_ptr(), k.data_ptr(),
@@ -353,6 +366,238 @@ def append_kv_paged(k, v, k_cache, v_cache, kv_indptr, kv_indices, kv_len, q=Non
             None if k_norm is None else k_norm.data_ptr(), eps, None if qo_indptr is None else qo_indptr.data_ptr(),
             kv_indptr.data_ptr(), kv_indices.data_ptr(), kv_indices.numel(), kv_len.data_ptr(), T, batch, hq, hkv, D, page,
             P, _pack7(qs[0], qs[1], qs[2], ks[0], ks[1], vs[0], vs[1]), dt, torch._C._cuda_getCurrentRawStream(index))
+    return out
+
+
+def _positions(positions, T, cos):
+    if positions.dtype is not torch.int32 or positions.shape != (T,) or not positions.is_contiguous():
+        _fail(f"positions must be contiguous int32 [{T}]")
+    if cos is None:
+        _fail("positions choose rows of cos and sin: give these too")
+
+
+_E4M3, _E8M0 = torch.float8_e4m3fn, torch.float8_e8m0fnu
+
+
+def _cache_fp8(k_cache, v_cache, k_scale, v_scale):
+    """Checks of a cache in 8 bits -> its shape."""
+    if k_cache.dtype is not _E4M3 or v_cache.dtype is not _E4M3:
+        _fail(f"caches must be float8_e4m3fn, got {k_cache.dtype}, {v_cache.dtype}")
+    if k_scale is None or v_scale is None or k_scale.dtype is not _E8M0 or v_scale.dtype is not _E8M0:
+        _fail("a cache in e4m3 needs k_scale and v_scale in float8_e8m0fnu")
+    cshape = k_cache.shape
+    if len(cshape) != 4 or v_cache.shape != cshape or k_scale.shape != cshape[:3] or v_scale.shape != cshape[:3]:
+        _fail("the caches must be [P, page, Hkv, D], their scales [P, page, Hkv]")
+    if not (k_cache.is_contiguous() and v_cache.is_contiguous() and k_scale.is_contiguous() and v_scale.is_contiguous()):
+        _fail("caches and scales must be contiguous (row-major)")
+    return cshape
+
+
+def append_kv_paged_fp8(k, v, k_cache, v_cache, k_scale, v_scale, kv_indptr, kv_indices, kv_len, q=None, cos=None, sin=None,
+                        q_norm=None, k_norm=None, eps: float = 1e-6, qo_indptr=None, positions=None, out=None):
+    """append_kv_paged into caches in 8 bits: codes float8_e4m3fn [P, page, Hkv, D], scales
+    float8_e8m0fnu [P, page, Hkv].
+
+    A token's head is rounded once, from fp32 to e4m3 codes times the smallest power of two that
+    holds its largest magnitude (half a step of e4m3: 2^-4 of a value, 2^-10 of the scale below 2^-6 of
+    it).  A head with a NaN or an infinity gets the scale NaN and reads as NaN.  The other arguments
+    are append_kv_paged's; 8-bit caches have no page bounds."""
+    dtype = k.dtype
+    dt = dtype_code(dtype)
+    for t in (v, q, q_norm, k_norm):
+        if t is not None and t.dtype is not dtype:
+            _fail(f"operand dtype {t.dtype} differs from k's {dtype}")
+    P, page, h2, d2 = _cache_fp8(k_cache, v_cache, k_scale, v_scale)
+    kshape = k.shape
+    if len(kshape) != 3 or v.shape != kshape:
+        _fail("k and v must be [T, Hkv, D]")
+    T, hkv, D = kshape
+    if h2 != hkv or d2 != D:
+        _fail(f"cache heads {(h2, d2)} differ from k's {(hkv, D)}")
+    batch = _page_table(T, kv_indptr, kv_indices, kv_len, qo_indptr)
+    for w in (q_norm, k_norm):
+        if w is not None and (w.shape != (D,) or not w.is_contiguous()):
+            _fail(f"norm weights must be contiguous [{D}]")
+    tdt, npos = 0, 0
+    if cos is not None or sin is not None:
+        if cos is None or sin is None:
+            _fail("cos and sin come together")
+        tshape, ttype = cos.shape, cos.dtype
+        if len(tshape) != 2 or tshape[1] != D or sin.shape != tshape or sin.dtype is not ttype:
+            _fail(f"cos and sin must be [positions, {D}] of one dtype")
+        if ttype is not dtype and ttype is not torch.float32:
+            _fail(f"tables must be float32 or {dtype}, got {ttype}")
+        _dense(cos, sin)
+        tdt, npos = _DTYPE_ALL[ttype], tshape[0]
+    if positions is not None:
+        _positions(positions, T, cos)
+    hq, qs = 0, (0, 0, 0)
+    ks, vs = k.stride(), v.stride()
+    if q is not None:
+        qs, qshape = q.stride(), q.shape
+        if len(qshape) == 4:
+            if qshape[0] != T or qshape[1] != hkv or qshape[3] != D:
+                _fail(f"q must be [{T}, {hkv}, heads, {D}]")
+            hq = hkv * qshape[2]
+        else:
+            if len(qshape) != 3 or qshape[0] != T or qshape[2] != D or qshape[1] % hkv:
+                _fail(f"q must be [{T}, heads, {D}] with a multiple of {hkv} heads")
+            hq = qshape[1]
+            qs = (qs[0], qs[1] * (hq // hkv), qs[1], qs[2])
+        if qs[3] != 1 and q.numel():
+            _fail("the last dim of q must be contiguous")
+        out = q.new_empty((T, hq, D)) if out is None else _output(out, (T, hq, D), q)
+    elif out is not None or q_norm is not None:
+        _fail("out and q_norm need q")
+    if (ks[2] != 1 or vs[2] != 1) and T:
+        _fail("the last dim of k and v must be contiguous")
+    index = _one_device(k, v, k_cache, v_cache, k_scale, v_scale, kv_indptr, kv_indices, kv_len, q, cos, sin, q_norm, k_norm,
+                        qo_indptr, positions, out)
+    if T == 0:
+        return out
+    _launch(index, lib().yr_hip_append_kv_paged_fp8, "append_kv_paged_fp8", None if q is None else q.data_ptr(), k.data_ptr(),
+            v.data_ptr(), None if q is None else out.data_ptr(), k_cache.data_ptr(), v_cache.data_ptr(), k_scale.data_ptr(),
+            v_scale.data_ptr(), None if cos is None else cos.data_ptr(), None if cos is None else sin.data_ptr(), tdt, npos,
+            None if q_norm is None else q_norm.data_ptr(), None if k_norm is None else k_norm.data_ptr(), eps,
+            None if positions is None else positions.data_ptr(), None if qo_indptr is None else qo_indptr.data_ptr(),
+            kv_indptr.data_ptr(), kv_indices.data_ptr(), kv_indices.numel(), kv_len.data_ptr(), T, batch, hq, hkv, D, page, P,
+            _pack7(qs[0], qs[1], qs[2], ks[0], ks[1], vs[0], vs[1]), dt, torch._C._cuda_getCurrentRawStream(index))
+    return out
+
+
+def read_kv_paged_fp8(k_cache, v_cache, k_scale, v_scale, kv_indptr, kv_indices, kv_len, out_indptr, total: int,
+                      dtype=torch.bfloat16, out=None):
+    """Values of an 8-bit cache in 16 bits: (k, v), each [total, Hkv, D].
+
+    Row out_indptr[b] + i is token i of sequence b (out_indptr int32, one more entry than kv_len); a
+    token that the sequence does not have, or whose page is missing, reads as 0, and rows behind the
+    last sequence are left as they were (out: a pair of tensors).  bf16 holds the values exactly
+    (down to its smallest normal number), f16 rounds them once."""
+    if dtype not in _TORCH_DT:
+        _fail(f"unsupported dtype {dtype} (float16/bfloat16 only)")
+    P, page, hkv, D = _cache_fp8(k_cache, v_cache, k_scale, v_scale)
+    if total < 0:
+        _fail("total must not be negative")
+    batch = _page_table(total, kv_indptr, kv_indices, kv_len, out_indptr)
+    if out_indptr is None:
+        _fail("out_indptr is needed")
+    shape = (total, hkv, D)
+    if out is None:
+        k, v = k_cache.new_empty(shape, dtype=dtype), k_cache.new_empty(shape, dtype=dtype)
+    else:
+        k, v = out
+        for t in out:
+            if tuple(t.shape) != shape or t.dtype is not dtype or not t.is_contiguous():
+                _fail(f"out must be two contiguous tensors {shape} {dtype}")
+    index = _one_device(k_cache, v_cache, k_scale, v_scale, kv_indptr, kv_indices, kv_len, out_indptr, k, v)
+    if total == 0:
+        return k, v
+    _launch(index, lib().yr_hip_read_kv_paged_fp8, "read_kv_paged_fp8", k_cache.data_ptr(), v_cache.data_ptr(),
+            k_scale.data_ptr(), v_scale.data_ptr(), kv_indptr.data_ptr(), kv_indices.data_ptr(), kv_indices.numel(),
+            kv_len.data_ptr(), out_indptr.data_ptr(), k.data_ptr(), v.data_ptr(), total, batch, hkv, D, page, P,
+            _TORCH_DT[dtype], torch._C._cuda_getCurrentRawStream(index))
+    return k, v
+
+
+def gqa_tree_paged(q, k_cache, v_cache, kv_indptr, kv_indices, kv_len, tree_mask=None, qo_indptr=None, k_scale=None,
+                   v_scale=None, max_kv_len: int | None = None, out=None):
+    """Paged GQA attention of new rows q [T, Hq, D]: single tokens, trees of drafted tokens, chunks of
+    prompts, over caches [P, page, Hkv, D] of q's dtype, or float8_e4m3fn with k_scale, v_scale
+    [P, page, Hkv] (float8_e8m0fnu).
+
+    A row sees every token before its sequence's new ones; of the new ones those up to itself or,
+    with tree_mask [T, n] (bool, last dim contiguous), those j with tree_mask[row, j] (none from n
+    on).  A row without a token, or whose scores are all -inf, is 0.  max_kv_len, about the largest
+    kv_len, says how finely the work is split (None: read on the host); it does not limit what is seen."""
+    dtype = q.dtype
+    dt = dtype_code(dtype)
+    if k_cache.dtype is _E4M3:
+        cdt = _lib.DTYPE_E4M3
+        cshape = _cache_fp8(k_cache, v_cache, k_scale, v_scale)
+    else:
+        cdt, cshape = dt, k_cache.shape
+        if k_cache.dtype is not dtype or v_cache.dtype is not dtype:
+            _fail(f"cache dtypes {k_cache.dtype}, {v_cache.dtype} differ from q's {dtype}")
+        if k_scale is not None or v_scale is not None:
+            _fail("k_scale and v_scale go with caches in e4m3")
+        if len(cshape) != 4 or v_cache.shape != cshape:
+            _fail("the caches must be [P, page, Hkv, D]")
+        _dense(k_cache, v_cache)
+    qshape = q.shape
+    if len(qshape) != 3 or cshape[3] != qshape[2]:
+        _fail("q must be [T, Hq, D], the caches [P, page, Hkv, D]")
+    _dense(q)
+    T, hq, D = qshape
+    P, page, hkv, _ = cshape
+    batch = _page_table(T, kv_indptr, kv_indices, kv_len, qo_indptr)
+    mask_at, mask_row, mask_cols = None, 0, 0
+    if tree_mask is not None:
+        if tree_mask.dtype is not torch.bool or tree_mask.dim() != 2 or tree_mask.shape[0] != T or tree_mask.shape[1] < 1:
+            _fail(f"tree_mask must be bool [{T}, n], n at least 1")
+        mask_at, (mask_row, inner), mask_cols = tree_mask.data_ptr(), tree_mask.stride(), tree_mask.shape[1]
+        if inner != 1 and mask_cols > 1:
+            _fail("the last dim of tree_mask must be contiguous")
+    out = torch.empty_like(q) if out is None else _output(out, qshape, q)
+    index = _one_device(q, k_cache, v_cache, kv_indptr, kv_indices, kv_len, tree_mask, qo_indptr, k_scale, v_scale, out)
+    if T == 0:
+        return out
+    if max_kv_len is None:
+        max_kv_len = int(kv_len.max().item())
+    max_kv_len = max(max_kv_len, 1)
+    stream = torch._C._cuda_getCurrentRawStream(index)
+    L = lib()
+    nb = L.yr_hip_gqa_tree_workspace(T, batch, qo_indptr is not None, hq, hkv, D, max_kv_len, cdt)
+    ws = _scratch(nb, q.device, stream)
+    _launch(index, L.yr_hip_gqa_tree_paged, "gqa_tree_paged", q.data_ptr(), k_cache.data_ptr(), v_cache.data_ptr(),
+            _at(k_scale), _at(v_scale), mask_at, mask_row, mask_cols, _at(qo_indptr), kv_indptr.data_ptr(),
+            kv_indices.data_ptr(), kv_indices.numel(), kv_len.data_ptr(), out.data_ptr(), T, batch, hq, hkv, D, page, P,
+            max_kv_len, cdt, dt, _at(ws), nb, stream)
+    return out
+
+
+def keep_kv_paged(k_cache, v_cache, kv_indptr, kv_indices, kv_len, path, qo_indptr=None, k_scale=None, v_scale=None,
+                  page_bounds=None, out=None):
+    """Keeps the accepted path of each sequence's tree of drafted tokens: its tokens move, in the caches
+    (16 bits, or e4m3 with their scales), to the front of the sequence's new slots.  Returns the new
+    lengths, int32 [B].
+
+    path [B, m] (int32): numbers of new tokens, ascending from the front; the first entry that is not
+    larger than the one before it, negative, or no new token ends it (-1 behind the path).  page_bounds
+    [P, Hkv, 2, D] (16 bits) grow to hold the kept keys.  What lies behind the new length is no longer
+    part of the sequence; no two sequences may share a page of their new tokens."""
+    cshape, cdtype = k_cache.shape, k_cache.dtype
+    if cdtype is _E4M3:
+        dt = _lib.DTYPE_E4M3
+        _cache_fp8(k_cache, v_cache, k_scale, v_scale)
+        if page_bounds is not None:
+            _fail("page_bounds go with caches in 16 bits")
+    else:
+        dt = dtype_code(cdtype)
+        if v_cache.dtype is not cdtype or len(cshape) != 4 or v_cache.shape != cshape:
+            _fail("the caches must be [P, page, Hkv, D] of one dtype")
+        if k_scale is not None or v_scale is not None:
+            _fail("k_scale and v_scale go with caches in e4m3")
+        if page_bounds is not None and (page_bounds.dtype is not cdtype or page_bounds.shape != (cshape[0], cshape[2], 2, cshape[3])):
+            _fail(f"page_bounds must be {(cshape[0], cshape[2], 2, cshape[3])} {cdtype}")
+        _dense(k_cache, v_cache, page_bounds)
+    P, page, hkv, D = cshape
+    batch = kv_len.numel()
+    pshape = path.shape
+    if path.dtype is not torch.int32 or len(pshape) != 2 or pshape[0] != batch or pshape[1] < 1 or not path.is_contiguous():
+        _fail(f"path must be contiguous int32 [{batch}, m], m at least 1")
+    # (new rows: a sequence has as many as its qo_indptr says)
+    _page_table(batch, kv_indptr, kv_indices, kv_len, qo_indptr)
+    if out is None:
+        out = torch.empty_like(kv_len)
+    elif out.shape != kv_len.shape or out.dtype is not torch.int32 or not out.is_contiguous() or out.data_ptr() == kv_len.data_ptr():
+        _fail(f"out must be another contiguous int32 tensor {tuple(kv_len.shape)}")
+    index = _one_device(k_cache, v_cache, kv_indptr, kv_indices, kv_len, path, qo_indptr, k_scale, v_scale, page_bounds, out)
+    if batch == 0:
+        return out
+    _launch(index, lib().yr_hip_keep_kv_paged, "keep_kv_paged", k_cache.data_ptr(), v_cache.data_ptr(), _at(k_scale),
+            _at(v_scale), _at(page_bounds), path.data_ptr(), pshape[1], _at(qo_indptr), kv_indptr.data_ptr(),
+            kv_indices.data_ptr(), kv_indices.numel(), kv_len.data_ptr(), out.data_ptr(), batch, hkv, D, page, P, dt,
+            torch._C._cuda_getCurrentRawStream(index))
     return out
 
 
