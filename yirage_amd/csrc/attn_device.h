@@ -56,4 +56,20 @@ __device__ __forceinline__ void lds_load16(const uint16_t* g, uint16_t* lds_base
                                    16, 0, 0);
 }
 
+// 4 bytes (or 1, zero-extended) per lane: lane l's land at lds_base + 4 l bytes
+__device__ __forceinline__ void lds_load4(const void* g, uint32_t* lds_base) {
+  __builtin_amdgcn_global_load_lds((const __attribute__((address_space(1))) void*)(g),
+                                   reinterpret_cast<__attribute__((address_space(3))) void*>(
+                                       reinterpret_cast<__attribute__((address_space(3))) char*>(
+                                           reinterpret_cast<uintptr_t>(lds_base))),
+                                   4, 0, 0);
+}
+__device__ __forceinline__ void lds_load1(const void* g, uint32_t* lds_base) {
+  __builtin_amdgcn_global_load_lds((const __attribute__((address_space(1))) void*)(g),
+                                   reinterpret_cast<__attribute__((address_space(3))) void*>(
+                                       reinterpret_cast<__attribute__((address_space(3))) char*>(
+                                           reinterpret_cast<uintptr_t>(lds_base))),
+                                   1, 0, 0);
+}
+
 }  // namespace yr

@@ -24,7 +24,8 @@ namespace yr {
 
 constexpr int TR_WAVES = 4;
 constexpr int TR_TARGET_WG = 512;  // two per CU
-constexpr int TR_MIN_BLOCKS = 4;   // of a split
+constexpr int TR_MIN_BLOCKS = 4;   // of a part
+constexpr int tr_block(int row_bytes) { return 8192 / row_bytes < 64 ? 8192 / row_bytes : 64; }  // tokens
 
 struct TreeArgs {
   Ragged r;
@@ -35,43 +36,143 @@ struct TreeArgs {
   const uint8_t* vs;
   const uint8_t* mask;  // [rows][mask_cols], rows mask_row apart, or null
   uint16_t* out;
-  float* partial;       // [tiles][hkv][splits][tt G][D + 4]: O, m, l
-  uint32_t* tickets;    // [tiles][hkv]
+  float* partial;       // [hkv][parts][2][tt G][D + 4]: O, m, l
+  int4* split;          // [hkv][parts]: the tile that begins in a part and ends in another: first row, columns, its parts (0: none)
   long long mask_row;
-  int mask_cols, hq, hkv, tt, splits;  // tt: rows per tile
+  int mask_cols, hq, hkv, tt, parts;  // rows per tile; ranges of a kv head's units (0: a workgroup a tile)
   uint32_t page_mul, page_shift;       // x / page = x page_mul >> page_shift for x < 2^31
   float scale_log2;
 };
 
-// Tile `tile` of a batch cut into tiles of up to `rows` rows of one sequence: the sequence
-// (batch: none) and the tile's first row within it.  64 sequences at a time, each wave for
-// itself.
-__device__ __forceinline__ int2 seek_tile(const Ragged& r, int tile, int rows) {
-  if (!r.qo_indptr) return make_int2(tile, 0);
-  const int lane = threadIdx.x % kWave;
-  int left = tile;
-  for (int b = 0; b < r.batch; b += kWave) {
-    int n = 0;
-    if (b + lane < r.batch) {
-      const int row0 = min(max(gptr(r.qo_indptr)[b + lane], 0), r.rows);
-      n = (min(max(gptr(r.qo_indptr)[b + lane + 1], row0), r.rows) - row0 + rows - 1) / rows;
+// Work.  A sequence of n new rows has ceil(n / tt) tiles, and a tile counts for as many units
+// as tokens its last row may see.  The units of a kv head, one sequence after another, are
+// cut into `parts` equal ranges, a workgroup each: lengths that differ leave no workgroup
+// waiting, a long sequence is split and several short ones share a workgroup.  (32 sequences
+// of 4 to 8 K tokens, two workgroups of each: TIME.)
+struct SeqWork {
+  SeqRows s;
+  int tiles;
+  long long units;
+};
+__device__ __forceinline__ long long units_before(const TreeArgs& a, const SeqRows& s, int tile) {
+  if (a.mask) return (long long)tile * max(s.len, 1);
+  return (long long)tile * max(s.len - s.n, 0) + (long long)a.tt * tile * (tile + 1) / 2;
+}
+__device__ __forceinline__ SeqWork seq_work(const TreeArgs& a, int b) {
+  SeqWork w;
+  w.tiles = 0;
+  w.units = 0;
+  if (b < a.r.batch) {
+    w.s = seq_rows(a.r, b);
+    w.tiles = (w.s.n + a.tt - 1) / a.tt;
+    w.units = units_before(a, w.s, w.tiles);
+  }
+  return w;
+}
+__device__ __forceinline__ long long lane64(long long x, int lane) {  // (uniform lane)
+  return (long long)(uint32_t)__builtin_amdgcn_readlane((int)(uint32_t)x, lane) |
+         (long long)__builtin_amdgcn_readlane((int)(x >> 32), lane) << 32;
+}
+__device__ __forceinline__ long long first64(long long x) { return lane64(x, 0); }
+// sum over the lanes up to this one, in registers
+template <int CTRL, int ROWS>
+__device__ __forceinline__ long long dpp_add64(long long x) {
+  const int lo = __builtin_amdgcn_update_dpp(0, (int)(uint32_t)x, CTRL, ROWS, 0xf, false);
+  const int hi = __builtin_amdgcn_update_dpp(0, (int)(x >> 32), CTRL, ROWS, 0xf, false);
+  return x + ((long long)(uint32_t)lo | (long long)hi << 32);
+}
+__device__ __forceinline__ long long scan64(long long x) {
+  x = dpp_add64<0x111, 0xf>(x);  // rows of 16 lanes: 1, 2, 4, 8 to the right
+  x = dpp_add64<0x112, 0xf>(x);
+  x = dpp_add64<0x114, 0xf>(x);
+  x = dpp_add64<0x118, 0xf>(x);
+  x = dpp_add64<0x142, 0xa>(x);  // lane 15 of rows 0 and 2 to the rows behind them
+  return dpp_add64<0x143, 0xc>(x);  // lane 31 to the upper half
+}
+// Units of a kv head.  Each wave for itself, a sequence a lane; w: the first 64 sequences.
+__device__ __forceinline__ long long all_units(const TreeArgs& a, const SeqWork& w) {
+  long long sum = w.units;
+  for (int b = kWave; b < a.r.batch; b += kWave) sum += seq_work(a, b + (int)threadIdx.x % kWave).units;
+  return lane64(scan64(sum), kWave - 1);
+}
+// A tile: its sequence (batch: none), number in it, first unit and units.
+struct TileAt {
+  SeqRows s;
+  int b, tile;
+  long long from, units;
+};
+__device__ __forceinline__ SeqRows seq_of_lane(const SeqRows& s, int lane) {  // (uniform lane)
+  return SeqRows{__builtin_amdgcn_readlane(s.row0, lane), __builtin_amdgcn_readlane(s.n, lane), __builtin_amdgcn_readlane(s.len, lane),
+                 __builtin_amdgcn_readlane(s.pg0, lane), __builtin_amdgcn_readlane(s.npg, lane)};
+}
+// The one that unit x falls into.
+__device__ __forceinline__ TileAt find_unit(const TreeArgs& a, SeqWork w, long long x) {
+  TileAt t;
+  t.b = a.r.batch;
+  long long before = 0;
+  for (int b = 0; b < a.r.batch; b += kWave) {
+    if (b > 0) w = seq_work(a, b + (int)threadIdx.x % kWave);
+    const long long sum = scan64(w.units);
+    const uint64_t past = __ballot(before + sum > x);
+    if (past) {
+      const int i = __builtin_ctzll(past);
+      t.b = b + i;
+      t.s = seq_of_lane(w.s, i);
+      before += lane64(sum - w.units, i);
+      // the last tile that begins at or before x
+      int lo = 0, hi = __builtin_amdgcn_readlane(w.tiles, i);
+      while (hi - lo > 1) {
+        const int mid = (lo + hi) / 2;
+        if (before + units_before(a, t.s, mid) <= x) lo = mid;
+        else hi = mid;
+      }
+      t.tile = lo;
+      t.from = before + units_before(a, t.s, lo);
+      t.units = before + units_before(a, t.s, lo + 1) - t.from;
+      return t;
     }
-    int sum = n;
-#pragma unroll
-    for (int o = 1; o < kWave; o <<= 1) {
-      const int v = __shfl_up(sum, o);
-      if (lane >= o) sum += v;
-    }
+    before += lane64(sum, kWave - 1);
+  }
+  return t;
+}
+// Tile `index` of all (a workgroup each, where there are many more than run at once).
+__device__ __forceinline__ TileAt find_index(const TreeArgs& a, SeqWork w, int index) {
+  TileAt t;
+  t.b = a.r.batch;
+  t.tile = 0;
+  t.from = 0;
+  t.units = 1;
+  if (!a.r.qo_indptr) {
+    t.b = index;
+    t.s = seq_rows(a.r, index);
+    return t;
+  }
+  long long left = index;
+  for (int b = 0; b < a.r.batch; b += kWave) {
+    if (b > 0) w = seq_work(a, b + (int)threadIdx.x % kWave);
+    const long long sum = scan64(w.tiles);
     const uint64_t past = __ballot(sum > left);
     if (past) {
       const int i = __builtin_ctzll(past);
-      return make_int2(b + i, (left - __builtin_amdgcn_readlane(sum - n, i)) * rows);
+      t.b = b + i;
+      t.s = seq_of_lane(w.s, i);
+      t.tile = (int)(left - lane64(sum - w.tiles, i));
+      return t;
     }
-    left -= __builtin_amdgcn_readlane(sum, kWave - 1);
+    left -= lane64(sum, kWave - 1);
   }
-  return make_int2(r.batch, 0);
+  return t;
 }
 
+// The units are cut into `parts` ranges that differ by one at most: where range w begins, and
+// the one that holds unit u.
+__device__ __forceinline__ long long part_start(long long units, int parts, int w) {
+  return units / parts * w + min((long long)w, units % parts);
+}
+__device__ __forceinline__ int part_of(long long units, int parts, long long u) {
+  const long long per = units / parts, more = units % parts, cut = (per + 1) * more;
+  return __builtin_amdgcn_readfirstlane((int)(u < cut ? u / (per + 1) : more + (u - cut) / per));
+}
 // 8 consecutive e4m3 codes of LDS rows, transposed across each 16-lane group: lanes 2 e
 // and 2 e + 1 address the halves of row e's 16 bytes, lane i receives byte i of rows 0 .. 7.
 typedef int v2i32 __attribute__((ext_vector_type(2)));
@@ -104,6 +205,26 @@ __device__ __forceinline__ int tv_swz(int row) {
   else return RB == 256 ? ((row & 7) << 1) | ((row >> 3) & 1) : (row & 3) << 1;
 }
 
+// Bytes j .. j + 3 of a row of n, 0 for those outside of it.  (One load of 4 bytes inside the
+// row, whatever its alignment.)
+__device__ __forceinline__ uint32_t mask4(const uint8_t* row, int n, int j) {
+  if (n >= 4) {
+    const int at = min(max(j, 0), n - 4), off = j - at;
+    uint32_t w;
+    __builtin_memcpy(&w, (const YR_G uint8_t*)gptr(row) + at, 4);
+    return off <= -4 || off >= 4 ? 0 : off < 0 ? w << (-8 * off) : w >> (8 * off);
+  }
+  uint32_t w = 0;
+  for (int i = 0; i < 4; i++)
+    if (j + i >= 0 && j + i < n) w |= (uint32_t)gptr(row)[j + i] << (8 * i);
+  return w;
+}
+// bit i: byte i is not 0
+__device__ __forceinline__ uint32_t nonzero4(uint32_t w) {
+  const uint32_t top = (((w & 0x7f7f7f7fu) + 0x7f7f7f7fu) | w) >> 7;
+  return (top & 1) | (top >> 7 & 2) | (top >> 14 & 4) | (top >> 21 & 8);
+}
+
 // A value that is infinite or NaN among the 16 bytes
 template <int DT, bool Q8>
 __device__ __forceinline__ bool not_finite(uint4 v) {
@@ -122,62 +243,50 @@ __device__ __forceinline__ bool not_finite(uint4 v) {
   return bad;
 }
 
-// Q8: a cache in e4m3.  NC: groups of 16 columns of a wave.
+// 4 results of a tile's column: channels d0 .. of row t0 + column / G, head column % G
+template <int DT, int D>
+__device__ __forceinline__ void put_result(const TreeArgs& a, int hk, int t0, int column, int d0, f32x4 O, float L) {
+  const int G = a.hq / a.hkv;
+  O *= L > 0.f || L != L ? 1.f / L : 0.f;  // (nothing seen: 0)
+  *(YR_G uint64_t*)(a.out + ((size_t)(t0 + column / G) * a.hq + (size_t)hk * G + column % G) * D + d0) =
+      (uint64_t)pack2<DT>(O[2], O[3]) << 32 | pack2<DT>(O[0], O[1]);
+}
+
+// Q8: a cache in e4m3.  NC: groups of 16 columns of a wave.  K and V go straight from memory
+// into LDS; page ids and scales come ahead of them, a token a lane.  The loads are counted,
+// so that each wait names what has to have landed.
 //
-// K and V go straight into the wave's LDS slots; its next K block is requested as soon as
-// this one's fragments are in registers and its next V block after P V, so one of the two
-// is always in flight.  Page ids and scales come two blocks ahead, in registers, a token a
-// lane; the loads of a block are counted, so that each wait names what has to have landed.
-template <int DT, bool Q8, int D, int NC>
+// SHARE false: a tile's columns fit one wave, its tokens are split over the waves.  Each has a
+// slot for K and one for V; its next K block is requested as soon as this one's fragments
+// are in registers and its next V block after P V, so one of the two is always in flight.
+//
+// SHARE true: each wave has its own columns (rows of up to 64 NC / G tokens) and all work on
+// the same block, so K and V are moved to LDS once for all of them.  The slots are a ring,
+// three blocks ahead, with one barrier a block.
+template <int DT, bool Q8, int D, int NC, bool SHARE>
 __global__ __launch_bounds__(TR_WAVES * kWave, 2) void tree_kernel(TreeArgs a) {
   constexpr int T = TR_WAVES * kWave;
   constexpr int RB = Q8 ? D : 2 * D;                   // bytes of a token's head
-  constexpr int BT = 8192 / RB < 64 ? 8192 / RB : 64;  // tokens of a block
+  constexpr int BT = tr_block(RB);                     // tokens of a block
   constexpr int CPR = RB / 16, RPI = kWave / CPR;      // chunks per row, rows per load instruction
   constexpr int NL = BT / RPI, NB = BT / 16;           // loads per operand, groups of 16 tokens
-  constexpr int NSMALL = Q8 ? 3 : 1;                   // loads of a block's scales and ids
-  constexpr int DTV = Q8 ? DT_BF16 : DT;               // type of V and P in the second product
+  constexpr int NSMALL = Q8 ? 3 : 1;                   // loads of a block's ids and scales
+  constexpr int NP = NL / TR_WAVES;                    // a wave's share of a block's loads
+  constexpr bool REL = Q8 && DT == DT_F16;
   __shared__ __attribute__((aligned(16))) uint8_t s_k[TR_WAVES][BT * RB];
   __shared__ __attribute__((aligned(16))) uint8_t s_v[TR_WAVES][BT * RB];
   __shared__ __attribute__((aligned(16))) float s_ks[TR_WAVES][BT], s_vs[TR_WAVES][BT];
+  __shared__ __attribute__((aligned(16))) uint32_t s_small[TR_WAVES][NSMALL][kWave];  // by wave or slot: ids, scale bytes
   __shared__ float s_m[TR_WAVES][16 * NC], s_l[TR_WAVES][16 * NC];
   static_assert(16 * D * 4 <= BT * RB, "a wave's O of 16 columns fits a slot");
   static_assert(NC <= 2, "O lies over a V and a K slot");
+  static_assert(NL % TR_WAVES == 0, "waves load equal shares");
   const int tid = threadIdx.x, lane = tid % kWave;
   const int wave = __builtin_amdgcn_readfirstlane(tid / kWave);
-  const int hk = blockIdx.x % a.hkv, rest = blockIdx.x / a.hkv;
-  const int split = rest % a.splits, tile = rest / a.splits, pair = tile * a.hkv + hk;
+  const int hk = blockIdx.x % a.hkv, w0 = blockIdx.x / a.hkv;
   const int G = a.hq / a.hkv, col = lane % 16, grp = lane / 16;
+  const int cols = a.tt * G;
 
-  const int2 at = seek_tile(a.r, tile, a.tt);
-  const int b = __builtin_amdgcn_readfirstlane(at.x), i0 = __builtin_amdgcn_readfirstlane(at.y);
-  if (b >= a.r.batch) return;
-  const SeqRows s = seq_rows(a.r, b);
-  const int nt = min(a.tt, s.n - i0), t0 = s.row0 + i0, first = s.len - s.n, p0 = first + i0;  // rows, first row, its place
-  // tokens that some row may see (and the page table has)
-  const int end = (int)min((long long)(a.mask ? s.len : min(s.len, p0 + nt)), (long long)s.npg * a.r.page);
-  const int plain = a.mask ? first : p0 + 1;             // tokens before this one are seen by all
-
-  // ---- this lane's query rows: column 16 c + col = row i of the tile, head g
-  int qi[NC];
-  uint4 qf[NC][D / 32];
-#pragma unroll
-  for (int c = 0; c < NC; c++) {
-    const int qg = (16 * c + col) % G;
-    qi[c] = (16 * c + col) / G;
-    const uint16_t* src = a.q + ((size_t)(t0 + qi[c]) * a.hq + (size_t)hk * G + qg) * D;
-#pragma unroll
-    for (int st = 0; st < D / 32; st++) {
-      qf[c][st] = make_uint4(0, 0, 0, 0);
-      if (qi[c] < nt) qf[c][st] = ldg16(src + (Q8 ? 16 * (4 * (st / 2) + grp) + 8 * (st % 2) : 32 * st + 8 * grp));
-    }
-  }
-  const int nblk = end > 0 ? (end + BT - 1) / BT : 0;
-  const int per = (nblk + a.splits - 1) / a.splits;
-  const int blk0 = min(split * per, nblk), blk1 = min(blk0 + per, nblk);
-
-  uint8_t* const ks = s_k[wave];
-  uint8_t* const vs = s_v[wave];
   // fragment offsets within a block: K's chunk of row col (groups of 16 rows add 16 RB), V's of
   // this lane's row (32 rows add 32 RB)
   uint32_t koff[RB / 64], voff[D / 16];
@@ -192,414 +301,607 @@ __global__ __launch_bounds__(TR_WAVES * kWave, 2) void tree_kernel(TreeArgs a) {
 #pragma unroll
     for (int dt = 0; dt < D / 16; dt++) voff[dt] = r0 * RB + 16 * ((2 * dt + qc) ^ tv_swz<Q8, RB>(r0)) + qh;
   }
-
-  // A block's tokens, one a lane (lane % BT): entry of the page table, then the place in the cache
-  // (0 where there is none) and which lanes have one.
-  struct Block {
-    uint32_t place;
-    uint64_t have;
-  };
-  auto token = [&](int blk) __attribute__((always_inline)) -> uint32_t { return (uint32_t)(blk * BT + lane % BT); };
-  auto entry = [&](uint32_t x) __attribute__((always_inline)) -> uint32_t {
-    return (uint32_t)((uint64_t)x * a.page_mul >> a.page_shift);
-  };
-  auto load_id = [&](int blk) __attribute__((always_inline)) -> int {
-    return gptr(a.r.kv_indices)[s.pg0 + min((int)entry(token(min(blk, nblk))), s.npg - 1)];
-  };
-  auto place = [&](int blk, int id) __attribute__((always_inline)) -> Block {
-    const uint32_t x = token(min(blk, nblk)), e = entry(x);
-    const bool ok = (int)x < end && (int)e < s.npg && (unsigned)id < (unsigned)a.r.num_pages;
-    Block t;
-    t.place = ok ? (uint32_t)id * (uint32_t)a.r.page + (x - e * (uint32_t)a.r.page) : 0;
-    t.have = __ballot(ok);
-    return t;
-  };
   const size_t tok_bytes = (size_t)a.hkv * RB;
-  auto issue = [&](uint32_t where, auto is_k_c) __attribute__((always_inline)) {
-    constexpr bool IS_K = decltype(is_k_c)::value;
-    const uint8_t* const base = (IS_K ? a.kc : a.vc) + (size_t)hk * RB;
-    uint8_t* const dst = IS_K ? ks : vs;
-#pragma unroll
-    for (int u = 0; u < NL; u++) {
-      const int row = RPI * u + lane / CPR;
-      const uint32_t from = (uint32_t)__shfl((int)where, row);
-      const int chunk = (lane % CPR) ^ (IS_K ? tk_swz<RB>(row) : tv_swz<Q8, RB>(row));
-      lds_load16(reinterpret_cast<const uint16_t*>(base + from * tok_bytes + 16 * chunk),
-                 reinterpret_cast<uint16_t*>(dst + 1024 * u));
-    }
-  };
-  auto scale = [&](const uint8_t* p, uint32_t where) __attribute__((always_inline)) -> uint32_t {
-    return gptr(p)[(size_t)where * a.hkv + hk];
-  };
-  auto scale_value = [](uint32_t byte) __attribute__((always_inline)) -> float {
-    return byte == 255 ? NAN : __uint_as_float(byte << 23);
-  };
 
-  float m_i[NC], l_i[NC];
-  bool far = false;  // some row's m_i is beyond kFarScore
-  f32x4 acc[NC][D / 16];
-#pragma unroll
-  for (int c = 0; c < NC; c++) {
-    m_i[c] = -INFINITY;
-    l_i[c] = 0.f;
-#pragma unroll
-    for (int dt = 0; dt < D / 16; dt++) acc[c][dt] = f32x4{0.f, 0.f, 0.f, 0.f};
+  // ---- this workgroup's units
+  long long units = 0, x = 0, x1 = 1;
+  int parts = 1;
+  SeqWork work0 = seq_work(a, lane);
+  if (a.parts) {
+    if (tid == 0) a.split[(size_t)hk * a.parts + w0].z = 0;
+    units = all_units(a, work0);
+    parts = (int)min((long long)a.parts, max(units / (TR_MIN_BLOCKS * BT), 1ll));
+    if (w0 >= parts) return;
+    x = part_start(units, parts, w0);
+    x1 = part_start(units, parts, w0 + 1);
   }
+  while (true) {
+    const TileAt at = a.parts ? find_unit(a, work0, x) : find_index(a, work0, w0);
+    if (at.b >= a.r.batch) return;
+    const SeqRows s = at.s;
+    const int i0 = at.tile * a.tt;
+    const long long u0 = a.parts ? x - at.from : 0, u1 = a.parts ? min(x1 - at.from, at.units) : 1;
+    x += u1 - u0;
+    const bool whole = u1 - u0 == at.units;
+    const int nt = min(a.tt, s.n - i0), t0 = s.row0 + i0, first = s.len - s.n, p0 = first + i0;  // rows, first row, its place
+    // tokens that some row may see (and the page table has), those before `plain` all rows
+    const int end = (int)min((long long)(a.mask ? s.len : min(s.len, p0 + nt)), (long long)s.npg * a.r.page);
+    const int plain = a.mask ? first : p0 + 1;
+    const int nblk = end > 0 ? (end + BT - 1) / BT : 0;
+    const int blk0 = (int)first64(u0 * nblk / at.units), blk1 = (int)first64(u1 * nblk / at.units);
 
-  Block cur, nxt;                                // this block and the next
-  uint32_t kb = 0, vb = 0, kb_next = 0, vb_next = 0;  // their scales
-  int id_ahead = 0;                              // of the block after
-  // LAST: there is no next block (a copy of its own: every path knows how many loads are in flight)
-  auto consume = [&](int blk, auto last_c) __attribute__((always_inline)) {
-    constexpr bool LAST = decltype(last_c)::value;
-    // K has landed; V and the small loads may be on their way
-    asm volatile("s_waitcnt vmcnt(%0)" ::"n"(LAST ? NL : NL + NSMALL) : "memory");
-    if constexpr (Q8) {
+    // ---- this lane's query rows: its column of group c is row qi of the tile, head (column % G)
+    const int col0 = SHARE ? wave * 16 * NC : 0;
+    int qi[NC];
+    uint4 qf[NC][D / 32];
+#pragma unroll
+    for (int c = 0; c < NC; c++) {
+      const int cw = col0 + 16 * c + col;
+      qi[c] = cw / G;
+      const uint16_t* src = a.q + ((size_t)(t0 + qi[c]) * a.hq + (size_t)hk * G + cw % G) * D;
+#pragma unroll
+      for (int st = 0; st < D / 32; st++) {
+        qf[c][st] = make_uint4(0, 0, 0, 0);
+        if (qi[c] < nt) qf[c][st] = ldg16(src + (Q8 ? 16 * (4 * (st / 2) + grp) + 8 * (st % 2) : 32 * st + 8 * grp));
+      }
+    }
+
+    // A block's tokens, one a lane (lane % BT): entry of the page table, then the place in the cache
+    // (0 where there is none) and which lanes have one.
+    struct Block {
+      uint32_t place;
+      uint64_t have;
+    };
+    auto token = [&](int blk) __attribute__((always_inline)) -> uint32_t { return (uint32_t)(min(blk, nblk) * BT + lane % BT); };
+    auto entry = [&](uint32_t x) __attribute__((always_inline)) -> uint32_t {
+      return (uint32_t)((uint64_t)x * a.page_mul >> a.page_shift);
+    };
+    auto id_at = [&](int blk) __attribute__((always_inline)) -> const int32_t* {
+      return a.r.kv_indices + s.pg0 + min((int)entry(token(blk)), s.npg - 1);
+    };
+    auto place = [&](int blk, int id) __attribute__((always_inline)) -> Block {
+      const uint32_t x = token(blk), e = entry(x);
+      const bool ok = (int)x < end && (int)e < s.npg && (unsigned)id < (unsigned)a.r.num_pages;
+      Block t;
+      t.place = ok ? (uint32_t)id * (uint32_t)a.r.page + (x - e * (uint32_t)a.r.page) : 0;
+      t.have = __ballot(ok);
+      return t;
+    };
+    // loads u0 .. u0 + N - 1 of a block's K or V
+    auto issue = [&](uint32_t where, const uint8_t* cache, uint8_t* dst, auto is_k_c, auto n_c, int u0) __attribute__((always_inline)) {
+      constexpr bool IS_K = decltype(is_k_c)::value;
+      const uint8_t* const base = cache + (size_t)hk * RB;
+#pragma unroll
+      for (int u = 0; u < decltype(n_c)::value; u++) {
+        const int row = RPI * (u0 + u) + lane / CPR;
+        const uint32_t from = (uint32_t)__shfl((int)where, row);
+        const int chunk = (lane % CPR) ^ (IS_K ? tk_swz<RB>(row) : tv_swz<Q8, RB>(row));
+        lds_load16(reinterpret_cast<const uint16_t*>(base + from * tok_bytes + 16 * chunk),
+                   reinterpret_cast<uint16_t*>(dst + 1024 * (u0 + u)));
+      }
+    };
+
+    float m_i[NC], l_i[NC];
+    bool far = false;  // some row's m_i is beyond kFarScore
+    f32x4 acc[NC][D / 16];
+#pragma unroll
+    for (int c = 0; c < NC; c++) {
+      m_i[c] = -INFINITY;
+      l_i[c] = 0.f;
+#pragma unroll
+      for (int dt = 0; dt < D / 16; dt++) acc[c][dt] = f32x4{0.f, 0.f, 0.f, 0.f};
+    }
+
+    // e8m0 -> float (byte 0 is 2^-127)
+    auto scale_value = [](int byte) __attribute__((always_inline)) -> float {
+      return byte == 255 ? NAN : __uint_as_float(byte > 0 ? (uint32_t)byte << 23 : 0x400000u);
+    };
+    // f16: V's scales go onto the weights relative to the largest so far, so that these keep
+    // to f16's range (an accumulator stands for itself times 2^(top - 127)).
+    int top = -1000;
+    auto put_scales = [&](int kb, int vb, uint64_t have) __attribute__((always_inline)) {
+      if constexpr (REL) {
+        const int mine = (have >> lane & 1) && vb != 255 ? vb : -1000;
+        if (__builtin_amdgcn_ballot_w64(mine > top)) {
+          int most = mine;
+#pragma unroll
+          for (int o = 32; o > 0; o >>= 1) most = max(most, __shfl_xor(most, o, kWave));
+          most = __builtin_amdgcn_readfirstlane(most);
+          const float f = __uint_as_float((uint32_t)max(top - most + 127, 0) << 23);
+          top = most;
+#pragma unroll
+          for (int c = 0; c < NC; c++)
+#pragma unroll
+            for (int dt = 0; dt < D / 16; dt++) acc[c][dt] *= f;
+        }
+      }
       s_ks[wave][lane % BT] = scale_value(kb);
-      s_vs[wave][lane % BT] = scale_value(vb);
-      asm volatile("" ::: "memory");
-    }
-    f32x4 sc[NC][NB];
-#pragma unroll
-    for (int n = 0; n < NB; n++) {
-#pragma unroll
-      for (int c = 0; c < NC; c++) sc[c][n] = f32x4{0.f, 0.f, 0.f, 0.f};
-      float kscale = 1.f;
-      if constexpr (Q8) kscale = s_ks[wave][16 * n + col];
-#pragma unroll
-      for (int j = 0; j < RB / 64; j++) {
-        const uint4 w = *reinterpret_cast<const uint4*>(&ks[koff[j] + 16 * n * RB]);
-        if constexpr (Q8) {
-          const uint2 f0 = e4m3x4<DT>(w.x, kscale), f1 = e4m3x4<DT>(w.y, kscale), f2 = e4m3x4<DT>(w.z, kscale),
-                      f3 = e4m3x4<DT>(w.w, kscale);
-#pragma unroll
-          for (int c = 0; c < NC; c++) {
-            sc[c][n] = mfma16<DT>(make_uint4(f0.x, f0.y, f1.x, f1.y), qf[c][2 * j], sc[c][n]);
-            sc[c][n] = mfma16<DT>(make_uint4(f2.x, f2.y, f3.x, f3.y), qf[c][2 * j + 1], sc[c][n]);
-          }
-        } else {
-#pragma unroll
-          for (int c = 0; c < NC; c++) sc[c][n] = mfma16<DT>(w, qf[c][j], sc[c][n]);
-        }
-      }
-    }
-    asm volatile("s_waitcnt lgkmcnt(0)" ::: "memory");  // every K fragment is in registers
-    if constexpr (!LAST) issue(nxt.place, std::true_type{});
-    // mask: this lane's tokens are 16 n + 4 grp + i
-    const int pos0 = blk * BT;
-    const bool masked = pos0 + BT > plain || cur.have != ~0ull;  // (uniform)
-    uint32_t seen[NC];
-#pragma unroll
-    for (int c = 0; c < NC; c++) seen[c] = ~0u;
-    if (masked) {
-#pragma unroll
-      for (int c = 0; c < NC; c++) {
-        const int rel = pos0 - first, lim = (a.mask ? first : p0 + qi[c] + 1) - pos0;
-        const uint8_t* const row = a.mask + (size_t)(t0 + min(qi[c], nt - 1)) * a.mask_row;
-        seen[c] = 0;
-#pragma unroll 1
-        for (int e = 0; e < 4 * NB; e++) {
-          const int x = 16 * (e / 4) + 4 * grp + e % 4;
-          bool ok = x < lim;
-          if (a.mask && !ok && rel + x < a.mask_cols) ok = gptr(row)[rel + x] != 0;
-          if (ok && (cur.have >> x & 1)) seen[c] |= 1u << e;
-        }
-#pragma unroll
-        for (int n = 0; n < NB; n++)
-#pragma unroll
-          for (int i = 0; i < 4; i++) sc[c][n][i] = seen[c] >> (4 * n + i) & 1 ? sc[c][n][i] : -INFINITY;
-      }
-    }
-    bool grow = false;
-    float mnew[NC];
-#pragma unroll
-    for (int c = 0; c < NC; c++) {
-      float mx = -INFINITY;
-#pragma unroll
-      for (int n = 0; n < NB; n++)
-#pragma unroll
-        for (int i = 0; i < 4; i++) mx = fmaxf(mx, sc[c][n][i]);
-      mx = max_xor32(max_xor16(mx)) * a.scale_log2;
-      mnew[c] = mx > m_i[c] + kLazy ? mx : m_i[c];
-      grow |= mx > m_i[c] + kLazy;
-    }
-    if (__builtin_amdgcn_ballot_w64(grow)) {
-      far = false;
-#pragma unroll
-      for (int c = 0; c < NC; c++) {
-        const float alpha = m_i[c] == -INFINITY ? 0.f : __builtin_amdgcn_exp2f(m_i[c] - mnew[c]);
-        m_i[c] = mnew[c];
-        far |= __builtin_amdgcn_ballot_w64(fabsf(m_i[c]) > kFarScore && m_i[c] > -INFINITY) != 0;
-        l_i[c] *= alpha;
-#pragma unroll
-        for (int dt = 0; dt < D / 16; dt++) acc[c][dt] *= alpha;
-      }
-    }
-    f32x4 vscale[NB];
-    if constexpr (Q8) {
-#pragma unroll
-      for (int n = 0; n < NB; n++) vscale[n] = *reinterpret_cast<const f32x4*>(&s_vs[wave][16 * n + 4 * grp]);
-    }
-    uint2 pb[NC][NB];
-#pragma unroll
-    for (int c = 0; c < NC; c++) {
-      float mref = m_i[c] == -INFINITY ? 0.f : m_i[c], scl = a.scale_log2;
-      if (far) {  // (uniform; a row goes by its own maximum, so its weights agree)
-#pragma unroll
-        for (int n = 0; n < NB; n++)
-#pragma unroll
-          for (int i = 0; i < 4; i++) sc[c][n][i] = far_exponent(sc[c][n][i], scl, mref);
-        mref = 0.f;
-        scl = 1.f;
-      }
-      mref -= kPBias<DTV>;
+      s_vs[wave][lane % BT] = !REL ? scale_value(vb) : vb == 255 ? NAN : __uint_as_float((uint32_t)min(max(vb - top + 127, 0), 127) << 23);
+    };
+
+    // Some row may not see some token of the block (uniform, also over waves)
+    auto is_masked = [&](int blk, uint64_t have) __attribute__((always_inline)) -> bool { return (blk + 1) * BT > plain || have != ~0ull; };
+    // One block for this wave's columns.  after_k: K's fragments are in registers; before_v: V
+    // is needed.
+    auto compute = [&](int blk, uint64_t have, const uint8_t* kt, uint8_t* vt, auto after_k, auto before_v) __attribute__((always_inline)) {
+      f32x4 sc[NC][NB];
 #pragma unroll
       for (int n = 0; n < NB; n++) {
-        f32x4 p;
 #pragma unroll
-        for (int i = 0; i < 4; i++) {
-          p[i] = __builtin_amdgcn_exp2f(fmaf(sc[c][n][i], scl, -mref));
-          l_i[c] += p[i];
-          if constexpr (Q8) p[i] *= vscale[n][i];
-        }
-        if (Q8 && masked) {  // an unseen token's scale may be NaN
+        for (int c = 0; c < NC; c++) sc[c][n] = f32x4{0.f, 0.f, 0.f, 0.f};
+        float kscale = 1.f;
+        if constexpr (Q8) kscale = s_ks[wave][16 * n + col];
 #pragma unroll
-          for (int i = 0; i < 4; i++) p[i] = seen[c] >> (4 * n + i) & 1 ? p[i] : 0.f;
+        for (int j = 0; j < RB / 64; j++) {
+          const uint4 w = *reinterpret_cast<const uint4*>(&kt[koff[j] + 16 * n * RB]);
+          if constexpr (Q8) {
+            const uint2 f0 = e4m3x4<DT>(w.x, kscale), f1 = e4m3x4<DT>(w.y, kscale), f2 = e4m3x4<DT>(w.z, kscale),
+                        f3 = e4m3x4<DT>(w.w, kscale);
+#pragma unroll
+            for (int c = 0; c < NC; c++) {
+              sc[c][n] = mfma16<DT>(make_uint4(f0.x, f0.y, f1.x, f1.y), qf[c][2 * j], sc[c][n]);
+              sc[c][n] = mfma16<DT>(make_uint4(f2.x, f2.y, f3.x, f3.y), qf[c][2 * j + 1], sc[c][n]);
+            }
+          } else {
+#pragma unroll
+            for (int c = 0; c < NC; c++) sc[c][n] = mfma16<DT>(w, qf[c][j], sc[c][n]);
+          }
         }
-        pb[c][n] = make_uint2(pack2<DTV>(p[0], p[1]), pack2<DTV>(p[2], p[3]));
       }
-    }
-    // V has landed; the small loads and the next K may be on their way
-    if constexpr (!LAST) asm volatile("s_waitcnt vmcnt(%0)" ::"n"(NL + NSMALL) : "memory");
-    else asm volatile("s_waitcnt vmcnt(0)" ::: "memory");
-    // Infinity or NaN in a token's V would reach the rows that do not see it as 0 * inf: such
-    // tokens leave the block and are added to those that do, one by one.
-    if (masked) {
-      uint64_t bad = 0;
-#pragma unroll 1
-      for (int u = 0; u < NL; u++) {
-        const uint4 w = *reinterpret_cast<const uint4*>(vs + 1024 * u + 16 * lane);
-        const uint64_t lanes = __ballot(not_finite<DT, Q8>(w));
-        for (int x = 0; x < RPI; x++)
-          if (lanes >> (x * CPR) & (CPR == 64 ? ~0ull : (1ull << CPR) - 1)) bad |= 1ull << (RPI * u + x);
-      }
-      for (; bad; bad &= bad - 1) {
-        const int x = __builtin_ctzll(bad);
-        const uint8_t* const row = vs + x * RB;
-        const int swz = tv_swz<Q8, RB>(x);
+      after_k();
+      // mask: this lane's tokens are 16 n + 4 grp + i
+      const int pos0 = blk * BT;
+      const bool masked = is_masked(blk, have);
+      uint32_t seen[NC];
+#pragma unroll
+      for (int c = 0; c < NC; c++) seen[c] = ~0u;
+      if (masked) {
 #pragma unroll
         for (int c = 0; c < NC; c++) {
-          uint2 w = make_uint2(0, 0);
+          const int rel = pos0 - first, lim = (a.mask ? first : p0 + qi[c] + 1) - pos0;
+          const uint8_t* const row = a.mask + (size_t)(t0 + min(qi[c], nt - 1)) * a.mask_row;
+          seen[c] = 0;
+          uint32_t bytes[NB];
+          if (a.mask) {
+#pragma unroll
+            for (int n = 0; n < NB; n++) bytes[n] = mask4(row, a.mask_cols, rel + 16 * n + 4 * grp);
+          }
+#pragma unroll
+          for (int n = 0; n < NB; n++) {
+            const int x = 16 * n + 4 * grp;
+            uint32_t four = (1u << min(max(lim - x, 0), 4)) - 1;
+            if (a.mask) four |= nonzero4(bytes[n]);
+            seen[c] |= (four & (uint32_t)(have >> x) & 15) << (4 * n);
+          }
 #pragma unroll
           for (int n = 0; n < NB; n++)
-            if (x / 16 == n) w = pb[c][n];
-          const uint32_t h = x & 2 ? w.y : w.x;
-          // (the lane group that holds the token tells the others; -1: not seen)
-          const float mine = seen[c] >> (4 * (x / 16) + x % 4) & 1 ? (x & 1 ? hi16<DTV>(h) : lo16<DTV>(h)) : -1.f;
-          const float p = __shfl(mine, x % 16 / 4 * 16 + col);
 #pragma unroll
-          for (int dt = 0; dt < D / 16; dt++) {  // channels 16 dt + 4 grp + i
-            uint2 v;
-            if constexpr (Q8) v = e4m3x4<DT_BF16>(*reinterpret_cast<const uint32_t*>(row + 16 * (dt ^ swz) + 4 * grp), 1.f);
-            else v = *reinterpret_cast<const uint2*>(row + 16 * ((2 * dt + grp / 2) ^ swz) + 8 * (grp % 2));
-            const float f[4] = {lo16<DTV>(v.x), hi16<DTV>(v.x), lo16<DTV>(v.y), hi16<DTV>(v.y)};
-#pragma unroll
-            for (int i = 0; i < 4; i++) acc[c][dt][i] = p < 0.f ? acc[c][dt][i] : fmaf(p, f[i], acc[c][dt][i]);
-            __builtin_amdgcn_sched_barrier(0);  // (rare: no registers for it)
-          }
+            for (int i = 0; i < 4; i++) sc[c][n][i] = seen[c] >> (4 * n + i) & 1 ? sc[c][n][i] : -INFINITY;
         }
-        asm volatile("s_waitcnt lgkmcnt(0)" ::: "memory");
-        if (lane < CPR) *reinterpret_cast<uint4*>(vs + x * RB + 16 * lane) = make_uint4(0, 0, 0, 0);
-        asm volatile("s_waitcnt lgkmcnt(0)" ::: "memory");
       }
-    }
+      bool grow = false;
+      float mnew[NC];
 #pragma unroll
-    for (int m = 0; m < NB / 2; m++)
+      for (int c = 0; c < NC; c++) {
+        float mx = -INFINITY;
 #pragma unroll
-      for (int dt = 0; dt < D / 16; dt++) {
-        uint4 vf;
-        if constexpr (Q8) {
-          const uint2 w = lds_tr8(&vs[voff[dt] + 32 * m * RB]);
-          const uint2 f0 = e4m3x4<DTV>(w.x, 1.f), f1 = e4m3x4<DTV>(w.y, 1.f);
-          vf = make_uint4(f0.x, f0.y, f1.x, f1.y);
-        } else {
-          const uint2 lo = lds_tr4(reinterpret_cast<const uint16_t*>(&vs[voff[dt] + 32 * m * RB]));
-          const uint2 hi = lds_tr4(reinterpret_cast<const uint16_t*>(&vs[voff[dt] + (32 * m + 16) * RB]));
-          vf = make_uint4(lo.x, lo.y, hi.x, hi.y);
+        for (int n = 0; n < NB; n++)
+#pragma unroll
+          for (int i = 0; i < 4; i++) mx = fmaxf(mx, sc[c][n][i]);
+        mx = max_xor32(max_xor16(mx)) * a.scale_log2;
+        mnew[c] = mx > m_i[c] + kLazy ? mx : m_i[c];
+        grow |= mx > m_i[c] + kLazy;
+      }
+      if (__builtin_amdgcn_ballot_w64(grow)) {
+        far = false;
+#pragma unroll
+        for (int c = 0; c < NC; c++) {
+          const float alpha = m_i[c] == -INFINITY ? 0.f : __builtin_amdgcn_exp2f(m_i[c] - mnew[c]);
+          m_i[c] = mnew[c];
+          far |= __builtin_amdgcn_ballot_w64(fabsf(m_i[c]) > kFarScore && m_i[c] > -INFINITY) != 0;
+          l_i[c] *= alpha;
+#pragma unroll
+          for (int dt = 0; dt < D / 16; dt++) acc[c][dt] *= alpha;
         }
-#pragma unroll
-        for (int c = 0; c < NC; c++)
-          acc[c][dt] = mfma16<DTV>(vf, make_uint4(pb[c][2 * m].x, pb[c][2 * m].y, pb[c][2 * m + 1].x, pb[c][2 * m + 1].y),
-                                   acc[c][dt]);
       }
-    asm volatile("s_waitcnt lgkmcnt(0)" ::: "memory");  // every V fragment is in registers
-    if constexpr (!LAST) {
-      issue(nxt.place, std::false_type{});
-      cur = nxt;
-      kb = kb_next;
-      vb = vb_next;
-      nxt = place(blk + 2 * TR_WAVES, id_ahead);
-      asm volatile("" ::: "memory");
+      f32x4 vscale[NB];
       if constexpr (Q8) {
-        kb_next = scale(a.ks, nxt.place);
-        vb_next = scale(a.vs, nxt.place);
+#pragma unroll
+        for (int n = 0; n < NB; n++) vscale[n] = *reinterpret_cast<const f32x4*>(&s_vs[wave][16 * n + 4 * grp]);
       }
-      id_ahead = load_id(blk + 3 * TR_WAVES);
-      asm volatile("" ::: "memory");
-    }
-  };
-  // wave w takes blocks w, w + TR_WAVES, .. of the split (a fixed order)
-  if (blk0 + wave < blk1) {
-    int blk = blk0 + wave;
-    const int id0 = load_id(blk), id1 = load_id(blk + TR_WAVES);
-    cur = place(blk, id0);
-    nxt = place(blk + TR_WAVES, id1);
-    if constexpr (Q8) {
-      kb = scale(a.ks, cur.place);
-      vb = scale(a.vs, cur.place);
-    }
-    asm volatile("" ::: "memory");
-    issue(cur.place, std::true_type{});
-    issue(cur.place, std::false_type{});
-    asm volatile("" ::: "memory");
-    if constexpr (Q8) {
-      kb_next = scale(a.ks, nxt.place);
-      vb_next = scale(a.vs, nxt.place);
-    }
-    id_ahead = load_id(blk + 2 * TR_WAVES);
-    asm volatile("" ::: "memory");
-    for (; blk + TR_WAVES < blk1; blk += TR_WAVES) consume(blk, std::false_type{});
-    consume(blk, std::true_type{});
-  }
-
-  // ---- the waves merge: O over each wave's own V slot (and K slot)
+      uint2 pb[NC][NB];
 #pragma unroll
-  for (int c = 0; c < NC; c++) {
-    l_i[c] = add_xor32(add_xor16(l_i[c]));
-    float* const os = reinterpret_cast<float*>(c == 0 ? vs : ks);
+      for (int c = 0; c < NC; c++) {
+        float mref = m_i[c] == -INFINITY ? 0.f : m_i[c], scl = a.scale_log2;
+        if (far) {  // (uniform; a row goes by its own maximum, so its weights agree)
 #pragma unroll
-    for (int dt = 0; dt < D / 16; dt++) *reinterpret_cast<f32x4*>(os + col * D + 16 * dt + 4 * grp) = acc[c][dt];
-    if (grp == 0) {
-      s_m[wave][16 * c + col] = m_i[c];
-      s_l[wave][16 * c + col] = l_i[c];
-    }
-  }
-  __syncthreads();
-  const int live = min(TR_WAVES, blk1 - blk0);  // waves that had a block
-  const int rows = nt * G;
-  for (int idx = tid; idx < rows * (D / 4); idx += T) {
-    const int row = idx / (D / 4), d0 = idx % (D / 4) * 4;
-    float M = -INFINITY, L = 0.f;
-    f32x4 O = {0.f, 0.f, 0.f, 0.f};
-    for (int w = 0; w < live; w++) M = fmaxf(M, s_m[w][row]);
-    for (int w = 0; w < live; w++) {
-      const float f = s_m[w][row] == -INFINITY ? 0.f : __builtin_amdgcn_exp2f(s_m[w][row] - M);
-      const uint8_t* const os = row < 16 ? s_v[w] : s_k[w];
-      const f32x4 v = *reinterpret_cast<const f32x4*>(reinterpret_cast<const float*>(os) + row % 16 * D + d0);
-      L += s_l[w][row] * f;
-      O += v * f;
-    }
-    if (a.splits == 1) {
-      const float inv = L > 0.f || L != L ? 1.f / L : 0.f;
-      O *= inv;
-      *(YR_G uint64_t*)(a.out + ((size_t)(t0 + row / G) * a.hq + (size_t)hk * G + row % G) * D + d0) =
-          (uint64_t)pack2<DT>(O[2], O[3]) << 32 | pack2<DT>(O[0], O[1]);
-    } else {
-      float* rec = a.partial + (((size_t)pair * a.splits + split) * a.tt * G + row) * (D + 4);
-      st_agent4(rec + d0, make_float4(O[0], O[1], O[2], O[3]));
-      if (d0 == 0) st_agent4(rec + D, make_float4(M, L, 0.f, 0.f));
-    }
-  }
-  if (a.splits == 1) return;
-
-  // ---- the splits meet in the workgroup that arrives last: a thread takes 4 dims of one row
-  // over every SG-th split, 8 records in flight, and the SG parts meet in LDS (a fixed order)
-  if (!arrive_last(&a.tickets[pair], a.splits)) return;
-  constexpr int MU = 8;
-  const int items = rows * (D / 4);
-  const int SG = items * 2 <= T ? T / items : 1;
-  f32x4* const so = reinterpret_cast<f32x4*>(&s_v[0][0]);
-  float2* const sml = reinterpret_cast<float2*>(&s_k[0][0]);
-  for (int item0 = 0; item0 < items; item0 += T) {  // (one turn where SG > 1)
-    const int item = SG > 1 ? tid % items : item0 + tid, j = SG > 1 ? tid / items : 0;
-    const int row = item / (D / 4), d0 = item % (D / 4) * 4;
-    float M = -INFINITY, L = 0.f;
-    f32x4 O = {0.f, 0.f, 0.f, 0.f};
-    const bool work = item < items && j < SG;
-    if (work) {
-      const float* base = a.partial + ((size_t)pair * a.splits * a.tt * G + row) * (D + 4);
-      const size_t next = (size_t)a.tt * G * (D + 4);
-      for (int s0 = j; s0 < a.splits; s0 += SG * MU) {
-        float4 ml[MU], ov[MU];
+          for (int n = 0; n < NB; n++)
 #pragma unroll
-        for (int u = 0; u < MU; u++) {
-          ml[u] = make_float4(-INFINITY, 0.f, 0.f, 0.f);
-          ov[u] = make_float4(0.f, 0.f, 0.f, 0.f);
-          if (s0 + u * SG < a.splits) {
-            ml[u] = ld_agent4(base + (size_t)(s0 + u * SG) * next + D);
-            ov[u] = ld_agent4(base + (size_t)(s0 + u * SG) * next + d0);
+            for (int i = 0; i < 4; i++) sc[c][n][i] = far_exponent(sc[c][n][i], scl, mref);
+          mref = 0.f;
+          scl = 1.f;
+        }
+        mref -= kPBias<DT>;
+#pragma unroll
+        for (int n = 0; n < NB; n++) {
+          f32x4 p;
+#pragma unroll
+          for (int i = 0; i < 4; i++) {
+            p[i] = __builtin_amdgcn_exp2f(fmaf(sc[c][n][i], scl, -mref));
+            l_i[c] += p[i];
+            if constexpr (Q8) p[i] *= vscale[n][i];
+          }
+          if (Q8 && masked) {  // an unseen token's scale may be NaN
+#pragma unroll
+            for (int i = 0; i < 4; i++) p[i] = seen[c] >> (4 * n + i) & 1 ? p[i] : 0.f;
+          }
+          pb[c][n] = make_uint2(pack2<DT>(p[0], p[1]), pack2<DT>(p[2], p[3]));
+        }
+      }
+      before_v();
+      // Infinity or NaN in a token's V would reach the rows that do not see it as 0 * inf: such
+      // tokens are left out of the product and added to those that do, one by one.
+      if (masked) {
+        uint64_t bad = 0;
+#pragma unroll 1
+        for (int u = 0; u < NL; u++) {
+          const uint4 w = *reinterpret_cast<const uint4*>(vt + 1024 * u + 16 * lane);
+          const uint64_t lanes = __ballot(not_finite<DT, Q8>(w));
+          for (int x = 0; x < RPI; x++)
+            if (lanes >> (x * CPR) & ((1ull << CPR) - 1)) bad |= 1ull << (RPI * u + x);
+        }
+#pragma unroll 1
+        for (uint64_t left = bad; left; left &= left - 1) {
+          const int x = __builtin_ctzll(left);
+          const uint8_t* const row = vt + x * RB;
+          const int swz = tv_swz<Q8, RB>(x);
+#pragma unroll
+          for (int c = 0; c < NC; c++) {
+            uint2 w = make_uint2(0, 0);
+#pragma unroll
+            for (int n = 0; n < NB; n++)
+              if (x / 16 == n) w = pb[c][n];
+            const uint32_t h = x & 2 ? w.y : w.x;
+            // (the lane group that holds the token tells the others; -1: not seen)
+            const float mine = seen[c] >> (4 * (x / 16) + x % 4) & 1 ? (x & 1 ? hi16<DT>(h) : lo16<DT>(h)) : -1.f;
+            const float p = __shfl(mine, x % 16 / 4 * 16 + col);
+#pragma unroll
+            for (int dt = 0; dt < D / 16; dt++) {  // channels 16 dt + 4 grp + i
+              uint2 v;
+              if constexpr (Q8) v = e4m3x4<DT>(*reinterpret_cast<const uint32_t*>(row + 16 * (dt ^ swz) + 4 * grp), 1.f);
+              else v = *reinterpret_cast<const uint2*>(row + 16 * ((2 * dt + grp / 2) ^ swz) + 8 * (grp % 2));
+              const float f[4] = {lo16<DT>(v.x), hi16<DT>(v.x), lo16<DT>(v.y), hi16<DT>(v.y)};
+#pragma unroll
+              for (int i = 0; i < 4; i++) acc[c][dt][i] = p < 0.f ? acc[c][dt][i] : fmaf(p, f[i], acc[c][dt][i]);
+              __builtin_amdgcn_sched_barrier(0);  // (rare: no registers for it)
+            }
           }
         }
-        float mb = M;
-#pragma unroll
-        for (int u = 0; u < MU; u++) mb = fmaxf(mb, ml[u].x);
-        const float f0 = M == -INFINITY ? 0.f : __builtin_amdgcn_exp2f(M - mb);
-        L *= f0;
-        O *= f0;
-#pragma unroll
-        for (int u = 0; u < MU; u++) {
-          const float f = ml[u].x == -INFINITY ? 0.f : __builtin_amdgcn_exp2f(ml[u].x - mb);
-          L += ml[u].y * f;
-          O += f32x4{ov[u].x, ov[u].y, ov[u].z, ov[u].w} * f;
+        if (bad) {  // (the same for all waves of a shared block)
+          if constexpr (SHARE) __syncthreads();
+          if (!SHARE || wave == 0) {
+            for (uint64_t left = bad; left; left &= left - 1)
+              if (lane < CPR) *reinterpret_cast<uint4*>(vt + __builtin_ctzll(left) * RB + 16 * lane) = make_uint4(0, 0, 0, 0);
+          }
+          asm volatile("s_waitcnt lgkmcnt(0)" ::: "memory");
+          if constexpr (SHARE) __syncthreads();
         }
-        M = mb;
+      }
+#pragma unroll
+      for (int m = 0; m < NB / 2; m++)
+#pragma unroll
+        for (int dt = 0; dt < D / 16; dt++) {
+          uint4 vf;
+          if constexpr (Q8) {
+            const uint2 w = lds_tr8(&vt[voff[dt] + 32 * m * RB]);
+            const uint2 f0 = e4m3x4<DT>(w.x, 1.f), f1 = e4m3x4<DT>(w.y, 1.f);
+            vf = make_uint4(f0.x, f0.y, f1.x, f1.y);
+          } else {
+            const uint2 lo = lds_tr4(reinterpret_cast<const uint16_t*>(&vt[voff[dt] + 32 * m * RB]));
+            const uint2 hi = lds_tr4(reinterpret_cast<const uint16_t*>(&vt[voff[dt] + (32 * m + 16) * RB]));
+            vf = make_uint4(lo.x, lo.y, hi.x, hi.y);
+          }
+#pragma unroll
+          for (int c = 0; c < NC; c++)
+            acc[c][dt] = mfma16<DT>(vf, make_uint4(pb[c][2 * m].x, pb[c][2 * m].y, pb[c][2 * m + 1].x, pb[c][2 * m + 1].y),
+                                    acc[c][dt]);
+        }
+    };
+
+    if constexpr (!SHARE) {
+      uint8_t* const ks = s_k[wave];
+      uint8_t* const vs = s_v[wave];
+      constexpr auto kk = std::true_type{};
+      constexpr auto vv = std::false_type{};
+      constexpr auto all = std::integral_constant<int, NL>{};
+      Block cur, nxt;  // this block and the next
+      uint32_t (*const small)[kWave] = s_small[wave];
+      // The next block's scales and the ids of the one after: into LDS, like the rest, since a
+      // register's load among loads into LDS is waited for with all of them.
+      auto small_loads = [&](int ahead) __attribute__((always_inline)) {
+        lds_load4(id_at(ahead), small[0]);
+        if constexpr (Q8) {
+          const size_t where = (size_t)nxt.place * a.hkv + hk;
+          lds_load1(a.ks + where, small[1]);
+          lds_load1(a.vs + where, small[2]);
+        }
+        asm volatile("" ::: "memory");
+      };
+      // LAST: there is no next block (a copy of its own: every path knows how many loads are in flight)
+      auto consume = [&](int blk, auto last_c) __attribute__((always_inline)) {
+        constexpr bool LAST = decltype(last_c)::value;
+        // K has landed; V and the small loads may be on their way
+        asm volatile("s_waitcnt vmcnt(%0)" ::"n"(LAST ? NL : NL + NSMALL) : "memory");
+        compute(
+            blk, cur.have, ks, vs,
+            [&]() __attribute__((always_inline)) {
+              asm volatile("s_waitcnt lgkmcnt(0)" ::: "memory");
+              if constexpr (!LAST) issue(nxt.place, a.kc, ks, kk, all, 0);
+            },
+            [&]() __attribute__((always_inline)) {  // the small loads and the next K may be on their way
+              if constexpr (!LAST) asm volatile("s_waitcnt vmcnt(%0)" ::"n"(NL + NSMALL) : "memory");
+              else asm volatile("s_waitcnt vmcnt(0)" ::: "memory");
+            });
+        asm volatile("s_waitcnt lgkmcnt(0)" ::: "memory");  // every V fragment is in registers
+        if constexpr (!LAST) {
+          issue(nxt.place, a.vc, vs, vv, all, 0);
+          cur = nxt;
+          // the small loads of the last turn have landed
+          asm volatile("s_waitcnt vmcnt(%0)" ::"n"(2 * NL) : "memory");
+          const int id = (int)small[0][lane];
+          if constexpr (Q8) put_scales((int)small[1][lane], (int)small[2][lane], cur.have);
+          nxt = place(blk + 2 * TR_WAVES, id);
+          asm volatile("s_waitcnt lgkmcnt(0)" ::: "memory");
+          small_loads(blk + 3 * TR_WAVES);
+        }
+      };
+      // wave w takes blocks w, w + TR_WAVES, .. (a fixed order)
+      if (blk0 + wave < blk1) {
+        int blk = blk0 + wave;
+        const int id0 = *gptr(id_at(blk)), id1 = *gptr(id_at(blk + TR_WAVES));
+        cur = place(blk, id0);
+        nxt = place(blk + TR_WAVES, id1);
+        if constexpr (Q8) {
+          const size_t where = (size_t)cur.place * a.hkv + hk;
+          put_scales(gptr(a.ks)[where], gptr(a.vs)[where], cur.have);
+        }
+        asm volatile("" ::: "memory");
+        issue(cur.place, a.kc, ks, kk, all, 0);
+        issue(cur.place, a.vc, vs, vv, all, 0);
+        asm volatile("" ::: "memory");
+        small_loads(blk + 2 * TR_WAVES);
+        for (; blk + TR_WAVES < blk1; blk += TR_WAVES) consume(blk, std::false_type{});
+        consume(blk, std::true_type{});
+      }
+    } else {
+      constexpr int GROUP = 2 * NP + 1;  // a wave's loads of a block
+      const int n = blk1 - blk0;
+      const bool idle = nt * G <= col0;  // (no columns)
+      constexpr auto share = std::integral_constant<int, NP>{};
+      // block t, in slot t % 4: this wave's part of K and V, its scales (one wave K's, one V's), and
+      // the ids of block t + 3 (the others, each the same)
+      auto issue_block = [&](int t, uint32_t where) __attribute__((always_inline)) {
+        const int slot = t % TR_WAVES;
+        issue(where, a.kc, s_k[slot], std::true_type{}, share, wave * NP);
+        issue(where, a.vc, s_v[slot], std::false_type{}, share, wave * NP);
+        const size_t head = (size_t)where * a.hkv + hk;
+        if (Q8 && wave < 2) lds_load1((wave == 0 ? a.ks : a.vs) + head, s_small[slot][NSMALL > 1 ? 1 + wave : 0]);
+        else lds_load4(id_at(blk0 + t + 3), s_small[(t + 3) % TR_WAVES][0]);
+        asm volatile("" ::: "memory");
+      };
+      uint64_t have[3] = {0, 0, 0};  // of this block and the next two
+      if (n > 0) {
+        int id[3];
+#pragma unroll
+        for (int t = 0; t < 3; t++) id[t] = *gptr(id_at(blk0 + t));
+#pragma unroll
+        for (int t = 0; t < 3; t++) {
+          const Block p = place(blk0 + t, id[t]);
+          have[t] = p.have;
+          if (t < n) issue_block(t, p.place);
+        }
+      }
+      for (int t = 0; t < n; t++) {
+        // this wave's part of the block has landed; those of up to two more may be on their way
+        if (t + 2 < n) asm volatile("s_waitcnt vmcnt(%0) lgkmcnt(0)" ::"n"(2 * GROUP) : "memory");
+        else if (t + 1 < n) asm volatile("s_waitcnt vmcnt(%0) lgkmcnt(0)" ::"n"(GROUP) : "memory");
+        else asm volatile("s_waitcnt vmcnt(0) lgkmcnt(0)" ::: "memory");
+        __builtin_amdgcn_s_barrier();  // every wave's part has, and the block before is read out
+        asm volatile("" ::: "memory");
+        const int slot = t % TR_WAVES;
+        int kb = 0, vb = 0;
+        if constexpr (Q8) {
+          kb = (int)s_small[slot][1][lane];
+          vb = (int)s_small[slot][2][lane];
+        }
+        uint64_t have3 = 0;
+        if (t + 3 < n) {
+          const Block p = place(blk0 + t + 3, (int)s_small[(t + 3) % TR_WAVES][0][lane]);
+          have3 = p.have;
+          asm volatile("s_waitcnt lgkmcnt(0)" ::: "memory");
+          issue_block(t + 3, p.place);
+        }
+        if (!idle || is_masked(blk0 + t, have[0])) {  // (a masked block may need barriers)
+          if constexpr (Q8) put_scales(kb, vb, have[0]);
+          compute(blk0 + t, have[0], s_k[slot], s_v[slot], [] {}, [] {});
+        }
+        have[0] = have[1];
+        have[1] = have[2];
+        have[2] = have3;
       }
     }
-    if (SG > 1) {
-      if (work) {
-        so[j * items + item] = O;
-        if (d0 == 0) sml[j * 16 * NC + row] = make_float2(M, L);
+
+    // ---- results, or this workgroup's part of them
+#pragma unroll
+    for (int c = 0; c < NC; c++) {
+      l_i[c] = add_xor32(add_xor16(l_i[c]));
+      if constexpr (REL) {
+        const float f = scale_value(max(top, 0));
+#pragma unroll
+        for (int dt = 0; dt < D / 16; dt++) acc[c][dt] *= f;
+      }
+    }
+    const int rows = nt * G;
+    auto put_out = [&](int row, int d0, f32x4 O, float L) __attribute__((always_inline)) { put_result<DT, D>(a, hk, t0, row, d0, O, L); };
+    // a part has two records: of a tile that began before it, and of one that goes on behind it
+    float* mine = nullptr;
+    if (!whole) {
+      mine = a.partial + (((size_t)hk * a.parts + w0) * 2 + (u0 == 0)) * cols * (D + 4);
+      if (u0 == 0 && tid == 0)
+        a.split[(size_t)hk * a.parts + w0] = make_int4(t0, rows, part_of(units, parts, x - u1 + at.units - 1) - w0 + 1, 0);
+    }
+    auto put_record = [&](int row, int d0, f32x4 v) __attribute__((always_inline)) {
+      *reinterpret_cast<f32x4*>(mine + (size_t)row * (D + 4) + d0) = v;
+    };
+    if constexpr (SHARE) {
+#pragma unroll
+      for (int c = 0; c < NC; c++) {
+        const int row = col0 + 16 * c + col;
+        if (row < rows) {
+          if (!whole && grp == 0) put_record(row, D, f32x4{m_i[c], l_i[c], 0.f, 0.f});
+#pragma unroll
+          for (int dt = 0; dt < D / 16; dt++) {
+            const f32x4 O = acc[c][dt];
+            if (whole) put_out(row, 16 * dt + 4 * grp, O, l_i[c]);
+            else put_record(row, 16 * dt + 4 * grp, O);
+          }
+        }
+      }
+    } else {
+      // the waves merge: O over each wave's own V slot (and K slot)
+#pragma unroll
+      for (int c = 0; c < NC; c++) {
+        float* const os = reinterpret_cast<float*>(c == 0 ? s_v[wave] : s_k[wave]);
+#pragma unroll
+        for (int dt = 0; dt < D / 16; dt++) *reinterpret_cast<f32x4*>(os + col * D + 16 * dt + 4 * grp) = acc[c][dt];
+        if (grp == 0) {
+          s_m[wave][16 * c + col] = m_i[c];
+          s_l[wave][16 * c + col] = l_i[c];
+        }
       }
       __syncthreads();
-      if (!work || j > 0) return;
-      float mb = -INFINITY;
-      for (int u = 0; u < SG; u++) mb = fmaxf(mb, sml[u * 16 * NC + row].x);
-      L = 0.f;
-      O = f32x4{0.f, 0.f, 0.f, 0.f};
-      for (int u = 0; u < SG; u++) {
-        const float2 v = sml[u * 16 * NC + row];
-        const float f = v.x == -INFINITY ? 0.f : __builtin_amdgcn_exp2f(v.x - mb);
-        L += v.y * f;
-        O += so[u * items + item] * f;
+      const int live = min(TR_WAVES, blk1 - blk0);  // waves that had a block
+      for (int idx = tid; idx < rows * (D / 4); idx += T) {
+        const int row = idx / (D / 4), d0 = idx % (D / 4) * 4;
+        float M = -INFINITY, L = 0.f;
+        f32x4 O = {0.f, 0.f, 0.f, 0.f};
+        for (int w = 0; w < live; w++) M = fmaxf(M, s_m[w][row]);
+        for (int w = 0; w < live; w++) {
+          const float f = s_m[w][row] == -INFINITY ? 0.f : __builtin_amdgcn_exp2f(s_m[w][row] - M);
+          const uint8_t* const os = row < 16 ? s_v[w] : s_k[w];
+          const f32x4 v = *reinterpret_cast<const f32x4*>(reinterpret_cast<const float*>(os) + row % 16 * D + d0);
+          L += s_l[w][row] * f;
+          O += v * f;
+        }
+        if (whole) {
+          put_out(row, d0, O, L);
+        } else {
+          put_record(row, d0, O);
+          if (d0 == 0) put_record(row, D, f32x4{M, L, 0.f, 0.f});
+        }
       }
     }
-    if (work) {
-      const float inv = L > 0.f || L != L ? 1.f / L : 0.f;
-      O *= inv;
-      *(YR_G uint64_t*)(a.out + ((size_t)(t0 + row / G) * a.hq + (size_t)hk * G + row % G) * D + d0) =
-          (uint64_t)pack2<DT>(O[2], O[3]) << 32 | pack2<DT>(O[0], O[1]);
-    }
+
+    if (x >= x1) return;
+    __syncthreads();  // the slots are free again
+    work0 = seq_work(a, lane);
   }
 }
 
-// Groups of 16 columns, rows per tile, tiles and splits of a call.
+// Split tiles: the parts of one, 256 of its results' quads a workgroup.  Where there are fewer
+// quads, SG threads share one (every SG-th part each) and meet in LDS.  (A workgroup that
+// arrives last in the kernel above would take 38 us for 32 rows and 32 parts.)
+constexpr int TC_THREADS = 256, TC_AHEAD = 16;
+template <int DT, int D>
+__global__ __launch_bounds__(TC_THREADS) void tree_join_kernel(TreeArgs a) {
+  const int hk = blockIdx.x % a.hkv, w0 = blockIdx.x / a.hkv, tid = threadIdx.x;
+  const int4 at = a.split[(size_t)hk * a.parts + w0];  // first row, columns, parts
+  const int items = at.y * (D / 4), item0 = blockIdx.y * TC_THREADS;
+  if (at.z == 0 || item0 >= items) return;
+  const int SG = items * 2 <= TC_THREADS ? TC_THREADS / items : 1;
+  const int item = SG > 1 ? tid % items : item0 + tid, j = SG > 1 ? tid / items : 0;
+  const int row = item / (D / 4), d0 = item % (D / 4) * 4;
+  const size_t rec = (size_t)a.tt * (a.hq / a.hkv) * (D + 4);
+  const float* const base = a.partial + ((size_t)hk * a.parts + w0) * 2 * rec + (size_t)row * (D + 4);
+  float M = -INFINITY, L = 0.f;
+  f32x4 O = {0.f, 0.f, 0.f, 0.f};
+  const bool work = item < items && j < SG;
+  if (work) {
+    for (int p = j; p < at.z; p += SG * TC_AHEAD) {
+      float2 ml[TC_AHEAD];
+      f32x4 ov[TC_AHEAD];
+#pragma unroll
+      for (int u = 0; u < TC_AHEAD; u++) {
+        const int q = p + u * SG;
+        ml[u] = make_float2(-INFINITY, 0.f);
+        ov[u] = f32x4{0.f, 0.f, 0.f, 0.f};
+        if (q < at.z) {
+          const float* const r = base + (q == 0 ? rec : 2 * rec * q);  // (the first part's is its second record)
+          ml[u] = *reinterpret_cast<const float2*>(r + D);
+          ov[u] = *reinterpret_cast<const f32x4*>(r + d0);
+        }
+      }
+      float mb = M;
+#pragma unroll
+      for (int u = 0; u < TC_AHEAD; u++) mb = fmaxf(mb, ml[u].x);
+      const float f0 = M == -INFINITY ? 0.f : __builtin_amdgcn_exp2f(M - mb);
+      L *= f0;
+      O *= f0;
+#pragma unroll
+      for (int u = 0; u < TC_AHEAD; u++) {
+        const float f = ml[u].x == -INFINITY ? 0.f : __builtin_amdgcn_exp2f(ml[u].x - mb);
+        L += ml[u].y * f;
+        O += ov[u] * f;
+      }
+      M = mb;
+    }
+  }
+  if (SG > 1) {  // (a fixed order)
+    __shared__ f32x4 so[TC_THREADS];
+    __shared__ float2 sml[TC_THREADS];
+    so[tid] = O;
+    sml[tid] = make_float2(M, L);
+    __syncthreads();
+    if (j > 0) return;
+    float mb = -INFINITY;
+    for (int u = 0; u < SG; u++) mb = fmaxf(mb, sml[u * items + item].x);
+    L = 0.f;
+    O = f32x4{0.f, 0.f, 0.f, 0.f};
+    for (int u = 0; u < SG; u++) {
+      const float2 v = sml[u * items + item];
+      const float f = v.x == -INFINITY ? 0.f : __builtin_amdgcn_exp2f(v.x - mb);
+      L += v.y * f;
+      O += so[u * items + item] * f;
+    }
+  }
+  if (work) put_result<DT, D>(a, hk, at.x, row, d0, O, L);
+}
+
+// Columns of a tile, rows per tile, parts of a kv head's units (0: a tile a workgroup) of a call.
 struct TreePlan {
   long long tiles;
-  int nc, tt, splits;
+  int nc;
+  bool share;
+  int tt, parts;
 };
 static TreePlan tree_plan(bool ragged, int rows, int batch, int hkv, int G, int d, int max_kv_len, bool e4m3) {
   TreePlan p;
   const long long cols = ((long long)rows + batch - 1) / batch * G;  // of a sequence, on average
-  p.nc = cols <= 16 ? 1 : 2;
-  p.tt = ragged ? 16 * p.nc / G : 1;
+  p.share = cols > 32;
+  p.nc = cols <= 16 || (cols > 32 && cols <= 64) ? 1 : 2;
+  p.tt = ragged ? 16 * p.nc * (p.share ? TR_WAVES : 1) / G : 1;
   p.tiles = ragged ? (long long)rows / p.tt + batch : rows;
   if (p.tiles > rows) p.tiles = rows;
-  const int rb = e4m3 ? d : 2 * d, bt = 8192 / rb < 64 ? 8192 / rb : 64;
-  const long long pairs = p.tiles * hkv, blocks = ((long long)max_kv_len + bt - 1) / bt;
-  long long sp = (TR_TARGET_WG + pairs - 1) / pairs;
-  if (sp > blocks / TR_MIN_BLOCKS) sp = blocks / TR_MIN_BLOCKS;
-  if (pairs > kMaxTickets || sp < 1) sp = 1;
-  p.splits = (int)sp;
+  const int bt = tr_block(e4m3 ? d : 2 * d);
+  long long most = TR_TARGET_WG / hkv;
+  if (most < 1) most = 1;
+  p.parts = (int)most;
+  if (p.tiles >= 4 * most) {
+    p.parts = 0;
+  } else if (max_kv_len > 0) {
+    const long long blocks = p.tiles * (((long long)max_kv_len + bt - 1) / bt), need = blocks / TR_MIN_BLOCKS + 1;
+    if (need < most) p.parts = (int)need;
+  }
   return p;
 }
 
@@ -607,21 +909,24 @@ static TreePlan tree_plan(bool ragged, int rows, int batch, int hkv, int G, int 
 
 using namespace yr;
 
+static bool tree_shape(int rows, int batch, int hq, int hkv, int d) {
+  return rows > 0 && batch > 0 && hkv > 0 && hq >= hkv && hq % hkv == 0 && hq / hkv <= 16 && (d == 64 || d == 128);
+}
+
 extern "C" size_t yr_hip_gqa_tree_workspace(int rows, int batch, int ragged, int hq, int hkv, int d, int max_kv_len, int cache_dtype) {
-  if (rows <= 0 || batch <= 0 || hkv <= 0 || hq < hkv || hq % hkv || hq / hkv > 16 || d <= 0 || max_kv_len <= 0) return 0;
+  if (!tree_shape(rows, batch, hq, hkv, d)) return 0;
   const TreePlan p = tree_plan(ragged != 0, rows, batch, hkv, hq / hkv, d, max_kv_len, cache_dtype == YR_DTYPE_E4M3);
-  if (p.splits == 1) return 0;
-  return kTicketBytes + (size_t)p.tiles * hkv * p.splits * p.tt * (hq / hkv) * (d + 4) * sizeof(float);
+  if (p.parts == 0) return 0;
+  return kTicketBytes + (size_t)p.parts * hkv * (2 * p.tt * (hq / hkv) * (d + 4) * sizeof(float) + sizeof(int4));
 }
 
 extern "C" int yr_hip_gqa_tree_plan(int rows, int batch, int ragged, int hq, int hkv, int d, int max_kv_len, int cache_dtype, int* plan3) {
   const char* nm = "yr_hip_gqa_tree_plan";
-  if (!plan3 || rows <= 0 || batch <= 0 || hkv <= 0 || hq < hkv || hq % hkv || hq / hkv > 16 || d <= 0 || max_kv_len <= 0)
-    return fail(YR_E_INVALID, "%s: shape", nm);
+  if (!plan3 || !tree_shape(rows, batch, hq, hkv, d)) return fail(YR_E_INVALID, "%s: shape", nm);
   const TreePlan p = tree_plan(ragged != 0, rows, batch, hkv, hq / hkv, d, max_kv_len, cache_dtype == YR_DTYPE_E4M3);
-  plan3[0] = p.nc;
+  plan3[0] = 16 * p.nc * (p.share ? TR_WAVES : 1);
   plan3[1] = p.tt;
-  plan3[2] = p.splits;
+  plan3[2] = p.parts;
   return YR_OK;
 }
 
@@ -643,13 +948,13 @@ extern "C" int yr_hip_gqa_tree_paged(const void* q, const void* k_cache, const v
     return fail(YR_E_INVALID, "%s: a cache in e4m3 comes with its scales, one in 16 bits without", nm);
   const int G = hq / hkv;
   if (G < 1 || G > 16) return fail(YR_E_INVALID, "%s: group size %d (1 to 16)", nm, G);
-  if (max_kv_len <= 0) return fail(YR_E_INVALID, "%s: max_kv_len must be positive", nm);
   if (tree_mask && (mask_cols < 1 || mask_row < 0)) return fail(YR_E_INVALID, "%s: tree_mask has at least one column", nm);
   if (((uintptr_t)q | (uintptr_t)k_cache | (uintptr_t)v_cache | (uintptr_t)out) & 15)
     return fail(YR_E_INVALID, "%s: pointers must be 16-byte aligned", nm);
   if ((long long)num_pages * page_size > 0xffffffffll) return fail(YR_E_INVALID, "%s: a cache of more than 2^32 tokens", nm);
   const TreePlan p = tree_plan(qo_indptr != nullptr, rows, batch, hkv, G, d, max_kv_len, e4m3);
-  if (p.tiles * hkv * p.splits > 0x7fffffff || (long long)rows * hkv > 0x7fffffff) return fail(YR_E_INVALID, "%s: too many rows", nm);
+  const long long grid = (p.parts ? p.parts : p.tiles) * hkv;
+  if (grid > 0x7fffffff || (long long)rows * hkv > 0x7fffffff) return fail(YR_E_INVALID, "%s: too many rows", nm);
   const size_t need = yr_hip_gqa_tree_workspace(rows, batch, qo_indptr != nullptr, hq, hkv, d, max_kv_len, cache_dtype);
   if (need > workspace_bytes || (need && !workspace))
     return fail(YR_E_WORKSPACE, "%s: workspace %zu < %zu", nm, workspace_bytes, need);
@@ -662,27 +967,37 @@ extern "C" int yr_hip_gqa_tree_paged(const void* q, const void* k_cache, const v
   a.mask_row = mask_row;
   a.mask_cols = mask_cols;
   a.out = (uint16_t*)out;
-  a.tickets = (uint32_t*)workspace;
-  a.partial = need ? (float*)((char*)workspace + kTicketBytes) : nullptr;
+  // (the tickets of other operators that share a workspace stay as they are)
+  a.split = need ? (int4*)((char*)workspace + kTicketBytes) : nullptr;
+  a.partial = need ? (float*)(a.split + (size_t)p.parts * hkv) : nullptr;
   a.hq = hq;
   a.hkv = hkv;
   a.tt = p.tt;
-  a.splits = p.splits;
+  a.parts = p.parts;
   // 2^(31 + s) / page rounded up, page <= 2^s: the error is below 1 / page for x < 2^31
   int sh = 0;
   while ((1ll << sh) < page_size) sh++;
   a.page_mul = (uint32_t)(((1ull << (31 + sh)) + page_size - 1) / page_size);
   a.page_shift = 31 + sh;
   a.scale_log2 = kLog2e / sqrtf((float)d);
-  const unsigned grid = (unsigned)(p.tiles * hkv * p.splits);
   hipStream_t st = (hipStream_t)stream;
-#define YR_TR(DT_, Q_, D_, N_)                                  \
-  if (dtype == DT_ && e4m3 == Q_ && d == D_ && p.nc == N_)      \
-    hipLaunchKernelGGL((tree_kernel<DT_, Q_, D_, N_>), dim3(grid), dim3(TR_WAVES * kWave), 0, st, a);
-#define YR_TR2(DT_, Q_) YR_TR(DT_, Q_, 64, 1) YR_TR(DT_, Q_, 64, 2) YR_TR(DT_, Q_, 128, 1) YR_TR(DT_, Q_, 128, 2)
-  YR_TR2(DT_F16, false) YR_TR2(DT_F16, true) YR_TR2(DT_BF16, false) YR_TR2(DT_BF16, true)
+#define YR_TR(DT_, Q_, D_, N_, S_)                                                  \
+  if (dtype == DT_ && e4m3 == Q_ && d == D_ && p.nc == N_ && p.share == S_)         \
+    hipLaunchKernelGGL((tree_kernel<DT_, Q_, D_, N_, S_>), dim3((unsigned)grid), dim3(TR_WAVES * kWave), 0, st, a);
+#define YR_TR2(DT_, Q_, D_) \
+  YR_TR(DT_, Q_, D_, 1, false) YR_TR(DT_, Q_, D_, 2, false) YR_TR(DT_, Q_, D_, 1, true) YR_TR(DT_, Q_, D_, 2, true)
+  YR_TR2(DT_F16, false, 64) YR_TR2(DT_F16, false, 128) YR_TR2(DT_F16, true, 64) YR_TR2(DT_F16, true, 128)
+  YR_TR2(DT_BF16, false, 64) YR_TR2(DT_BF16, false, 128) YR_TR2(DT_BF16, true, 64) YR_TR2(DT_BF16, true, 128)
 #undef YR_TR2
 #undef YR_TR
+  YR_CHECK_LAUNCH(nm);
+  if (p.parts) {
+    const dim3 joins((unsigned)(p.parts * hkv), (unsigned)((p.tt * G * (d / 4) + TC_THREADS - 1) / TC_THREADS));
+#define YR_TJ(DT_, D_) \
+  if (dtype == DT_ && d == D_) hipLaunchKernelGGL((tree_join_kernel<DT_, D_>), joins, dim3(TC_THREADS), 0, st, a);
+    YR_TJ(DT_F16, 64) YR_TJ(DT_F16, 128) YR_TJ(DT_BF16, 64) YR_TJ(DT_BF16, 128)
+#undef YR_TJ
+  }
   YR_CHECK_LAUNCH(nm);
   return YR_OK;
 }

@@ -507,8 +507,9 @@ def gqa_tree_paged(q, k_cache, v_cache, kv_indptr, kv_indices, kv_len, tree_mask
 
     A row sees every token before its sequence's new ones; of the new ones those up to itself or,
     with tree_mask [T, n] (bool, last dim contiguous), those j with tree_mask[row, j] (none from n
-    on).  A row without a token, or whose scores are all -inf, is 0.  max_kv_len, about the largest
-    kv_len, says how finely the work is split (None: read on the host); it does not limit what is seen."""
+    on).  A row without a token, or whose scores are all -inf, is 0.  max_kv_len, about the
+    largest kv_len, spares a small call workgroups that find nothing to do; it does not limit what
+    is seen, and nothing is read on the host without it."""
     dtype = q.dtype
     dt = dtype_code(dtype)
     if k_cache.dtype is _E4M3:
@@ -541,9 +542,7 @@ def gqa_tree_paged(q, k_cache, v_cache, kv_indptr, kv_indices, kv_len, tree_mask
     index = _one_device(q, k_cache, v_cache, kv_indptr, kv_indices, kv_len, tree_mask, qo_indptr, k_scale, v_scale, out)
     if T == 0:
         return out
-    if max_kv_len is None:
-        max_kv_len = int(kv_len.max().item())
-    max_kv_len = max(max_kv_len, 1)
+    max_kv_len = 0 if max_kv_len is None else int(max_kv_len)
     stream = torch._C._cuda_getCurrentRawStream(index)
     L = lib()
     nb = L.yr_hip_gqa_tree_workspace(T, batch, qo_indptr is not None, hq, hkv, D, max_kv_len, cdt)
