@@ -25,6 +25,7 @@ namespace yr {
 constexpr int TR_WAVES = 4;
 constexpr int TR_TARGET_WG = 512;  // two per CU
 constexpr int TR_MIN_BLOCKS = 4;   // of a part
+constexpr int TR_WAVE_BLOCKS = 8;  // of a wave, for several heads to share a workgroup
 constexpr int tr_block(int row_bytes) { return 8192 / row_bytes < 64 ? 8192 / row_bytes : 64; }  // tokens
 
 struct TreeArgs {
@@ -36,10 +37,11 @@ struct TreeArgs {
   const uint8_t* vs;
   const uint8_t* mask;  // [rows][mask_cols], rows mask_row apart, or null
   uint16_t* out;
-  float* partial;       // [hkv][parts][2][tt G][D + 4]: O, m, l
-  int4* split;          // [hkv][parts]: the tile that begins in a part and ends in another: first row, columns, its parts (0: none)
+  float* partial;       // [hkv][parts heads][2][tt G][D + 4]: O, m, l
+  int4* split;          // the parts of this call, then [hkv][parts heads]: the tile that begins in a part and ends in another: first row, columns, its parts (0: none)
   long long mask_row;
-  int mask_cols, hq, hkv, tt, parts;  // rows per tile; ranges of a kv head's units (0: a workgroup a tile)
+  int mask_cols, hq, hkv, tt;  // rows per tile
+  int parts, log_heads;        // workgroups per kv head (0: one a tile); kv heads that may share one
   uint32_t page_mul, page_shift;       // x / page = x page_mul >> page_shift for x < 2^31
   float scale_log2;
 };
@@ -283,7 +285,6 @@ __global__ __launch_bounds__(TR_WAVES * kWave, 2) void tree_kernel(TreeArgs a) {
   static_assert(NL % TR_WAVES == 0, "waves load equal shares");
   const int tid = threadIdx.x, lane = tid % kWave;
   const int wave = __builtin_amdgcn_readfirstlane(tid / kWave);
-  const int hk = blockIdx.x % a.hkv, w0 = blockIdx.x / a.hkv;
   const int G = a.hq / a.hkv, col = lane % 16, grp = lane / 16;
   const int cols = a.tt * G;
 
@@ -307,17 +308,26 @@ __global__ __launch_bounds__(TR_WAVES * kWave, 2) void tree_kernel(TreeArgs a) {
   long long units = 0, x = 0, x1 = 1;
   int parts = 1;
   SeqWork work0 = seq_work(a, lane);
+  // Up to 4 kv heads share a workgroup, a wave (or two) each, where a wave has enough to do:
+  // they read neighbouring bytes at about the same time (loads alone, 128 bytes a head: 5.2 TB/s
+  // with a workgroup a head, 6.0 with 4 heads in one).
+  if (a.parts) units = all_units(a, work0);
+  const bool shared = !SHARE && !(a.parts && units < (long long)TR_WAVE_BLOCKS * BT * TR_WAVES * a.parts);
+  const int log_heads = shared ? a.log_heads : 0, heads = 1 << log_heads, groups = a.hkv >> log_heads;
+  const int w0 = __builtin_amdgcn_readfirstlane(blockIdx.x / groups), hk0 = (blockIdx.x - w0 * groups) << log_heads;
+  const int streams = TR_WAVES >> log_heads, stream = SHARE ? 0 : wave & (streams - 1);  // waves of a head
+  const int hk = SHARE ? hk0 : hk0 + (wave << log_heads) / TR_WAVES;                      // this wave's
+  const int most = a.parts << a.log_heads;
   if (a.parts) {
-    if (tid == 0) a.split[(size_t)hk * a.parts + w0].z = 0;
-    units = all_units(a, work0);
-    parts = (int)min((long long)a.parts, max(units / (TR_MIN_BLOCKS * BT), 1ll));
+    parts = (int)min((long long)a.parts << log_heads, max(units / (TR_MIN_BLOCKS * BT), 1ll));
+    if (blockIdx.x == 0 && tid == 0) a.split[0].x = units ? parts : 0;
     if (w0 >= parts) return;
     x = part_start(units, parts, w0);
     x1 = part_start(units, parts, w0 + 1);
   }
   while (true) {
     const TileAt at = a.parts ? find_unit(a, work0, x) : find_index(a, work0, w0);
-    if (at.b >= a.r.batch) return;
+    if (at.b >= a.r.batch) return;  // (only without parts)
     const SeqRows s = at.s;
     const int i0 = at.tile * a.tt;
     const long long u0 = a.parts ? x - at.from : 0, u1 = a.parts ? min(x1 - at.from, at.units) : 1;
@@ -650,17 +660,17 @@ __global__ __launch_bounds__(TR_WAVES * kWave, 2) void tree_kernel(TreeArgs a) {
           asm volatile("s_waitcnt vmcnt(%0)" ::"n"(2 * NL) : "memory");
           const int id = (int)small[0][lane];
           if constexpr (Q8) put_scales((int)small[1][lane], (int)small[2][lane], cur.have);
-          nxt = place(blk + 2 * TR_WAVES, id);
+          nxt = place(blk + 2 * streams, id);
           asm volatile("s_waitcnt lgkmcnt(0)" ::: "memory");
-          small_loads(blk + 3 * TR_WAVES);
+          small_loads(blk + 3 * streams);
         }
       };
-      // wave w takes blocks w, w + TR_WAVES, .. (a fixed order)
-      if (blk0 + wave < blk1) {
-        int blk = blk0 + wave;
-        const int id0 = *gptr(id_at(blk)), id1 = *gptr(id_at(blk + TR_WAVES));
+      // a head's waves take blocks in turn (a fixed order)
+      if (blk0 + stream < blk1) {
+        int blk = blk0 + stream;
+        const int id0 = *gptr(id_at(blk)), id1 = *gptr(id_at(blk + streams));
         cur = place(blk, id0);
-        nxt = place(blk + TR_WAVES, id1);
+        nxt = place(blk + streams, id1);
         if constexpr (Q8) {
           const size_t where = (size_t)cur.place * a.hkv + hk;
           put_scales(gptr(a.ks)[where], gptr(a.vs)[where], cur.have);
@@ -669,8 +679,8 @@ __global__ __launch_bounds__(TR_WAVES * kWave, 2) void tree_kernel(TreeArgs a) {
         issue(cur.place, a.kc, ks, kk, all, 0);
         issue(cur.place, a.vc, vs, vv, all, 0);
         asm volatile("" ::: "memory");
-        small_loads(blk + 2 * TR_WAVES);
-        for (; blk + TR_WAVES < blk1; blk += TR_WAVES) consume(blk, std::false_type{});
+        small_loads(blk + 2 * streams);
+        for (; blk + streams < blk1; blk += streams) consume(blk, std::false_type{});
         consume(blk, std::true_type{});
       }
     } else {
@@ -742,28 +752,29 @@ __global__ __launch_bounds__(TR_WAVES * kWave, 2) void tree_kernel(TreeArgs a) {
       }
     }
     const int rows = nt * G;
-    auto put_out = [&](int row, int d0, f32x4 O, float L) __attribute__((always_inline)) { put_result<DT, D>(a, hk, t0, row, d0, O, L); };
     // a part has two records: of a tile that began before it, and of one that goes on behind it
-    float* mine = nullptr;
-    if (!whole) {
-      mine = a.partial + (((size_t)hk * a.parts + w0) * 2 + (u0 == 0)) * cols * (D + 4);
-      if (u0 == 0 && tid == 0)
-        a.split[(size_t)hk * a.parts + w0] = make_int4(t0, rows, part_of(units, parts, x - u1 + at.units - 1) - w0 + 1, 0);
+    auto record = [&](int head) __attribute__((always_inline)) -> float* {
+      return a.partial + (((size_t)head * most + w0) * 2 + (u0 == 0)) * cols * (D + 4);
+    };
+    if (a.parts && x >= x1 && tid == 0) {  // its last tile: the parts that this one begins, if it does
+      const int n = !whole && u0 == 0 ? part_of(units, parts, x - u1 + at.units - 1) - w0 + 1 : 0;
+      for (int h = hk0; h < hk0 + heads; h++) a.split[1 + (size_t)h * most + w0] = make_int4(t0, rows, n, 0);
     }
-    auto put_record = [&](int row, int d0, f32x4 v) __attribute__((always_inline)) {
-      *reinterpret_cast<f32x4*>(mine + (size_t)row * (D + 4) + d0) = v;
+    auto put_record = [&](float* rec, int row, int d0, f32x4 v) __attribute__((always_inline)) {
+      *reinterpret_cast<f32x4*>(rec + (size_t)row * (D + 4) + d0) = v;
     };
     if constexpr (SHARE) {
+      float* const mine = record(hk);
 #pragma unroll
       for (int c = 0; c < NC; c++) {
         const int row = col0 + 16 * c + col;
         if (row < rows) {
-          if (!whole && grp == 0) put_record(row, D, f32x4{m_i[c], l_i[c], 0.f, 0.f});
+          if (!whole && grp == 0) put_record(mine, row, D, f32x4{m_i[c], l_i[c], 0.f, 0.f});
 #pragma unroll
           for (int dt = 0; dt < D / 16; dt++) {
             const f32x4 O = acc[c][dt];
-            if (whole) put_out(row, 16 * dt + 4 * grp, O, l_i[c]);
-            else put_record(row, 16 * dt + 4 * grp, O);
+            if (whole) put_result<DT, D>(a, hk, t0, row, 16 * dt + 4 * grp, O, l_i[c]);
+            else put_record(mine, row, 16 * dt + 4 * grp, O);
           }
         }
       }
@@ -780,13 +791,14 @@ __global__ __launch_bounds__(TR_WAVES * kWave, 2) void tree_kernel(TreeArgs a) {
         }
       }
       __syncthreads();
-      const int live = min(TR_WAVES, blk1 - blk0);  // waves that had a block
-      for (int idx = tid; idx < rows * (D / 4); idx += T) {
-        const int row = idx / (D / 4), d0 = idx % (D / 4) * 4;
+      const int live = min(streams, blk1 - blk0);  // waves of a head that had a block
+      const int quads = rows * (D / 4);
+      for (int idx = tid; idx < quads * heads; idx += T) {
+        const int head = idx / quads, row = idx % quads / (D / 4), d0 = idx % (D / 4) * 4, wa = head * streams;
         float M = -INFINITY, L = 0.f;
         f32x4 O = {0.f, 0.f, 0.f, 0.f};
-        for (int w = 0; w < live; w++) M = fmaxf(M, s_m[w][row]);
-        for (int w = 0; w < live; w++) {
+        for (int w = wa; w < wa + live; w++) M = fmaxf(M, s_m[w][row]);
+        for (int w = wa; w < wa + live; w++) {
           const float f = s_m[w][row] == -INFINITY ? 0.f : __builtin_amdgcn_exp2f(s_m[w][row] - M);
           const uint8_t* const os = row < 16 ? s_v[w] : s_k[w];
           const f32x4 v = *reinterpret_cast<const f32x4*>(reinterpret_cast<const float*>(os) + row % 16 * D + d0);
@@ -794,10 +806,10 @@ __global__ __launch_bounds__(TR_WAVES * kWave, 2) void tree_kernel(TreeArgs a) {
           O += v * f;
         }
         if (whole) {
-          put_out(row, d0, O, L);
+          put_result<DT, D>(a, hk0 + head, t0, row, d0, O, L);
         } else {
-          put_record(row, d0, O);
-          if (d0 == 0) put_record(row, D, f32x4{M, L, 0.f, 0.f});
+          put_record(record(hk0 + head), row, d0, O);
+          if (d0 == 0) put_record(record(hk0 + head), row, D, f32x4{M, L, 0.f, 0.f});
         }
       }
     }
@@ -814,15 +826,15 @@ __global__ __launch_bounds__(TR_WAVES * kWave, 2) void tree_kernel(TreeArgs a) {
 constexpr int TC_THREADS = 256, TC_AHEAD = 16;
 template <int DT, int D>
 __global__ __launch_bounds__(TC_THREADS) void tree_join_kernel(TreeArgs a) {
-  const int hk = blockIdx.x % a.hkv, w0 = blockIdx.x / a.hkv, tid = threadIdx.x;
-  const int4 at = a.split[(size_t)hk * a.parts + w0];  // first row, columns, parts
+  const int hk = blockIdx.x % a.hkv, w0 = blockIdx.x / a.hkv, tid = threadIdx.x, most = a.parts << a.log_heads;
+  const int4 at = a.split[1 + (size_t)hk * most + w0];  // first row, columns, parts
   const int items = at.y * (D / 4), item0 = blockIdx.y * TC_THREADS;
-  if (at.z == 0 || item0 >= items) return;
+  if (w0 >= a.split[0].x || at.z == 0 || item0 >= items) return;
   const int SG = items * 2 <= TC_THREADS ? TC_THREADS / items : 1;
   const int item = SG > 1 ? tid % items : item0 + tid, j = SG > 1 ? tid / items : 0;
   const int row = item / (D / 4), d0 = item % (D / 4) * 4;
   const size_t rec = (size_t)a.tt * (a.hq / a.hkv) * (D + 4);
-  const float* const base = a.partial + ((size_t)hk * a.parts + w0) * 2 * rec + (size_t)row * (D + 4);
+  const float* const base = a.partial + ((size_t)hk * most + w0) * 2 * rec + (size_t)row * (D + 4);
   float M = -INFINITY, L = 0.f;
   f32x4 O = {0.f, 0.f, 0.f, 0.f};
   const bool work = item < items && j < SG;
@@ -882,7 +894,7 @@ struct TreePlan {
   long long tiles;
   int nc;
   bool share;
-  int tt, parts;
+  int tt, parts, log_heads;
 };
 static TreePlan tree_plan(bool ragged, int rows, int batch, int hkv, int G, int d, int max_kv_len, bool e4m3) {
   TreePlan p;
@@ -893,6 +905,7 @@ static TreePlan tree_plan(bool ragged, int rows, int batch, int hkv, int G, int 
   p.tiles = ragged ? (long long)rows / p.tt + batch : rows;
   if (p.tiles > rows) p.tiles = rows;
   const int bt = tr_block(e4m3 ? d : 2 * d);
+  p.log_heads = p.share ? 0 : hkv % 4 == 0 ? 2 : hkv % 2 == 0 ? 1 : 0;
   long long most = TR_TARGET_WG / hkv;
   if (most < 1) most = 1;
   p.parts = (int)most;
@@ -917,7 +930,7 @@ extern "C" size_t yr_hip_gqa_tree_workspace(int rows, int batch, int ragged, int
   if (!tree_shape(rows, batch, hq, hkv, d)) return 0;
   const TreePlan p = tree_plan(ragged != 0, rows, batch, hkv, hq / hkv, d, max_kv_len, cache_dtype == YR_DTYPE_E4M3);
   if (p.parts == 0) return 0;
-  return kTicketBytes + (size_t)p.parts * hkv * (2 * p.tt * (hq / hkv) * (d + 4) * sizeof(float) + sizeof(int4));
+  return kTicketBytes + sizeof(int4) + ((size_t)p.parts << p.log_heads) * hkv * (2 * p.tt * (hq / hkv) * (d + 4) * sizeof(float) + sizeof(int4));
 }
 
 extern "C" int yr_hip_gqa_tree_plan(int rows, int batch, int ragged, int hq, int hkv, int d, int max_kv_len, int cache_dtype, int* plan3) {
@@ -953,7 +966,7 @@ extern "C" int yr_hip_gqa_tree_paged(const void* q, const void* k_cache, const v
     return fail(YR_E_INVALID, "%s: pointers must be 16-byte aligned", nm);
   if ((long long)num_pages * page_size > 0xffffffffll) return fail(YR_E_INVALID, "%s: a cache of more than 2^32 tokens", nm);
   const TreePlan p = tree_plan(qo_indptr != nullptr, rows, batch, hkv, G, d, max_kv_len, e4m3);
-  const long long grid = (p.parts ? p.parts : p.tiles) * hkv;
+  const long long grid = p.parts ? (long long)p.parts * hkv : p.tiles * (hkv >> p.log_heads);
   if (grid > 0x7fffffff || (long long)rows * hkv > 0x7fffffff) return fail(YR_E_INVALID, "%s: too many rows", nm);
   const size_t need = yr_hip_gqa_tree_workspace(rows, batch, qo_indptr != nullptr, hq, hkv, d, max_kv_len, cache_dtype);
   if (need > workspace_bytes || (need && !workspace))
@@ -969,11 +982,12 @@ extern "C" int yr_hip_gqa_tree_paged(const void* q, const void* k_cache, const v
   a.out = (uint16_t*)out;
   // (the tickets of other operators that share a workspace stay as they are)
   a.split = need ? (int4*)((char*)workspace + kTicketBytes) : nullptr;
-  a.partial = need ? (float*)(a.split + (size_t)p.parts * hkv) : nullptr;
+  a.partial = need ? (float*)(a.split + 1 + ((size_t)p.parts << p.log_heads) * hkv) : nullptr;
   a.hq = hq;
   a.hkv = hkv;
   a.tt = p.tt;
   a.parts = p.parts;
+  a.log_heads = p.log_heads;
   // 2^(31 + s) / page rounded up, page <= 2^s: the error is below 1 / page for x < 2^31
   int sh = 0;
   while ((1ll << sh) < page_size) sh++;
@@ -992,7 +1006,7 @@ extern "C" int yr_hip_gqa_tree_paged(const void* q, const void* k_cache, const v
 #undef YR_TR
   YR_CHECK_LAUNCH(nm);
   if (p.parts) {
-    const dim3 joins((unsigned)(p.parts * hkv), (unsigned)((p.tt * G * (d / 4) + TC_THREADS - 1) / TC_THREADS));
+    const dim3 joins((unsigned)((p.parts << p.log_heads) * hkv), (unsigned)((p.tt * G * (d / 4) + TC_THREADS - 1) / TC_THREADS));
 #define YR_TJ(DT_, D_) \
   if (dtype == DT_ && d == D_) hipLaunchKernelGGL((tree_join_kernel<DT_, D_>), joins, dim3(TC_THREADS), 0, st, a);
     YR_TJ(DT_F16, 64) YR_TJ(DT_F16, 128) YR_TJ(DT_BF16, 64) YR_TJ(DT_BF16, 128)
