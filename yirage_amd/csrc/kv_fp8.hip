@@ -159,10 +159,10 @@ struct Read8Args {
   int hkv;
 };
 
-// 16 codes and their scale -> 16 values of 16 bits.  Exact in bf16 wherever the value
+// 8 codes and their scale -> 8 values of 16 bits.  Exact in bf16 wherever the value
 // is normal, rounded once in f16; a scale of NaN gives NaN.
 template <int DT>
-__device__ __forceinline__ void values16(uint4 c, uint32_t scale, uint4* out) {
+__device__ __forceinline__ uint4 values8(uint2 c, uint32_t scale) {
   const float s = __uint_as_float(scale << 23);
   auto two = [&](uint32_t w, auto hi) __attribute__((always_inline)) -> uint32_t {
     if constexpr (DT == DT_BF16) return __builtin_bit_cast(uint32_t, __builtin_amdgcn_cvt_scalef32_pk_bf16_fp8(w, s, hi.value));
@@ -170,11 +170,12 @@ __device__ __forceinline__ void values16(uint4 c, uint32_t scale, uint4* out) {
   };
   constexpr std::false_type lo;
   constexpr std::true_type hi;
-  out[0] = make_uint4(two(c.x, lo), two(c.x, hi), two(c.y, lo), two(c.y, hi));
-  out[1] = make_uint4(two(c.z, lo), two(c.z, hi), two(c.w, lo), two(c.w, hi));
+  return make_uint4(two(c.x, lo), two(c.x, hi), two(c.y, lo), two(c.y, hi));
 }
 
-constexpr int R8_TOKENS = 8;  // of a wave: lane i looks up token i % R8_TOKENS
+// A wave takes R8_TOKENS tokens: lane i looks up token i % R8_TOKENS, then the wave passes over
+// their pieces of 8 codes, R8_AHEAD of them a lane on their way.  Bound by memory.
+constexpr int R8_TOKENS = 8, R8_AHEAD = 8;
 
 template <int DT, int D>
 __global__ __launch_bounds__(256) void read8_kernel(Read8Args a) {
@@ -192,31 +193,43 @@ __global__ __launch_bounds__(256) void read8_kernel(Read8Args a) {
       place = id < 0 ? -1 : (long long)id * r.page + p % r.page;
     }
   }
-  const int per = a.hkv * D / 16, total = n * per;  // 16-code pieces of a token
+  const int per = a.hkv * (D / 8), total = n * per;  // pieces of a token
   int u = lane / per, i = lane % per;
   const int du = kWave / per, di = kWave % per;
-  for (int at = lane; at - lane < total; at += kWave) {
-    const int token = min(u, n - 1);
-    const long long from = (long long)(uint32_t)__shfl((int)(uint32_t)place, token) | (long long)__shfl((int)(place >> 32), token) << 32;
-    if (at < total && from >= -1) {
-      uint4 ko[2], vo[2];
-      ko[0] = ko[1] = vo[0] = vo[1] = make_uint4(0, 0, 0, 0);
-      if (from >= 0) {
-        const size_t head = (size_t)from * a.hkv + i / (D / 16), piece = (size_t)from * per + i;
-        values16<DT>(ldg16(a.kc + piece * 16), gptr(a.ks)[head], ko);
-        values16<DT>(ldg16(a.vc + piece * 16), gptr(a.vs)[head], vo);
+  for (int at = lane; at - lane < total; at += kWave * R8_AHEAD) {
+    long long from[R8_AHEAD];
+    size_t to[R8_AHEAD];
+    uint2 kw[R8_AHEAD], vw[R8_AHEAD];
+    uint32_t kb[R8_AHEAD], vb[R8_AHEAD];
+#pragma unroll
+    for (int x = 0; x < R8_AHEAD; x++) {
+      const int token = min(u, n - 1);
+      from[x] = (long long)(uint32_t)__shfl((int)(uint32_t)place, token) | (long long)__shfl((int)(place >> 32), token) << 32;
+      if (at + x * kWave >= total) from[x] = -2;
+      to[x] = ((size_t)(t0 + u) * per + i) * 8;
+      const size_t row = (size_t)max(from[x], 0ll), head = row * a.hkv + i / (D / 8), piece = (row * per + i) * 8;
+      kw[x] = vw[x] = make_uint2(0, 0);
+      kb[x] = vb[x] = 0;
+      if (from[x] >= 0) {
+        const uint64_t k = *(const YR_G uint64_t*)(a.kc + piece);
+        const uint64_t v = *(const YR_G uint64_t*)(a.vc + piece);
+        kw[x] = make_uint2((uint32_t)k, (uint32_t)(k >> 32));
+        vw[x] = make_uint2((uint32_t)v, (uint32_t)(v >> 32));
+        kb[x] = gptr(a.ks)[head];
+        vb[x] = gptr(a.vs)[head];
       }
-      const size_t to = ((size_t)(t0 + u) * per + i) * 16;
-      stg16_stream(a.k + to, ko[0]);
-      stg16_stream(a.k + to + 8, ko[1]);
-      stg16_stream(a.v + to, vo[0]);
-      stg16_stream(a.v + to + 8, vo[1]);
+      u += du;
+      i += di;
+      if (i >= per) {
+        i -= per;
+        u++;
+      }
     }
-    u += du;
-    i += di;
-    if (i >= per) {
-      i -= per;
-      u++;
+#pragma unroll
+    for (int x = 0; x < R8_AHEAD; x++) {
+      if (from[x] < -1) continue;
+      stg16_stream(a.k + to[x], values8<DT>(kw[x], kb[x]));
+      stg16_stream(a.v + to[x], values8<DT>(vw[x], vb[x]));
     }
   }
 }

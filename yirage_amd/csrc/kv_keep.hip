@@ -57,15 +57,15 @@ __global__ __launch_bounds__(KEEP_THREADS) void keep_kernel(KeepArgs a) {
   while (more) {
     int n = 0, from[KEEP_AHEAD];
 #pragma unroll
+    for (int u = 0; u < KEEP_AHEAD; u++) from[u] = kept + u < a.depth ? gptr(path)[kept + u] : -1;
+#pragma unroll
     for (int u = 0; u < KEEP_AHEAD; u++) {
-      from[u] = 0;
+      more = more && from[u] > last && from[u] < s.n;
       if (more) {
-        const int p = kept + n < a.depth ? gptr(path)[kept + n] : -1;
-        more = p > last && p < s.n;
-        if (more) {
-          from[u] = last = p;
-          n++;
-        }
+        last = from[u];
+        n++;
+      } else {
+        from[u] = 0;
       }
     }
     // (a token without a place is neither read nor written)
@@ -77,11 +77,12 @@ __global__ __launch_bounds__(KEEP_THREADS) void keep_kernel(KeepArgs a) {
     for (int u = 0; u < KEEP_AHEAD; u++) {
       const int p = first + from[u], q = first + kept + u;
       const bool some = u < n && p >= 0 && q >= 0;
-      const int f = some ? page_id(r, s, p / r.page) : -1;
-      page[u] = some ? page_id(r, s, q / r.page) : -1;
+      const int up = some ? p / r.page : -1, uq = some ? q / r.page : -1;
+      const int f = page_id(r, s, up);
+      page[u] = page_id(r, s, uq);
       if (f < 0) page[u] = -1;
-      src[u] = (long long)max(f, 0) * r.page + (some ? p % r.page : 0);
-      dst[u] = (long long)max(page[u], 0) * r.page + (some ? q % r.page : 0);
+      src[u] = (long long)max(f, 0) * r.page + p - up * r.page;
+      dst[u] = (long long)max(page[u], 0) * r.page + q - uq * r.page;
     }
 #pragma unroll
     for (int u = 0; u < KEEP_AHEAD; u++) {
