@@ -14,7 +14,7 @@
 //
 // In 8 bits a fragment is converted between LDS and MFMA.  The conversion multiplies by
 // a power of two, so a key is read with its scale for nothing and, in bf16, without
-// rounding; a fragment of V holds 8 tokens, whose scales go onto the weights instead.
+// rounding; a fragment of V holds 8 tokens, whose scales go into the weights' exponents instead.
 #include <type_traits>
 
 #include "attn_device.h"
@@ -25,8 +25,11 @@ namespace yr {
 constexpr int TR_WAVES = 4;
 constexpr int TR_TARGET_WG = 512;  // two per CU
 constexpr int TR_MIN_BLOCKS = 4;   // of a part
+constexpr int TR_TILE_COST = 192;  // of a tile's start, in tokens
 constexpr int TR_WAVE_BLOCKS = 8;  // of a wave, for several heads to share a workgroup
-constexpr int tr_block(int row_bytes) { return 8192 / row_bytes < 64 ? 8192 / row_bytes : 64; }  // tokens
+// Tokens of a block: a lane's each, half as many where a wave has a block of its own and a
+// token 256 bytes (shared ones of 32: a chunk of 2048 rows in 16 bits 744 us for 629).
+constexpr int tr_block(int row_bytes, bool share) { return row_bytes == 256 && !share ? 32 : 64; }
 
 struct TreeArgs {
   Ragged r;
@@ -43,11 +46,11 @@ struct TreeArgs {
   int mask_cols, hq, hkv, tt;  // rows per tile
   int parts, log_heads;        // workgroups per kv head (0: one a tile); kv heads that may share one
   uint32_t page_mul, page_shift;       // x / page = x page_mul >> page_shift for x < 2^31
-  float scale_log2;
+  float scale_log2, scale_inv;
 };
 
 // Work.  A sequence of n new rows has ceil(n / tt) tiles, and a tile counts for as many units
-// as tokens its last row may see.  The units of a kv head, one sequence after another, are
+// as tokens its last row may see, and TR_TILE_COST for its start.  The units of a kv head, one sequence after another, are
 // cut into `parts` equal ranges, a workgroup each: lengths that differ leave no workgroup
 // waiting, a long sequence is split and several short ones share a workgroup.  (32 sequences
 // of 4 to 8 K tokens, two workgroups of each: TIME.)
@@ -57,8 +60,8 @@ struct SeqWork {
   long long units;
 };
 __device__ __forceinline__ long long units_before(const TreeArgs& a, const SeqRows& s, int tile) {
-  if (a.mask) return (long long)tile * max(s.len, 1);
-  return (long long)tile * max(s.len - s.n, 0) + (long long)a.tt * tile * (tile + 1) / 2;
+  if (a.mask) return (long long)tile * (s.len + TR_TILE_COST);
+  return (long long)tile * (max(s.len - s.n, 0) + TR_TILE_COST) + (long long)a.tt * tile * (tile + 1) / 2;
 }
 __device__ __forceinline__ SeqWork seq_work(const TreeArgs& a, int b) {
   SeqWork w;
@@ -263,21 +266,21 @@ __device__ __forceinline__ void put_result(const TreeArgs& a, int hk, int t0, in
 // are in registers and its next V block after P V, so one of the two is always in flight.
 //
 // SHARE true: each wave has its own columns (rows of up to 64 NC / G tokens) and all work on
-// the same block, so K and V are moved to LDS once for all of them.  The slots are a ring,
-// three blocks ahead, with one barrier a block.
+// the same block, so K and V are moved to LDS once for all of them.  The slots are a ring with
+// one barrier a block.
 template <int DT, bool Q8, int D, int NC, bool SHARE>
 __global__ __launch_bounds__(TR_WAVES * kWave, 2) void tree_kernel(TreeArgs a) {
   constexpr int T = TR_WAVES * kWave;
   constexpr int RB = Q8 ? D : 2 * D;                   // bytes of a token's head
-  constexpr int BT = tr_block(RB);                     // tokens of a block
+  constexpr int BT = tr_block(RB, SHARE);              // tokens of a block
+  constexpr int SLOTS = SHARE && RB == 256 ? 2 : 4;    // of K and of V in LDS
   constexpr int CPR = RB / 16, RPI = kWave / CPR;      // chunks per row, rows per load instruction
   constexpr int NL = BT / RPI, NB = BT / 16;           // loads per operand, groups of 16 tokens
   constexpr int NSMALL = Q8 ? 3 : 1;                   // loads of a block's ids and scales
   constexpr int NP = NL / TR_WAVES;                    // a wave's share of a block's loads
-  constexpr bool REL = Q8 && DT == DT_F16;
-  __shared__ __attribute__((aligned(16))) uint8_t s_k[TR_WAVES][BT * RB];
-  __shared__ __attribute__((aligned(16))) uint8_t s_v[TR_WAVES][BT * RB];
-  __shared__ __attribute__((aligned(16))) float s_ks[TR_WAVES][BT], s_vs[TR_WAVES][BT];
+  __shared__ __attribute__((aligned(16))) uint8_t s_k[SLOTS][BT * RB];
+  __shared__ __attribute__((aligned(16))) uint8_t s_v[SLOTS][BT * RB];
+  __shared__ __attribute__((aligned(16))) float s_ks[TR_WAVES][BT], s_ev[TR_WAVES][BT], s_iv[TR_WAVES][BT], s_fv[TR_WAVES][BT];
   __shared__ __attribute__((aligned(16))) uint32_t s_small[TR_WAVES][NSMALL][kWave];  // by wave or slot: ids, scale bytes
   __shared__ float s_m[TR_WAVES][16 * NC], s_l[TR_WAVES][16 * NC];
   static_assert(16 * D * 4 <= BT * RB, "a wave's O of 16 columns fits a slot");
@@ -302,7 +305,7 @@ __global__ __launch_bounds__(TR_WAVES * kWave, 2) void tree_kernel(TreeArgs a) {
 #pragma unroll
     for (int dt = 0; dt < D / 16; dt++) voff[dt] = r0 * RB + 16 * ((2 * dt + qc) ^ tv_swz<Q8, RB>(r0)) + qh;
   }
-  const size_t tok_bytes = (size_t)a.hkv * RB;
+  const uint32_t tok_bytes = (uint32_t)a.hkv * RB;
 
   // ---- this workgroup's units
   long long units = 0, x = 0, x1 = 1;
@@ -386,7 +389,7 @@ __global__ __launch_bounds__(TR_WAVES * kWave, 2) void tree_kernel(TreeArgs a) {
         const int row = RPI * (u0 + u) + lane / CPR;
         const uint32_t from = (uint32_t)__shfl((int)where, row);
         const int chunk = (lane % CPR) ^ (IS_K ? tk_swz<RB>(row) : tv_swz<Q8, RB>(row));
-        lds_load16(reinterpret_cast<const uint16_t*>(base + from * tok_bytes + 16 * chunk),
+        lds_load16(reinterpret_cast<const uint16_t*>(base + (uint64_t)from * tok_bytes + 16 * chunk),
                    reinterpret_cast<uint16_t*>(dst + 1024 * (u0 + u)));
       }
     };
@@ -402,31 +405,28 @@ __global__ __launch_bounds__(TR_WAVES * kWave, 2) void tree_kernel(TreeArgs a) {
       for (int dt = 0; dt < D / 16; dt++) acc[c][dt] = f32x4{0.f, 0.f, 0.f, 0.f};
     }
 
-    // e8m0 -> float (byte 0 is 2^-127)
-    auto scale_value = [](int byte) __attribute__((always_inline)) -> float {
-      return byte == 255 ? NAN : __uint_as_float(byte > 0 ? (uint32_t)byte << 23 : 0x400000u);
-    };
-    // f16: V's scales go onto the weights relative to the largest so far, so that these keep
-    // to f16's range (an accumulator stands for itself times 2^(top - 127)).
-    int top = -1000;
+    // Scales.  K's go into the conversion.  V's, 2^e, are added to the scores, as e in the exponent
+    // (the start of the sums that are the scores: no instruction a weight):
+    //   P = 2^(x + e - m),  O += P code,  L += P 2^-e,  m the running maximum of x + e
+    // so that P keeps to its type's range whatever the scales are.  A token whose scale is below 2^-60,
+    // or 2^-60 of the largest so far, takes that instead (its part in L would be lost otherwise),
+    // and its weight the rest on its way to O.
+    int top = 0;       // the largest scale byte so far
+    bool low = false;  // some token of the block has less than its scale in e
     auto put_scales = [&](int kb, int vb, uint64_t have) __attribute__((always_inline)) {
-      if constexpr (REL) {
-        const int mine = (have >> lane & 1) && vb != 255 ? vb : -1000;
-        if (__builtin_amdgcn_ballot_w64(mine > top)) {
-          int most = mine;
+      const bool ok = (have >> lane & 1) && vb != 255;
+      if (__builtin_amdgcn_ballot_w64(ok && vb > top)) {
+        int most = ok ? vb : 0;
 #pragma unroll
-          for (int o = 32; o > 0; o >>= 1) most = max(most, __shfl_xor(most, o, kWave));
-          most = __builtin_amdgcn_readfirstlane(most);
-          const float f = __uint_as_float((uint32_t)max(top - most + 127, 0) << 23);
-          top = most;
-#pragma unroll
-          for (int c = 0; c < NC; c++)
-#pragma unroll
-            for (int dt = 0; dt < D / 16; dt++) acc[c][dt] *= f;
-        }
+        for (int o = 32; o > 0; o >>= 1) most = max(most, __shfl_xor(most, o, kWave));
+        top = max(top, __builtin_amdgcn_readfirstlane(most));
       }
-      s_ks[wave][lane % BT] = scale_value(kb);
-      s_vs[wave][lane % BT] = !REL ? scale_value(vb) : vb == 255 ? NAN : __uint_as_float((uint32_t)min(max(vb - top + 127, 0), 127) << 23);
+      const int least = max(top - 60, 67), e = min(max(vb, least), 254);
+      low = __builtin_amdgcn_ballot_w64(ok && vb < least) != 0;
+      s_ks[wave][lane % BT] = __uint_as_float((uint32_t)kb << 23);  // (what the conversion takes: 0 is 2^-127, 255 NaN)
+      s_ev[wave][lane % BT] = vb == 255 ? NAN : (float)(e - 127) * a.scale_inv;
+      s_iv[wave][lane % BT] = __uint_as_float(e < 254 ? (uint32_t)(254 - e) << 23 : 0x400000u);
+      s_fv[wave][lane % BT] = __uint_as_float((uint32_t)max(vb - e + 127, 0) << 23);
     };
 
     // Some row may not see some token of the block (uniform, also over waves)
@@ -437,10 +437,14 @@ __global__ __launch_bounds__(TR_WAVES * kWave, 2) void tree_kernel(TreeArgs a) {
       f32x4 sc[NC][NB];
 #pragma unroll
       for (int n = 0; n < NB; n++) {
-#pragma unroll
-        for (int c = 0; c < NC; c++) sc[c][n] = f32x4{0.f, 0.f, 0.f, 0.f};
+        f32x4 start = {0.f, 0.f, 0.f, 0.f};
         float kscale = 1.f;
-        if constexpr (Q8) kscale = s_ks[wave][16 * n + col];
+        if constexpr (Q8) {
+          start = *reinterpret_cast<const f32x4*>(&s_ev[wave][16 * n + 4 * grp]);
+          kscale = s_ks[wave][16 * n + col];
+        }
+#pragma unroll
+        for (int c = 0; c < NC; c++) sc[c][n] = start;
 #pragma unroll
         for (int j = 0; j < RB / 64; j++) {
           const uint4 w = *reinterpret_cast<const uint4*>(&kt[koff[j] + 16 * n * RB]);
@@ -458,6 +462,9 @@ __global__ __launch_bounds__(TR_WAVES * kWave, 2) void tree_kernel(TreeArgs a) {
           }
         }
       }
+      // (the other wave of the SIMD is given way to in the softmax: its matrix instructions and these
+      // vector ones then overlap; a chunk of 2048 rows after 14 K tokens 672 -> 635 us)
+      __builtin_amdgcn_s_setprio(0);
       after_k();
       // mask: this lane's tokens are 16 n + 4 grp + i
       const int pos0 = blk * BT;
@@ -514,40 +521,34 @@ __global__ __launch_bounds__(TR_WAVES * kWave, 2) void tree_kernel(TreeArgs a) {
           for (int dt = 0; dt < D / 16; dt++) acc[c][dt] *= alpha;
         }
       }
-      f32x4 vscale[NB];
-      if constexpr (Q8) {
-#pragma unroll
-        for (int n = 0; n < NB; n++) vscale[n] = *reinterpret_cast<const f32x4*>(&s_vs[wave][16 * n + 4 * grp]);
-      }
       uint2 pb[NC][NB];
-#pragma unroll
-      for (int c = 0; c < NC; c++) {
-        float mref = m_i[c] == -INFINITY ? 0.f : m_i[c], scl = a.scale_log2;
-        if (far) {  // (uniform; a row goes by its own maximum, so its weights agree)
-#pragma unroll
-          for (int n = 0; n < NB; n++)
-#pragma unroll
-            for (int i = 0; i < 4; i++) sc[c][n][i] = far_exponent(sc[c][n][i], scl, mref);
-          mref = 0.f;
-          scl = 1.f;
-        }
-        mref -= kPBias<DT>;
+      auto weights = [&](auto plain_c) __attribute__((always_inline)) {
+        constexpr bool PLAIN = decltype(plain_c)::value;
 #pragma unroll
         for (int n = 0; n < NB; n++) {
-          f32x4 p;
+          f32x4 iv, fv;
+          if constexpr (Q8) iv = *reinterpret_cast<const f32x4*>(&s_iv[wave][16 * n + 4 * grp]);
+          if constexpr (Q8 && !PLAIN) fv = *reinterpret_cast<const f32x4*>(&s_fv[wave][16 * n + 4 * grp]);
 #pragma unroll
-          for (int i = 0; i < 4; i++) {
-            p[i] = __builtin_amdgcn_exp2f(fmaf(sc[c][n][i], scl, -mref));
-            l_i[c] += p[i];
-            if constexpr (Q8) p[i] *= vscale[n][i];
-          }
-          if (Q8 && masked) {  // an unseen token's scale may be NaN
+          for (int c = 0; c < NC; c++) {
+            const float m = m_i[c] == -INFINITY ? 0.f : m_i[c];
+            f32x4 p;
 #pragma unroll
-            for (int i = 0; i < 4; i++) p[i] = seen[c] >> (4 * n + i) & 1 ? p[i] : 0.f;
+            for (int i = 0; i < 4; i++) {
+              // (a row goes by its own maximum, so its weights agree)
+              float x = PLAIN ? fmaf(sc[c][n][i], a.scale_log2, kPBias<DT> - m) : far_exponent(sc[c][n][i], a.scale_log2, m) + kPBias<DT>;
+              p[i] = __builtin_amdgcn_exp2f(x);
+              if constexpr (Q8) l_i[c] = fmaf(p[i], iv[i], l_i[c]);
+              else l_i[c] += p[i];
+              if constexpr (Q8 && !PLAIN) p[i] *= fv[i];
+            }
+            pb[c][n] = make_uint2(pack2<DT>(p[0], p[1]), pack2<DT>(p[2], p[3]));
           }
-          pb[c][n] = make_uint2(pack2<DT>(p[0], p[1]), pack2<DT>(p[2], p[3]));
         }
-      }
+      };
+      if (far || low) weights(std::false_type{});  // (uniform)
+      else weights(std::true_type{});
+      __builtin_amdgcn_s_setprio(1);
       before_v();
       // Infinity or NaN in a token's V would reach the rows that do not see it as 0 * inf: such
       // tokens are left out of the product and added to those that do, one by one.
@@ -684,60 +685,61 @@ __global__ __launch_bounds__(TR_WAVES * kWave, 2) void tree_kernel(TreeArgs a) {
         consume(blk, std::true_type{});
       }
     } else {
+      constexpr int AHEAD = SLOTS - 1;
       constexpr int GROUP = 2 * NP + 1;  // a wave's loads of a block
       const int n = blk1 - blk0;
       const bool idle = nt * G <= col0;  // (no columns)
       constexpr auto share = std::integral_constant<int, NP>{};
-      // block t, in slot t % 4: this wave's part of K and V, its scales (one wave K's, one V's), and
-      // the ids of block t + 3 (the others, each the same)
+      // block t, in slot t % SLOTS: this wave's part of K and V, its scales (one wave K's, one V's), and
+      // the ids of block t + AHEAD (the others, each the same)
       auto issue_block = [&](int t, uint32_t where) __attribute__((always_inline)) {
-        const int slot = t % TR_WAVES;
+        const int slot = t % SLOTS;
         issue(where, a.kc, s_k[slot], std::true_type{}, share, wave * NP);
         issue(where, a.vc, s_v[slot], std::false_type{}, share, wave * NP);
         const size_t head = (size_t)where * a.hkv + hk;
         if (Q8 && wave < 2) lds_load1((wave == 0 ? a.ks : a.vs) + head, s_small[slot][NSMALL > 1 ? 1 + wave : 0]);
-        else lds_load4(id_at(blk0 + t + 3), s_small[(t + 3) % TR_WAVES][0]);
+        else lds_load4(id_at(blk0 + t + AHEAD), s_small[(t + AHEAD) % SLOTS][0]);
         asm volatile("" ::: "memory");
       };
-      uint64_t have[3] = {0, 0, 0};  // of this block and the next two
+      uint64_t have[AHEAD] = {};  // of this block and those on their way
       if (n > 0) {
-        int id[3];
+        int id[AHEAD];
 #pragma unroll
-        for (int t = 0; t < 3; t++) id[t] = *gptr(id_at(blk0 + t));
+        for (int t = 0; t < AHEAD; t++) id[t] = *gptr(id_at(blk0 + t));
 #pragma unroll
-        for (int t = 0; t < 3; t++) {
+        for (int t = 0; t < AHEAD; t++) {
           const Block p = place(blk0 + t, id[t]);
           have[t] = p.have;
           if (t < n) issue_block(t, p.place);
         }
       }
       for (int t = 0; t < n; t++) {
-        // this wave's part of the block has landed; those of up to two more may be on their way
-        if (t + 2 < n) asm volatile("s_waitcnt vmcnt(%0) lgkmcnt(0)" ::"n"(2 * GROUP) : "memory");
-        else if (t + 1 < n) asm volatile("s_waitcnt vmcnt(%0) lgkmcnt(0)" ::"n"(GROUP) : "memory");
+        // this wave's part of the block has landed; those behind it may be on their way
+        if (AHEAD > 2 && t + 2 < n) asm volatile("s_waitcnt vmcnt(%0) lgkmcnt(0)" ::"n"(2 * GROUP) : "memory");
+        else if (AHEAD > 1 && t + 1 < n) asm volatile("s_waitcnt vmcnt(%0) lgkmcnt(0)" ::"n"(GROUP) : "memory");
         else asm volatile("s_waitcnt vmcnt(0) lgkmcnt(0)" ::: "memory");
         __builtin_amdgcn_s_barrier();  // every wave's part has, and the block before is read out
         asm volatile("" ::: "memory");
-        const int slot = t % TR_WAVES;
+        const int slot = t % SLOTS;
         int kb = 0, vb = 0;
         if constexpr (Q8) {
           kb = (int)s_small[slot][1][lane];
           vb = (int)s_small[slot][2][lane];
         }
-        uint64_t have3 = 0;
-        if (t + 3 < n) {
-          const Block p = place(blk0 + t + 3, (int)s_small[(t + 3) % TR_WAVES][0][lane]);
-          have3 = p.have;
+        uint64_t have_new = 0;
+        if (t + AHEAD < n) {
+          const Block p = place(blk0 + t + AHEAD, (int)s_small[(t + AHEAD) % SLOTS][0][lane]);
+          have_new = p.have;
           asm volatile("s_waitcnt lgkmcnt(0)" ::: "memory");
-          issue_block(t + 3, p.place);
+          issue_block(t + AHEAD, p.place);
         }
         if (!idle || is_masked(blk0 + t, have[0])) {  // (a masked block may need barriers)
           if constexpr (Q8) put_scales(kb, vb, have[0]);
           compute(blk0 + t, have[0], s_k[slot], s_v[slot], [] {}, [] {});
         }
-        have[0] = have[1];
-        have[1] = have[2];
-        have[2] = have3;
+#pragma unroll
+        for (int u = 0; u + 1 < AHEAD; u++) have[u] = have[u + 1];
+        have[AHEAD - 1] = have_new;
       }
     }
 
@@ -745,11 +747,6 @@ __global__ __launch_bounds__(TR_WAVES * kWave, 2) void tree_kernel(TreeArgs a) {
 #pragma unroll
     for (int c = 0; c < NC; c++) {
       l_i[c] = add_xor32(add_xor16(l_i[c]));
-      if constexpr (REL) {
-        const float f = scale_value(max(top, 0));
-#pragma unroll
-        for (int dt = 0; dt < D / 16; dt++) acc[c][dt] *= f;
-      }
     }
     const int rows = nt * G;
     // a part has two records: of a tile that began before it, and of one that goes on behind it
@@ -904,7 +901,7 @@ static TreePlan tree_plan(bool ragged, int rows, int batch, int hkv, int G, int 
   p.tt = ragged ? 16 * p.nc * (p.share ? TR_WAVES : 1) / G : 1;
   p.tiles = ragged ? (long long)rows / p.tt + batch : rows;
   if (p.tiles > rows) p.tiles = rows;
-  const int bt = tr_block(e4m3 ? d : 2 * d);
+  const int bt = tr_block(e4m3 ? d : 2 * d, p.share);
   p.log_heads = p.share ? 0 : hkv % 4 == 0 ? 2 : hkv % 2 == 0 ? 1 : 0;
   long long most = TR_TARGET_WG / hkv;
   if (most < 1) most = 1;
@@ -964,6 +961,7 @@ extern "C" int yr_hip_gqa_tree_paged(const void* q, const void* k_cache, const v
   if (tree_mask && (mask_cols < 1 || mask_row < 0)) return fail(YR_E_INVALID, "%s: tree_mask has at least one column", nm);
   if (((uintptr_t)q | (uintptr_t)k_cache | (uintptr_t)v_cache | (uintptr_t)out) & 15)
     return fail(YR_E_INVALID, "%s: pointers must be 16-byte aligned", nm);
+  if (hkv > 1 << 20) return fail(YR_E_INVALID, "%s: too many heads", nm);
   if ((long long)num_pages * page_size > 0xffffffffll) return fail(YR_E_INVALID, "%s: a cache of more than 2^32 tokens", nm);
   const TreePlan p = tree_plan(qo_indptr != nullptr, rows, batch, hkv, G, d, max_kv_len, e4m3);
   const long long grid = p.parts ? (long long)p.parts * hkv : p.tiles * (hkv >> p.log_heads);
@@ -994,6 +992,7 @@ extern "C" int yr_hip_gqa_tree_paged(const void* q, const void* k_cache, const v
   a.page_mul = (uint32_t)(((1ull << (31 + sh)) + page_size - 1) / page_size);
   a.page_shift = 31 + sh;
   a.scale_log2 = kLog2e / sqrtf((float)d);
+  a.scale_inv = 1.f / a.scale_log2;
   hipStream_t st = (hipStream_t)stream;
 #define YR_TR(DT_, Q_, D_, N_, S_)                                                  \
   if (dtype == DT_ && e4m3 == Q_ && d == D_ && p.nc == N_ && p.share == S_)         \
