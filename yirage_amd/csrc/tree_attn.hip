@@ -26,6 +26,7 @@ constexpr int TR_WAVES = 4;
 constexpr int TR_TARGET_WG = 512;  // two per CU
 constexpr int TR_MIN_BLOCKS = 4;   // of a part
 constexpr int TR_TILE_COST = 192;  // of a tile's start, in tokens
+constexpr int TR_SHORT = 512;      // tiles of that many tokens on average are not split
 constexpr int TR_WAVE_BLOCKS = 8;  // of a wave, for several heads to share a workgroup
 // Tokens of a block: a lane's each, half as many where a wave has a block of its own and a
 // token 256 bytes (shared ones of 32: a chunk of 2048 rows in 16 bits 744 us for 629).
@@ -94,10 +95,15 @@ __device__ __forceinline__ long long scan64(long long x) {
   x = dpp_add64<0x142, 0xa>(x);  // lane 15 of rows 0 and 2 to the rows behind them
   return dpp_add64<0x143, 0xc>(x);  // lane 31 to the upper half
 }
-// Units of a kv head.  Each wave for itself, a sequence a lane; w: the first 64 sequences.
-__device__ __forceinline__ long long all_units(const TreeArgs& a, const SeqWork& w) {
-  long long sum = w.units;
-  for (int b = kWave; b < a.r.batch; b += kWave) sum += seq_work(a, b + (int)threadIdx.x % kWave).units;
+// Units and tiles of a kv head.  Each wave for itself, a sequence a lane; w: the first 64 sequences.
+__device__ __forceinline__ long long all_units(const TreeArgs& a, const SeqWork& w, long long* tiles) {
+  long long sum = w.units, count = w.tiles;
+  for (int b = kWave; b < a.r.batch; b += kWave) {
+    const SeqWork more = seq_work(a, b + (int)threadIdx.x % kWave);
+    sum += more.units;
+    count += more.tiles;
+  }
+  *tiles = lane64(scan64(count), kWave - 1);
   return lane64(scan64(sum), kWave - 1);
 }
 // A tile: its sequence (batch: none), number in it, first unit and units.
@@ -314,14 +320,20 @@ __global__ __launch_bounds__(TR_WAVES * kWave, 2) void tree_kernel(TreeArgs a) {
   // Up to 4 kv heads share a workgroup, a wave (or two) each, where a wave has enough to do:
   // they read neighbouring bytes at about the same time (loads alone, 128 bytes a head: 5.2 TB/s
   // with a workgroup a head, 6.0 with 4 heads in one).
-  if (a.parts) units = all_units(a, work0);
-  const bool shared = !SHARE && !(a.parts && units < (long long)TR_WAVE_BLOCKS * BT * TR_WAVES * a.parts);
+  bool split = a.parts > 0;  // else a tile a workgroup
+  if (split) {
+    long long tiles;
+    units = all_units(a, work0, &tiles);
+    split = tiles > a.parts || units > tiles * (TR_SHORT + TR_TILE_COST);
+    if (!split && blockIdx.x == 0 && tid == 0) a.split[0].x = 0;
+  }
+  const bool shared = !SHARE && !(a.parts && (!split || units < (long long)TR_WAVE_BLOCKS * BT * TR_WAVES * a.parts));
   const int log_heads = shared ? a.log_heads : 0, heads = 1 << log_heads, groups = a.hkv >> log_heads;
   const int w0 = __builtin_amdgcn_readfirstlane(blockIdx.x / groups), hk0 = (blockIdx.x - w0 * groups) << log_heads;
   const int streams = TR_WAVES >> log_heads, stream = SHARE ? 0 : wave & (streams - 1);  // waves of a head
   const int hk = SHARE ? hk0 : hk0 + (wave << log_heads) / TR_WAVES;                      // this wave's
   const int most = a.parts << a.log_heads;
-  if (a.parts) {
+  if (split) {
     parts = (int)min((long long)a.parts << log_heads, max(units / (TR_MIN_BLOCKS * BT), 1ll));
     if (blockIdx.x == 0 && tid == 0) a.split[0].x = units ? parts : 0;
     if (w0 >= parts) return;
@@ -329,11 +341,11 @@ __global__ __launch_bounds__(TR_WAVES * kWave, 2) void tree_kernel(TreeArgs a) {
     x1 = part_start(units, parts, w0 + 1);
   }
   while (true) {
-    const TileAt at = a.parts ? find_unit(a, work0, x) : find_index(a, work0, w0);
+    const TileAt at = split ? find_unit(a, work0, x) : find_index(a, work0, w0);
     if (at.b >= a.r.batch) return;  // (only without parts)
     const SeqRows s = at.s;
     const int i0 = at.tile * a.tt;
-    const long long u0 = a.parts ? x - at.from : 0, u1 = a.parts ? min(x1 - at.from, at.units) : 1;
+    const long long u0 = split ? x - at.from : 0, u1 = split ? min(x1 - at.from, at.units) : 1;
     x += u1 - u0;
     const bool whole = u1 - u0 == at.units;
     const int nt = min(a.tt, s.n - i0), t0 = s.row0 + i0, first = s.len - s.n, p0 = first + i0;  // rows, first row, its place
@@ -753,7 +765,7 @@ __global__ __launch_bounds__(TR_WAVES * kWave, 2) void tree_kernel(TreeArgs a) {
     auto record = [&](int head) __attribute__((always_inline)) -> float* {
       return a.partial + (((size_t)head * most + w0) * 2 + (u0 == 0)) * cols * (D + 4);
     };
-    if (a.parts && x >= x1 && tid == 0) {  // its last tile: the parts that this one begins, if it does
+    if (split && x >= x1 && tid == 0) {  // its last tile: the parts that this one begins, if it does
       const int n = !whole && u0 == 0 ? part_of(units, parts, x - u1 + at.units - 1) - w0 + 1 : 0;
       for (int h = hk0; h < hk0 + heads; h++) a.split[1 + (size_t)h * most + w0] = make_int4(t0, rows, n, 0);
     }
@@ -906,11 +918,12 @@ static TreePlan tree_plan(bool ragged, int rows, int batch, int hkv, int G, int 
   long long most = TR_TARGET_WG / hkv;
   if (most < 1) most = 1;
   p.parts = (int)most;
-  if (p.tiles >= 4 * most) {
+  if (p.tiles >= 4 * most || (max_kv_len > 0 && max_kv_len <= TR_SHORT)) {
     p.parts = 0;
+    if (p.tiles * (hkv >> p.log_heads) < TR_TARGET_WG) p.log_heads = 0;
   } else if (max_kv_len > 0) {
-    const long long blocks = p.tiles * (((long long)max_kv_len + bt - 1) / bt), need = blocks / TR_MIN_BLOCKS + 1;
-    if (need < most) p.parts = (int)need;
+    const long long blocks = p.tiles * (((long long)max_kv_len + TR_TILE_COST + bt - 1) / bt), need = blocks / TR_MIN_BLOCKS + 1;
+    if (need < most) p.parts = (int)(need < p.tiles ? p.tiles : need);
   }
   return p;
 }
