@@ -344,10 +344,11 @@ def append_kv_paged(k, v, k_cache, v_cache, kv_indptr, kv_indices, kv_len, q=Non
         _fail("the last dim of k and v must be contiguous")
     if q is not None:
         out = q.new_empty((T, hq, D)) if out is None else _output(out, (T, hq, D), q)
+    if positions is not None:
+        _positions(positions, T, cos)
     index = _one_device(k, v, k_cache, v_cache, kv_indptr, kv_indices, kv_len, q, cos, sin, q_norm, k_norm, qo_indptr,
                         page_bounds, out)
     if positions is not None:
-        _positions(positions, T, cos)
         _one_device(k, positions)
         if T:
             _launch(index, lib().yr_hip_append_kv_paged_at, "append_kv_paged", _at(q), k.data_ptr(), v.data_ptr(),
