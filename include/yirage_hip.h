@@ -218,11 +218,11 @@ int yr_hip_read_kv_paged_fp8(const void* k_cache, const void* v_cache, const voi
  * hq / hkv <= 16.  A row without a token, or whose scores are all -inf, is 0.
  * max_kv_len, about the largest kv_len, decides how finely the work is split; it does not
  * limit what is seen.  Softmax statistics are fp32; the weights are rounded to dtype before they
- * meet v (to bf16 with a cache in 8 bits). */
+ * meet v.  Two launches where tokens are split over workgroups, one otherwise. */
 size_t yr_hip_gqa_tree_workspace(int rows, int batch, int ragged, int hq, int hkv, int d, int max_kv_len,
                                  int cache_dtype); /* ragged: a call with qo_indptr */
-/* The kernel a call runs on (host only): plan3 = {groups of 16 columns (rows times heads of a kv
- * head) of a wave, rows of a sequence per tile, splits of a tile's tokens}. */
+/* The kernel a call runs on (host only): plan3 = {columns (rows times heads of a kv head) of a tile,
+ * rows of a sequence per tile, workgroups that share a kv head's tokens (0: a tile a workgroup)}. */
 int yr_hip_gqa_tree_plan(int rows, int batch, int ragged, int hq, int hkv, int d, int max_kv_len, int cache_dtype,
                          int* plan3);
 int yr_hip_gqa_tree_paged(const void* q, const void* k_cache, const void* v_cache, const void* k_scale,

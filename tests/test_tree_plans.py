@@ -15,13 +15,13 @@ def plan(rows, batch, hq, hkv, d, most, cache, ragged=True):
 
 
 @pytest.mark.parametrize("args,want", [
-    ((1, 1, 32, 8, 128, 32768, _lib.DTYPE_E4M3, False), (16, 1, 64)), ((32, 32, 32, 8, 128, 8192, _lib.DTYPE_BF16, False), (16, 1, 64)),
-    ((8, 1, 32, 8, 128, 32768, _lib.DTYPE_E4M3), (32, 8, 64)), ((16, 1, 32, 8, 128, 32768, _lib.DTYPE_E4M3), (64, 16, 64)),
+    ((1, 1, 32, 8, 128, 32768, _lib.DTYPE_E4M3, False), (16, 1, 32)), ((32, 32, 32, 8, 128, 8192, _lib.DTYPE_BF16, False), (16, 1, 32)),
+    ((8, 1, 32, 8, 128, 32768, _lib.DTYPE_E4M3), (32, 8, 32)), ((16, 1, 32, 8, 128, 32768, _lib.DTYPE_E4M3), (64, 16, 64)),
     ((64, 1, 32, 8, 128, 32768, _lib.DTYPE_F16), (128, 32, 64)), ((2048, 1, 32, 8, 128, 16384, _lib.DTYPE_F16), (128, 32, 64)),
     ((2048, 1, 35, 7, 64, 16384, _lib.DTYPE_F16), (128, 25, 73)),  # 5 heads a group: 125 columns
     ((1, 1, 32, 8, 128, 512, _lib.DTYPE_E4M3, False), (16, 1, 0)),  # short: not split
     ((300, 300, 16, 8, 64, 4096, _lib.DTYPE_E4M3, False), (16, 1, 0)),  # enough of them
-    ((1, 1, 32, 8, 128, 0, _lib.DTYPE_E4M3, False), (16, 1, 64)),  # no length given
+    ((1, 1, 32, 8, 128, 0, _lib.DTYPE_E4M3, False), (16, 1, 32)),  # no length given
 ])
 def test_plans(args, want):
     assert plan(*args) == want

@@ -6,15 +6,22 @@
 // over the tokens before the sequence's new ones, and of the new ones those at or before
 // row t's place, or those that tree_mask[t] names.
 //
-// A tile is up to 16 NC / G consecutive rows of one sequence with their G heads (the
-// columns of the products, which are transposed: S^T = K Q^T and O^T += V^T P^T on MFMA
-// 16x16x32; a lane holds one query row of each 16).  The tile's tokens are split over
-// workgroups and their waves; each wave streams its blocks through LDS slots of its own,
-// with an online softmax, and waves and splits merge at the end.
+// A tile is consecutive rows of one sequence with their G heads: 16, 32, 64 or 128 columns of
+// the products, which are transposed (S^T = K Q^T and O^T += V^T P^T on MFMA 16x16x32; a
+// lane holds one query row of each 16).  Up to 32 columns every wave holds all of them and the
+// waves split the tokens; wider tiles share each block of tokens, 16 or 32 columns a wave (16
+// sequences' trees of 16 nodes and 4 heads, 64 columns: 69 us, as private tiles of 32 columns 93).  One pass with a running maximum;
+// statistics and O are fp32.  The weights are rounded to q's type before they meet V (half a step
+// of a weight each; their sum takes them unrounded).
 //
 // In 8 bits a fragment is converted between LDS and MFMA.  The conversion multiplies by
 // a power of two, so a key is read with its scale for nothing and, in bf16, without
-// rounding; a fragment of V holds 8 tokens, whose scales go into the weights' exponents instead.
+// rounding (f16 rounds keys below 2^-14); a fragment of V holds 8 tokens, whose scales go into the
+// weights' exponents instead.
+//
+// Bound: single rows by memory (32 sequences of 4 to 8 K tokens in 8 bits, 436 MB, 88 us, 5.0 TB/s), one long row by the chain of ids, first block, merge and join;
+// chunks by issue: MFMA takes half of a SIMD's cycles and the exponentials, conversions and LDS reads the
+// rest (2048 rows after 14 K tokens, 503 GFLOP, 620 us, 0.81 PFLOP/s).
 #include <type_traits>
 
 #include "attn_device.h"
@@ -22,12 +29,19 @@
 
 namespace yr {
 
+// The figures of these choices are replayed calls of 32 / 8 heads of 128, a graph's launch included.
 constexpr int TR_WAVES = 4;
-constexpr int TR_TARGET_WG = 512;  // two per CU
-constexpr int TR_MIN_BLOCKS = 4;   // of a part
-constexpr int TR_TILE_COST = 192;  // of a tile's start, in tokens
-constexpr int TR_SHORT = 512;      // tiles of that many tokens on average are not split
-constexpr int TR_WAVE_BLOCKS = 8;  // of a wave, for several heads to share a workgroup
+// Workgroups: one a CU where each has loads enough of its own on their way (one row over 32 K tokens
+// 32.6 us, with 512 of them 35.7, 320: 39.2; 32 rows of d = 64 65, 70 and 85), two where waves wait for
+// a shared block (64-node trees 144 us, with 256 194, 1024: 160; a chunk of 2048 641, 1083, 659).
+constexpr int TR_PRIVATE_WG = 256, TR_SHARED_WG = 512;
+// From that many tiles (of all kv heads) on each has a workgroup: 500 sequences of 1000 tokens 170 us,
+// in equal parts 195; fewer are cut (300 of 1500 tokens 162 us, a workgroup each 175, 160 of 2000: 122 and 128).
+constexpr int TR_MANY = 2048;
+constexpr int TR_MIN_BLOCKS = 4;   // of a part: one row over 8 K tokens 24.6 us, with 2 26.9, with 8 25.5
+constexpr int TR_TILE_COST = 192;  // of a tile's start, in tokens: a prompt of 2048 103 us, without 153
+constexpr int TR_SHORT = 512;      // tiles of so many tokens on average are not split: 7 trees over 57 tokens 18 us for 35
+constexpr int TR_WAVE_BLOCKS = 8;  // of a wave, for several heads to share a workgroup: 32 rows of d = 64 70 us, never 94; with 2 one row 37.3 for 35.7
 // Tokens of a block: a lane's each, half as many where a wave has a block of its own and a
 // token 256 bytes (shared ones of 32: a chunk of 2048 rows in 16 bits 744 us for 629).
 constexpr int tr_block(int row_bytes, bool share) { return row_bytes == 256 && !share ? 32 : 64; }
@@ -42,7 +56,8 @@ struct TreeArgs {
   const uint8_t* mask;  // [rows][mask_cols], rows mask_row apart, or null
   uint16_t* out;
   float* partial;       // [hkv][parts heads][2][tt G][D + 4]: O, m, l
-  int4* split;          // the parts of this call, then [hkv][parts heads]: the tile that begins in a part and ends in another: first row, columns, its parts (0: none)
+  int4* split;          // .x the parts of this call; then [hkv][parts heads]: first row, columns and parts (0: none)
+                        // of the tile that begins in a part and ends in another
   long long mask_row;
   int mask_cols, hq, hkv, tt;  // rows per tile
   int parts, log_heads;        // workgroups per kv head (0: one a tile); kv heads that may share one
@@ -51,10 +66,11 @@ struct TreeArgs {
 };
 
 // Work.  A sequence of n new rows has ceil(n / tt) tiles, and a tile counts for as many units
-// as tokens its last row may see, and TR_TILE_COST for its start.  The units of a kv head, one sequence after another, are
-// cut into `parts` equal ranges, a workgroup each: lengths that differ leave no workgroup
-// waiting, a long sequence is split and several short ones share a workgroup.  (32 sequences
-// of 4 to 8 K tokens, two workgroups of each: TIME.)
+// as tokens its last row may see, and TR_TILE_COST for its start.  The units of a kv head, one
+// sequence after another, are cut into `parts` equal ranges, a workgroup each: lengths that differ
+// leave no workgroup waiting, a long sequence is split and several short ones share a workgroup.
+// (Each tile split as often as the longest needs: 64-node trees over 16 bits 169 us for 145, one
+// row over 32 K tokens 29 for 25.)  The cut is made on the device, from lengths that no host reads.
 struct SeqWork {
   SeqRows s;
   int tiles;
@@ -830,8 +846,8 @@ __global__ __launch_bounds__(TR_WAVES * kWave, 2) void tree_kernel(TreeArgs a) {
 }
 
 // Split tiles: the parts of one, 256 of its results' quads a workgroup.  Where there are fewer
-// quads, SG threads share one (every SG-th part each) and meet in LDS.  (A workgroup that
-// arrives last in the kernel above would take 38 us for 32 rows and 32 parts.)
+// quads, SG threads share one (every SG-th part each) and meet in LDS.  (Joined by the last
+// workgroup of a tile to arrive in the kernel above: 38 us for 32 rows and 32 parts; here 5 to 14.)
 constexpr int TC_THREADS = 256, TC_AHEAD = 16;
 template <int DT, int D>
 __global__ __launch_bounds__(TC_THREADS) void tree_join_kernel(TreeArgs a) {
@@ -915,12 +931,13 @@ static TreePlan tree_plan(bool ragged, int rows, int batch, int hkv, int G, int 
   if (p.tiles > rows) p.tiles = rows;
   const int bt = tr_block(e4m3 ? d : 2 * d, p.share);
   p.log_heads = p.share ? 0 : hkv % 4 == 0 ? 2 : hkv % 2 == 0 ? 1 : 0;
-  long long most = TR_TARGET_WG / hkv;
+  const int target = p.share ? TR_SHARED_WG : TR_PRIVATE_WG;
+  long long most = target / hkv;
   if (most < 1) most = 1;
   p.parts = (int)most;
-  if (p.tiles >= 4 * most || (max_kv_len > 0 && max_kv_len <= TR_SHORT)) {
+  if (p.tiles * hkv >= TR_MANY || (max_kv_len > 0 && max_kv_len <= TR_SHORT)) {
     p.parts = 0;
-    if (p.tiles * (hkv >> p.log_heads) < TR_TARGET_WG) p.log_heads = 0;
+    if (p.tiles * (hkv >> p.log_heads) < TR_SHARED_WG) p.log_heads = 0;
   } else if (max_kv_len > 0) {
     const long long blocks = p.tiles * (((long long)max_kv_len + TR_TILE_COST + bt - 1) / bt), need = blocks / TR_MIN_BLOCKS + 1;
     if (need < most) p.parts = (int)(need < p.tiles ? p.tiles : need);
