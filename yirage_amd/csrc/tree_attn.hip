@@ -39,7 +39,9 @@ constexpr int TR_PRIVATE_WG = 256, TR_SHARED_WG = 512;
 // in equal parts 195; fewer are cut (300 of 1500 tokens 162 us, a workgroup each 175, 160 of 2000: 122 and 128).
 constexpr int TR_MANY = 2048;
 constexpr int TR_MIN_BLOCKS = 4;   // of a part: one row over 8 K tokens 24.6 us, with 2 26.9, with 8 25.5
-constexpr int TR_TILE_COST = 192;  // of a tile's start, in tokens: a prompt of 2048 103 us, without 153
+// Of a tile's start, in tokens, at its front (spread over its tokens: 64-node trees 144 us for 132, a prompt of
+// 2048 104 for 95, without 153): 16 trees of 15 nodes 56 us, with 128 59, with 320 62.
+constexpr int TR_TILE_COST = 192;
 constexpr int TR_SHORT = 512;      // tiles of so many tokens on average are not split: 7 trees over 57 tokens 18 us for 35
 constexpr int TR_WAVE_BLOCKS = 8;  // of a wave, for several heads to share a workgroup: 32 rows of d = 64 70 us, never 94; with 2 one row 37.3 for 35.7
 // Tokens of a block: a lane's each, half as many where a wave has a block of its own and a
@@ -191,14 +193,17 @@ __device__ __forceinline__ TileAt find_index(const TreeArgs& a, SeqWork w, int i
   return t;
 }
 
-// The units are cut into `parts` ranges that differ by one at most: where range w begins, and
-// the one that holds unit u.
+// The units behind the first tile's start (every part has one such start) are cut into `parts` ranges
+// that differ by one at most: where range w begins, and the one that holds unit u.  (In fp64 instead
+// of 64-bit divisions the kernel needs more registers: 64-node trees 155 us for 131.)
 __device__ __forceinline__ long long part_start(long long units, int parts, int w) {
-  return units / parts * w + min((long long)w, units % parts);
+  const long long cut = max(units - TR_TILE_COST, 0ll);
+  return w == 0 ? 0 : TR_TILE_COST + cut / parts * w + min((long long)w, cut % parts);
 }
 __device__ __forceinline__ int part_of(long long units, int parts, long long u) {
-  const long long per = units / parts, more = units % parts, cut = (per + 1) * more;
-  return __builtin_amdgcn_readfirstlane((int)(u < cut ? u / (per + 1) : more + (u - cut) / per));
+  const long long cut = max(units - TR_TILE_COST, 0ll), per = cut / parts, more = cut % parts, longer = (per + 1) * more;
+  const long long at = max(u - TR_TILE_COST, 0ll);
+  return __builtin_amdgcn_readfirstlane((int)(at < longer ? at / (per + 1) : more + (at - longer) / max(per, 1ll)));
 }
 // 8 consecutive e4m3 codes of LDS rows, transposed across each 16-lane group: lanes 2 e
 // and 2 e + 1 address the halves of row e's 16 bytes, lane i receives byte i of rows 0 .. 7.
@@ -369,7 +374,12 @@ __global__ __launch_bounds__(TR_WAVES * kWave, 2) void tree_kernel(TreeArgs a) {
     const int end = (int)min((long long)(a.mask ? s.len : min(s.len, p0 + nt)), (long long)s.npg * a.r.page);
     const int plain = a.mask ? first : p0 + 1;
     const int nblk = end > 0 ? (end + BT - 1) / BT : 0;
-    const int blk0 = (int)first64(u0 * nblk / at.units), blk1 = (int)first64(u1 * nblk / at.units);
+    // (a tile's first TR_TILE_COST units stand for its start and hold no blocks)
+    const long long tokens = split ? max(at.units - TR_TILE_COST, 1ll) : 1;
+    auto block_at = [&](long long u) __attribute__((always_inline)) -> int {
+      return (int)first64((split ? max(u - TR_TILE_COST, 0ll) : u) * nblk / tokens);
+    };
+    const int blk0 = block_at(u0), blk1 = block_at(u1);
 
     // ---- this lane's query rows: its column of group c is row qi of the tile, head (column % G)
     const int col0 = SHARE ? wave * 16 * NC : 0;
