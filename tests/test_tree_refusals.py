@@ -94,6 +94,18 @@ def test_tree_workspace():
     assert _lib.lib().yr_hip_gqa_tree_workspace(1024, 1024, 0, 32, 8, 128, 4096, _lib.DTYPE_F16) == 0
 
 
+def test_new_lengths_beside_the_old():
+    """Overlapping lengths are refused, neighbouring ones are not."""
+    both, t = torch.zeros(8, dtype=torch.int32), _step()
+    args = lambda lens: (t["kc"], t["vc"], t["ptr"], t["idx"], lens, t["path"])
+    for at, text in ((1, "another"), (2, "GPU"), (0, "another")):
+        with pytest.raises(YirageHipError, match=text):
+            F.keep_kv_paged(*args(both[:2]), k_scale=t["ks"], v_scale=t["vs"], out=both[at: at + 2])
+    for at in (4092, 4096, 4100):  # kv_len is 4096 there, of two sequences
+        rc, msg = _keep(out=ctypes.c_void_p(at))
+        assert rc == -1 and "place of their own" in msg, (at, msg)
+
+
 def _keep(**change):
     a = dict(kc=FAKE, vc=FAKE, ks=FAKE, vs=FAKE, bounds=None, path=FAKE, depth=4, qo=FAKE, ptr=FAKE, idx=FAKE, nidx=4, lens=FAKE,
              out=ctypes.c_void_p(8192), batch=2, hkv=8, d=128, page=64, pages=4, dt=_lib.DTYPE_E4M3, stream=None)
@@ -204,6 +216,8 @@ def test_nothing_to_do(monkeypatch):
     assert F.gqa_tree_paged(empty["q"], t["kc"], t["vc"], t["ptr"], t["idx"], t["lens"], qo_indptr=qo, k_scale=t["ks"], v_scale=t["vs"]).shape == (0, 8, 64)
     k, v = F.read_kv_paged_fp8(t["kc"], t["vc"], t["ks"], t["vs"], t["ptr"], t["idx"], t["lens"], qo, 0)
     assert k.shape == v.shape == (0, 2, 64)
+    assert F.keep_kv_paged(t["kc"], t["vc"], _i32(0), none, none, torch.zeros((0, 3), dtype=torch.int32), k_scale=t["ks"], v_scale=t["vs"],
+                           out=none.clone()).shape == (0,)
     kept = F.keep_kv_paged(t["kc"], t["vc"], _i32(0), none, none, torch.zeros((0, 3), dtype=torch.int32), k_scale=t["ks"], v_scale=t["vs"])
     assert kept.shape == (0,)
 

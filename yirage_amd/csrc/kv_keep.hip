@@ -156,7 +156,9 @@ extern "C" int yr_hip_keep_kv_paged(void* k_cache, void* v_cache, void* k_scale,
   if (depth < 1) return fail(YR_E_INVALID, "%s: a path has at least one entry", nm);
   if (((uintptr_t)k_cache | (uintptr_t)v_cache | (uintptr_t)page_bounds) & 15)
     return fail(YR_E_INVALID, "%s: pointers must be 16-byte aligned", nm);
-  if (len_out == kv_len) return fail(YR_E_INVALID, "%s: the new lengths need a place of their own", nm);
+  // (sequences are read and written in any order)
+  const intptr_t apart = (intptr_t)len_out - (intptr_t)kv_len, size = (intptr_t)batch * (intptr_t)sizeof(int32_t);
+  if (apart < size && -apart < size) return fail(YR_E_INVALID, "%s: the new lengths need a place of their own", nm);
   if (hkv > 1 << 20) return fail(YR_E_INVALID, "%s: too many heads", nm);
   a.kc = (uint8_t*)k_cache;
   a.vc = (uint8_t*)v_cache;

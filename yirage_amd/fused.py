@@ -589,7 +589,7 @@ def keep_kv_paged(k_cache, v_cache, kv_indptr, kv_indices, kv_len, path, qo_indp
     _page_table(batch, kv_indptr, kv_indices, kv_len, qo_indptr)
     if out is None:
         out = torch.empty_like(kv_len)
-    elif out.shape != kv_len.shape or out.dtype is not torch.int32 or not out.is_contiguous() or out.data_ptr() == kv_len.data_ptr():
+    elif out.shape != kv_len.shape or out.dtype is not torch.int32 or not out.is_contiguous() or abs(out.data_ptr() - kv_len.data_ptr()) < 4 * batch:
         _fail(f"out must be another contiguous int32 tensor {tuple(kv_len.shape)}")
     index = _one_device(k_cache, v_cache, kv_indptr, kv_indices, kv_len, path, qo_indptr, k_scale, v_scale, page_bounds, out)
     if batch == 0:
