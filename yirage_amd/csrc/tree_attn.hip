@@ -44,6 +44,9 @@ constexpr int TR_MIN_BLOCKS = 4;   // of a part: one row over 8 K tokens 24.6 us
 constexpr int TR_TILE_COST = 192;
 constexpr int TR_SHORT = 512;      // tiles of so many tokens on average are not split: 7 trees over 57 tokens 18 us for 35
 constexpr int TR_WAVE_BLOCKS = 8;  // of a wave, for several heads to share a workgroup: 32 rows of d = 64 70 us, never 94; with 2 one row 37.3 for 35.7
+// Fragments that are read from LDS ahead of their products (left to the compiler each was waited for:
+// a chunk of 2048 rows over 16 bits 620 us for 568, 64-node trees 132 for 123; 1 ahead 577 and 124, 4: 563 and 126).
+constexpr int TR_FRAGMENTS = 2;
 // Tokens of a block: a lane's each, half as many where a wave has a block of its own and a
 // token 256 bytes (shared ones of 32: a chunk of 2048 rows in 16 bits 744 us for 629).
 constexpr int tr_block(int row_bytes, bool share) { return row_bytes == 256 && !share ? 32 : 64; }
@@ -473,31 +476,40 @@ __global__ __launch_bounds__(TR_WAVES * kWave, 2) void tree_kernel(TreeArgs a) {
     // is needed.
     auto compute = [&](int blk, uint64_t have, const uint8_t* kt, uint8_t* vt, auto after_k, auto before_v) __attribute__((always_inline)) {
       f32x4 sc[NC][NB];
+      float kscale[NB];
 #pragma unroll
       for (int n = 0; n < NB; n++) {
         f32x4 start = {0.f, 0.f, 0.f, 0.f};
-        float kscale = 1.f;
         if constexpr (Q8) {
           start = *reinterpret_cast<const f32x4*>(&s_ev[wave][16 * n + 4 * grp]);
-          kscale = s_ks[wave][16 * n + col];
+          kscale[n] = s_ks[wave][16 * n + col];
         }
 #pragma unroll
         for (int c = 0; c < NC; c++) sc[c][n] = start;
+      }
+      uint4 kw[TR_FRAGMENTS + 1];
+      auto k_read = [&](int s) __attribute__((always_inline)) {
+        kw[s % (TR_FRAGMENTS + 1)] = *reinterpret_cast<const uint4*>(&kt[koff[s / NB] + 16 * (s % NB) * RB]);
+      };
 #pragma unroll
-        for (int j = 0; j < RB / 64; j++) {
-          const uint4 w = *reinterpret_cast<const uint4*>(&kt[koff[j] + 16 * n * RB]);
-          if constexpr (Q8) {
-            const uint2 f0 = e4m3x4<DT>(w.x, kscale), f1 = e4m3x4<DT>(w.y, kscale), f2 = e4m3x4<DT>(w.z, kscale),
-                        f3 = e4m3x4<DT>(w.w, kscale);
+      for (int s = 0; s < TR_FRAGMENTS; s++) k_read(s);
 #pragma unroll
-            for (int c = 0; c < NC; c++) {
-              sc[c][n] = mfma16<DT>(make_uint4(f0.x, f0.y, f1.x, f1.y), qf[c][2 * j], sc[c][n]);
-              sc[c][n] = mfma16<DT>(make_uint4(f2.x, f2.y, f3.x, f3.y), qf[c][2 * j + 1], sc[c][n]);
-            }
-          } else {
+      for (int s = 0; s < NB * (RB / 64); s++) {
+        if (s + TR_FRAGMENTS < NB * (RB / 64)) k_read(s + TR_FRAGMENTS);
+        __builtin_amdgcn_sched_barrier(0);
+        const int n = s % NB, j = s / NB;
+        const uint4 w = kw[s % (TR_FRAGMENTS + 1)];
+        if constexpr (Q8) {
+          const uint2 f0 = e4m3x4<DT>(w.x, kscale[n]), f1 = e4m3x4<DT>(w.y, kscale[n]), f2 = e4m3x4<DT>(w.z, kscale[n]),
+                      f3 = e4m3x4<DT>(w.w, kscale[n]);
 #pragma unroll
-            for (int c = 0; c < NC; c++) sc[c][n] = mfma16<DT>(w, qf[c][j], sc[c][n]);
+          for (int c = 0; c < NC; c++) {
+            sc[c][n] = mfma16<DT>(make_uint4(f0.x, f0.y, f1.x, f1.y), qf[c][2 * j], sc[c][n]);
+            sc[c][n] = mfma16<DT>(make_uint4(f2.x, f2.y, f3.x, f3.y), qf[c][2 * j + 1], sc[c][n]);
           }
+        } else {
+#pragma unroll
+          for (int c = 0; c < NC; c++) sc[c][n] = mfma16<DT>(w, qf[c][j], sc[c][n]);
         }
       }
       // (the other wave of the SIMD is given way to in the softmax: its matrix instructions and these
@@ -636,25 +648,38 @@ __global__ __launch_bounds__(TR_WAVES * kWave, 2) void tree_kernel(TreeArgs a) {
           if constexpr (SHARE) __syncthreads();
         }
       }
-#pragma unroll
-      for (int m = 0; m < NB / 2; m++)
-#pragma unroll
-        for (int dt = 0; dt < D / 16; dt++) {
-          uint4 vf;
-          if constexpr (Q8) {
-            const uint2 w = lds_tr8(&vt[voff[dt] + 32 * m * RB]);
-            const uint2 f0 = e4m3x4<DT>(w.x, 1.f), f1 = e4m3x4<DT>(w.y, 1.f);
-            vf = make_uint4(f0.x, f0.y, f1.x, f1.y);
-          } else {
-            const uint2 lo = lds_tr4(reinterpret_cast<const uint16_t*>(&vt[voff[dt] + 32 * m * RB]));
-            const uint2 hi = lds_tr4(reinterpret_cast<const uint16_t*>(&vt[voff[dt] + (32 * m + 16) * RB]));
-            vf = make_uint4(lo.x, lo.y, hi.x, hi.y);
-          }
-#pragma unroll
-          for (int c = 0; c < NC; c++)
-            acc[c][dt] = mfma16<DT>(vf, make_uint4(pb[c][2 * m].x, pb[c][2 * m].y, pb[c][2 * m + 1].x, pb[c][2 * m + 1].y),
-                                    acc[c][dt]);
+      constexpr int DV = D / 16;
+      uint4 vw[TR_FRAGMENTS + 1];
+      auto v_read = [&](int s) __attribute__((always_inline)) {
+        const int m = s / DV, dt = s % DV;
+        uint4& to = vw[s % (TR_FRAGMENTS + 1)];
+        if constexpr (Q8) {
+          const uint2 w = lds_tr8(&vt[voff[dt] + 32 * m * RB]);
+          to.x = w.x;
+          to.y = w.y;
+        } else {
+          const uint2 lo = lds_tr4(reinterpret_cast<const uint16_t*>(&vt[voff[dt] + 32 * m * RB]));
+          const uint2 hi = lds_tr4(reinterpret_cast<const uint16_t*>(&vt[voff[dt] + (32 * m + 16) * RB]));
+          to = make_uint4(lo.x, lo.y, hi.x, hi.y);
         }
+      };
+#pragma unroll
+      for (int s = 0; s < TR_FRAGMENTS; s++) v_read(s);
+#pragma unroll
+      for (int s = 0; s < NB / 2 * DV; s++) {
+        if (s + TR_FRAGMENTS < NB / 2 * DV) v_read(s + TR_FRAGMENTS);
+        __builtin_amdgcn_sched_barrier(0);
+        const int m = s / DV, dt = s % DV;
+        uint4 vf = vw[s % (TR_FRAGMENTS + 1)];
+        if constexpr (Q8) {
+          const uint2 f0 = e4m3x4<DT>(vf.x, 1.f), f1 = e4m3x4<DT>(vf.y, 1.f);
+          vf = make_uint4(f0.x, f0.y, f1.x, f1.y);
+        }
+#pragma unroll
+        for (int c = 0; c < NC; c++)
+          acc[c][dt] = mfma16<DT>(vf, make_uint4(pb[c][2 * m].x, pb[c][2 * m].y, pb[c][2 * m + 1].x, pb[c][2 * m + 1].y),
+                                  acc[c][dt]);
+      }
     };
 
     if constexpr (!SHARE) {
