@@ -10,18 +10,21 @@
 // the products, which are transposed (S^T = K Q^T and O^T += V^T P^T on MFMA 16x16x32; a
 // lane holds one query row of each 16).  Up to 32 columns every wave holds all of them and the
 // waves split the tokens; wider tiles share each block of tokens, 16 or 32 columns a wave (16
-// sequences' trees of 16 nodes and 4 heads, 64 columns: 69 us, as private tiles of 32 columns 93).  One pass with a running maximum;
-// statistics and O are fp32.  The weights are rounded to q's type before they meet V (half a step
-// of a weight each; their sum takes them unrounded).
+// sequences' trees of 16 nodes and 4 heads, 64 columns: 69 us, as private tiles of 32 columns 93).
+// One pass with a running maximum; statistics and O are fp32.  The weights are rounded to q's type
+// before they meet V (half a step of a weight each; their sum takes them unrounded).
 //
 // In 8 bits a fragment is converted between LDS and MFMA.  The conversion multiplies by
 // a power of two, so a key is read with its scale for nothing and, in bf16, without
 // rounding (f16 rounds keys below 2^-14); a fragment of V holds 8 tokens, whose scales go into the
 // weights' exponents instead.
 //
-// Bound: single rows by memory (32 sequences of 4 to 8 K tokens in 8 bits, 436 MB, 88 us, 5.0 TB/s), one long row by the chain of ids, first block, merge and join;
-// chunks by issue: MFMA takes half of a SIMD's cycles and the exponentials, conversions and LDS reads the
-// rest (2048 rows after 14 K tokens, 503 GFLOP, 620 us, 0.81 PFLOP/s).
+// Bound: single rows by memory (32 sequences of 4 to 8 K tokens in 8 bits, 436 MB, 84 us, 5.2 TB/s), one
+// long row by the chain of ids, first block, merge and join (32 K tokens: 20 + 4 us); chunks by issue and
+// the waits between MFMA and softmax of two waves a SIMD (2048 rows after 14 K tokens in 8 bits, 503 GFLOP,
+// 610 us, 0.82 PFLOP/s: VALU 64 % and MFMA 35 % of a SIMD's cycles).  Of the two workgroups of a CU the one
+// that starts first runs some 10 % faster; larger shares for those: the chunk 620 -> 607, a prompt of
+// 2048 90 -> 100, so not kept.
 #include <type_traits>
 
 #include "attn_device.h"
@@ -35,8 +38,9 @@ constexpr int TR_WAVES = 4;
 // 32.6 us, with 512 of them 35.7, 320: 39.2; 32 rows of d = 64 65, 70 and 85), two where waves wait for
 // a shared block (64-node trees 144 us, with 256 194, 1024: 160; a chunk of 2048 641, 1083, 659).
 constexpr int TR_PRIVATE_WG = 256, TR_SHARED_WG = 512;
-// From that many tiles (of all kv heads) on each has a workgroup: 500 sequences of 1000 tokens 170 us,
-// in equal parts 195; fewer are cut (300 of 1500 tokens 162 us, a workgroup each 175, 160 of 2000: 122 and 128).
+// From that many tiles (of all kv heads) on each has a workgroup: 500 sequences of 1000 tokens 170 us, in equal
+// parts 195, 200 trees of 8 nodes 118 and 142; 160 sequences of 2000 tokens are cut, 122 us for 128.
+// (300 of 1500, the cut's worst miss: 175 us, in equal parts 162.)
 constexpr int TR_MANY = 2048;
 constexpr int TR_MIN_BLOCKS = 4;   // of a part: one row over 8 K tokens 24.6 us, with 2 26.9, with 8 25.5
 // Of a tile's start, in tokens, at its front (spread over its tokens: 64-node trees 144 us for 132, a prompt of
@@ -882,8 +886,9 @@ __global__ __launch_bounds__(TR_WAVES * kWave, 2) void tree_kernel(TreeArgs a) {
 
 // Split tiles: the parts of one, 256 of its results' quads a workgroup.  Where there are fewer
 // quads, SG threads share one (every SG-th part each) and meet in LDS.  (Joined by the last
-// workgroup of a tile to arrive in the kernel above: 38 us for 32 rows and 32 parts; here 5 to 14.)
-constexpr int TC_THREADS = 256, TC_AHEAD = 16;
+// workgroup of a tile to arrive in the kernel above: 38 us for 32 rows and 32 parts; here 4 to 17.)
+// TC_AHEAD of a thread's parts are on their way, where it has few TC_FEW (a chunk's, two each: 23 us for 17).
+constexpr int TC_THREADS = 256, TC_AHEAD = 16, TC_FEW = 4;
 template <int DT, int D>
 __global__ __launch_bounds__(TC_THREADS) void tree_join_kernel(TreeArgs a) {
   const int hk = blockIdx.x % a.hkv, w0 = blockIdx.x / a.hkv, tid = threadIdx.x, most = a.parts << a.log_heads;
@@ -898,12 +903,13 @@ __global__ __launch_bounds__(TC_THREADS) void tree_join_kernel(TreeArgs a) {
   float M = -INFINITY, L = 0.f;
   f32x4 O = {0.f, 0.f, 0.f, 0.f};
   const bool work = item < items && j < SG;
-  if (work) {
-    for (int p = j; p < at.z; p += SG * TC_AHEAD) {
-      float2 ml[TC_AHEAD];
-      f32x4 ov[TC_AHEAD];
+  auto merge = [&](auto ahead_c) __attribute__((always_inline)) {
+    constexpr int AHEAD = decltype(ahead_c)::value;  // parts of this thread on their way
+    for (int p = j; p < at.z; p += SG * AHEAD) {
+      float2 ml[AHEAD];
+      f32x4 ov[AHEAD];
 #pragma unroll
-      for (int u = 0; u < TC_AHEAD; u++) {
+      for (int u = 0; u < AHEAD; u++) {
         const int q = p + u * SG;
         ml[u] = make_float2(-INFINITY, 0.f);
         ov[u] = f32x4{0.f, 0.f, 0.f, 0.f};
@@ -915,18 +921,22 @@ __global__ __launch_bounds__(TC_THREADS) void tree_join_kernel(TreeArgs a) {
       }
       float mb = M;
 #pragma unroll
-      for (int u = 0; u < TC_AHEAD; u++) mb = fmaxf(mb, ml[u].x);
+      for (int u = 0; u < AHEAD; u++) mb = fmaxf(mb, ml[u].x);
       const float f0 = M == -INFINITY ? 0.f : __builtin_amdgcn_exp2f(M - mb);
       L *= f0;
       O *= f0;
 #pragma unroll
-      for (int u = 0; u < TC_AHEAD; u++) {
+      for (int u = 0; u < AHEAD; u++) {
         const float f = ml[u].x == -INFINITY ? 0.f : __builtin_amdgcn_exp2f(ml[u].x - mb);
         L += ml[u].y * f;
         O += ov[u] * f;
       }
       M = mb;
     }
+  };
+  if (work) {
+    if (at.z <= SG * TC_FEW) merge(std::integral_constant<int, TC_FEW>{});
+    else merge(std::integral_constant<int, TC_AHEAD>{});
   }
   if (SG > 1) {  // (a fixed order)
     __shared__ f32x4 so[TC_THREADS];
