@@ -129,6 +129,40 @@ def test_scales_of_v(kind, news, hq, d, dt):
         _check(b, q, k, v * 2.0 ** 120, (out.double() * 2.0 ** 120), None, 127, least=2.0 ** -13)
 
 
+@DTS
+@WIDTHS
+def test_large_scores_over_8_bits(news, hq, d, dt):
+    """Scores beyond 2^20, where V's exponents are lost beside them: the largest of each row takes the weight,
+    and its value comes back exactly."""
+    gen = torch.Generator().manual_seed(12)
+    hkv, page, lens = 2, 16, [330, 700]
+    b = Batch(lens, news, page, seed=5)
+    q = (torch.randn((b.rows, hq, d), generator=gen) * 2.0 ** 8).to(dt)
+    kc, vc, ks, vs = random_cache(b.pool, page, hkv, d, gen, 118, 122)
+    top = 134 if dt is torch.float16 else 160  # (keys that f16 holds)
+    ks = torch.randint(top - 4, top, ks.shape, generator=gen, dtype=torch.uint8).view(E8M0)
+    k, v = values(kc, ks), values(vc, vs)
+    out = F.gqa_tree_paged(q.cuda(), kc.cuda(), vc.cuda(), *b.args(), qo_indptr=b.qo(), k_scale=ks.cuda(), v_scale=vs.cuda()).cpu()
+    assert out.isfinite().all()
+    checked, row, G = 0, 0, hq // hkv
+    for s, (L, n) in enumerate(zip(b.lens, b.news)):
+        ids = torch.from_numpy(b.indices[b.kv_ptr[s]:b.kv_ptr[s + 1]]).long()
+        for i in range(n):
+            at = torch.arange(L - n + i + 1)
+            for h in range(hkv):
+                kk, vv = k[ids[at // page], at % page, h], v[ids[at // page], at % page, h]
+                qs = q[row, h * G:(h + 1) * G].double()
+                score = qs @ kk.t()
+                best = score.topk(2, -1).values
+                # sums of d terms in fp32 are at most 2^-17 of their magnitudes off; V's exponents are below 128
+                sure = best[:, 0] - best[:, 1] > (2.0 ** -16 * (qs.abs() @ kk.abs().t()).amax(-1) + 128 + 40) * math.sqrt(d)
+                for g in sure.nonzero()[:, 0].tolist():
+                    checked += 1
+                    assert torch.equal(out[row, h * G + g], vv[score[g].argmax()].to(dt))
+            row += 1
+    assert checked > 3 * b.rows
+
+
 def test_two_streams_at_once():
     """Calls on two streams have workspaces of their own."""
     gen, dt = torch.Generator().manual_seed(6), torch.bfloat16

@@ -64,7 +64,10 @@ __device__ __forceinline__ int quantise16(const float* x, uint2* codes) {
 }
 
 // A wave takes up to A8_ROWS * RPW of a token's rows, q heads first, then k's and v's: its
-// lanes keep the token's angles for all of theirs.
+// lanes keep the token's angles for all of theirs, and the search for the token's sequence and
+// page runs while the rows are on their way.  12.4k tokens of 32 and 8 heads of 128 in bf16, 281 MB:
+// 53 us, 5.3 TB/s, bound by memory (a copy of that size 55); one token 4.8 us, bound by latency.
+// (The sequence searched for by all lanes at once instead of by halving: 56.5 us.)
 template <int DT, int D, bool F32>
 __global__ __launch_bounds__(A8_THREADS) void append8_kernel(Append8Args a) {
   constexpr int LPR = D / 16, RPW = kWave / LPR, WAVES = A8_THREADS / kWave;  // lanes per row, rows per wave and pass
@@ -174,7 +177,9 @@ __device__ __forceinline__ uint4 values8(uint2 c, uint32_t scale) {
 }
 
 // A wave takes R8_TOKENS tokens: lane i looks up token i % R8_TOKENS, then the wave passes over
-// their pieces of 8 codes, R8_AHEAD of them a lane on their way.  Bound by memory.
+// their pieces of 8 codes, R8_AHEAD of them a lane on their way, so that a store of the wave is 1 KB
+// in a piece.  131 K tokens of 8 heads of 128, 619 MB: 121 us, 5.1 TB/s, what a copy reaches (16 codes
+// a lane, stores of 16 bytes every 32: 148 us).
 constexpr int R8_TOKENS = 8, R8_AHEAD = 8;
 
 template <int DT, int D>
