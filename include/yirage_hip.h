@@ -235,7 +235,8 @@ int yr_hip_gqa_tree_paged(const void* q, const void* k_cache, const void* v_cach
 /* Moves the accepted path of each sequence's drafted tokens to the front of its new slots:
  * slot kv_len[b] - n + j takes what slot kv_len[b] - n + path[b][j] held, n the sequence's
  * new tokens (by qo_indptr; NULL: 1).  path[batch][depth] ascends; the first entry that does
- * not, is negative or not below n ends it.  len_out[b] = kv_len[b] - n + entries.  dtype is the
+ * not, is negative or not below n ends it.  len_out[b] = kv_len[b] - n + entries (a place of its
+ * own; no two sequences may share a page of their new tokens).  dtype is the
  * cache's: f16 or bf16 (scales NULL; page_bounds, or NULL, grow to hold the kept keys) or
  * YR_DTYPE_E4M3 (with scales, without bounds). */
 int yr_hip_keep_kv_paged(void* k_cache, void* v_cache, void* k_scale, void* v_scale, void* page_bounds,
