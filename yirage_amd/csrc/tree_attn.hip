@@ -179,8 +179,11 @@ __device__ __forceinline__ TileAt find_index(const TreeArgs& a, SeqWork w, int i
   t.from = 0;
   t.units = 1;
   if (!a.r.qo_indptr) {
-    t.b = index;
-    t.s = seq_rows(a.r, index);
+    // (a call made for more parts than it has sequences: those behind the last have no tables to read)
+    if (index < a.r.batch) {
+      t.b = index;
+      t.s = seq_rows(a.r, index);
+    }
     return t;
   }
   long long left = index;
@@ -370,7 +373,7 @@ __global__ __launch_bounds__(TR_WAVES * kWave, 2) void tree_kernel(TreeArgs a) {
   }
   while (true) {
     const TileAt at = split ? find_unit(a, work0, x) : find_index(a, work0, w0);
-    if (at.b >= a.r.batch) return;  // (only without parts)
+    if (at.b >= a.r.batch) return;  // (no tile left: a tile a workgroup, or no new rows)
     const SeqRows s = at.s;
     const int i0 = at.tile * a.tt;
     const long long u0 = split ? x - at.from : 0, u1 = split ? min(x1 - at.from, at.units) : 1;
