@@ -285,6 +285,14 @@ __device__ __forceinline__ bool not_finite(uint4 v) {
   return bad;
 }
 
+// A row's sum of weights at maximum m, as one at maximum `to`.  In 8 bits the maximum is that of score and V's exponent
+// together and the sum one of scores alone: it can count where 2^(m - to) is below fp32's range (64 tokens of scale
+// 2^-60 before 64 of 2^93: without them twice the value), so it moves in two steps.
+__device__ __forceinline__ float sum_at(float l, float m, float to) {
+  const float half = m == -INFINITY ? 0.f : __builtin_amdgcn_exp2f(0.5f * (m - to));
+  return l * half * half;
+}
+
 // 4 results of a tile's column: channels d0 .. of row t0 + column / G, head column % G
 template <int DT, int D>
 __device__ __forceinline__ void put_result(const TreeArgs& a, int hk, int t0, int column, int d0, f32x4 O, float L) {
@@ -571,9 +579,10 @@ __global__ __launch_bounds__(TR_WAVES * kWave, 2) void tree_kernel(TreeArgs a) {
 #pragma unroll
         for (int c = 0; c < NC; c++) {
           const float alpha = m_i[c] == -INFINITY ? 0.f : __builtin_amdgcn_exp2f(m_i[c] - mnew[c]);
+          if constexpr (Q8) l_i[c] = sum_at(l_i[c], m_i[c], mnew[c]);
+          else l_i[c] *= alpha;
           m_i[c] = mnew[c];
           far |= __builtin_amdgcn_ballot_w64(fabsf(m_i[c]) > kFarScore && m_i[c] > -INFINITY) != 0;
-          l_i[c] *= alpha;
 #pragma unroll
           for (int dt = 0; dt < D / 16; dt++) acc[c][dt] *= alpha;
         }
@@ -869,7 +878,8 @@ __global__ __launch_bounds__(TR_WAVES * kWave, 2) void tree_kernel(TreeArgs a) {
           const float f = s_m[w][row] == -INFINITY ? 0.f : __builtin_amdgcn_exp2f(s_m[w][row] - M);
           const uint8_t* const os = row < 16 ? s_v[w] : s_k[w];
           const f32x4 v = *reinterpret_cast<const f32x4*>(reinterpret_cast<const float*>(os) + row % 16 * D + d0);
-          L += s_l[w][row] * f;
+          if constexpr (Q8) L += sum_at(s_l[w][row], s_m[w][row], M);
+          else L += s_l[w][row] * f;
           O += v * f;
         }
         if (whole) {
@@ -926,12 +936,12 @@ __global__ __launch_bounds__(TC_THREADS) void tree_join_kernel(TreeArgs a) {
 #pragma unroll
       for (int u = 0; u < AHEAD; u++) mb = fmaxf(mb, ml[u].x);
       const float f0 = M == -INFINITY ? 0.f : __builtin_amdgcn_exp2f(M - mb);
-      L *= f0;
+      L = sum_at(L, M, mb);
       O *= f0;
 #pragma unroll
       for (int u = 0; u < AHEAD; u++) {
         const float f = ml[u].x == -INFINITY ? 0.f : __builtin_amdgcn_exp2f(ml[u].x - mb);
-        L += ml[u].y * f;
+        L += sum_at(ml[u].y, ml[u].x, mb);
         O += ov[u] * f;
       }
       M = mb;
@@ -955,7 +965,7 @@ __global__ __launch_bounds__(TC_THREADS) void tree_join_kernel(TreeArgs a) {
     for (int u = 0; u < SG; u++) {
       const float2 v = sml[u * items + item];
       const float f = v.x == -INFINITY ? 0.f : __builtin_amdgcn_exp2f(v.x - mb);
-      L += v.y * f;
+      L += sum_at(v.y, v.x, mb);
       O += so[u * items + item] * f;
     }
   }
