@@ -464,11 +464,13 @@ __global__ __launch_bounds__(TR_WAVES * kWave, 2) void tree_kernel(TreeArgs a) {
     // Scales.  K's go into the conversion.  V's, 2^e, are added to the scores, as e in the exponent
     // (the start of the sums that are the scores: no instruction a weight):
     //   P = 2^(x + e - m),  O += P code,  L += P 2^-e,  m the running maximum of x + e
-    // so that P keeps to its type's range whatever the scales are.  A token whose scale is below 2^-60,
-    // or 2^-60 of the largest so far, takes that instead (its part in L would be lost otherwise),
-    // and its weight the rest on its way to O.
+    // so that P keeps to its type's range whatever the scales are, by each row's own maximum: a token that
+    // a row does not see, or that counts little, takes no bits from it.  Where a token's scale is below 2^-60 of the
+    // largest so far, P may be 0 and its part in L is not: there L += 2^(x - m), in two factors like all that L is
+    // multiplied by.  A scale below 2^-60 counts as that (L stays in range) and its weight takes the rest on its
+    // way to O.
     int top = 0;       // the largest scale byte so far
-    bool low = false;  // some token of the block has less than its scale in e
+    bool low = false;  // some token of the block has a scale for that
     auto put_scales = [&](int kb, int vb, uint64_t have) __attribute__((always_inline)) {
       const bool ok = (have >> lane & 1) && vb != 255;
       if (__builtin_amdgcn_ballot_w64(ok && vb > top)) {
@@ -477,8 +479,8 @@ __global__ __launch_bounds__(TR_WAVES * kWave, 2) void tree_kernel(TreeArgs a) {
         for (int o = 32; o > 0; o >>= 1) most = max(most, __shfl_xor(most, o, kWave));
         top = max(top, __builtin_amdgcn_readfirstlane(most));
       }
-      const int least = max(top - 60, 67), e = min(max(vb, least), 254);
-      low = __builtin_amdgcn_ballot_w64(ok && vb < least) != 0;
+      const int e = min(max(vb, 67), 254);
+      low = __builtin_amdgcn_ballot_w64(ok && vb < max(top - 60, 67)) != 0;
       s_ks[wave][lane % BT] = __uint_as_float((uint32_t)kb << 23);  // (what the conversion takes: 0 is 2^-127, 255 NaN)
       s_ev[wave][lane % BT] = vb == 255 ? NAN : (float)(e - 127) * a.scale_inv;
       s_iv[wave][lane % BT] = __uint_as_float(e < 254 ? (uint32_t)(254 - e) << 23 : 0x400000u);
@@ -604,9 +606,15 @@ __global__ __launch_bounds__(TR_WAVES * kWave, 2) void tree_kernel(TreeArgs a) {
               // (a row goes by its own maximum, so its weights agree)
               float x = PLAIN ? fmaf(sc[c][n][i], a.scale_log2, kPBias<DT> - m) : far_exponent(sc[c][n][i], a.scale_log2, m) + kPBias<DT>;
               p[i] = __builtin_amdgcn_exp2f(x);
-              if constexpr (Q8) l_i[c] = fmaf(p[i], iv[i], l_i[c]);
-              else l_i[c] += p[i];
-              if constexpr (Q8 && !PLAIN) p[i] *= fv[i];
+              if constexpr (Q8 && !PLAIN) {
+                const float root = __builtin_amdgcn_exp2f(0.5f * (x + (float)((int)(__float_as_uint(iv[i]) >> 23) - 127)));
+                l_i[c] = fmaf(root, root, l_i[c]);
+                p[i] *= fv[i];
+              } else if constexpr (Q8) {
+                l_i[c] = fmaf(p[i], iv[i], l_i[c]);
+              } else {
+                l_i[c] += p[i];
+              }
             }
             pb[c][n] = make_uint2(pack2<DT>(p[0], p[1]), pack2<DT>(p[2], p[3]));
           }
