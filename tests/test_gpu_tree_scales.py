@@ -118,3 +118,41 @@ def test_large_scales_with_small_weights(news, hq, d, dt):
                 moved += int(((p[:, others] @ vv[others] - ref).abs() > 8 * tol).sum())
             row += 1
     assert moved > 100
+
+
+@DTS
+@WIDTHS
+@pytest.mark.parametrize("low,high", [(118, 142), (137, 142), (60, 121)])
+def test_scales_of_keys(low, high, news, hq, d, dt):
+    """Keys beyond what 16 bits of q's type hold, alone and among ordinary ones, and far below."""
+    print("case", low, high, news, hq, d, dt, flush=True)
+    gen = torch.Generator().manual_seed(24)
+    hkv, page, lens = 2, 16, [330, 700]
+    b = Batch(lens, news, page, seed=5)
+    big = high > 127
+    q = (torch.randn((b.rows, hq, d), generator=gen) * (2.0 ** -12 if big else 1)).to(dt)
+    kc, vc, _, vs = random_cache(b.pool, page, hkv, d, gen, 118, 122)
+    if big:
+        kc = (kc.float() / 16).to(E4M3)
+    ks = torch.randint(low, high, (b.pool, page, hkv), generator=gen, dtype=torch.uint8).view(E8M0)
+    k, v = values(kc, ks), values(vc, vs)
+    assert not big or k.abs().max() > 2 * 65504
+    out = F.gqa_tree_paged(q.cuda(), kc.cuda(), vc.cuda(), *b.args(), qo_indptr=b.qo(), k_scale=ks.cuda(), v_scale=vs.cuda()).cpu()
+    _check(b, q, k, v, out, None, 9)
+
+
+def test_largest_keys_of_f16():
+    """f16's largest keys, appended: their codes stand for 65536, which f16 itself does not hold."""
+    gen = torch.Generator().manual_seed(25)
+    dt, hq, hkv, d, page, L = torch.float16, 4, 1, 64, 16, 90
+    b = Batch([L], [L], page)
+    k = torch.where(torch.rand((L, hkv, d), generator=gen) < 0.5, -65504.0, 65504.0).to(dt)
+    v = torch.randn((L, hkv, d), generator=gen).to(dt)
+    q = (torch.randn((L, hq, d), generator=gen) * 2.0 ** -14).to(dt)
+    kc, vc = (torch.zeros((b.pool, page, hkv, d), dtype=torch.uint8, device="cuda").view(E4M3) for _ in range(2))
+    ks, vs = (torch.zeros((b.pool, page, hkv), dtype=torch.uint8, device="cuda").view(E8M0) for _ in range(2))
+    F.append_kv_paged_fp8(k.cuda(), v.cuda(), kc, vc, ks, vs, *b.args(), qo_indptr=b.qo())
+    stored = values(kc.cpu(), ks.cpu())
+    assert stored.abs().max() == 65536
+    out = F.gqa_tree_paged(q.cuda(), kc, vc, *b.args(), qo_indptr=b.qo(), k_scale=ks, v_scale=vs).cpu()
+    _check(b, q, stored, values(vc.cpu(), vs.cpu()), out, None, 9)

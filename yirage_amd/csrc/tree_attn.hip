@@ -15,8 +15,8 @@
 // before they meet V (half a step of a weight each; their sum takes them unrounded).
 //
 // In 8 bits a fragment is converted between LDS and MFMA.  The conversion multiplies by
-// a power of two, so a key is read with its scale for nothing and, in bf16, without
-// rounding (f16 rounds keys below 2^-14); a fragment of V holds 8 tokens, whose scales go into the
+// a power of two, so a key is read with its scale for nothing and without rounding (down to
+// bf16's smallest normal number); a fragment of V holds 8 tokens, whose scales go into the
 // weights' exponents instead.
 //
 // Bound: single rows by memory (32 sequences of 4 to 8 K tokens in 8 bits, 436 MB, 84 us, 5.2 TB/s), one
@@ -326,6 +326,7 @@ __global__ __launch_bounds__(TR_WAVES * kWave, 2) void tree_kernel(TreeArgs a) {
   __shared__ __attribute__((aligned(16))) uint8_t s_k[SLOTS][BT * RB];
   __shared__ __attribute__((aligned(16))) uint8_t s_v[SLOTS][BT * RB];
   __shared__ __attribute__((aligned(16))) float s_ks[TR_WAVES][BT], s_ev[TR_WAVES][BT], s_iv[TR_WAVES][BT], s_fv[TR_WAVES][BT];
+  __shared__ __attribute__((aligned(16))) float s_rk[Q8 && DT == DT_F16 ? TR_WAVES : 1][BT], s_rv[Q8 && DT == DT_F16 ? TR_WAVES : 1][BT];
   __shared__ __attribute__((aligned(16))) uint32_t s_small[TR_WAVES][NSMALL][kWave];  // by wave or slot: ids, scale bytes
   __shared__ float s_m[TR_WAVES][16 * NC], s_l[TR_WAVES][16 * NC];
   static_assert(16 * D * 4 <= BT * RB, "a wave's O of 16 columns fits a slot");
@@ -461,8 +462,9 @@ __global__ __launch_bounds__(TR_WAVES * kWave, 2) void tree_kernel(TreeArgs a) {
       for (int dt = 0; dt < D / 16; dt++) acc[c][dt] = f32x4{0.f, 0.f, 0.f, 0.f};
     }
 
-    // Scales.  K's go into the conversion.  V's, 2^e, are added to the scores, as e in the exponent
-    // (the start of the sums that are the scores: no instruction a weight):
+    // Scales.  K's go into the conversion (f16 holds every code times 2^-15 to 2^7: of a scale beyond these the
+    // rest multiplies the token's scores, and V's exponent follows).  V's, 2^e, are added to the scores, as e in the
+    // exponent (the start of the sums that are the scores: no instruction a weight):
     //   P = 2^(x + e - m),  O += P code,  L += P 2^-e,  m the running maximum of x + e
     // so that P keeps to its type's range whatever the scales are, by each row's own maximum: a token that
     // a row does not see, or that counts little, takes no bits from it.  Where a token's scale is below 2^-60 of the
@@ -471,20 +473,32 @@ __global__ __launch_bounds__(TR_WAVES * kWave, 2) void tree_kernel(TreeArgs a) {
     // way to O.
     int top = 0;       // the largest scale byte so far
     bool low = false;  // some token of the block has a scale for that
+    bool wide = false; // some key's scale is beyond what f16 holds
     auto put_scales = [&](int kb, int vb, uint64_t have) __attribute__((always_inline)) {
-      const bool ok = (have >> lane & 1) && vb != 255;
-      if (__builtin_amdgcn_ballot_w64(ok && vb > top)) {
-        int most = ok ? vb : 0;
+      const bool ok = have >> lane & 1;
+      const int e = min(max(vb, 67), 254);
+      float ev = vb == 255 ? NAN : (float)(e - 127) * a.scale_inv;
+      low = wide = false;
+      // (rare, and the first block)
+      if (__builtin_amdgcn_ballot_w64(ok && (vb > top || vb < max(top - 60, 67) || (DT == DT_F16 && (unsigned)(kb - 112) > 22)))) {
+        int most = ok && vb != 255 ? max(vb, top) : top;
 #pragma unroll
         for (int o = 32; o > 0; o >>= 1) most = max(most, __shfl_xor(most, o, kWave));
-        top = max(top, __builtin_amdgcn_readfirstlane(most));
+        top = __builtin_amdgcn_readfirstlane(most);
+        low = __builtin_amdgcn_ballot_w64(ok && vb < max(top - 60, 67)) != 0;
+        if constexpr (DT == DT_F16) {
+          const int held = kb == 255 ? kb : min(max(kb, 112), 134);
+          wide = __builtin_amdgcn_ballot_w64(ok && kb != held) != 0;
+          s_rk[wave][lane % BT] = __uint_as_float((uint32_t)(kb - held + 127) << 23);
+          s_rv[wave][lane % BT] = kb != held ? ev : 0.f;
+          ev = kb != held ? 0.f : ev;
+          kb = held;
+        }
       }
-      const int e = min(max(vb, 67), 254);
-      low = __builtin_amdgcn_ballot_w64(ok && vb < max(top - 60, 67)) != 0;
       s_ks[wave][lane % BT] = __uint_as_float((uint32_t)kb << 23);  // (what the conversion takes: 0 is 2^-127, 255 NaN)
-      s_ev[wave][lane % BT] = vb == 255 ? NAN : (float)(e - 127) * a.scale_inv;
+      s_ev[wave][lane % BT] = ev;
       s_iv[wave][lane % BT] = __uint_as_float(e < 254 ? (uint32_t)(254 - e) << 23 : 0x400000u);
-      s_fv[wave][lane % BT] = __uint_as_float((uint32_t)max(vb - e + 127, 0) << 23);
+      s_fv[wave][lane % BT] = __uint_as_float((uint32_t)(vb - e + 127) << 23);
     };
 
     // Some row may not see some token of the block (uniform, also over waves)
@@ -539,6 +553,19 @@ __global__ __launch_bounds__(TR_WAVES * kWave, 2) void tree_kernel(TreeArgs a) {
       uint32_t seen[NC];
 #pragma unroll
       for (int c = 0; c < NC; c++) seen[c] = ~0u;
+      if constexpr (Q8 && DT == DT_F16) {
+        if (wide) {  // (uniform)
+#pragma unroll
+          for (int n = 0; n < NB; n++) {
+            const f32x4 rest = *reinterpret_cast<const f32x4*>(&s_rk[wave][16 * n + 4 * grp]);
+            const f32x4 ev = *reinterpret_cast<const f32x4*>(&s_rv[wave][16 * n + 4 * grp]);
+#pragma unroll
+            for (int c = 0; c < NC; c++)
+#pragma unroll
+              for (int i = 0; i < 4; i++) sc[c][n][i] = fmaf(sc[c][n][i], rest[i], ev[i]);
+          }
+        }
+      }
       if (masked) {
 #pragma unroll
         for (int c = 0; c < NC; c++) {
@@ -594,9 +621,13 @@ __global__ __launch_bounds__(TR_WAVES * kWave, 2) void tree_kernel(TreeArgs a) {
         constexpr bool PLAIN = decltype(plain_c)::value;
 #pragma unroll
         for (int n = 0; n < NB; n++) {
-          f32x4 iv, fv;
+          f32x4 iv, fv, hv;  // 2^-e; the rest of V's scale; -e / 2
           if constexpr (Q8) iv = *reinterpret_cast<const f32x4*>(&s_iv[wave][16 * n + 4 * grp]);
-          if constexpr (Q8 && !PLAIN) fv = *reinterpret_cast<const f32x4*>(&s_fv[wave][16 * n + 4 * grp]);
+          if constexpr (Q8 && !PLAIN) {
+            fv = *reinterpret_cast<const f32x4*>(&s_fv[wave][16 * n + 4 * grp]);
+#pragma unroll
+            for (int i = 0; i < 4; i++) hv[i] = 0.5f * (float)((int)(__float_as_uint(iv[i]) >> 23) - 127);
+          }
 #pragma unroll
           for (int c = 0; c < NC; c++) {
             const float m = m_i[c] == -INFINITY ? 0.f : m_i[c];
@@ -607,7 +638,7 @@ __global__ __launch_bounds__(TR_WAVES * kWave, 2) void tree_kernel(TreeArgs a) {
               float x = PLAIN ? fmaf(sc[c][n][i], a.scale_log2, kPBias<DT> - m) : far_exponent(sc[c][n][i], a.scale_log2, m) + kPBias<DT>;
               p[i] = __builtin_amdgcn_exp2f(x);
               if constexpr (Q8 && !PLAIN) {
-                const float root = __builtin_amdgcn_exp2f(0.5f * (x + (float)((int)(__float_as_uint(iv[i]) >> 23) - 127)));
+                const float root = __builtin_amdgcn_exp2f(fmaf(0.5f, x, hv[i]));
                 l_i[c] = fmaf(root, root, l_i[c]);
                 p[i] *= fv[i];
               } else if constexpr (Q8) {
