@@ -218,7 +218,9 @@ int yr_hip_read_kv_paged_fp8(const void* k_cache, const void* v_cache, const voi
  * hq / hkv <= 16.  A row without a token, or whose scores are all -inf, is 0.
  * max_kv_len, about the largest kv_len, decides how finely the work is split; it does not
  * limit what is seen.  Softmax statistics are fp32; the weights are rounded to dtype before they
- * meet v.  Two launches where tokens are split over workgroups, one otherwise. */
+ * meet v.  One launch where no workspace is needed, otherwise two that meet in it: a call on the
+ * stream that uses the same workspace must not come between them (threads that share a stream
+ * and a workspace call one at a time). */
 size_t yr_hip_gqa_tree_workspace(int rows, int batch, int ragged, int hq, int hkv, int d, int max_kv_len,
                                  int cache_dtype); /* ragged: a call with qo_indptr */
 /* The kernel a call runs on (host only): plan3 = {columns (rows times heads of a kv head) of a tile,

@@ -10,6 +10,7 @@ from __future__ import annotations
 
 import ctypes
 import struct
+import threading
 from typing import NamedTuple
 
 import torch
@@ -186,6 +187,7 @@ def argmax(x, n_valid: int | None = None, out=None):
 # each property once.
 _TICKET_BYTES = 65536  # what a workspace has zeroed at rest
 _scratch_cache: dict = {}
+_scratch_locks: dict = {}
 _DTYPE_ALL = {**_TORCH_DT, torch.float32: _lib.DTYPE_F32}
 _pack7 = struct.Struct("7q").pack  # seven int64 in memory, as a pointer argument takes them
 
@@ -242,6 +244,18 @@ def _scratch(nbytes: int, device, stream: int):
         with torch.cuda.device(device):  # (allocated and cleared on its stream)
             ws = _scratch_cache[key] = torch.zeros(max(nbytes, 1 << 20), dtype=torch.uint8, device=device)
     return ws
+
+
+def _launch_with(ws, index: int, stream: int, fn, what: str, *args):
+    """_launch of a call with scratch.  Some are two launches that meet in it, and it is every thread's
+    on that stream: calls follow one another under a lock, so that none comes between the two."""
+    if ws is None:
+        return _launch(index, fn, what, *args)
+    lock = _scratch_locks.get((index, stream))
+    if lock is None:
+        lock = _scratch_locks.setdefault((index, stream), threading.Lock())
+    with lock:
+        _launch(index, fn, what, *args)
 
 
 def _at(t):
@@ -548,7 +562,7 @@ def gqa_tree_paged(q, k_cache, v_cache, kv_indptr, kv_indices, kv_len, tree_mask
     L = lib()
     nb = L.yr_hip_gqa_tree_workspace(T, batch, qo_indptr is not None, hq, hkv, D, max_kv_len, cdt)
     ws = _scratch(nb, q.device, stream)
-    _launch(index, L.yr_hip_gqa_tree_paged, "gqa_tree_paged", q.data_ptr(), k_cache.data_ptr(), v_cache.data_ptr(),
+    _launch_with(ws, index, stream, L.yr_hip_gqa_tree_paged, "gqa_tree_paged", q.data_ptr(), k_cache.data_ptr(), v_cache.data_ptr(),
             _at(k_scale), _at(v_scale), mask_at, mask_row, mask_cols, _at(qo_indptr), kv_indptr.data_ptr(),
             kv_indices.data_ptr(), kv_indices.numel(), kv_len.data_ptr(), out.data_ptr(), T, batch, hq, hkv, D, page, P,
             max_kv_len, cdt, dt, _at(ws), nb, stream)
@@ -634,7 +648,7 @@ def select_pages(q, page_bounds, kv_indptr, kv_indices, kv_len, page_size: int, 
     stream = torch._C._cuda_getCurrentRawStream(index)
     nb = lib().yr_hip_select_pages_workspace(T, hkv, page_size, max_kv_len)
     ws = _scratch(nb, q.device, stream)
-    _launch(index, lib().yr_hip_select_pages, "select_pages", q.data_ptr(), page_bounds.data_ptr(), _at(qo_indptr),
+    _launch_with(ws, index, stream, lib().yr_hip_select_pages, "select_pages", q.data_ptr(), page_bounds.data_ptr(), _at(qo_indptr),
             kv_indptr.data_ptr(), kv_indices.data_ptr(), kv_indices.numel(), kv_len.data_ptr(), out.data_ptr(), T, batch,
             hq, hkv, D, page_size, P, max_kv_len, top_pages, first_pages, last_pages, dt,
             _at(ws), nb, stream)
@@ -666,7 +680,7 @@ def gqa_sparse_paged(q, k_cache, v_cache, kv_indptr, kv_indices, kv_len, pages, 
     stream = torch._C._cuda_getCurrentRawStream(index)
     nb = lib().yr_hip_gqa_sparse_workspace(T, batch, qo_indptr is not None, hq, hkv, D, page, top)
     ws = _scratch(nb, q.device, stream)
-    _launch(index, lib().yr_hip_gqa_sparse_paged, "gqa_sparse_paged", q.data_ptr(), k_cache.data_ptr(),
+    _launch_with(ws, index, stream, lib().yr_hip_gqa_sparse_paged, "gqa_sparse_paged", q.data_ptr(), k_cache.data_ptr(),
             v_cache.data_ptr(), _at(qo_indptr), kv_indptr.data_ptr(), kv_indices.data_ptr(), kv_indices.numel(),
             kv_len.data_ptr(), pages.data_ptr(), out.data_ptr(), T, batch, hq, hkv, D, page, P, top, dt,
             _at(ws), nb, stream)
@@ -711,7 +725,7 @@ def token_logprobs(logits, tokens, top_n: int = 0, n_valid: int | None = None) -
     nb = lib().yr_hip_token_logprobs_workspace(rows, n_valid, top_n, dt)
     ws = _scratch(nb, logits.device, stream)
     at = flat.data_ptr()
-    _launch(index, lib().yr_hip_token_logprobs, "token_logprobs", logits.data_ptr(), tokens.data_ptr(), at + 12 * cut,
+    _launch_with(ws, index, stream, lib().yr_hip_token_logprobs, "token_logprobs", logits.data_ptr(), tokens.data_ptr(), at + 12 * cut,
             at + 12 * cut + 4 * rows, at + 8 * cut, at, rows, n, n_valid, logits.stride(0) if rows > 1 else n, top_n, dt,
             _at(ws), nb, stream)
     return res
