@@ -156,3 +156,14 @@ def test_largest_keys_of_f16():
     assert stored.abs().max() == 65536
     out = F.gqa_tree_paged(q.cuda(), kc, vc, *b.args(), qo_indptr=b.qo(), k_scale=ks, v_scale=vs).cpu()
     _check(b, q, stored, values(vc.cpu(), vs.cpu()), out, None, 9)
+
+
+def test_reading_beyond_f16():
+    """What f16 does not hold reads as infinity of its sign, what rounds to its largest number as that."""
+    b = Batch([16], [16], 16)
+    codes = torch.linspace(-448, 448, 64).to(E4M3).expand(b.pool, 16, 1, 64).contiguous()
+    scales = (torch.arange(16, dtype=torch.uint8) + 130).view(1, 16, 1).expand(b.pool, 16, 1).contiguous().view(E8M0)
+    ref = values(codes, scales)[0].half()
+    assert ref.isinf().any() and ref.isfinite().any()
+    for x in F.read_kv_paged_fp8(codes.cuda(), codes.cuda(), scales.cuda(), scales.cuda(), *b.args(), b.qo(), 16, dtype=torch.float16):
+        assert torch.equal(x.cpu(), ref)

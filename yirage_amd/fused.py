@@ -486,8 +486,8 @@ def read_kv_paged_fp8(k_cache, v_cache, k_scale, v_scale, kv_indptr, kv_indices,
 
     Row out_indptr[b] + i is token i of sequence b (out_indptr int32, one more entry than kv_len); a
     token that the sequence does not have, or whose page is missing, reads as 0, and rows behind the
-    last sequence are left as they were (out: a pair of tensors).  bf16 holds the values exactly
-    (down to its smallest normal number), f16 rounds them once."""
+    last sequence are left as they were (out: two tensors).  bf16 holds the values exactly
+    (down to its smallest normal number), f16 rounds them once (to infinity from 65520 on)."""
     if dtype not in _TORCH_DT:
         _fail(f"unsupported dtype {dtype} (float16/bfloat16 only)")
     P, page, hkv, D = _cache_fp8(k_cache, v_cache, k_scale, v_scale)
@@ -500,10 +500,11 @@ def read_kv_paged_fp8(k_cache, v_cache, k_scale, v_scale, kv_indptr, kv_indices,
     if out is None:
         k, v = k_cache.new_empty(shape, dtype=dtype), k_cache.new_empty(shape, dtype=dtype)
     else:
+        if len(out) != 2 or any(tuple(t.shape) != shape or t.dtype is not dtype or not t.is_contiguous() for t in out):
+            _fail(f"out must be two contiguous tensors {shape} {dtype}")
         k, v = out
-        for t in out:
-            if tuple(t.shape) != shape or t.dtype is not dtype or not t.is_contiguous():
-                _fail(f"out must be two contiguous tensors {shape} {dtype}")
+        if abs(k.data_ptr() - v.data_ptr()) < 2 * k.numel():
+            _fail("the two results must lie apart")
     index = _one_device(k_cache, v_cache, k_scale, v_scale, kv_indptr, kv_indices, kv_len, out_indptr, k, v)
     if total == 0:
         return k, v
