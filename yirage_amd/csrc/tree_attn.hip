@@ -477,7 +477,11 @@ __global__ __launch_bounds__(TR_WAVES * kWave, 2) void tree_kernel(TreeArgs a) {
     auto put_scales = [&](int kb, int vb, uint64_t have) __attribute__((always_inline)) {
       const bool ok = have >> lane & 1;
       const int e = min(max(vb, 67), 254);
-      float ev = vb == 255 ? NAN : (float)(e - 127) * a.scale_inv;
+      const float ev = vb == 255 ? NAN : (float)(e - 127) * a.scale_inv;
+      s_ks[wave][lane % BT] = __uint_as_float((uint32_t)kb << 23);  // (what the conversion takes: 0 is 2^-127, 255 NaN)
+      s_ev[wave][lane % BT] = ev;
+      s_iv[wave][lane % BT] = __uint_as_float(e < 254 ? (uint32_t)(254 - e) << 23 : 0x400000u);
+      s_fv[wave][lane % BT] = __uint_as_float((uint32_t)(vb - e + 127) << 23);
       low = wide = false;
       // (rare, and the first block)
       if (__builtin_amdgcn_ballot_w64(ok && (vb > top || vb < max(top - 60, 67) || (DT == DT_F16 && (unsigned)(kb - 112) > 22)))) {
@@ -489,16 +493,14 @@ __global__ __launch_bounds__(TR_WAVES * kWave, 2) void tree_kernel(TreeArgs a) {
         if constexpr (DT == DT_F16) {
           const int held = kb == 255 ? kb : min(max(kb, 112), 134);
           wide = __builtin_amdgcn_ballot_w64(ok && kb != held) != 0;
-          s_rk[wave][lane % BT] = __uint_as_float((uint32_t)(kb - held + 127) << 23);
-          s_rv[wave][lane % BT] = kb != held ? ev : 0.f;
-          ev = kb != held ? 0.f : ev;
-          kb = held;
+          if (wide) {
+            s_ks[wave][lane % BT] = __uint_as_float((uint32_t)held << 23);
+            s_ev[wave][lane % BT] = kb != held ? 0.f : ev;
+            s_rk[wave][lane % BT] = __uint_as_float((uint32_t)(kb - held + 127) << 23);
+            s_rv[wave][lane % BT] = kb != held ? ev : 0.f;
+          }
         }
       }
-      s_ks[wave][lane % BT] = __uint_as_float((uint32_t)kb << 23);  // (what the conversion takes: 0 is 2^-127, 255 NaN)
-      s_ev[wave][lane % BT] = ev;
-      s_iv[wave][lane % BT] = __uint_as_float(e < 254 ? (uint32_t)(254 - e) << 23 : 0x400000u);
-      s_fv[wave][lane % BT] = __uint_as_float((uint32_t)(vb - e + 127) << 23);
     };
 
     // Some row may not see some token of the block (uniform, also over waves)
