@@ -19,10 +19,11 @@
 // bf16's smallest normal number); a fragment of V holds 8 tokens, whose scales go into the
 // weights' exponents instead.
 //
-// Bound: single rows by memory (32 sequences of 4 to 8 K tokens in 8 bits, 436 MB, 84 us, 5.2 TB/s), one
+// Bound: single rows by memory (32 sequences of 4 to 8 K tokens in 8 bits, 436 MB, 84 us, 5.2 TB/s; in 16 bits 865 MB,
+// 152 us, 5.7), one
 // long row by the chain of ids, first block, merge and join (32 K tokens: 20 + 4 us); chunks by issue and
 // the waits between MFMA and softmax of two waves a SIMD (2048 rows after 14 K tokens in 8 bits, 503 GFLOP,
-// 610 us, 0.82 PFLOP/s: VALU 64 % and MFMA 35 % of a SIMD's cycles).  Of the two workgroups of a CU the one
+// 599 us, 0.84 PFLOP/s: VALU 65 % and MFMA 36 % of a SIMD's cycles).  Of the two workgroups of a CU the one
 // that starts first runs some 10 % faster; larger shares for those: the chunk 620 -> 607, a prompt of
 // 2048 90 -> 100, so not kept.
 #include <type_traits>
@@ -39,8 +40,10 @@ constexpr int TR_WAVES = 4;
 // a shared block (64-node trees 144 us, with 256 194, 1024: 160; a chunk of 2048 641, 1083, 659).
 constexpr int TR_PRIVATE_WG = 256, TR_SHARED_WG = 512;
 // From that many tiles (of all kv heads) on each has a workgroup: 500 sequences of 1000 tokens 170 us, in equal
-// parts 195, 200 trees of 8 nodes 118 and 142; 160 sequences of 2000 tokens are cut, 122 us for 128.
-// (300 of 1500, the cut's worst miss: 175 us, in equal parts 162.)
+// parts 195, 200 trees of 8 nodes 118 and 142; 160 sequences of 2000 tokens are cut, 122 us for 128 (300 of
+// 1500: 175 us, in equal parts 162).  All of these of one length.  The rule asks for no length, and a sequence much
+// longer than the rest is then one workgroup's: 256 single rows, one over 32 K tokens and the others over 1 K,
+// take 1000 us, 255 of them, which are cut, 125.
 constexpr int TR_MANY = 2048;
 constexpr int TR_MIN_BLOCKS = 4;   // of a part: one row over 8 K tokens 24.6 us, with 2 26.9, with 8 25.5
 // Of a tile's start, in tokens, at its front (spread over its tokens: 64-node trees 144 us for 132, a prompt of
@@ -76,8 +79,8 @@ struct TreeArgs {
 
 // Work.  A sequence of n new rows has ceil(n / tt) tiles, and a tile counts for as many units
 // as tokens its last row may see, and TR_TILE_COST for its start.  The units of a kv head, one
-// sequence after another, are cut into `parts` equal ranges, a workgroup each: lengths that differ
-// leave no workgroup waiting, a long sequence is split and several short ones share a workgroup.
+// sequence after another, are cut into `parts` equal ranges, a workgroup each (below TR_MANY tiles): lengths
+// that differ leave no workgroup waiting, a long sequence is split and several short ones share a workgroup.
 // (Each tile split as often as the longest needs: 64-node trees over 16 bits 169 us for 145, one
 // row over 32 K tokens 29 for 25.)  The cut is made on the device, from lengths that no host reads.
 struct SeqWork {
@@ -467,7 +470,8 @@ __global__ __launch_bounds__(TR_WAVES * kWave, 2) void tree_kernel(TreeArgs a) {
     // exponent (the start of the sums that are the scores: no instruction a weight):
     //   P = 2^(x + e - m),  O += P code,  L += P 2^-e,  m the running maximum of x + e
     // so that P keeps to its type's range whatever the scales are, by each row's own maximum: a token that
-    // a row does not see, or that counts little, takes no bits from it.  Where a token's scale is below 2^-60 of the
+    // a row does not see, or that counts little, takes no bits from it (f16 holds all of a weight's down to 2^-21 of
+    // the row's largest 2^(x + e), bf16 to 2^-126).  Where a token's scale is below 2^-60 of the
     // largest so far, P may be 0 and its part in L is not: there L += 2^(x - m), in two factors like all that L is
     // multiplied by.  A scale below 2^-60 counts as that (L stays in range) and its weight takes the rest on its
     // way to O.
