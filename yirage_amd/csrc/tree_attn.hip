@@ -19,13 +19,12 @@
 // bf16's smallest normal number); a fragment of V holds 8 tokens, whose scales go into the
 // weights' exponents instead.
 //
-// Bound: single rows by memory (32 sequences of 4 to 8 K tokens in 8 bits, 436 MB, 84 us, 5.2 TB/s; in 16 bits 865 MB,
-// 152 us, 5.7), one
-// long row by the chain of ids, first block, merge and join (32 K tokens: 20 + 4 us); chunks by issue and
-// the waits between MFMA and softmax of two waves a SIMD (2048 rows after 14 K tokens in 8 bits, 503 GFLOP,
-// 599 us, 0.84 PFLOP/s: VALU 65 % and MFMA 36 % of a SIMD's cycles).  Of the two workgroups of a CU the one
-// that starts first runs some 10 % faster; larger shares for those: the chunk 620 -> 607, a prompt of
-// 2048 90 -> 100, so not kept.
+// Bound: single rows by memory (32 sequences of 4 to 8 K tokens in 8 bits, 436 MB, 84 us, 5.2 TB/s; in 16 bits
+// 865 MB, 152 us, 5.7 TB/s), one long row by the chain of ids, first block, merge and join (32 K tokens: 20 + 4 us);
+// chunks by issue and the waits between MFMA and softmax of two waves a SIMD (2048 rows after 14 K tokens in 8 bits,
+// 503 GFLOP, 599 us, 0.84 PFLOP/s: VALU 65 % and MFMA 36 % of a SIMD's cycles).  Of the two workgroups of a CU the
+// one that starts first runs some 10 % faster; larger shares for those: the chunk 620 -> 607, a prompt of 2048
+// 90 -> 100, so not kept.
 #include <type_traits>
 
 #include "attn_device.h"
